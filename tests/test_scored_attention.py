@@ -1,0 +1,338 @@
+"""Attention with transformed scores: layouts, refusals and the reference on the CPU, the sm_100a kernels against the
+definition in 64 bits on the GPU, with element-wise bounds that follow from where the kernels round."""
+import math
+
+import pytest
+import torch
+
+from turbo_dllm_b200.ops.attention import MaskLayout, block_diffusion_layout
+from turbo_dllm_b200.ops.scored_attention import (DEAD_KEY, ScoreTransform, _seen_keys, document_layout, document_positions,
+                                                  scored_attention, scored_attention_reference)
+
+D = 128
+HALF = torch.finfo(torch.bfloat16).eps / 2     # a rounding to bf16 is off by at most half a step, relative
+# everything held in 32 bits: exponentials (two of them behind a cap, whose error grows with the cap's log2 e factor, 72
+# for the largest cap here, at 2^-22 each), sums over at most a few thousand terms, the stored lse
+FINE = 2.0 ** -14
+
+
+def exact(q, k, v, layout, tr, scale, dout=None):
+    """The definition in 64 bits, head by head, and the largest error a kernel may show in each output: P and dS are
+    rounded to bf16 as operands of the next product, out enters the row sum dO.out rounded, every result is rounded."""
+    nq, Hq, _ = q.shape
+    Hkv = k.shape[1]
+    G = Hq // Hkv
+    vis = layout.dense_mask()
+    q, k, v = (t.detach().double() for t in (q, k, v))
+    q = torch.where(vis.any(1)[:, None, None], q, torch.zeros_like(q))
+    k, v = (torch.where(vis.any(0)[:, None, None], t, torch.zeros_like(t)) for t in (k, v))
+    res = {n: torch.zeros_like(t) for n, t in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
+    res["lse"] = torch.full((Hq, nq), -math.inf, dtype=torch.float64, device=q.device)
+    tol = {n: torch.zeros_like(t) for n, t in res.items()}
+    for h in range(Hq):
+        qh, kh, vh = q[:, h], k[:, h // G], v[:, h // G]
+        s = scale * (qh @ kh.t())
+        t = torch.zeros_like(s)
+        z = s
+        if tr is not None and tr.softcap:
+            t = torch.tanh(s / tr.softcap)
+            z = tr.softcap * t
+        if tr is not None and tr.biased:
+            z = z - tr.slopes[h].double() * (tr.q_pos.double()[:, None] - tr.k_pos.double()[None]).abs()
+        z = z.masked_fill(~vis, -math.inf)
+        top = z.amax(-1, keepdim=True).clamp_min(-1e300)
+        e = torch.exp(z - top)
+        total = e.sum(-1, keepdim=True)
+        p = e / total.clamp_min(1e-300)
+        o = p @ vh
+        res["out"][:, h] = o
+        live = total[:, 0] > 0
+        res["lse"][h, live] = (top + torch.log(total))[live, 0]
+        a = p @ vh.abs()
+        eo = HALF * (o.abs() + a) + FINE * a
+        tol["out"][:, h] = eo
+        tol["lse"][h] = FINE * (1 + res["lse"][h].abs().nan_to_num(posinf=0))
+        if dout is None:
+            continue
+        do = torch.where(vis.any(1)[:, None], dout[:, h].detach().double(), torch.zeros_like(qh))
+        dp = do @ vh.t()
+        delta = (do * o).sum(-1, keepdim=True)
+        f = 1 - t * t
+        ds = p * f * (dp - delta)
+        res["dq"][:, h] = scale * (ds @ kh)
+        res["dk"][:, h // G] += scale * (ds.t() @ qh)
+        res["dv"][:, h // G] += p.t() @ do
+        edelta = (do.abs() * eo).sum(-1, keepdim=True)
+        eds = HALF * ds.abs() + p * f * edelta + p * (f + FINE) * FINE * (dp.abs() + delta.abs())
+        eds = eds + HALF * eds
+        tol["dq"][:, h] += scale * (eds @ kh.abs())
+        tol["dk"][:, h // G] += scale * (eds.t() @ qh.abs())
+        tol["dv"][:, h // G] += (HALF + FINE) * (p.t() @ do.abs())
+    for n in ("dq", "dk", "dv"):
+        tol[n] += HALF * (res[n].abs() + tol[n])
+    return res, tol
+
+
+def near(got, want, tol, name):
+    got = got.detach().double()
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fin), name
+    over = ((got - want).abs() - tol)[fin]
+    # 1e-6: sums of products that cancel to zero
+    assert over.numel() == 0 or float(over.max()) <= 1e-6, (name, float(over.max()), float((got - want).abs()[fin].max()))
+
+
+def transform_for(kind, Hq, qpos, kpos, device):
+    cap = {"cap": 50.0, "smallcap": 3.0, "both": 20.0}.get(kind, 0.0)
+    if kind in ("bias", "both"):
+        slopes = torch.exp2(-8.0 * (torch.arange(Hq, dtype=torch.float32) + 1) / Hq).to(device)
+        return ScoreTransform(cap, slopes, qpos.to(device), kpos.to(device))
+    return ScoreTransform(cap) if cap else None
+
+
+# ------------------------------------------------------------------------------------------------ CPU
+def test_document_layout_masks():
+    L = document_layout([3, 0, 5], prefix=[2, 0, 3], rows=11)
+    m = L.dense_mask()
+    want = torch.zeros(11, 11, dtype=torch.bool)
+    for s, n, pre in ((0, 3, 2), (3, 5, 3)):
+        for i in range(n):
+            want[s + i, s:s + max(i + 1, pre)] = True
+    assert torch.equal(m, want)
+    full = document_layout([3, 5], causal=False).dense_mask()
+    assert torch.equal(full, torch.block_diag(torch.ones(3, 3), torch.ones(5, 5)).bool())
+    assert document_positions([3, 0, 5], rows=11).tolist() == [0, 1, 2, 0, 1, 2, 3, 4, 0, 0, 0]
+    assert document_layout([]).nq == 0
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_seen_keys_match_the_dense_mask(seed):
+    g = torch.Generator().manual_seed(seed)
+    lo = torch.randint(0, 60, (23,), generator=g)
+    hi = lo + torch.randint(-5, 20, (23,), generator=g)
+    grp = -torch.randint(0, 6, (23,), generator=g)
+    code = torch.randint(-8, 80, (57,), generator=g)
+    code[5] = DEAD_KEY
+    L = MaskLayout(*(t.to(torch.int32) for t in (lo, hi, grp, code)))
+    want = L.dense_mask().any(0)
+    # a query of grp 0 sees no noisy key: codes are negative there
+    assert torch.equal(_seen_keys(L), want)
+
+
+@pytest.mark.parametrize("kind", ["none", "cap", "smallcap", "bias", "both"])
+def test_reference_gradients_against_differences(kind):
+    torch.manual_seed(1)
+    lens, rows = [4, 0, 3], 9
+    L = document_layout(lens, prefix=[2, 0, 0], rows=rows)
+    pos = document_positions(lens, rows=rows)
+    tr = transform_for(kind, 4, pos, pos, "cpu")
+    x = [torch.randn(rows, h, 8, dtype=torch.float64).requires_grad_() for h in (4, 2, 2)]
+    assert torch.autograd.gradcheck(lambda *t: scored_attention(*t, L, tr), x)
+    out, lse = scored_attention(*x, L, tr, return_lse=True)
+    assert not lse.requires_grad and bool(torch.isinf(lse[:, 7:]).all()) and float(out[7:].abs().max()) == 0
+
+
+def test_reference_matches_the_plain_operator_and_ignores_dead_rows():
+    from turbo_dllm_b200.ops.attention import attention_reference
+
+    torch.manual_seed(2)
+    p = torch.arange(24)
+    L = block_diffusion_layout(p, p // 8, p, 8)
+    q, k, v = (torch.randn(48, h, 16) for h in (4, 2, 2))
+    assert torch.allclose(scored_attention(q, k, v, L), attention_reference(q, k, v, L)[0], atol=1e-6)
+    L = document_layout([20, 11], rows=40)
+    clean = scored_attention(q[:40], k[:40], v[:40], L)
+    for t in (q, k, v):
+        t[31:40] = float("nan")
+    got = scored_attention(q[:40], k[:40], v[:40], L)
+    assert torch.equal(got, clean)
+
+
+def test_refusals():
+    L = document_layout([4, 4])
+    pos = document_positions([4, 4])
+    q, k = torch.zeros(8, 4, 16), torch.zeros(8, 2, 16)
+    for bad in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="softcap"):
+            ScoreTransform(bad)
+    s = torch.ones(4)
+    with pytest.raises(ValueError, match="together"):
+        ScoreTransform(0.0, s)
+    with pytest.raises(ValueError, match="float32"):
+        ScoreTransform(0.0, s.double(), pos, pos)
+    with pytest.raises(ValueError, match="no gradient"):
+        ScoreTransform(0.0, s.clone().requires_grad_(), pos, pos)
+    with pytest.raises(ValueError, match="int32"):
+        ScoreTransform(0.0, s, pos.float(), pos)
+    with pytest.raises(ValueError, match="slopes"):
+        scored_attention(q, k, k, L, ScoreTransform(0.0, torch.ones(3), pos, pos))
+    with pytest.raises(ValueError, match="position"):
+        scored_attention(q, k, k, L, ScoreTransform(0.0, s, pos[:5], pos))
+    with pytest.raises(ValueError, match="divide"):
+        scored_attention(q[:, :3], k, k, L)
+    with pytest.raises(ValueError, match="layout describes"):
+        scored_attention(q[:5], k, k, L)
+    with pytest.raises(ValueError, match="share"):
+        scored_attention(q, k.double(), k.double(), L)
+    with pytest.raises(ValueError, match="need q"):
+        scored_attention(q, k, k[:, :1], L)
+    with pytest.raises(ValueError, match="rows"):
+        document_layout([4, 4], rows=7)
+    with pytest.raises(ValueError, match="prefix"):
+        document_layout([4, 4], prefix=[5, 0])
+    with pytest.raises(ValueError, match="negative"):
+        document_layout([4, -1])
+    far = torch.full((8,), 1 << 24, dtype=torch.int32)
+    with pytest.raises(ValueError, match="positions"):
+        ScoreTransform(0.0, s, far, pos)._padded(128, 128)
+
+
+def test_padded_positions_follow_the_tensors():
+    pos = document_positions([5])
+    tr = ScoreTransform(0.0, torch.ones(2), pos, pos)
+    assert tr._padded(128, 128)[1][4] == 4
+    pos[4] = 9
+    assert tr._padded(128, 128)[1][4] == 9
+
+
+# ------------------------------------------------------------------------------------------------ GPU
+def _operands(nq, nk, Hq, Hkv, seed, packed=False, gain=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    if packed:
+        rows = torch.randn(nq, (Hq + 2 * Hkv) * D, generator=g, device="cuda").bfloat16() * gain
+        return (rows[:, :Hq * D].view(nq, Hq, D), rows[:, Hq * D:(Hq + Hkv) * D].view(nk, Hkv, D),
+                rows[:, (Hq + Hkv) * D:].view(nk, Hkv, D))
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")   # noqa: E731
+    return (r(nq, Hq, D) * gain).bfloat16(), r(nk, Hkv, D).bfloat16(), r(nk, Hkv, D).bfloat16()
+
+
+def run_case(q, k, v, layout, tr, backward=True, seed=3):
+    from turbo_dllm_b200.kernels import native
+
+    scale = 1.0 / math.sqrt(D)
+    q, k, v = (t.detach().requires_grad_(backward) for t in (q, k, v))
+    out, lse = scored_attention(q, k, v, layout, tr, return_lse=True)
+    dout = torch.randn(out.shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").bfloat16()
+    got = {"out": out, "lse": lse}
+    if backward:
+        got.update(zip(("dq", "dk", "dv"), torch.autograd.grad(out, [q, k, v], dout)))
+    torch.cuda.synchronize()
+    native.raise_on_device_error()
+    want, tol = exact(q, k, v, layout, tr, scale, dout if backward else None)
+    for n, t in got.items():
+        near(t, want[n], tol[n], n)
+    return got
+
+
+def blocks(tokens, block, device="cuda", window=None):
+    p = torch.arange(tokens, device=device)
+    L = block_diffusion_layout(p, p // block, p, block, window=window)
+    return L, torch.cat([p, p]).to(torch.int32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["none", "cap", "smallcap", "bias", "both"])
+@pytest.mark.parametrize("lens,prefix,rows", [([1], None, 1), ([5, 0, 2], None, 7), ([128], None, 128), ([129], [40], 129),
+                                             ([100, 1, 200, 30], [0, 1, 150, 30], 345), ([700], [1], 719)])
+def test_documents(kind, lens, prefix, rows):
+    L = document_layout(lens, prefix=prefix, rows=rows, device="cuda")
+    pos = document_positions(lens, rows=rows, device="cuda")
+    run_case(*_operands(rows, rows, 4, 2, 0, packed=True), L, transform_for(kind, 4, pos, pos, "cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["cap", "both"])
+@pytest.mark.parametrize("Hq,Hkv", [(1, 1), (3, 1), (8, 2), (6, 6)])
+def test_blocks(kind, Hq, Hkv):
+    L, pos = blocks(256, 32)
+    run_case(*_operands(512, 512, Hq, Hkv, 1), L, transform_for(kind, Hq, pos, pos, "cuda"))
+
+
+@pytest.mark.gpu
+def test_windows_and_keys_of_another_length():
+    L, pos = blocks(384, 16, window=100)
+    run_case(*_operands(768, 768, 4, 2, 2), L, transform_for("both", 4, pos, pos, "cuda"))
+    p = torch.arange(500, device="cuda")
+    L = block_diffusion_layout(p[96:160], p[96:160] // 32, p[:77], 32, key_clean_pos=p[::3])
+    qpos = torch.cat([p[96:160], p[:77]]).to(torch.int32)
+    kpos = torch.cat([p[96:160], p[::3]]).to(torch.int32)
+    run_case(*_operands(L.nq, L.nk, 4, 2, 3), L, transform_for("both", 4, qpos, kpos, "cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -3.0e38])
+def test_contents_of_dead_rows_do_not_matter(junk):
+    lens, rows = [90, 130], 300
+    L = document_layout(lens, rows=rows, device="cuda")
+    pos = document_positions(lens, rows=rows, device="cuda")
+    tr = transform_for("both", 4, pos, pos, "cuda")
+    q, k, v = (t.clone() for t in _operands(rows, rows, 4, 2, 4))
+    for t in (q, k, v):
+        t[220:] = junk
+    got = run_case(q, k, v, L, tr)
+    assert float(got["out"][220:].abs().max()) == 0 and all(float(got[n][220:].abs().max()) == 0 for n in ("dq", "dk", "dv"))
+
+
+@pytest.mark.gpu
+def test_masks_that_leave_every_row_empty():
+    z = torch.zeros(70, dtype=torch.int32, device="cuda")
+    L = MaskLayout(z, z, z, z + 5)
+    got = run_case(*_operands(70, 70, 2, 1, 5), L, ScoreTransform(10.0))
+    assert float(got["dk"].abs().max()) == 0
+
+
+@pytest.mark.gpu
+def test_strides_and_alignment():
+    L = document_layout([150], device="cuda")
+    q, k, v = _operands(150, 150, 4, 2, 6)
+    base = scored_attention(q, k, v, L, ScoreTransform(20.0))
+    odd = torch.empty(150 * 4 * D + 1, dtype=torch.bfloat16, device="cuda")[1:].view(150, 4, D)    # 2-byte aligned base
+    odd.copy_(q)
+    heads_first = k.permute(1, 0, 2).contiguous().permute(1, 0, 2)
+    wide = torch.zeros(150, 2, 2 * D, dtype=torch.bfloat16, device="cuda")
+    wide[..., :D] = v
+    assert torch.equal(scored_attention(odd, heads_first, wide[..., :D], L, ScoreTransform(20.0)), base)
+    qg = odd.detach().requires_grad_()
+    out = scored_attention(qg, heads_first, wide[..., :D], L, ScoreTransform(20.0))
+    (dq,) = torch.autograd.grad(out, [qg], torch.ones((), dtype=out.dtype, device="cuda").expand_as(out))
+    assert torch.isfinite(dq).all()
+
+
+@pytest.mark.gpu
+def test_empty_operands_and_other_types():
+    e = torch.empty(0, 4, D, dtype=torch.bfloat16, device="cuda")
+    L = document_layout([], device="cuda")
+    out, lse = scored_attention(e, e[:, :2], e[:, :2], L, ScoreTransform(5.0), return_lse=True)
+    assert out.shape == (0, 4, D) and lse.shape == (4, 0)
+    z = torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 4, D, device="cuda").bfloat16().requires_grad_()
+    out, lse = scored_attention(q, e[:, :2], e[:, :2], MaskLayout(z, z + 9, z, z[:0]), return_lse=True)
+    assert float(out.abs().max()) == 0 and bool(torch.isinf(lse).all())
+    x = torch.randn(40, 2, 64, device="cuda")
+    L = document_layout([40], device="cuda")
+    ref = scored_attention_reference(x.double(), x.double(), x.double(), L, ScoreTransform(3.0))[0]
+    assert torch.allclose(scored_attention(x, x, x, L, ScoreTransform(3.0)).double(), ref, atol=1e-5)
+    from turbo_dllm_b200.kernels.native import NativeKernelError
+
+    with pytest.raises(NativeKernelError, match="head_dim"):
+        scored_attention(x.bfloat16(), x.bfloat16(), x.bfloat16(), L)
+
+
+@pytest.mark.gpu
+def test_another_stream_and_a_captured_graph():
+    L = document_layout([200], device="cuda")
+    q, k, v = _operands(200, 200, 4, 2, 7)
+    tr = ScoreTransform(20.0)
+    want = scored_attention(q, k, v, L, tr)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = scored_attention(q, k, v, L, tr)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = scored_attention(q, k, v, L, tr)
+    q.copy_(q.flip(0))
+    graph.replay()
+    assert torch.equal(held, scored_attention(q, k, v, L, tr))

@@ -115,6 +115,23 @@ int tdllm_attn_merge_bwd(const void* go, const void* out, const float* lse, cons
                          const float* lse_s, void* go_s, float* dlse_s, long long nrh, int D,
                          void* stream);
 
+// ---- attention with transformed scores (score_mod.cuh) ----------------------
+// As tdllm_attn_fwd / tdllm_attn_bwd_fused, on scores cap*tanh(scale*q.k/cap) - slope_h*|q_pos - k_pos|. softcap 0: no
+// cap; slope2 null: no bias, else [Hq] slopes times log2(e), with positions as floats padded to nq_pad / nk_pad.
+// Contents of query rows and keys that take part in no visible pair do not matter (keys: code -2^31).
+int tdllm_attn_fwd_scored(const void* q, const void* k, const void* v, void* o, float* lse, int nq, int nk, int Hq,
+                          int Hkv, long long ldq, long long ldk, long long ldv, long long ldo, const int* q_lo,
+                          const int* q_hi, const int* q_grp, const int* k_code, const int* tile_ptr,
+                          const int* tile_idx, const int* order, int n_qtiles, float scale, float softcap,
+                          const float* slope2, const float* q_pos, const float* k_pos, void* stream);
+int tdllm_attn_bwd_scored(const void* q, const void* k, const void* v, const void* o, const void* dout, void* dq,
+                          void* dk, void* dv, const float* lse, float* delta, float* acc, int nq, int nk, int Hq,
+                          int Hkv, long long ldq, long long ldk, long long ldv, long long ldo, long long lddo,
+                          long long lddq, long long lddk, long long lddv, const int* q_lo, const int* q_hi,
+                          const int* q_grp, const int* k_code, const int* w_ptr, const int* w_idx,
+                          const int* w_order, int n_work, int n_qtiles, int n_ktiles, float scale, float softcap,
+                          const float* slope2, const float* q_pos, const float* k_pos, void* stream);
+
 // ---- block-diffusion attention (head_dim 128) ------------------------------
 int tdllm_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int nq,
                    int nk, int Hq, int Hkv, long long ldq, long long ldk, long long ldv,

@@ -30,6 +30,10 @@
 // goes to shared memory as bf16 (one 128-byte swizzled row of 64 queries per key): the B operand
 // of the dQᵀ product, whose A operand is the K tile read MN-major (same bytes as the Sᵀ product).
 //
+// Transformed scores (template argument MOD, score_mod.cuh): the probabilities come from the transformed scores, and
+// dS gets the factor 1 - tanh^2 of the cap. Rows of Q and dO whose query sees no key, and rows of K that no query sees,
+// are overwritten with zeros in shared memory before the gradient products read them.
+//
 // Context-sharded form (template argument CSBP): key tiles [0, nlt) are this rank's own rows, key tiles from
 // nlt on are clean rows of the other ranks of the context-parallel group (their K|V were brought into
 // kv_rem by the forward kernel). The dK/dV partial sums of a remote key tile never touch this GPU's memory:
@@ -45,6 +49,7 @@
 // flash_bwd_sm100.py: five products, dQ by reduce-add) and the owner-major clean dK/dV
 // buffers of dllm_parallel/core/attention/context_parallel_attention.py:820-885.
 #include "common.cuh"
+#include "score_mod.cuh"
 #include "api.h"
 
 namespace tdllm {
@@ -96,6 +101,7 @@ struct Params {
   const float* lse2;   // [Hq, nq_pad] −lse·log2e (−inf = row without keys)
   const float* delta;  // [Hq, nq_pad] −scale · rowsum(dO∘O)
   float scale_log2, scale;
+  score::Mod mod;      // MOD != 0: the score transform
 };
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -121,7 +127,7 @@ __device__ __forceinline__ void red_add_peer_f32x4(float* dst, uint32_t a, uint3
                : "memory");
 }
 
-template <bool CSBP>
+template <bool CSBP, int MOD>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                       const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -341,6 +347,19 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     float* red = (float*)(sRed + grp * RED_BYTES);
     const bool issuer = (qd == 0 && lane == 0);   // issues and tracks this group's reduce-add copies
     int st = b;   // stage of unit 2*it + b
+    [[maybe_unused]] float kpos = 0.f, slope2 = 0.f;
+    if constexpr ((MOD & score::BIAS) != 0) kpos = p.mod.k_pos[kt * 128 + row];
+    if constexpr (MOD != 0) {
+      // dead keys: both slots clear them (the same zeros), each before its own first arrival
+      if (items > 0 && __any_sync(0xffffffffu, kcode == score::DEAD_KEY)) {
+        if (kcode == score::DEAD_KEY && mbar_wait_spin(bar_kv, 0, KID, 34)) {
+          uint4* krow = reinterpret_cast<uint4*>(sK + sub * KV_HALF_BYTES + row * 128);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) krow[e] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+      }
+    }
     for (int it = 0; it < items; ++it) {
       const int ent = list[it % n];
       const int qrow0 = (ent >> 1) * 128 + b * 64 + sub * 32;
@@ -358,7 +377,37 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           tmem_ld16(t_s + sub * 32 + c * 16, rs);
           tmem_ld16(t_s + 64 + sub * 32 + c * 16, rp);
           tmem_ld_wait();
-          if (ent & 1) {
+          if constexpr (MOD != 0) {
+            const bool masked = ent & 1;
+            if constexpr ((MOD & score::BIAS) != 0) slope2 = __ldg(p.mod.slope2 + kvh * G + it / n);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              float pv[2], ds[2];
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                const int g = qrow0 + c * 16 + e + t;
+                float z = __uint_as_float(rs[e + t]), f = 1.f;
+                if constexpr ((MOD & score::CAP) != 0) {
+                  const float r = score::cap_r(z, p.mod);
+                  z = score::cap_z(r, p.mod);
+                  f = score::cap_slope(r);
+                } else {
+                  z *= p.scale_log2;
+                }
+                if constexpr ((MOD & score::BIAS) != 0) z = fmaf(-slope2, fabsf(__ldg(p.mod.q_pos + g) - kpos), z);
+                float pr = fast_exp2(z + sl[c * 16 + e + t]);
+                float u = fmaf(__uint_as_float(rp[e + t]), p.scale, sd[c * 16 + e + t]) * (pr * f);
+                if (masked && !key_visible(kcode, __ldg(p.q_lo + g), __ldg(p.q_hi + g), __ldg(p.q_grp + g))) {
+                  pr = 0.f;   // (selected, not multiplied: a dead row or key may have left NaN in either product)
+                  u = 0.f;
+                }
+                pv[t] = pr;
+                ds[t] = u;
+              }
+              pk[c * 8 + (e >> 1)] = pack_bf16x2(pv[0], pv[1]);
+              dk[c * 8 + (e >> 1)] = pack_bf16x2(ds[0], ds[1]);
+            }
+          } else if (ent & 1) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
               const float4 l4 = *reinterpret_cast<const float4*>(sl + c * 16 + e);
@@ -418,6 +467,18 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           for (int j = 0; j < 4; ++j)
             *reinterpret_cast<uint4*>(srow + sw128_offset(row, sub * 4 + j)) =
                 make_uint4(dk[4 * j], dk[4 * j + 1], dk[4 * j + 2], dk[4 * j + 3]);
+        }
+        if constexpr (MOD != 0) {
+          // queries without a visible key (lse2 = -inf): four threads per query clear one half row of Q or dO each
+          if (ent & 1) {
+            const int t = qd * 32 + lane, qi = t >> 2, piece = t & 3;
+            if (sl[qi] == -INFINITY) {
+              uint8_t* tile = (piece & 2) ? sdO : sQ;
+              uint4* zrow = reinterpret_cast<uint4*>(tile + st * QS_BYTES + (piece & 1) * QS_HALF_BYTES + (sub * 32 + qi) * 128);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) zrow[e] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
         }
         tmem_st_wait();
         fence_proxy_async_smem();

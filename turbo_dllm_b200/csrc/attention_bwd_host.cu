@@ -114,39 +114,42 @@ __global__ void acc_cast_kernel(const float* __restrict__ acc, __nv_bfloat16* __
 // accumulators, zeroed here). Work items (`w_*`): for chunk c of query tiles and key tile kt, item
 // c*n_ktiles + kt lists the chunk's query tiles that see the key tile (w_ptr has one entry per item
 // plus one); `w_order` names the non-empty items, chunk by chunk.
-extern "C" int tdllm_attn_bwd_fused(const void* q, const void* k, const void* v, const void* o,
-                                    const void* dout, void* dq, void* dk, void* dv, const float* lse,
-                                    float* delta, float* acc, int nq, int nk, int Hq, int Hkv,
-                                    long long ldq, long long ldk, long long ldv, long long ldo,
-                                    long long lddo, long long lddq, long long lddk, long long lddv,
-                                    const int* q_lo, const int* q_hi, const int* q_grp,
-                                    const int* k_code, const int* w_ptr, const int* w_idx,
-                                    const int* w_order, int n_work, int n_qtiles, int n_ktiles,
-                                    float scale, void* stream) {
+template <int MOD>
+static int attn_bwd_fused_launch(const char* who, const void* q, const void* k, const void* v, const void* o,
+                                 const void* dout, void* dq, void* dk, void* dv, const float* lse,
+                                 float* delta, float* acc, int nq, int nk, int Hq, int Hkv,
+                                 long long ldq, long long ldk, long long ldv, long long ldo,
+                                 long long lddo, long long lddq, long long lddk, long long lddv,
+                                 const int* q_lo, const int* q_hi, const int* q_grp,
+                                 const int* k_code, const int* w_ptr, const int* w_idx,
+                                 const int* w_order, int n_work, int n_qtiles, int n_ktiles,
+                                 float scale, const score::Mod& mod, void* stream) {
   if (nq <= 0 || nk <= 0) return 0;
   if (Hq % Hkv) {
-    tdllm_host::set_last_error("attn_bwd_fused: %d query heads do not divide over %d KV heads", Hq, Hkv);
+    tdllm_host::set_last_error("%s: %d query heads do not divide over %d KV heads", who, Hq, Hkv);
     return 1;
   }
   const long long lds[8] = {ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv};
   const void* ptrs[8] = {q, k, v, o, dout, dq, dk, dv};
   for (int i = 0; i < 8; ++i)
     if ((lds[i] % 8) || ((uintptr_t)ptrs[i] % 16)) {
-      tdllm_host::set_last_error("attn_bwd_fused: operand %d needs 16-byte aligned base and row stride", i);
+      tdllm_host::set_last_error("%s: operand %d needs 16-byte aligned base and row stride", who, i);
       return 1;
     }
   if ((uintptr_t)acc % 128) {
-    tdllm_host::set_last_error("attn_bwd_fused: accumulator scratch must be 128-byte aligned");
+    tdllm_host::set_last_error("%s: accumulator scratch must be 128-byte aligned", who);
     return 1;
   }
-  static bool attr_set = false;
-  if (!attr_set) {
-    if (cudaFuncSetAttribute(attn_fused::attn_bwd_fused_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  static bool attr_set[64] = {false};   // a function attribute belongs to one device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    if (cudaFuncSetAttribute(attn_fused::attn_bwd_fused_kernel<false, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              attn_fused::SMEM_BYTES) != cudaSuccess) {
-      tdllm_host::set_last_error("attn_bwd_fused: cudaFuncSetAttribute failed");
+      tdllm_host::set_last_error("%s: cudaFuncSetAttribute failed", who);
       return 2;
     }
-    attr_set = true;
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   cudaStream_t s = (cudaStream_t)stream;
   const int nq_pad = n_qtiles * 128, nk_pad = n_ktiles * 128;
@@ -192,9 +195,10 @@ extern "C" int tdllm_attn_bwd_fused(const void* q, const void* k, const void* v,
     p.tile_ptr = w_ptr; p.tile_idx = w_idx; p.order = w_order;
     p.lse2 = delta + (size_t)Hq * nq_pad; p.delta = delta;
     p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
+    p.mod = mod;
     attn_fused::PushPlan pp;
     memset(&pp, 0, sizeof(pp));
-    attn_fused::attn_bwd_fused_kernel<false><<<n_work * Hkv, attn_fused::THREADS, attn_fused::SMEM_BYTES, s>>>(
+    attn_fused::attn_bwd_fused_kernel<false, MOD><<<n_work * Hkv, attn_fused::THREADS, attn_fused::SMEM_BYTES, s>>>(
         tq, tdo, tk, tv, tdk, tdv, tacc, tk, tv, p, pp);
   }
   {
@@ -206,10 +210,50 @@ extern "C" int tdllm_attn_bwd_fused(const void* q, const void* k, const void* v,
   }
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
-    tdllm_host::set_last_error("attn_bwd_fused launch: %s", cudaGetErrorString(e));
+    tdllm_host::set_last_error("%s launch: %s", who, cudaGetErrorString(e));
     return 4;
   }
   return 0;
+}
+
+extern "C" int tdllm_attn_bwd_fused(const void* q, const void* k, const void* v, const void* o,
+                                    const void* dout, void* dq, void* dk, void* dv, const float* lse,
+                                    float* delta, float* acc, int nq, int nk, int Hq, int Hkv,
+                                    long long ldq, long long ldk, long long ldv, long long ldo,
+                                    long long lddo, long long lddq, long long lddk, long long lddv,
+                                    const int* q_lo, const int* q_hi, const int* q_grp,
+                                    const int* k_code, const int* w_ptr, const int* w_idx,
+                                    const int* w_order, int n_work, int n_qtiles, int n_ktiles,
+                                    float scale, void* stream) {
+  score::Mod mod;
+  memset(&mod, 0, sizeof(mod));
+  return attn_bwd_fused_launch<0>("attn_bwd_fused", q, k, v, o, dout, dq, dk, dv, lse, delta, acc, nq, nk, Hq, Hkv, ldq,
+                                  ldk, ldv, ldo, lddo, lddq, lddk, lddv, q_lo, q_hi, q_grp, k_code, w_ptr, w_idx, w_order,
+                                  n_work, n_qtiles, n_ktiles, scale, mod, stream);
+}
+
+// The same for transformed scores (arguments as in tdllm_attn_fwd_scored).
+extern "C" int tdllm_attn_bwd_scored(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                                     void* dq, void* dk, void* dv, const float* lse, float* delta, float* acc, int nq,
+                                     int nk, int Hq, int Hkv, long long ldq, long long ldk, long long ldv, long long ldo,
+                                     long long lddo, long long lddq, long long lddk, long long lddv, const int* q_lo,
+                                     const int* q_hi, const int* q_grp, const int* k_code, const int* w_ptr,
+                                     const int* w_idx, const int* w_order, int n_work, int n_qtiles, int n_ktiles,
+                                     float scale, float softcap, const float* slope2, const float* q_pos,
+                                     const float* k_pos, void* stream) {
+  const score::Mod mod = score_mod_of(scale, softcap, slope2, q_pos, k_pos);
+#define TD_SCORED_BWD(M)                                                                                               \
+  return attn_bwd_fused_launch<score::SAFE | (M)>("attn_bwd_scored", q, k, v, o, dout, dq, dk, dv, lse, delta, acc,    \
+                                                  nq, nk, Hq, Hkv, ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv, q_lo,   \
+                                                  q_hi, q_grp, k_code, w_ptr, w_idx, w_order, n_work, n_qtiles,        \
+                                                  n_ktiles, scale, mod, stream)
+  switch ((softcap > 0.f ? score::CAP : 0) | (slope2 ? score::BIAS : 0)) {
+    case 0: TD_SCORED_BWD(0);
+    case score::CAP: TD_SCORED_BWD(score::CAP);
+    case score::BIAS: TD_SCORED_BWD(score::BIAS);
+    default: TD_SCORED_BWD(score::CAP | score::BIAS);
+  }
+#undef TD_SCORED_BWD
 }
 
 // Context-sharded one-pass backward. Keys as in tdllm_attn_fwd_csbp: this rank's nk_loc rows, then (from key
@@ -255,7 +299,7 @@ extern "C" int tdllm_attn_bwd_fused_csbp(
   }
   static bool attr_set = false;
   if (!attr_set) {
-    if (cudaFuncSetAttribute(attn_fused::attn_bwd_fused_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(attn_fused::attn_bwd_fused_kernel<true, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              attn_fused::SMEM_BYTES) != cudaSuccess) {
       tdllm_host::set_last_error("attn_bwd_fused_csbp: cudaFuncSetAttribute failed");
       return 2;
@@ -326,7 +370,7 @@ extern "C" int tdllm_attn_bwd_fused_csbp(
     }
     pp.n_rows = n_rem;
     pp.nlt = nlt;
-    attn_fused::attn_bwd_fused_kernel<true><<<n_work * Hkv, attn_fused::THREADS, attn_fused::SMEM_BYTES, s>>>(
+    attn_fused::attn_bwd_fused_kernel<true, 0><<<n_work * Hkv, attn_fused::THREADS, attn_fused::SMEM_BYTES, s>>>(
         tq, tdo, tk, tv, tdk, tdv, tacc, tkr, tvr, p, pp);
   }
   // every rank's partial sums for this rank's rows are in place once all ranks have passed this point

@@ -23,6 +23,10 @@
 // (mask_mod) and the predicate of dllm_parallel/core/attention/context_parallel_attention.py:119-144.
 // It returns (out, lse) so shard results can be merged across K/V owners.
 //
+// Transformed scores (template argument MOD, score_mod.cuh): a tanh cap and / or a bias by distance, applied to the
+// scores right after they leave TMEM, in log2 units; the row maximum, the lazy rescale and the exponentials then work
+// on the transformed values. Keys that no row sees have their V row overwritten with zeros before P.V reads the tile.
+//
 // Context-sharded form (template argument CSBP): key tiles [0, nlt) are this rank's own rows and are read
 // in place; key tiles [nlt, nlt + nrt) are clean K|V rows owned by the peers of the context-parallel group.
 // Two extra warps per CTA ("pullers") fetch those rows from the peers' symmetric staging buffers with plain
@@ -35,6 +39,7 @@
 #include <cstring>
 #include "common.cuh"
 #include "peer_pull.cuh"
+#include "score_mod.cuh"
 #include "api.h"
 
 namespace tdllm {
@@ -68,6 +73,7 @@ struct FwdParams {
   float* lse;          // [Hq, nq_pad]
   float scale_log2;    // softmax scale * log2(e)
   float scale;         // softmax scale
+  score::Mod mod;      // MOD != 0: the score transform
 };
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -96,7 +102,7 @@ __device__ __forceinline__ bool key_visible(int code, int lo, int hi, int grp) {
   return code >= 0 ? (code >= lo && code < hi) : (code == grp);
 }
 
-template <bool CSBP>
+template <bool CSBP, int MOD>
 __global__ void __launch_bounds__(CSBP ? THREADS_CSBP : THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
@@ -285,7 +291,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint32_t t_o = tmem_base + ((uint32_t)(qd * 32) << 16) + 256 + i * 128;
     float* xmine = sX + (i * 2 + sub) * 128 + row;
     const float* xother = sX + (i * 2 + (sub ^ 1)) * 128 + row;
-    float m_used = -INFINITY;  // max the stored probabilities are relative to (raw score units)
+    const float scl = MOD ? 1.f : p.scale_log2;   // transformed scores already are in log2 units
+    [[maybe_unused]] float slope2 = 0.f, qpos = 0.f;
+    if constexpr ((MOD & score::BIAS) != 0) {
+      slope2 = p.mod.slope2[min(h0 + i, h_last)];
+      qpos = p.mod.q_pos[grow];
+    }
+    float m_used = -INFINITY;  // max the stored probabilities are relative to (raw score units; log2 units if MOD)
     float l = 0.f;             // this thread's share of the row sum
     uint32_t r[64];
     bool ok = true;
@@ -298,6 +310,28 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tmem_ld32(t_s + sub * 64, r);
         tmem_ld32(t_s + sub * 64 + 32, r + 32);
         tmem_ld_wait();
+        if constexpr (MOD != 0) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            float z = __uint_as_float(r[e]);
+            if constexpr ((MOD & score::CAP) != 0) z = score::cap_z(score::cap_r(z, p.mod), p.mod);
+            else z *= p.scale_log2;
+            if constexpr ((MOD & score::BIAS) != 0)
+              z = fmaf(-slope2, fabsf(qpos - __ldg(p.mod.k_pos + (ent >> 1) * BKV + sub * 64 + e)), z);
+            r[e] = __float_as_uint(z);
+          }
+          if (ent & 1) {
+            // this thread's key of the tile (and half of its columns): a dead key's V row is zeroed
+            if (__ldg(p.k_code + (ent >> 1) * BKV + row) == score::DEAD_KEY) {
+              if (mbar_wait_spin(bar_vfull + 8 * (j & 1), (j >> 1) & 1, KID, 33)) {
+                uint4* vrow = reinterpret_cast<uint4*>(sV + (j & 1) * TILE_BYTES + sub * HALF_BYTES + row * 128);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+            fence_proxy_async_smem();
+          }
+        }
         if (ent & 1) {
           const int lo = __ldg(p.q_lo + grow), hi = __ldg(p.q_hi + grow), grp = __ldg(p.q_grp + grow);
 #pragma unroll
@@ -315,8 +349,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // lazy rescale: keep the old reference max unless the new one is 2^8 larger (both threads of a
       // row take the same decision: same inputs)
       float alpha = 1.f;
-      if (mx > -INFINITY && (m_used == -INFINITY || (mx - m_used) * p.scale_log2 > 8.f)) {
-        alpha = (m_used == -INFINITY) ? 0.f : fast_exp2((m_used - mx) * p.scale_log2);
+      if (mx > -INFINITY && (m_used == -INFINITY || (mx - m_used) * scl > 8.f)) {
+        alpha = (m_used == -INFINITY) ? 0.f : fast_exp2((m_used - mx) * scl);
         m_used = mx;
       }
       l *= alpha;
@@ -332,14 +366,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       // probabilities -> bf16 P in TMEM over the S columns; masked scores are -inf -> exactly 0
-      const float mref = (m_used == -INFINITY) ? 0.f : m_used * p.scale_log2;
+      const float mref = (m_used == -INFINITY) ? 0.f : m_used * scl;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t pk[8];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-          const float p0 = fast_exp2(fmaf(__uint_as_float(r[c * 16 + e]), p.scale_log2, -mref));
-          const float p1 = fast_exp2(fmaf(__uint_as_float(r[c * 16 + e + 1]), p.scale_log2, -mref));
+          const float p0 = fast_exp2(fmaf(__uint_as_float(r[c * 16 + e]), scl, -mref));
+          const float p1 = fast_exp2(fmaf(__uint_as_float(r[c * 16 + e + 1]), scl, -mref));
           l += p0 + p1;
           pk[e >> 1] = pack_bf16x2(p0, p1);
         }
@@ -382,7 +416,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       if (sub == 0)
-        p.lse[(size_t)min(h0 + i, h_last) * p.nq_pad + grow] = l > 0.f ? m_used * p.scale + __logf(l) : -INFINITY;
+        p.lse[(size_t)min(h0 + i, h_last) * p.nq_pad + grow] = l > 0.f ? m_used * (MOD ? 0.69314718055994531f : p.scale) + __logf(l) : -INFINITY;
       fence_proxy_async_smem();
       mbar_arrive(bar_epi + 8 * i);
       if (row == 0 && sub == 0) {
@@ -440,28 +474,28 @@ static int attn_fwd_check(const char* who, int Hq, int Hkv, const long long* lds
   return 0;
 }
 
-// q [nq, Hq*128] (row stride ldq), k/v [nk, Hkv*128], o [nq, Hq*128], lse [Hq, nq_pad].
-// Row metadata arrays are padded to nq_pad / nk_pad (multiples of 128) by the caller.
-extern "C" int tdllm_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
-                              int nq, int nk, int Hq, int Hkv, long long ldq, long long ldk,
-                              long long ldv, long long ldo, const int* q_lo, const int* q_hi,
-                              const int* q_grp, const int* k_code, const int* tile_ptr,
-                              const int* tile_idx, const int* order, int n_qtiles, float scale,
-                              void* stream) {
+// One-GPU launch, plain (MOD == 0) or with transformed scores.
+template <int MOD>
+static int attn_fwd_launch(const char* who, const void* q, const void* k, const void* v, void* o, float* lse, int nq,
+                           int nk, int Hq, int Hkv, long long ldq, long long ldk, long long ldv, long long ldo,
+                           const int* q_lo, const int* q_hi, const int* q_grp, const int* k_code, const int* tile_ptr,
+                           const int* tile_idx, const int* order, int n_qtiles, float scale, const score::Mod& mod,
+                           cudaStream_t stream) {
   using namespace tdllm::attn;
-  if (nq <= 0) return 0;
   const long long lds[4] = {ldq, ldk, ldv, ldo};
   const void* ptrs[4] = {q, k, v, o};
-  if (attn_fwd_check("attn_fwd", Hq, Hkv, lds, ptrs, 4)) return 1;
-  static bool attr_set = false;
-  if (!attr_set) {
-    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  if (attn_fwd_check(who, Hq, Hkv, lds, ptrs, 4)) return 1;
+  static bool attr_set[64] = {false};   // a function attribute belongs to one device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<false, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          SMEM_BYTES);
     if (e != cudaSuccess) {
-      tdllm_host::set_last_error("attn_fwd: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      tdllm_host::set_last_error("%s: cudaFuncSetAttribute: %s", who, cudaGetErrorString(e));
       return 2;
     }
-    attr_set = true;
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   CUtensorMap tq, tk, tv, to;
   if (tdllm_host::encode_rows_tmap(&tq, q, (long long)Hq * HD, nq, ldq, 128)) return 3;
@@ -476,16 +510,55 @@ extern "C" int tdllm_attn_fwd(const void* q, const void* k, const void* v, void*
   p.lse = lse;
   p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.mod = mod;
   PullPlan pl;
   memset(&pl, 0, sizeof(pl));
   const int grid = n_qtiles * Hkv * ((Hq / Hkv + 1) / 2);
-  attn_fwd_kernel<false><<<grid, THREADS, SMEM_BYTES, (cudaStream_t)stream>>>(tq, tk, tv, to, tk, tv, p, pl);
+  attn_fwd_kernel<false, MOD><<<grid, THREADS, SMEM_BYTES, stream>>>(tq, tk, tv, to, tk, tv, p, pl);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
-    tdllm_host::set_last_error("attn_fwd launch: %s", cudaGetErrorString(e));
+    tdllm_host::set_last_error("%s launch: %s", who, cudaGetErrorString(e));
     return 4;
   }
   return 0;
+}
+
+// q [nq, Hq*128] (row stride ldq), k/v [nk, Hkv*128], o [nq, Hq*128], lse [Hq, nq_pad].
+// Row metadata arrays are padded to nq_pad / nk_pad (multiples of 128) by the caller.
+extern "C" int tdllm_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
+                              int nq, int nk, int Hq, int Hkv, long long ldq, long long ldk,
+                              long long ldv, long long ldo, const int* q_lo, const int* q_hi,
+                              const int* q_grp, const int* k_code, const int* tile_ptr,
+                              const int* tile_idx, const int* order, int n_qtiles, float scale,
+                              void* stream) {
+  if (nq <= 0) return 0;
+  score::Mod mod;
+  memset(&mod, 0, sizeof(mod));
+  return attn_fwd_launch<0>("attn_fwd", q, k, v, o, lse, nq, nk, Hq, Hkv, ldq, ldk, ldv, ldo, q_lo, q_hi, q_grp, k_code,
+                            tile_ptr, tile_idx, order, n_qtiles, scale, mod, (cudaStream_t)stream);
+}
+
+// The same with transformed scores (score_mod.cuh). softcap 0 = none; slope2 null = no bias, else [Hq] slopes times
+// log2(e) with q_pos / k_pos, positions as floats padded to nq_pad / nk_pad.
+extern "C" int tdllm_attn_fwd_scored(const void* q, const void* k, const void* v, void* o, float* lse, int nq, int nk,
+                                     int Hq, int Hkv, long long ldq, long long ldk, long long ldv, long long ldo,
+                                     const int* q_lo, const int* q_hi, const int* q_grp, const int* k_code,
+                                     const int* tile_ptr, const int* tile_idx, const int* order, int n_qtiles,
+                                     float scale, float softcap, const float* slope2, const float* q_pos,
+                                     const float* k_pos, void* stream) {
+  if (nq <= 0 || nk <= 0) return 0;
+  const score::Mod mod = score_mod_of(scale, softcap, slope2, q_pos, k_pos);
+  cudaStream_t st = (cudaStream_t)stream;
+#define TD_SCORED_FWD(M)                                                                                              \
+  return attn_fwd_launch<score::SAFE | (M)>("attn_fwd_scored", q, k, v, o, lse, nq, nk, Hq, Hkv, ldq, ldk, ldv, ldo,  \
+                                            q_lo, q_hi, q_grp, k_code, tile_ptr, tile_idx, order, n_qtiles, scale, mod, st)
+  switch ((softcap > 0.f ? score::CAP : 0) | (slope2 ? score::BIAS : 0)) {
+    case 0: TD_SCORED_FWD(0);
+    case score::CAP: TD_SCORED_FWD(score::CAP);
+    case score::BIAS: TD_SCORED_FWD(score::BIAS);
+    default: TD_SCORED_FWD(score::CAP | score::BIAS);
+  }
+#undef TD_SCORED_FWD
 }
 
 // Context-sharded forward. Keys are this rank's nk_loc rows (k_loc / v_loc, read in place) followed, from key
@@ -516,7 +589,7 @@ extern "C" int tdllm_attn_fwd_csbp(const void* q, const void* k_loc, const void*
   }
   static bool attr_set = false;
   if (!attr_set) {
-    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<true, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          SMEM_BYTES);
     if (e != cudaSuccess) {
       tdllm_host::set_last_error("attn_fwd_csbp: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
@@ -574,7 +647,7 @@ extern "C" int tdllm_attn_fwd_csbp(const void* q, const void* k_loc, const void*
   p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f;
   const int grid = n_qtiles * Hkv * ((Hq / Hkv + 1) / 2);
-  attn_fwd_kernel<true><<<grid, THREADS_CSBP, SMEM_BYTES, st>>>(tq, tk, tv, to, tkr, tvr, p, pl);
+  attn_fwd_kernel<true, 0><<<grid, THREADS_CSBP, SMEM_BYTES, st>>>(tq, tk, tv, to, tkr, tvr, p, pl);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     tdllm_host::set_last_error("attn_fwd_csbp launch: %s", cudaGetErrorString(e));

@@ -1,0 +1,319 @@
+"""Attention with transformed scores: a tanh cap, a bias by distance, document and prefix masks.
+
+Per query row i, key j and head h, with the visibility of a `MaskLayout` (`ops/attention.py`):
+
+    z_ij = scale * q_i . k_j
+    z_ij = cap * tanh(z_ij / cap)                          softcap > 0
+    z_ij = z_ij - slope_h * |q_pos_i - k_pos_j|            slopes given
+    out_i = sum_j softmax_j(z_ij) v_j,   lse_i = log sum_j exp(z_ij)       over the visible j
+
+and backward, with P_ij = exp(z_ij - lse_i) and t_ij = tanh(scale * q_i . k_j / cap):
+
+    dZ_ij = P_ij (dO_i . v_j - dO_i . out_i)               dS_ij = dZ_ij (1 - t_ij^2)
+    dq_i = scale * sum_j dS_ij k_j     dk_j = scale * sum_i dS_ij q_i     dv_j = sum_i P_ij dO_i
+
+summed over the query heads that share a KV head. Rows that see no key give out = 0, lse = -inf and no gradient. Query
+rows without a visible key and keys that no row sees may hold anything, infinities and NaN included; a value that is not
+finite and that some row does see may reach the other rows of its 128-row tile.
+
+The block-diffusion masks come from `block_diffusion_layout`; `document_layout` gives packed documents (causal, or with
+a prefix that is read in both directions). On CUDA bf16 tensors with head width 128 the tcgen05 kernels run
+(`csrc/attention_fwd_sm100.cu`, `csrc/attention_bwd_fused_sm100.cu` with the transforms of `csrc/score_mod.cuh`);
+everything else takes `scored_attention_reference`. A layout's tile lists and a transform's padded positions are built on
+first use, which synchronises: run a call once before it is captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass, field
+
+import torch
+
+from ..kernels import native
+from ._util import ptr
+from .attention import MaskLayout, backward_chunk_tiles, backward_mode
+
+native.register_signatures({
+    "tdllm_attn_fwd_scored": (native.c_int, [native.c_void_p] * 5 + [native.c_int] * 4 + [native.c_ll] * 4
+                              + [native.c_void_p] * 7 + [native.c_int, native.c_float, native.c_float]
+                              + [native.c_void_p] * 4),
+    "tdllm_attn_bwd_scored": (native.c_int, [native.c_void_p] * 11 + [native.c_int] * 4 + [native.c_ll] * 8
+                              + [native.c_void_p] * 7 + [native.c_int, native.c_int, native.c_int, native.c_float,
+                                                         native.c_float] + [native.c_void_p] * 4),
+})
+
+DEAD_KEY = -(2 ** 31)      # key code that no query row matches
+MAX_POSITION = 1 << 24     # distances are taken between positions held as floats
+LOG2E = 1.4426950408889634
+
+
+@dataclass(frozen=True, eq=False)
+class ScoreTransform:
+    """What happens to the scores before the softmax.
+
+    softcap: cap of the tanh, 0 for none. slopes: [Hq] float32, one slope per query head, with q_pos [nq] and k_pos [nk]
+    (int32 or int64, absolute value below 2^24): the distance bias. Slopes are constants: they get no gradient."""
+
+    softcap: float = 0.0
+    slopes: torch.Tensor | None = None
+    q_pos: torch.Tensor | None = None
+    k_pos: torch.Tensor | None = None
+    _cache: dict = field(default_factory=dict, repr=False)
+
+    def __post_init__(self):
+        if not (math.isfinite(self.softcap) and self.softcap >= 0.0):
+            raise ValueError(f"softcap must be a finite number >= 0, got {self.softcap}")
+        given = [t is not None for t in (self.slopes, self.q_pos, self.k_pos)]
+        if any(given) and not all(given):
+            raise ValueError("a distance bias needs slopes, q_pos and k_pos together")
+        if self.slopes is None:
+            return
+        if self.slopes.dim() != 1 or self.slopes.dtype != torch.float32:
+            raise ValueError("slopes must be a float32 vector, one value per query head")
+        if self.slopes.requires_grad:
+            raise ValueError("slopes are constants of the bias and get no gradient; detach them")
+        for name, t in (("q_pos", self.q_pos), ("k_pos", self.k_pos)):
+            if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
+                raise ValueError(f"{name} must be a vector of int32 or int64")
+
+    @property
+    def biased(self) -> bool:
+        return self.slopes is not None
+
+    def _padded(self, nq_pad: int, nk_pad: int):
+        """(slopes * log2 e, q_pos, k_pos) as the kernels read them: floats, positions padded with zeros. Rebuilt when
+        one of the tensors has been written to since."""
+        version = (self.slopes._version, self.q_pos._version, self.k_pos._version, nq_pad, nk_pad)
+        hit = self._cache.get("padded")
+        if hit is not None and hit[0] == version:
+            return hit[1]
+        out = [(self.slopes * LOG2E).contiguous()]
+        for t, n in ((self.q_pos, nq_pad), (self.k_pos, nk_pad)):
+            if t.numel() and int(t.abs().max()) >= MAX_POSITION:
+                raise ValueError(f"positions of the distance bias must lie within +-{MAX_POSITION}")
+            f = torch.zeros(n, dtype=torch.float32, device=t.device)
+            f[: t.shape[0]] = t
+            out.append(f)
+        self._cache["padded"] = (version, tuple(out))
+        return self._cache["padded"][1]
+
+
+def document_layout(lengths, *, prefix=None, rows: int | None = None, causal: bool = True, device="cpu") -> MaskLayout:
+    """Packed documents: row i of a document sees that document's rows up to itself (all of them when not `causal`), and
+    at least the document's first `prefix[d]` rows, so that a prefix is read in both directions. `lengths` are the
+    documents' row counts in packing order (zero is allowed); rows behind the last document, up to `rows`, see nothing and
+    are seen by nothing."""
+    lens = torch.as_tensor(lengths, dtype=torch.int64).reshape(-1)
+    if lens.numel() and int(lens.min()) < 0:
+        raise ValueError("document lengths must not be negative")
+    pre = torch.zeros_like(lens) if prefix is None else torch.as_tensor(prefix, dtype=torch.int64).reshape(-1)
+    if pre.shape != lens.shape or bool((pre < 0).any()) or bool((pre > lens).any()):
+        raise ValueError("prefix needs one value per document, between 0 and its length")
+    total = int(lens.sum())
+    rows = total if rows is None else int(rows)
+    if rows < total:
+        raise ValueError(f"the documents have {total} rows, more than rows={rows}")
+    start = torch.repeat_interleave(lens.cumsum(0) - lens, lens)
+    stop = torch.repeat_interleave(lens.cumsum(0), lens)
+    first = torch.repeat_interleave(pre, lens)
+    at = torch.arange(total)
+    hi = torch.maximum(at + 1, start + first) if causal else stop
+    pad = rows - total
+    z = torch.zeros(pad, dtype=torch.int64)
+    out = [torch.cat([start, z]), torch.cat([hi, z]), torch.zeros(rows, dtype=torch.int64), torch.cat([at, z + DEAD_KEY])]
+    return MaskLayout(*(t.to(torch.int32).to(device) for t in out))
+
+
+def document_positions(lengths, *, rows: int | None = None, device="cpu") -> torch.Tensor:
+    """[rows] int32 positions inside the documents of `document_layout` (0 behind the last one)."""
+    lens = torch.as_tensor(lengths, dtype=torch.int64).reshape(-1)
+    total = int(lens.sum())
+    pos = torch.zeros(total if rows is None else int(rows), dtype=torch.int32)
+    pos[:total] = (torch.arange(total) - torch.repeat_interleave(lens.cumsum(0) - lens, lens)).to(torch.int32)
+    return pos.to(device)
+
+
+def _seen_keys(layout: MaskLayout) -> torch.Tensor:
+    """[nk] bool: keys that some query row sees."""
+    lo, hi, grp, code = (t.long() for t in (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code))
+    real = hi > lo
+    starts, stops = torch.sort(lo[real]).values, torch.sort(hi[real]).values
+    # intervals that contain c: those that start at or before it minus those that have ended by then
+    covered = torch.searchsorted(starts, code, right=True) > torch.searchsorted(stops, code, right=True)
+    return torch.where(code >= 0, covered, torch.isin(code, grp[grp < 0]))
+
+
+def _lists(layout: MaskLayout) -> dict:
+    """The layout's tile lists with the codes of keys that no row sees set to DEAD_KEY."""
+    if "scored" not in layout._cache:
+        L = dict(layout.tile_lists())
+        code = L["k_code"].clone()
+        code[: layout.nk].masked_fill_(~_seen_keys(layout), DEAD_KEY)
+        L["k_code"] = code
+        layout._cache["scored"] = L
+    return layout._cache["scored"]
+
+
+def scored_attention_reference(q, k, v, layout: MaskLayout, transform: ScoreTransform | None = None,
+                               scale: float | None = None):
+    """Dense-mask form in fp32 (in 64 bits for double inputs), differentiable. q [nq, Hq, D], k / v [nk, Hkv, D] ->
+    (out [nq, Hq, D] in q's dtype, lse [Hq, nq])."""
+    nq, Hq, D = q.shape
+    G = Hq // k.shape[1]
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    seen = layout.dense_mask().to(q.device)
+    row_live, key_live = seen.any(1), seen.any(0)
+    keep = lambda t, live: torch.where(live[:, None, None], t.to(wide), torch.zeros((), dtype=wide, device=t.device))  # noqa: E731
+    qf = keep(q, row_live).permute(1, 0, 2)
+    kf = keep(k, key_live).permute(1, 0, 2).repeat_interleave(G, dim=0)
+    vf = keep(v, key_live).permute(1, 0, 2).repeat_interleave(G, dim=0)
+    z = torch.matmul(qf, kf.transpose(1, 2)) * scale
+    if transform is not None and transform.softcap:
+        z = transform.softcap * torch.tanh(z / transform.softcap)
+    if transform is not None and transform.biased:
+        far = (transform.q_pos.to(wide)[:, None] - transform.k_pos.to(wide)[None, :]).abs()
+        z = z - transform.slopes.to(wide)[:, None, None] * far
+    z = z.masked_fill(~(seen | ~row_live[:, None]), float("-inf"))      # (rows without a key are taken out below)
+    if layout.nk == 0:
+        return torch.zeros_like(q), torch.full((Hq, nq), float("-inf"), dtype=wide, device=q.device)
+    lse = torch.logsumexp(z, dim=-1)
+    p = torch.where(row_live[None, :, None], torch.exp(z - lse[..., None]), torch.zeros((), dtype=wide, device=q.device))
+    out = torch.matmul(p, vf).permute(1, 0, 2)
+    return out.to(q.dtype), lse.masked_fill(~row_live[None], float("-inf"))
+
+
+def _check(q, k, v, layout: MaskLayout, transform: ScoreTransform | None) -> None:
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
+        raise ValueError(f"need q [nq, Hq, D] and k, v [nk, Hkv, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{q.shape[1]} query heads do not divide over {k.shape[1]} KV heads")
+    if not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
+        raise ValueError("q, k and v must share dtype and device")
+    meta = (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code)
+    if layout.nq != q.shape[0] or layout.nk != k.shape[0] or layout.q_hi.shape != layout.q_lo.shape \
+            or layout.q_grp.shape != layout.q_lo.shape:
+        raise ValueError(f"the layout describes {layout.nq} query rows and {layout.nk} keys, got {q.shape[0]} and {k.shape[0]}")
+    if any(t.device != q.device for t in meta):
+        raise ValueError(f"the layout must lie on {q.device}")
+    if transform is not None and transform.biased:
+        if transform.slopes.shape[0] != q.shape[1]:
+            raise ValueError(f"{transform.slopes.shape[0]} slopes for {q.shape[1]} query heads")
+        if transform.q_pos.shape[0] != q.shape[0] or transform.k_pos.shape[0] != k.shape[0]:
+            raise ValueError("q_pos and k_pos need one position per query row and per key")
+        if any(t.device != q.device for t in (transform.slopes, transform.q_pos, transform.k_pos)):
+            raise ValueError(f"slopes and positions must lie on {q.device}")
+
+
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """[n, H, 128] rows the tensor maps can address: packed heads, 16-byte aligned base and row stride."""
+    n, H, D = t.shape
+    if t.stride(2) == 1 and (H == 1 or t.stride(1) == D) and t.data_ptr() % 16 == 0 \
+            and (n == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= H * D)):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]     # (a single row's stride may be anything)
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _mod_args(transform: ScoreTransform | None, L: dict):
+    """(softcap, slope2, q_pos, k_pos) of a launch and the tensors behind the pointers."""
+    if transform is None:
+        return (0.0, None, None, None), ()
+    if not transform.biased:
+        return (float(transform.softcap), None, None, None), ()
+    kept = transform._padded(L["nq_pad"], L["nk_pad"])
+    return (float(transform.softcap), *(ptr(t) for t in kept)), kept
+
+
+def _forward(q, k, v, layout, transform, scale):
+    nq, Hq, D = q.shape
+    nk, Hkv, _ = k.shape
+    L = _lists(layout)
+    mod, _kept = _mod_args(transform, L)
+    out = torch.empty(nq, Hq, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(Hq, L["nq_pad"], dtype=torch.float32, device=q.device)
+    rc = native.lib().tdllm_attn_fwd_scored(
+        ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v),
+        out.stride(0), ptr(L["q_lo"]), ptr(L["q_hi"]), ptr(L["q_grp"]), ptr(L["k_code"]), ptr(L["f_ptr"]), ptr(L["f_idx"]),
+        ptr(L["f_order"]), L["nqt"], float(scale), *mod, _stream(q))
+    native.check(rc, "attn_fwd_scored")
+    return out, lse
+
+
+def _backward(q, k, v, out, dout, lse, layout, transform, scale):
+    nq, Hq, D = q.shape
+    nk, Hkv, _ = k.shape
+    L = _lists(layout)
+    W = layout.backward_work(backward_chunk_tiles())
+    mod, _kept = _mod_args(transform, L)
+    dev = q.device
+    dq, dk, dv = torch.empty(nq, Hq, D, dtype=q.dtype, device=dev), torch.empty_like(k, memory_format=torch.contiguous_format), \
+        torch.empty_like(v, memory_format=torch.contiguous_format)
+    delta = torch.empty(2, Hq, L["nq_pad"], dtype=torch.float32, device=dev)
+    # (allocated per call: two streams, or two captured graphs, must not add into one accumulator)
+    acc = torch.empty(L["nq_pad"] * Hq * D + 2 * L["nk_pad"] * Hkv * D, dtype=torch.float32, device=dev)
+    rc = native.lib().tdllm_attn_bwd_scored(
+        ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(lse), ptr(delta), ptr(acc),
+        nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v), _row_stride(out), _row_stride(dout),
+        dq.stride(0), dk.stride(0), dv.stride(0), ptr(L["q_lo"]), ptr(L["q_hi"]), ptr(L["q_grp"]), ptr(L["k_code"]),
+        ptr(W["w_ptr"]), ptr(W["w_idx"]), ptr(W["w_order"]), W["n_work"], L["nqt"], L["nkt"], float(scale), *mod, _stream(q))
+    native.check(rc, "attn_bwd_scored")
+    return dq, dk, dv
+
+
+class _ScoredAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, layout, transform, scale):
+        with torch.cuda.device(q.device):
+            q, k, v = _operand(q), _operand(k), _operand(v)
+            out, lse = _forward(q, k, v, layout, transform, scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.layout, ctx.transform, ctx.scale = layout, transform, scale
+        lse = lse[:, : q.shape[0]]
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _dlse):
+        q, k, v, out, lse = ctx.saved_tensors
+        with torch.cuda.device(q.device):
+            grads = _backward(q, k, v, out, _operand(dout), lse, ctx.layout, ctx.transform, ctx.scale)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
+
+
+def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: MaskLayout,
+                     transform: ScoreTransform | None = None, *, scale: float | None = None, return_lse: bool = False):
+    """q [nq, Hq, D], k / v [nk, Hkv, D] -> out [nq, Hq, D] (and lse [Hq, nq] float32, without gradient).
+
+    Operands may be views of a packed projection (packed heads, any row stride). The gradient of dQ is summed over key
+    tiles by fp32 adds whose order is not fixed, as in `block_attention`'s one-pass backward."""
+    _check(q, k, v, layout, transform)
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if not q.is_cuda or q.dtype != torch.bfloat16:
+        out, lse = scored_attention_reference(q, k, v, layout, transform, scale)
+        return (out, lse.detach()) if return_lse else out
+    if q.shape[2] != 128:
+        raise native.NativeKernelError("scored attention on bf16 CUDA tensors is built for head_dim 128 (no silent fallback)")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        if backward_mode() == "split":
+            raise native.NativeKernelError("scored attention has the one-pass backward only; unset TDLLM_ATTN_BWD=split")
+        if q.shape[0] == 0 or k.shape[0] == 0:
+            out, lse = scored_attention_reference(q, k, v, layout, transform, scale)
+        else:
+            out, lse = _ScoredAttention.apply(q, k, v, layout, transform, scale)
+    elif q.shape[0] == 0 or k.shape[0] == 0:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.full((q.shape[1], q.shape[0]), float("-inf"), dtype=torch.float32, device=q.device)
+    else:
+        with torch.cuda.device(q.device):
+            out, lse = _forward(_operand(q), _operand(k), _operand(v), layout, transform, scale)
+            lse = lse[:, : q.shape[0]]
+    return (out, lse) if return_lse else out
