@@ -82,6 +82,11 @@ int tdllm_swiglu_fwd(const void* gu, void* out, long long rows, int inter, void*
 int tdllm_swiglu_bwd(const void* dy, const void* gu, void* dgu, long long rows, int inter,
                      void* stream);
 
+// Rotary positions (rotary.cu): x [rows, H, D] with row and head strides in elements -> packed out; the first `part`
+// values of each head turn by pos * freqs, as pairs (i, i + part/2) (half) or (2i, 2i + 1); dir -1 turns back.
+int tdllm_rotary(const void* x, void* out, const int* pos, const float* freqs, int rows, int H, int D, int part,
+                 long long ld_row, long long ld_head, int half, int dtype, float scale, float dir, void* stream);
+
 // ---- wide-head attention: the masked softmax between the tensor-core products ----
 // S fp32 [R, N] (row stride lds) -> P bf16 [R, N] (row stride ldp), lse [R]. Row r uses the mask entries of
 // query (r % rows_per_head).

@@ -1,6 +1,8 @@
 """Helpers shared by the op wrappers: pointers, streams, parameter gradient sinks."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from ..kernels import native
@@ -24,6 +26,23 @@ def use_native(*tensors: torch.Tensor) -> bool:
         return False
     native.lib()
     return True
+
+
+_DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def dtype_code(t: torch.Tensor) -> int | None:
+    """Type argument of the kernels that take bf16, fp16 and fp32 CUDA tensors; None: the reference runs."""
+    if not t.is_cuda:
+        return None
+    return _DTYPE_CODES.get(t.dtype)
+
+
+def on_device(t: torch.Tensor):
+    """Makes the tensor's device the current one for a launch on it (and for `stream()`)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def grad_sink(param: torch.Tensor):
