@@ -1,0 +1,206 @@
+"""The norms around a block: refusals and the reference on the CPU, the kernels against 64 bits on the GPU."""
+import pytest
+import torch
+
+from turbo_dllm_b200.ops.norm import rmsnorm_reference, sandwich_norm
+
+EPS = 1e-6
+FINE = 2.0 ** -18    # 32-bit arithmetic: a row sum adds up to 16 values per thread and ten tree levels at 2^-24 each
+SUMS = 2.0 ** -15    # sums over rows: up to 400 sequential 32-bit additions
+
+
+def exact(x, res, wq, wp, gate, a, dy=None, dh=None):
+    """Outputs and gradients in 64 bits with the error each may have: half a step of the type on what is stored, FINE
+    (SUMS) of the summed magnitudes."""
+    half = torch.finfo(x.dtype).eps / 2
+    x, res, wq, wp = (t.detach().double() for t in (x, res, wq, wp))
+    gate = torch.ones((), dtype=torch.float64, device=x.device) if gate is None else gate.detach().double()
+    mean = lambda t: t.mean(-1, keepdim=True)   # noqa: E731
+    rx = (mean(x * x) + EPS).sqrt()
+    u = x / rx
+    b = gate * u * wq
+    h = a * res + b
+    size = (a * res).abs() + b.abs()
+    rh = (mean(h * h) + EPS).sqrt()
+    t = h / rh
+    tsize = size / rh * (1 + mean(size * size) / (rh * rh))
+    want = {"y": t * wp, "h": h}
+    tol = {"y": half * want["y"].abs() + FINE * tsize * wp.abs(), "h": half * h.abs() + FINE * size}
+    if dy is not None or dh is not None:
+        dy = torch.zeros_like(x) if dy is None else dy.detach().double()
+        dh = torch.zeros_like(x) if dh is None else dh.detach().double()
+        dt = dy * wp
+        d = dh + (dt - t * mean(dt * t)) / rh
+        dsize = dh.abs() + (dt.abs() + tsize * mean(dt.abs() * tsize)) / rh
+        gw = gate * wq
+        du = d * gw
+        want["x"] = (du - u * mean(du * u)) / rx
+        tol["x"] = half * want["x"].abs() + FINE * (dsize * gw.abs() + u.abs() * mean(dsize * gw.abs() * u.abs())) / rx
+        want["res"] = a * d
+        tol["res"] = half * want["res"].abs() + FINE * abs(a) * dsize
+        for n, term, mag in (("w_post", d * gate * u, dsize * gate.abs() * u.abs()), ("w_pre", dy * t, dy.abs() * tsize),
+                             ("gate", d * u * wq, dsize * u.abs() * wq.abs())):
+            if n == "gate" and gate.dim() == 2:
+                want[n], tol[n] = term, half * term.abs() + FINE * mag
+            else:
+                want[n] = term.sum(0)
+                tol[n] = half * want[n].abs() + SUMS * mag.sum(0)
+    return want, tol
+
+
+def near(got, want, tol, name):
+    tiny = torch.finfo(got.dtype).tiny
+    over = (got.detach().double() - want).abs() - tol - tiny
+    assert over.numel() == 0 or float(over.max()) <= 0, (name, float(over.max()))
+
+
+def operands(rows, H, gate, dtype, device, seed=0):
+    g = torch.Generator(device=device).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device=device)   # noqa: E731
+    out = dict(x=(0.7 * r(rows, H)).to(dtype), res=(1.5 * r(rows, H)).to(dtype), w_post=(1 + 0.2 * r(H)).to(dtype),
+               w_pre=(1 + 0.2 * r(H)).to(dtype))
+    if gate:
+        out["gate"] = r(*((H,) if gate == "channel" else (rows, H))).to(dtype)
+    return out, r(rows, H).to(dtype), r(rows, H).to(dtype)
+
+
+def run(t, dy, dh, a=0.9):
+    leaves = {n: v.detach().requires_grad_() for n, v in t.items()}
+    y, h = sandwich_norm(leaves["x"], leaves["res"], leaves["w_post"], leaves["w_pre"], gate=leaves.get("gate"), res_scale=a, eps=EPS)
+    outs, grads = zip(*[(o, g) for o, g in ((y, dy), (h, dh)) if g is not None])
+    got = dict(zip(leaves, torch.autograd.grad(outs, list(leaves.values()), grads, allow_unused=True)))
+    got = {n: torch.zeros_like(leaves[n]) if g is None else g for n, g in got.items()}
+    return {"y": y, "h": h, **got}
+
+
+# ------------------------------------------------------------------------------------------------ CPU
+@pytest.mark.parametrize("gate", [None, "channel", "full"])
+def test_reference(gate):
+    t, dy, dh = operands(5, 7, gate, torch.float64, "cpu")
+    want, _ = exact(t["x"], t["res"], t["w_post"], t["w_pre"], t.get("gate"), 0.9, dy, dh)
+    got = run(t, dy, dh)
+    for n in got:
+        assert torch.allclose(got[n], want[n], rtol=1e-10, atol=1e-12), n
+    leaves = [v.requires_grad_() for v in t.values()]
+    assert torch.autograd.gradcheck(lambda *v: sandwich_norm(*v[:4], gate=v[4] if gate else None, res_scale=0.9), leaves)
+
+
+def test_it_is_two_norms():
+    t, _, _ = operands(3, 8, None, torch.float32, "cpu")
+    y, h = sandwich_norm(t["x"].view(3, 1, 8), t["res"].view(3, 1, 8), t["w_post"], t["w_pre"])
+    want = t["res"] + rmsnorm_reference(t["x"], t["w_post"], EPS)[0]
+    assert y.shape == (3, 1, 8) and torch.allclose(h.view(3, 8), want)
+    assert torch.allclose(y.view(3, 8), rmsnorm_reference(want, t["w_pre"], EPS)[0], atol=1e-6)
+
+
+def test_refusals():
+    t, _, _ = operands(3, 8, None, torch.float32, "cpu")
+    x, res, wq, wp = t.values()
+    with pytest.raises(ValueError, match="one shape"):
+        sandwich_norm(x, res[:2], wq, wp)
+    with pytest.raises(ValueError, match="vectors"):
+        sandwich_norm(x, res, wq[:7], wp)
+    with pytest.raises(ValueError, match="gate"):
+        sandwich_norm(x, res, wq, wp, gate=x[:1])
+    with pytest.raises(ValueError, match="share"):
+        sandwich_norm(x, res, wq.double(), wp)
+    with pytest.raises(ValueError, match="one shape"):
+        sandwich_norm(x[:, :0], res[:, :0], wq[:0], wp[:0])
+
+
+# ------------------------------------------------------------------------------------------------ GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("gate", [None, "channel", "full"])
+@pytest.mark.parametrize("rows,H", [(1, 1), (3, 7), (5, 256), (33, 1000), (700, 1411), (2, 4096), (601, 4104), (3, 16384), (1300, 96),
+                                    (2, 16383)])
+def test_kernels(dtype, gate, rows, H):
+    t, dy, dh = operands(rows, H, gate, dtype, "cuda", rows + H)
+    want, tol = exact(t["x"], t["res"], t["w_post"], t["w_pre"], t.get("gate"), 0.9, dy, dh)
+    got = run(t, dy, dh)
+    for n in got:
+        near(got[n], want[n], tol[n], n)
+    again = run(t, dy, dh)
+    assert all(torch.equal(got[n], again[n]) for n in got)      # sums in a fixed order
+    y, h = sandwich_norm(t["x"], t["res"], t["w_post"], t["w_pre"], gate=t.get("gate"), res_scale=0.9, eps=EPS)
+    assert torch.equal(y, got["y"]) and torch.equal(h, got["h"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["dy", "dh"])
+@pytest.mark.parametrize("gate", [None, "full"])
+def test_one_incoming_gradient(which, gate):
+    t, dy, dh = operands(40, 512, gate, torch.bfloat16, "cuda")
+    dy, dh = (dy, None) if which == "dy" else (None, dh)
+    want, tol = exact(t["x"], t["res"], t["w_post"], t["w_pre"], t.get("gate"), 0.9, dy, dh)
+    got = run(t, dy, dh)
+    for n in got:
+        near(got[n], want[n], tol[n], n)
+
+
+@pytest.mark.gpu
+def test_strides_and_empty_rows():
+    t, dy, dh = operands(30, 256, "full", torch.bfloat16, "cuda")
+    base = run(t, dy, dh)
+    wide = torch.zeros(30, 3 * 256 + 1, dtype=torch.bfloat16, device="cuda")
+    views = {n: wide[:, i * 256 + 1:(i + 1) * 256 + 1] for i, n in enumerate(("x", "res", "gate"))}
+    for n, v in views.items():
+        v.copy_(t[n])
+    # (a base that is not 16-byte aligned goes value by value: other sums, the same bounds)
+    want, tol = exact(t["x"], t["res"], t["w_post"], t["w_pre"], t["gate"], 0.9, dy, dh)
+    for n, got in run({**t, **views}, dy, dh).items():
+        near(got, want[n], tol[n], n)
+    turned = {**t, "x": t["x"].t().contiguous().t()}
+    assert torch.equal(run(turned, dy, dh)["y"], base["y"])
+    none = {n: v[:0] if v.dim() == 2 else v for n, v in t.items()}
+    got = run(none, dy[:0], dh[:0])
+    assert got["y"].shape == (0, 256) and float(got["w_post"].abs().max()) == 0
+
+
+@pytest.mark.gpu
+def test_gradients_go_to_the_flat_buffers():
+    t, dy, dh = operands(60, 512, "channel", torch.bfloat16, "cuda")
+    plain = run(t, dy, dh)
+    for sink_type in (torch.float32, torch.bfloat16):
+        leaves = {n: v.detach().requires_grad_() for n, v in t.items()}
+        for n in ("w_post", "w_pre", "gate"):
+            leaves[n].main_grad = torch.full((512,), 7.0, dtype=sink_type, device="cuda")
+            leaves[n].grad_acc = False
+        for step in (1, 2):
+            y, h = sandwich_norm(leaves["x"], leaves["res"], leaves["w_post"], leaves["w_pre"], gate=leaves["gate"], res_scale=0.9, eps=EPS)
+            torch.autograd.backward([y, h], [dy, dh])
+            for n in ("w_post", "w_pre", "gate"):
+                assert leaves[n].grad is None and leaves[n].grad_acc
+                # (two roundings to bf16 apart: the plain result's and, for the second step, the buffer's)
+                assert torch.allclose(leaves[n].main_grad.float(), step * plain[n].float(), rtol=2.0 ** -6, atol=2.0 ** -8), (n, step)
+    from turbo_dllm_b200.kernels.native import NativeKernelError
+
+    leaves["w_post"].main_grad = torch.zeros(512, dtype=torch.float16, device="cuda")
+    y, h = sandwich_norm(leaves["x"], leaves["res"], leaves["w_post"], leaves["w_pre"])
+    with pytest.raises(NativeKernelError, match="gradient buffer"):
+        y.sum().backward()
+    x = torch.zeros(1, 16385, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(NativeKernelError, match="widths"):
+        sandwich_norm(x, x, x[0], x[0])
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs_side_by_side():
+    t, dy, dh = operands(300, 512, None, torch.bfloat16, "cuda")
+    u, ey, eh = operands(300, 512, None, torch.bfloat16, "cuda", seed=5)
+    want = [run(t, dy, dh), run(u, ey, eh)]
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for args in ((t, dy, dh), (u, ey, eh)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(run(*args))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for h, w in zip(held, want):
+        assert all(torch.equal(h[n], w[n]) for n in w)

@@ -1,4 +1,5 @@
-"""RMSNorm with optional fused residual add: h = x + res; y = h * rsqrt(mean(h²)+eps) * w.
+"""RMSNorm with optional fused residual add: h = x + res; y = h * rsqrt(mean(h²)+eps) * w. And the norms behind and
+in front of a block in one kernel, with the block's gate and a scaled residual (`sandwich_norm`).
 
 Reference counterpart: HF RMSNorm modules and TE `LayerNormLinear(normalization="RMSNorm")`
 (dllm_parallel/core/models/backbones/nemotron/model.py:3866-3960).
@@ -8,7 +9,18 @@ from __future__ import annotations
 import torch
 
 from ..kernels import native
-from ._util import grad_sink, mark_grad_written, ptr, scratch, stream, use_native
+from ._util import dtype_code, grad_sink, mark_grad_written, on_device, ptr, scratch, stream, use_native
+
+
+native.register_signatures({
+    "tdllm_sandwich_norm_fwd": (native.c_int, [native.c_void_p] * 8 + [native.c_ll] * 3 + [native.c_int] * 4
+                                + [native.c_float] * 2 + [native.c_void_p]),
+    "tdllm_sandwich_norm_parts": (native.c_int, [native.c_int]),
+    "tdllm_sandwich_norm_bwd": (native.c_int, [native.c_void_p] * 14 + [native.c_int] * 6 + [native.c_void_p]
+                                + [native.c_ll] * 3 + [native.c_int] * 4 + [native.c_float, native.c_void_p]),
+})
+
+SANDWICH_MAX_WIDTH = 16384
 
 
 def rmsnorm_reference(x, w, eps, res=None):
@@ -74,3 +86,121 @@ def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6,
         return _RMSNorm.apply(x, None, w, eps), x
     y, h = _RMSNorm.apply(x, res, w, eps)
     return y, h
+
+
+def sandwich_norm_reference(x, res, w_post, w_pre, gate=None, res_scale: float = 1.0, eps: float = 1e-6):
+    """(y, h) of `sandwich_norm` in fp32 (64 bits for double inputs), each rounded once; y is formed from the unrounded h."""
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    xf = x.to(wide)
+    b = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w_post.to(wide)
+    if gate is not None:
+        b = b * gate.to(wide)
+    h = res_scale * res.to(wide) + b
+    y = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps) * w_pre.to(wide)
+    return y.to(x.dtype), h.to(x.dtype)
+
+
+GATE_NONE, GATE_CHANNEL, GATE_FULL = 0, 1, 2
+
+
+def _rows2d(t: torch.Tensor) -> torch.Tensor:
+    """[rows, H] view with unit inner stride (a copy only where the tensor has none)."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _sandwich_forward(x, res, w_post, w_pre, gate, res_scale, eps, want_stats):
+    kind = GATE_NONE if gate is None else GATE_CHANNEL if gate.dim() == 1 else GATE_FULL
+    rows, H = x.shape
+    y, h = torch.empty(rows, H, dtype=x.dtype, device=x.device), torch.empty(rows, H, dtype=x.dtype, device=x.device)
+    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if want_stats else None
+    with on_device(x):
+        native.check(native.lib().tdllm_sandwich_norm_fwd(
+            ptr(x), ptr(res), ptr(w_post), ptr(w_pre), ptr(gate), ptr(y), ptr(h), ptr(stats), x.stride(0), res.stride(0),
+            gate.stride(0) if kind == GATE_FULL else 0, rows, H, kind, dtype_code(x), res_scale, eps, stream()),
+            "sandwich_norm_fwd")
+    return y, h, stats
+
+
+class _SandwichNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, res, w_post, w_pre, gate, res_scale, eps):
+        x2, res2 = _rows2d(x), _rows2d(res)
+        gate2 = gate if gate is None or gate.dim() == 1 else _rows2d(gate)
+        y, h, stats = _sandwich_forward(x2, res2, w_post, w_pre, gate2, res_scale, eps, True)
+        ctx.save_for_backward(x2, res2, w_post, w_pre, gate2, stats)
+        ctx.refs = (w_post, w_pre, gate if gate is not None and gate.dim() == 1 else None)
+        ctx.meta = (res_scale, x.shape)
+        ctx.set_materialize_grads(False)
+        return y.view(x.shape), h.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        x, res, w_post, w_pre, gate, stats = ctx.saved_tensors
+        res_scale, shape = ctx.meta
+        rows, H = x.shape
+        kind = GATE_NONE if gate is None else GATE_CHANNEL if gate.dim() == 1 else GATE_FULL
+        dy = None if dy is None else dy.reshape(rows, H).contiguous()
+        dh = None if dh is None else dh.reshape(rows, H).contiguous()
+        dx, dres = torch.empty(rows, H, dtype=x.dtype, device=x.device), torch.empty(rows, H, dtype=x.dtype, device=x.device)
+        dgate = torch.empty(rows, H, dtype=x.dtype, device=x.device) if kind == GATE_FULL else None
+        # vectors that own a slice of the flat gradient buffer are written (or added) there, the others are returned
+        targets, flags, returned, written = [], [], [], []
+        for vec, ref, need in zip((w_post, w_pre, gate if kind == GATE_CHANNEL else None), ctx.refs, ctx.needs_input_grad[2:5]):
+            sink, acc = (None, False) if vec is None or not need else grad_sink(ref)
+            if sink is not None and sink.dtype not in (torch.float32, x.dtype):
+                raise native.NativeKernelError(f"gradient buffer of {sink.dtype} for a {x.dtype} parameter")
+            grad = torch.empty_like(vec) if vec is not None and need and sink is None else None
+            to = sink if sink is not None else grad
+            targets.append(to)
+            flags += [int(to is not None and to.dtype == torch.float32), int(acc)]
+            returned.append(grad)
+            if sink is not None:
+                written.append(ref)
+        with on_device(x):
+            lib = native.lib()
+            # (allocated per call: streams and captured graphs do not share it)
+            part = torch.empty(lib.tdllm_sandwich_norm_parts(rows) * 2 * H, dtype=torch.float32, device=x.device)
+            native.check(lib.tdllm_sandwich_norm_bwd(
+                ptr(x), ptr(res), ptr(w_post), ptr(w_pre), ptr(gate), ptr(dy), ptr(dh), ptr(stats), ptr(dx), ptr(dres),
+                ptr(dgate), *(ptr(t) for t in targets), *flags, ptr(part), x.stride(0), res.stride(0),
+                gate.stride(0) if kind == GATE_FULL else 0, rows, H, kind, dtype_code(x), res_scale, stream()),
+                "sandwich_norm_bwd")
+        for ref in written:
+            mark_grad_written(ref)
+        return (dx.view(shape), dres.view(shape), returned[0], returned[1],
+                dgate.view(shape) if kind == GATE_FULL else returned[2], None, None)
+
+
+def sandwich_norm(x: torch.Tensor, res: torch.Tensor, w_post: torch.Tensor, w_pre: torch.Tensor, *,
+                  gate: torch.Tensor | None = None, res_scale: float = 1.0, eps: float = 1e-6):
+    """The norm behind a block and the norm in front of the next one, around the residual stream:
+
+        h = res_scale * res + gate * rmsnorm(x, w_post)        y = rmsnorm(h, w_pre)
+
+    x (the block's output) and res [..., H]; w_post, w_pre [H]; gate None, [H] (one learned value per channel) or x's
+    shape. Returns (y, h): the next block's input and the updated residual stream. CUDA tensors of bf16, fp16 and fp32 with
+    H <= 16384 run `csrc/sandwich_norm.cu`; y is formed from h before h is rounded. Others take `sandwich_norm_reference`."""
+    H = x.shape[-1] if x.dim() else 0
+    if x.dim() < 1 or H < 1 or res.shape != x.shape:
+        raise ValueError(f"x and res need one shape [..., H], got {tuple(x.shape)} and {tuple(res.shape)}")
+    if w_post.shape != (H,) or w_pre.shape != (H,):
+        raise ValueError(f"w_post and w_pre must be vectors of {H} values")
+    if gate is not None and gate.shape != (H,) and gate.shape != x.shape:
+        raise ValueError(f"gate must be a vector of {H} values or have x's shape, got {tuple(gate.shape)}")
+    given = [t for t in (res, w_post, w_pre, gate) if t is not None]
+    if any(t.dtype != x.dtype or t.device != x.device for t in given):
+        raise ValueError("x, res, the weights and the gate must share dtype and device")
+    if dtype_code(x) is None:
+        return sandwich_norm_reference(x, res, w_post, w_pre, gate, res_scale, eps)
+    if H > SANDWICH_MAX_WIDTH:
+        raise native.NativeKernelError(f"sandwich_norm kernels take widths up to {SANDWICH_MAX_WIDTH}, got {H}")
+    w_post, w_pre = w_post.contiguous(), w_pre.contiguous()
+    if gate is not None and gate.dim() == 1:
+        gate = gate.contiguous()
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *given)):
+        return _SandwichNorm.apply(x, res, w_post, w_pre, gate, float(res_scale), float(eps))
+    g2 = gate if gate is None or gate.dim() == 1 else _rows2d(gate)
+    y, h, _ = _sandwich_forward(_rows2d(x), _rows2d(res), w_post, w_pre, g2, float(res_scale), float(eps), False)
+    return y.view(x.shape), h.view(x.shape)
