@@ -259,6 +259,73 @@ def test_windows_and_keys_of_another_length():
     run_case(*_operands(L.nq, L.nk, 4, 2, 3), L, transform_for("both", 4, qpos, kpos, "cuda"))
 
 
+def step_layout(caches, new, device="cuda", capacity=None, window=None):
+    """`new` rows per sequence against its own clean cache (rows behind a cache's length hold nothing) and each other."""
+    s, span = len(caches), 1 << 20
+    cap = capacity or max(max(caches), 1)
+    seq = torch.arange(s, device=device)
+    n = torch.tensor(caches, device=device)
+    at = torch.arange(cap, device=device)
+    kc = torch.where(at[None] < n[:, None], seq[:, None] * span + at[None], torch.full((), DEAD_KEY, device=device)).reshape(-1)
+    sq, end = seq.repeat_interleave(new), n.repeat_interleave(new)
+    lo = sq * span + (0 if window is None else (end - window).clamp_min(0))
+    L = MaskLayout(*(t.to(torch.int32) for t in (lo, sq * span + end, -(sq + 1), torch.cat([kc, -(sq + 1)]))))
+    qpos = (end + torch.arange(new, device=device).repeat(s)).to(torch.int32)
+    return L, qpos, torch.cat([at.repeat(s).to(torch.int32), qpos])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["none", "cap", "bias", "both"])
+@pytest.mark.parametrize("caches,new,Hq,Hkv", [([1], 1, 1, 1), ([0], 1, 4, 2), ([5000], 1, 8, 2), ([700, 0, 1300], 1, 12, 4),
+                                               ([300, 129], 32, 8, 2), ([4000], 32, 4, 1), ([260, 1, 513], 17, 6, 2),
+                                               ([130], 128, 3, 1), ([2000], 5, 16, 2)])
+def test_few_rows(kind, caches, new, Hq, Hkv):
+    L, qpos, kpos = step_layout(caches, new)
+    run_case(*_operands(L.nq, L.nk, Hq, Hkv, 8), L, transform_for(kind, Hq, qpos, kpos, "cuda"))
+
+
+@pytest.mark.gpu
+def test_few_rows_against_caches_with_junk_behind_their_lengths():
+    L, qpos, kpos = step_layout([70, 900, 0], 9, capacity=1000)
+    q, k, v = _operands(L.nq, L.nk, 8, 2, 9)
+    dead = L.k_code == DEAD_KEY
+    k[dead] = float("nan")
+    v[dead] = float("inf")
+    run_case(q, k, v, L, transform_for("both", 8, qpos, kpos, "cuda"))
+    L, qpos, kpos = step_layout([3000], 2, window=300)
+    run_case(*_operands(L.nq, L.nk, 8, 2, 9), L, transform_for("cap", 8, qpos, kpos, "cuda"))
+
+
+@pytest.mark.gpu
+def test_few_rows_over_more_tiles_than_one_round():
+    """148 KV heads leave one split of the keys, whose 1095 tiles exceed the 1024 of one visibility round."""
+    L, qpos, kpos = step_layout([140000], 1)
+    q, k, v = _operands(L.nq, L.nk, 1, 1, 10, gain=1.0)
+    q, k, v = (t.expand(-1, 148, -1).contiguous() for t in (q, k, v))
+    out, lse = scored_attention(q, k, v, L, ScoreTransform(30.0), return_lse=True)
+    assert torch.equal(out, out[:, :1].expand_as(out)) and torch.equal(lse, lse[:1].expand_as(lse))
+    want, tol = exact(q[:, :1], k[:, :1], v[:, :1], L, ScoreTransform(30.0), 1.0 / math.sqrt(D))
+    near(out[:, :1], want["out"], tol["out"], "out")
+    near(lse[:1], want["lse"], tol["lse"], "lse")
+
+
+@pytest.mark.gpu
+def test_few_rows_graph_follows_the_metadata():
+    L, qpos, kpos = step_layout([500], 1, capacity=800)
+    q, k, v = _operands(L.nq, L.nk, 8, 2, 12)
+    tr = transform_for("both", 8, qpos, kpos, "cuda")
+    scored_attention(q, k, v, L, tr)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = scored_attention(q, k, v, L, tr)
+    M, mq, mk = step_layout([620], 1, capacity=800)
+    for a, b in ((L.q_hi, M.q_hi), (L.k_code, M.k_code), (tr.q_pos, mq), (tr.k_pos, mk)):
+        a.copy_(b)
+    graph.replay()
+    assert torch.equal(held, scored_attention(q, k, v, M, transform_for("both", 8, mq, mk, "cuda")))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("junk", [float("nan"), float("inf"), -3.0e38])
 def test_contents_of_dead_rows_do_not_matter(junk):

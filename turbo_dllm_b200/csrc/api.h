@@ -142,6 +142,13 @@ int tdllm_attn_fwd_scored(const void* q, const void* k, const void* v, void* o, 
                           const int* q_hi, const int* q_grp, const int* k_code, const int* tile_ptr,
                           const int* tile_idx, const int* order, int n_qtiles, float scale, float softcap,
                           const float* slope2, const float* q_pos, const float* k_pos, void* stream);
+// The forward for a few query rows against long keys, keys split over CTAs (attention_few_rows.cu). The mask's arrays are
+// the layout's own, unpadded; positions int32; scratch: tdllm_attn_few_rows_scratch floats.
+long long tdllm_attn_few_rows_scratch(int nq, int nk, int Hq, int Hkv);
+int tdllm_attn_few_rows(const void* q, const void* k, const void* v, void* o, float* lse, float* scratch, int nq, int nk,
+                        int Hq, int Hkv, long long ldq, long long ldk, long long ldv, long long ldo, long long ld_lse,
+                        const int* q_lo, const int* q_hi, const int* q_grp, const int* k_code, float scale,
+                        float softcap, const float* slopes, const int* q_pos, const int* k_pos, void* stream);
 int tdllm_attn_bwd_scored(const void* q, const void* k, const void* v, const void* o, const void* dout, void* dq,
                           void* dk, void* dv, const float* lse, float* delta, float* acc, int nq, int nk, int Hq,
                           int Hkv, long long ldq, long long ldk, long long ldv, long long ldo, long long lddo,

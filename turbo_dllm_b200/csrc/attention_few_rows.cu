@@ -1,0 +1,559 @@
+// Attention of a few new rows (one token, one block of new tokens, a batch of either) against a long cache, head width
+// 128, with the score transforms and the declarative mask of the tile kernels. Forward only.
+//
+// A call reads K and V once and does little with them, so it is bound by memory as long as every SM pulls: the keys are
+// split over CTAs. The G query heads of a KV head and the query rows are packed into one row axis (row r = query r / G,
+// head r % G), so a KV head's keys are read once for all of them; up to 128 packed rows share a CTA.
+//
+//   warps 0-7   each 16 packed rows x a share of the tile's keys (WR warps along the rows, 8 / WR along the keys):
+//               S = Q K^T with mma.m16n8k16 (Q fragments stay in registers), transform, mask, online softmax, O += P V.
+//               The products are a few percent of what one tile's 64 KB of loads take, until the 128 rows of a CTA are
+//               full, where both take about the same time.
+//   warp 8      brings in the tiles: TMA for K and V (three stages of 64 KB), plain loads for the keys' codes
+//
+// Split s takes the key tiles s, s + S, s + 2 S, ...: a sequence of a batch, or a sliding window, is a run of tiles, and
+// a stride spreads it evenly. Before the loop the warps test each of the CTA's tiles against the bounds of its rows'
+// masks; tiles that no row can see are never loaded. Every warp keeps its own running maximum, sum and accumulator (32
+// bits); they meet in shared memory at the end, and the splits' partial results (fp32, with their maximum and sum) in a
+// second small kernel, in a fixed order.
+//
+// Probabilities are rounded to bf16 for the product with V (as in the tile kernels), sums use them unrounded. V rows of
+// keys that none of a warp's 16 rows sees enter the product as zeros, whatever they hold.
+#include "common.cuh"
+#include "score_mod.cuh"
+#include "api.h"
+
+namespace tdllm {
+namespace few {
+
+constexpr int KID = 12;
+constexpr int HD = 128;
+constexpr int BK = 128;
+constexpr int STAGES = 3;
+constexpr int TILE_BYTES = BK * HD * 2;   // two halves of 64 columns: 128 rows x 128 bytes, swizzled
+constexpr int HALF_BYTES = TILE_BYTES / 2;
+constexpr int THREADS = 288;
+constexpr int ROUND = 1024;               // own tiles per visibility round
+constexpr int OFF_CODE = STAGES * 2 * TILE_BYTES;
+constexpr int OFF_KPOS = OFF_CODE + STAGES * BK * 4;
+constexpr int OFF_ML = OFF_KPOS + STAGES * BK * 4;          // [8 warps][16 rows] max, then sum
+constexpr int OFF_BITS = OFF_ML + 2 * 8 * 16 * 4;
+constexpr int OFF_BARS = OFF_BITS + ROUND / 8 + 32;
+constexpr int SMEM_BYTES = OFF_BARS + 64 + 1024;
+static_assert(8 * 16 * HD * 4 <= STAGES * 2 * TILE_BYTES, "the warps' accumulators reuse the stages");
+
+struct Params {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* o;
+  float* lse;
+  float* part_o;    // [splits][nq * Hq][128]
+  float* part_ml;   // [splits][nq * Hq][2]
+  const int *q_lo, *q_hi, *q_grp, *k_code, *q_pos, *k_pos;
+  const float* slopes;
+  long long ldq, ldo, ld_lse;
+  int nq, nk, Hq, Hkv, splits, row_tiles;
+  float scale_log2;
+  score::Mod mod;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ bool visible(int code, int lo, int hi, int grp) {
+  return code >= 0 ? (code >= lo && code < hi) : (code == grp);
+}
+
+// writes one finished row value range: 4 values of row r (packed index) starting at column c
+__device__ __forceinline__ void store_row4(const Params& p, int kvh, int G, int r, int c, const float* v) {
+  const int i = r / G, h = kvh * G + r % G;
+  uint2 w;
+  w.x = pack_bf16x2(v[0], v[1]);
+  w.y = pack_bf16x2(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p.o + (long long)i * p.ldo + h * HD + c) = w;
+}
+
+template <int WR, int MOD>
+__global__ void __launch_bounds__(THREADS, 1)
+few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  constexpr int KW = 8 / WR;           // warps along the keys
+  constexpr int SB = WR == 1 ? 1 : 2;  // 16-key blocks a warp takes at a time
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  int* s_code = (int*)(smem + OFF_CODE);
+  float* s_kpos = (float*)(smem + OFF_KPOS);
+  float* s_ml = (float*)(smem + OFF_ML);
+  uint32_t* s_bits = (uint32_t*)(smem + OFF_BITS);
+  int* s_bound = (int*)(s_bits + ROUND / 32);   // lo_min, hi_max, grp_min, grp_max
+  const uint32_t bar_full = smem_u32(smem + OFF_BARS), bar_empty = bar_full + 8 * STAGES;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.Hq / p.Hkv;
+  const int kvh = blockIdx.x % p.Hkv;
+  const int rt = (blockIdx.x / p.Hkv) % p.row_tiles;
+  const int split = blockIdx.x / (p.Hkv * p.row_tiles);
+  const int rows = p.nq * G;             // packed rows of a KV head
+  const int row0 = rt * 16 * WR;
+  const int nkt = (p.nk + BK - 1) / BK;
+  const int own = split < nkt ? (nkt - split + p.splits - 1) / p.splits : 0;
+
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 33);
+      mbar_init(bar_empty + 8 * s, 8);
+    }
+    fence_mbar_init();
+    s_bound[0] = 2147483647; s_bound[1] = -1; s_bound[2] = 0; s_bound[3] = score::DEAD_KEY;
+  }
+  __syncthreads();
+  {   // bounds of the rows' masks
+    const int i0 = row0 / G, i1 = min((row0 + 16 * WR - 1) / G, p.nq - 1);
+    for (int i = i0 + tid; i <= i1; i += THREADS) {
+      const int lo = p.q_lo[i], hi = p.q_hi[i], grp = p.q_grp[i];
+      if (lo < hi) {
+        atomicMin(s_bound, lo);
+        atomicMax(s_bound + 1, hi);
+      }
+      if (grp < 0) {
+        atomicMin(s_bound + 2, grp);
+        atomicMax(s_bound + 3, grp);
+      }
+    }
+  }
+  __syncthreads();
+  const int lo_min = s_bound[0], hi_max = s_bound[1], g_min = s_bound[2], g_max = s_bound[3];
+
+  // compute warps: rows and their metadata
+  const int wr = warp % WR, kw = warp / WR;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int ra = row0 + wr * 16 + g, rb = ra + 8;
+  uint32_t qf[8][4];
+  int lo[2] = {0, 0}, hi[2] = {0, 0}, grp[2] = {0, 0};
+  [[maybe_unused]] float slope2[2] = {0.f, 0.f}, qpos[2] = {0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float acc[16][4];
+  if (warp < 8) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = x ? rb : ra;
+      if (r < rows) {
+        const int i = r / G, h = kvh * G + r % G;
+        lo[x] = p.q_lo[i];
+        hi[x] = p.q_hi[i];
+        grp[x] = p.q_grp[i];
+        if constexpr ((MOD & score::BIAS) != 0) {
+          slope2[x] = p.slopes[h] * 1.4426950408889634f;
+          qpos[x] = (float)p.q_pos[i];
+        }
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (long long)i * p.ldq + h * HD) + t4;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          qf[k][x] = src[k * 8];
+          qf[k][x + 2] = src[k * 8 + 4];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) qf[k][x] = qf[k][x + 2] = 0u;
+      }
+    }
+  }
+
+  int it = 0;        // tiles through the pipeline so far: stage it % STAGES
+  bool ok = true;
+  for (int base = 0; base < own; base += ROUND) {
+    const int cnt = min(ROUND, own - base);
+    __syncthreads();   // the previous round's bits have been read
+    for (int i = tid; i < ROUND / 32; i += THREADS) s_bits[i] = 0u;
+    __syncthreads();
+    for (int o = warp; o < cnt; o += THREADS / 32) {
+      const int k0 = (split + (base + o) * p.splits) * BK;
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = k0 + e * 32 + lane;
+        const int c = k < p.nk ? __ldg(p.k_code + k) : score::DEAD_KEY;
+        any |= c >= 0 ? (c >= lo_min && c < hi_max) : (c >= g_min && c <= g_max && c != score::DEAD_KEY);
+      }
+      if (__any_sync(0xffffffffu, any) && lane == 0) atomicOr(s_bits + (o >> 5), 1u << (o & 31));
+    }
+    __syncthreads();
+    int total = 0;
+    for (int i = 0; i < (cnt + 31) / 32; ++i) total += __popc(s_bits[i]);
+    if (warp == 8) {
+      int j = 0;
+      for (int w = 0; w < (cnt + 31) / 32 && ok; ++w) {
+        uint32_t bits = s_bits[w];
+        while (bits && ok) {
+          const int o = w * 32 + __ffs(bits) - 1;
+          bits &= bits - 1;
+          const int k0 = (split + (base + o) * p.splits) * BK;
+          const int s = (it + j) % STAGES;
+          const uint32_t ph = ((it + j) / STAGES) & 1;
+          int code[4];
+          [[maybe_unused]] int kp[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = k0 + e * 32 + lane;
+            code[e] = k < p.nk ? __ldg(p.k_code + k) : score::DEAD_KEY;
+            if constexpr ((MOD & score::BIAS) != 0) kp[e] = k < p.nk ? __ldg(p.k_pos + k) : 0;
+          }
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, ph ^ 1, KID, 10));
+          if (!ok) break;
+          if (lane == 0) {
+            const uint32_t bar = bar_full + 8 * s;
+            const uint32_t dst = smem_u32(smem + s * 2 * TILE_BYTES);
+            mbar_expect_tx(bar, 2 * TILE_BYTES);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              tma_load_2d(dst + c * HALF_BYTES, &tm_k, bar, kvh * HD + c * 64, k0);
+              tma_load_2d(dst + TILE_BYTES + c * HALF_BYTES, &tm_v, bar, kvh * HD + c * 64, k0);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s_code[s * BK + e * 32 + lane] = code[e];
+            if constexpr ((MOD & score::BIAS) != 0) s_kpos[s * BK + e * 32 + lane] = (float)kp[e];
+          }
+          mbar_arrive(bar_full + 8 * s);
+          ++j;
+        }
+      }
+    } else {
+      for (int j = 0; j < total && ok; ++j) {
+        const int s = (it + j) % STAGES;
+        const uint32_t ph = ((it + j) / STAGES) & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_full + 8 * s, ph, KID, 20));
+        if (!ok) break;
+        const uint32_t kb = smem_u32(smem + s * 2 * TILE_BYTES), vb = kb + TILE_BYTES;
+        const int* codes = s_code + s * BK;
+        const float* kpos = s_kpos + s * BK;
+#pragma unroll 1
+        for (int b0 = kw * SB; b0 < 8; b0 += KW * SB) {   // SB blocks of 16 keys
+          float sc[SB * 2][4];
+#pragma unroll
+          for (int n = 0; n < SB * 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+#pragma unroll
+            for (int b = 0; b < SB; ++b) {
+              uint32_t kf[4];
+              const int key = (b0 + b) * 16 + (lane >> 4) * 8 + (lane & 7);
+              const int chunk = k * 2 + ((lane >> 3) & 1);
+              ldsm4(kb + (chunk >> 3) * HALF_BYTES + sw128_offset(key, chunk & 7), kf);
+              mma16816(sc[b * 2], qf[k], kf[0], kf[1]);
+              mma16816(sc[b * 2 + 1], qf[k], kf[2], kf[3]);
+            }
+          }
+          float mx[2] = {-INFINITY, -INFINITY};
+          uint32_t live[SB * 2];   // bit 0, 1: a row of this warp sees key 2 t4 (+1) of the 8
+#pragma unroll
+          for (int n = 0; n < SB * 2; ++n) {
+            const int key = b0 * 16 + n * 8 + t4 * 2;
+            const int c0 = codes[key], c1 = codes[key + 1];
+            live[n] = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int x = e >> 1, c = (e & 1) ? c1 : c0;
+              float z = sc[n][e];
+              if constexpr ((MOD & score::CAP) != 0) z = score::cap_z(score::cap_r(z, p.mod), p.mod);
+              else z *= p.scale_log2;
+              if constexpr ((MOD & score::BIAS) != 0) z = fmaf(-slope2[x], fabsf(qpos[x] - kpos[key + (e & 1)]), z);
+              const bool v = visible(c, lo[x], hi[x], grp[x]);
+              live[n] |= (uint32_t)v << (e & 1);
+              sc[n][e] = v ? z : -INFINITY;
+              mx[x] = fmaxf(mx[x], sc[n][e]);
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
+            mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
+          }
+#pragma unroll
+          for (int n = 0; n < SB * 2; ++n) {
+            live[n] |= __shfl_xor_sync(0xffffffffu, live[n], 4);
+            live[n] |= __shfl_xor_sync(0xffffffffu, live[n], 8);
+            live[n] |= __shfl_xor_sync(0xffffffffu, live[n], 16);
+          }
+          // the reference maximum moves only when the new one is 2^8 larger
+          float alpha[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            alpha[x] = 1.f;
+            if (mx[x] > -INFINITY && (m[x] == -INFINITY || mx[x] - m[x] > 8.f)) {
+              alpha[x] = m[x] == -INFINITY ? 0.f : score::exp2_approx(m[x] - mx[x]);
+              m[x] = mx[x];
+            }
+            l[x] *= alpha[x];
+          }
+          if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              acc[e][0] *= alpha[0];
+              acc[e][1] *= alpha[0];
+              acc[e][2] *= alpha[1];
+              acc[e][3] *= alpha[1];
+            }
+          }
+          const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+          for (int b = 0; b < SB; ++b) {
+            uint32_t pf[4], keep[2];
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {   // keys 0-7, 8-15 of the block
+              float* z = sc[b * 2 + hh];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                z[e] = score::exp2_approx(z[e] - ref[e >> 1]);
+                l[e >> 1] += z[e];
+              }
+              pf[hh * 2] = pack_bf16x2(z[0], z[1]);
+              pf[hh * 2 + 1] = pack_bf16x2(z[2], z[3]);
+              const uint32_t lv = live[b * 2 + hh];
+              keep[hh] = ((lv & 1u) ? 0xffffu : 0u) | ((lv & 2u) ? 0xffff0000u : 0u);
+            }
+            const bool all = __all_sync(0xffffffffu, (keep[0] & keep[1]) == 0xffffffffu);
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {   // 16 columns of V at a time
+              uint32_t vf[4];
+              const int key = (b0 + b) * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+              const int chunk = d * 2 + (lane >> 4);
+              ldsm4t(vb + (chunk >> 3) * HALF_BYTES + sw128_offset(key, chunk & 7), vf);
+              if (!all) {
+                vf[0] &= keep[0];
+                vf[1] &= keep[1];
+                vf[2] &= keep[0];
+                vf[3] &= keep[1];
+              }
+              mma16816(acc[d * 2], pf, vf[0], vf[1]);
+              mma16816(acc[d * 2 + 1], pf, vf[2], vf[3]);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_empty + 8 * s);
+      }
+    }
+    it += total;
+  }
+
+  // the warps' partial results meet in shared memory
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+  }
+  if (__syncthreads_or(!ok)) {
+    // a wait ran out: leave the results alone, give this CTA's own copies time to land
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    __syncthreads();
+    return;
+  }
+  float* s_acc = (float*)smem;   // [warp][16][128]
+  if (warp < 8) {
+    float* mine = s_acc + warp * 16 * HD;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      *reinterpret_cast<float2*>(mine + g * HD + e * 8 + t4 * 2) = make_float2(acc[e][0], acc[e][1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * HD + e * 8 + t4 * 2) = make_float2(acc[e][2], acc[e][3]);
+    }
+    if (t4 == 0) {
+      s_ml[warp * 16 + g] = m[0];
+      s_ml[warp * 16 + g + 8] = m[1];
+      s_ml[128 + warp * 16 + g] = l[0];
+      s_ml[128 + warp * 16 + g + 8] = l[1];
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < 16 * WR * (HD / 4); i += THREADS) {
+    const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+    const int row = row0 + r;
+    if (row >= rows) continue;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) top = fmaxf(top, s_ml[(k * WR + r / 16) * 16 + r % 16]);
+    float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (top > -INFINITY) {
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        const int w = k * WR + r / 16;
+        const float f = score::exp2_approx(s_ml[w * 16 + r % 16] - top);   // (-inf - top: 0)
+        sum += f * s_ml[128 + w * 16 + r % 16];
+        const float4 a = *reinterpret_cast<const float4*>(s_acc + (w * 16 + r % 16) * HD + c);
+        v[0] += f * a.x;
+        v[1] += f * a.y;
+        v[2] += f * a.z;
+        v[3] += f * a.w;
+      }
+    }
+    const long long out_row = (long long)(row / G) * p.Hq + kvh * G + row % G;
+    if (p.splits == 1) {
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= inv;
+      store_row4(p, kvh, G, row, c, v);
+      if (c == 0)
+        p.lse[(long long)(kvh * G + row % G) * p.ld_lse + row / G] =
+            sum > 0.f ? top * 0.69314718055994531f + __logf(sum) : -INFINITY;
+    } else {
+      const long long at = (long long)split * p.nq * p.Hq + out_row;
+      *reinterpret_cast<float4*>(p.part_o + at * HD + c) = make_float4(v[0], v[1], v[2], v[3]);
+      if (c == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(top, sum);
+    }
+  }
+}
+
+// One warp per (query row, head): joins the splits.
+__global__ void __launch_bounds__(128) few_rows_join_kernel(const Params p) {
+  const int lane = threadIdx.x & 31;
+  const long long n = (long long)p.nq * p.Hq;
+  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (at >= n) return;
+  float top = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_ml[(s * n + at) * 2]);
+  top = warp_max(top);
+  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (top > -INFINITY) {
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * n + at) * 2);
+      const float4 a = *reinterpret_cast<const float4*>(p.part_o + (s * n + at) * HD + lane * 4);
+      const float f = score::exp2_approx(ml.x - top);
+      sum += f * ml.y;
+      v[0] += f * a.x;
+      v[1] += f * a.y;
+      v[2] += f * a.z;
+      v[3] += f * a.w;
+    }
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const int i = (int)(at / p.Hq), h = (int)(at % p.Hq);
+  uint2 w;
+  w.x = pack_bf16x2(v[0] * inv, v[1] * inv);
+  w.y = pack_bf16x2(v[2] * inv, v[3] * inv);
+  *reinterpret_cast<uint2*>(p.o + (long long)i * p.ldo + h * HD + lane * 4) = w;
+  if (lane == 0)
+    p.lse[(long long)h * p.ld_lse + i] = sum > 0.f ? top * 0.69314718055994531f + __logf(sum) : -INFINITY;
+}
+
+struct Plan {
+  int wr, row_tiles, splits;
+};
+static Plan plan_of(int nq, int nk, int Hq, int Hkv) {
+  Plan pl;
+  const int rows = nq * (Hq / Hkv);
+  pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
+  pl.row_tiles = (rows + 16 * pl.wr - 1) / (16 * pl.wr);
+  const int nkt = (nk + BK - 1) / BK;
+  int s = tdllm_num_sms() / (Hkv * pl.row_tiles);
+  if (s > nkt) s = nkt;
+  pl.splits = s < 1 ? 1 : s;
+  return pl;
+}
+
+template <int WR, int MOD>
+static cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, cudaStream_t st) {
+  static bool attr_set[64] = {false};   // a function attribute belongs to one device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<WR, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  few_rows_kernel<WR, MOD><<<p.Hkv * p.row_tiles * p.splits, THREADS, SMEM_BYTES, st>>>(tk, tv, p);
+  return cudaGetLastError();
+}
+template <int MOD>
+static cudaError_t launch_wr(int wr, const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, cudaStream_t st) {
+  switch (wr) {
+    case 1: return launch<1, MOD>(tk, tv, p, st);
+    case 2: return launch<2, MOD>(tk, tv, p, st);
+    case 4: return launch<4, MOD>(tk, tv, p, st);
+    default: return launch<8, MOD>(tk, tv, p, st);
+  }
+}
+
+}  // namespace few
+}  // namespace tdllm
+
+using namespace tdllm;
+
+// floats of scratch that tdllm_attn_few_rows needs (0: the keys are not split)
+extern "C" long long tdllm_attn_few_rows_scratch(int nq, int nk, int Hq, int Hkv) {
+  if (nq <= 0 || nk <= 0 || Hkv <= 0 || Hq % Hkv) return 0;
+  const few::Plan pl = few::plan_of(nq, nk, Hq, Hkv);
+  return pl.splits > 1 ? (long long)pl.splits * nq * Hq * (few::HD + 2) : 0;
+}
+
+// q [nq, Hq*128], k / v [nk, Hkv*128], o [nq, Hq*128] (row strides in elements), lse [Hq][ld_lse]. The mask's arrays are
+// the layout's own (nothing padded, no tile lists); positions int32, slopes [Hq] (null: no bias).
+extern "C" int tdllm_attn_few_rows(const void* q, const void* k, const void* v, void* o, float* lse, float* scratch,
+                                   int nq, int nk, int Hq, int Hkv, long long ldq, long long ldk, long long ldv,
+                                   long long ldo, long long ld_lse, const int* q_lo, const int* q_hi, const int* q_grp,
+                                   const int* k_code, float scale, float softcap, const float* slopes, const int* q_pos,
+                                   const int* k_pos, void* stream) {
+  if (nq <= 0 || nk <= 0) return 0;
+  if (Hkv <= 0 || Hq % Hkv) {
+    tdllm_host::set_last_error("attn_few_rows: %d query heads do not divide over %d KV heads", Hq, Hkv);
+    return 1;
+  }
+  const long long lds[4] = {ldq, ldk, ldv, ldo};
+  const void* ptrs[4] = {q, k, v, o};
+  for (int i = 0; i < 4; ++i)
+    if ((lds[i] % 8) || ((uintptr_t)ptrs[i] % 16)) {
+      tdllm_host::set_last_error("attn_few_rows: operand %d needs a 16-byte aligned base and row stride", i);
+      return 1;
+    }
+  const few::Plan pl = few::plan_of(nq, nk, Hq, Hkv);
+  CUtensorMap tk, tv;
+  if (tdllm_host::encode_rows_tmap(&tk, k, (long long)Hkv * few::HD, nk, ldk, few::BK)) return 3;
+  if (tdllm_host::encode_rows_tmap(&tv, v, (long long)Hkv * few::HD, nk, ldv, few::BK)) return 3;
+  few::Params p;
+  p.q = (const __nv_bfloat16*)q;
+  p.o = (__nv_bfloat16*)o;
+  p.lse = lse;
+  p.part_o = scratch;
+  p.part_ml = scratch ? scratch + (long long)pl.splits * nq * Hq * few::HD : nullptr;
+  p.q_lo = q_lo; p.q_hi = q_hi; p.q_grp = q_grp; p.k_code = k_code; p.q_pos = q_pos; p.k_pos = k_pos;
+  p.slopes = slopes;
+  p.ldq = ldq; p.ldo = ldo; p.ld_lse = ld_lse;
+  p.nq = nq; p.nk = nk; p.Hq = Hq; p.Hkv = Hkv; p.splits = pl.splits; p.row_tiles = pl.row_tiles;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.mod = score_mod_of(scale, softcap, nullptr, nullptr, nullptr);
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  switch ((softcap > 0.f ? score::CAP : 0) | (slopes ? score::BIAS : 0)) {
+    case 0: e = few::launch_wr<0>(pl.wr, tk, tv, p, st); break;
+    case score::CAP: e = few::launch_wr<score::CAP>(pl.wr, tk, tv, p, st); break;
+    case score::BIAS: e = few::launch_wr<score::BIAS>(pl.wr, tk, tv, p, st); break;
+    default: e = few::launch_wr<score::CAP | score::BIAS>(pl.wr, tk, tv, p, st); break;
+  }
+  if (e == cudaSuccess && pl.splits > 1) {
+    const long long n = (long long)nq * Hq;
+    few::few_rows_join_kernel<<<(unsigned)((n + 3) / 4), 128, 0, st>>>(p);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) {
+    tdllm_host::set_last_error("attn_few_rows launch: %s", cudaGetErrorString(e));
+    return 4;
+  }
+  return 0;
+}

@@ -31,12 +31,15 @@ import torch
 
 from ..kernels import native
 from ._util import ptr
-from .attention import MaskLayout, backward_chunk_tiles, backward_mode
+from .attention import TILE, MaskLayout, backward_chunk_tiles, backward_mode
 
 native.register_signatures({
     "tdllm_attn_fwd_scored": (native.c_int, [native.c_void_p] * 5 + [native.c_int] * 4 + [native.c_ll] * 4
                               + [native.c_void_p] * 7 + [native.c_int, native.c_float, native.c_float]
                               + [native.c_void_p] * 4),
+    "tdllm_attn_few_rows_scratch": (native.c_ll, [native.c_int] * 4),
+    "tdllm_attn_few_rows": (native.c_int, [native.c_void_p] * 6 + [native.c_int] * 4 + [native.c_ll] * 5
+                            + [native.c_void_p] * 4 + [native.c_float] * 2 + [native.c_void_p] * 4),
     "tdllm_attn_bwd_scored": (native.c_int, [native.c_void_p] * 11 + [native.c_int] * 4 + [native.c_ll] * 8
                               + [native.c_void_p] * 7 + [native.c_int, native.c_int, native.c_int, native.c_float,
                                                          native.c_float] + [native.c_void_p] * 4),
@@ -45,6 +48,8 @@ native.register_signatures({
 DEAD_KEY = -(2 ** 31)      # key code that no query row matches
 MAX_POSITION = 1 << 24     # distances are taken between positions held as floats
 LOG2E = 1.4426950408889634
+# Up to this many query rows the forward splits the keys over the GPU instead of giving a CTA a 128-row query tile
+FEW_ROWS = 128
 
 
 @dataclass(frozen=True, eq=False)
@@ -232,9 +237,37 @@ def _mod_args(transform: ScoreTransform | None, L: dict):
     return (float(transform.softcap), *(ptr(t) for t in kept)), kept
 
 
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    return t.to(torch.int32).contiguous()
+
+
+def _forward_few_rows(q, k, v, layout, transform, scale):
+    """(out, lse [Hq, rows padded to 128]) with the keys split over CTAs. Reads the layout's and the transform's own
+    tensors at run time: nothing is built or cached, so a captured graph follows what is written to them."""
+    nq, Hq, D = q.shape
+    nk, Hkv, _ = k.shape
+    lib = native.lib()
+    out = torch.empty(nq, Hq, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(Hq, TILE, dtype=torch.float32, device=q.device)
+    n = lib.tdllm_attn_few_rows_scratch(nq, nk, Hq, Hkv)
+    part = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    meta = [_int32(t) for t in (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code)]
+    bias = [None] * 3
+    if transform is not None and transform.biased:
+        bias = [transform.slopes.contiguous(), _int32(transform.q_pos), _int32(transform.k_pos)]
+    rc = lib.tdllm_attn_few_rows(
+        ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(part), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k),
+        _row_stride(v), out.stride(0), TILE, *(ptr(t) for t in meta), float(scale),
+        0.0 if transform is None else float(transform.softcap), *(ptr(t) for t in bias), _stream(q))
+    native.check(rc, "attn_few_rows" if part is None else "attn_few_rows_split")
+    return out, lse
+
+
 def _forward(q, k, v, layout, transform, scale):
     nq, Hq, D = q.shape
     nk, Hkv, _ = k.shape
+    if nq <= FEW_ROWS:
+        return _forward_few_rows(q, k, v, layout, transform, scale)
     L = _lists(layout)
     mod, _kept = _mod_args(transform, L)
     out = torch.empty(nq, Hq, D, dtype=q.dtype, device=q.device)
