@@ -278,22 +278,24 @@ def step_layout(caches, new, device="cuda", capacity=None, window=None):
 @pytest.mark.parametrize("kind", ["none", "cap", "bias", "both"])
 @pytest.mark.parametrize("caches,new,Hq,Hkv", [([1], 1, 1, 1), ([0], 1, 4, 2), ([5000], 1, 8, 2), ([700, 0, 1300], 1, 12, 4),
                                                ([300, 129], 32, 8, 2), ([4000], 32, 4, 1), ([260, 1, 513], 17, 6, 2),
-                                               ([130], 128, 3, 1), ([2000], 5, 16, 2)])
+                                               ([130], 128, 3, 1), ([2000], 5, 16, 2),
+                                               ([1000], 100, 2, 2), ([300, 200], 64, 8, 1), ([5], 40, 16, 1)])
 def test_few_rows(kind, caches, new, Hq, Hkv):
     L, qpos, kpos = step_layout(caches, new)
     run_case(*_operands(L.nq, L.nk, Hq, Hkv, 8), L, transform_for(kind, Hq, qpos, kpos, "cuda"))
 
 
 @pytest.mark.gpu
-def test_few_rows_against_caches_with_junk_behind_their_lengths():
-    L, qpos, kpos = step_layout([70, 900, 0], 9, capacity=1000)
-    q, k, v = _operands(L.nq, L.nk, 8, 2, 9)
+@pytest.mark.parametrize("new,Hq", [(1, 8), (9, 8), (30, 8), (9, 6)])
+def test_few_rows_against_caches_with_junk_behind_their_lengths(new, Hq):
+    L, qpos, kpos = step_layout([70, 900, 0], new, capacity=1000)
+    q, k, v = _operands(L.nq, L.nk, Hq, 2, 9)
     dead = L.k_code == DEAD_KEY
     k[dead] = float("nan")
     v[dead] = float("inf")
-    run_case(q, k, v, L, transform_for("both", 8, qpos, kpos, "cuda"))
-    L, qpos, kpos = step_layout([3000], 2, window=300)
-    run_case(*_operands(L.nq, L.nk, 8, 2, 9), L, transform_for("cap", 8, qpos, kpos, "cuda"))
+    run_case(q, k, v, L, transform_for("both", Hq, qpos, kpos, "cuda"))
+    L, qpos, kpos = step_layout([3000], new, window=300)
+    run_case(*_operands(L.nq, L.nk, Hq, 2, 9), L, transform_for("cap", Hq, qpos, kpos, "cuda"))
 
 
 @pytest.mark.gpu

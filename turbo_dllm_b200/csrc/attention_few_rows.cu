@@ -420,6 +420,456 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   }
 }
 
+// ---------------------------------------------------------------------------
+// The same for more packed rows (and group sizes that divide 128): tcgen05 products on a 128-row tile
+// ---------------------------------------------------------------------------
+// One CTA owns 128 packed rows of a KV head and one split of the keys. Its tiles alternate between two softmax
+// pipelines of eight warps (two threads per row, 64 keys each) with their own scores and accumulator in TMEM, so that the
+// exponentials of one tile overlap the products of the next; the two accumulators are joined at the end like two splits.
+//   warps 0-15 softmax, warp 16 TMA (Q once: a 3-D box of 128 / G rows x G heads lands as packed rows; K and V, three
+//   stages), warp 17 issues the MMAs.  TMEM: S0 [0,128) S1 [128,256) O0 [256,384) O1 [384,512), P over S as bf16.
+// Tiles that every row sees whole skip the mask; in the others, V rows that no row of the CTA can see are overwritten
+// with zeros.
+namespace fewt {
+
+constexpr int KID = 13;
+constexpr int STAGES = 3;
+constexpr int THREADS = 576;
+constexpr int OFF_STAGE = TILE_BYTES;                             // behind Q
+constexpr int OFF_X = OFF_STAGE + STAGES * 2 * TILE_BYTES;        // row exchange [pipeline][half][128]
+constexpr int OFF_BITS = OFF_X + 2048;                            // visible tiles, then fully visible tiles
+constexpr int OFF_BOUND = OFF_BITS + 2 * ROUND / 8;
+constexpr int OFF_BARS = OFF_BOUND + 32;
+// no alignment slack: the kernel checks that its dynamic shared memory starts 1 KiB aligned
+constexpr int SMEM_BYTES = OFF_BARS + 256;
+static_assert(SMEM_BYTES <= 232448, "shared memory budget of one CTA");
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// walks the set bits of a bit map in order
+struct Walk {
+  const uint32_t* words;
+  int w;
+  uint32_t bits;
+  __device__ __forceinline__ explicit Walk(const uint32_t* b) : words(b), w(0), bits(b[0]) {}
+  __device__ __forceinline__ int next() {   // only called while bits are left
+    while (!bits) bits = words[++w];
+    const int o = w * 32 + __ffs(bits) - 1;
+    bits &= bits - 1;
+    return o;
+  }
+};
+
+template <int MOD>
+__global__ void __launch_bounds__(THREADS, 1)
+few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                 const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {   // swizzled tiles need 1 KiB alignment; nothing has been set up yet
+    if (threadIdx.x == 0) set_error(ERR_BAD_INDEX, KID, 1);
+    return;
+  }
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + OFF_STAGE;   // [stage][K | V]
+  float* sX = (float*)(smem + OFF_X);
+  uint32_t* s_vis = (uint32_t*)(smem + OFF_BITS);
+  uint32_t* s_full = s_vis + ROUND / 32;
+  int* s_bound = (int*)(smem + OFF_BOUND);   // lo_min, hi_max, grp_min, grp_max, lo_max, hi_min
+  const uint32_t b0 = smem_u32(smem + OFF_BARS);
+  const uint32_t bar_q = b0, bar_kfull = b0 + 8, bar_vfull = b0 + 32, bar_empty = b0 + 56;   // [3] each
+  const uint32_t bar_sfull = b0 + 80, bar_pfull = b0 + 96, bar_odone = b0 + 112;             // [2] each
+  uint32_t* tmem_slot = (uint32_t*)(smem + OFF_BARS + 128);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.Hq / p.Hkv;
+  const int kvh = blockIdx.x % p.Hkv;
+  const int rt = (blockIdx.x / p.Hkv) % p.row_tiles;
+  const int split = blockIdx.x / (p.Hkv * p.row_tiles);
+  const int rows = p.nq * G;
+  const int row0 = rt * 128;
+  const int nkt = (p.nk + BK - 1) / BK;
+  const int own = split < nkt ? (nkt - split + p.splits - 1) / p.splits : 0;   // at most ROUND (host)
+
+  if (tid == 0) {
+    mbar_init(bar_q, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_kfull + 8 * s, 1);
+      mbar_init(bar_vfull + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar_sfull + 8 * s, 1);
+      mbar_init(bar_pfull + 8 * s, 256);
+      mbar_init(bar_odone + 8 * s, 1);
+    }
+    fence_mbar_init();
+    s_bound[0] = 2147483647; s_bound[1] = -1; s_bound[2] = 0; s_bound[3] = score::DEAD_KEY;
+    s_bound[4] = -2147483647 - 1; s_bound[5] = 2147483647;
+  }
+  if (warp == 17) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  for (int i = tid; i < 2 * ROUND / 32; i += THREADS) s_vis[i] = 0u;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  {   // bounds of the rows' masks
+    const int i0 = row0 / G, i1 = min((row0 + 127) / G, p.nq - 1);
+    for (int i = i0 + tid; i <= i1; i += THREADS) {
+      const int lo = p.q_lo[i], hi = p.q_hi[i], grp = p.q_grp[i];
+      if (lo < hi) {
+        atomicMin(s_bound, lo);
+        atomicMax(s_bound + 1, hi);
+      }
+      if (grp < 0) {
+        atomicMin(s_bound + 2, grp);
+        atomicMax(s_bound + 3, grp);
+      }
+      atomicMax(s_bound + 4, lo);
+      atomicMin(s_bound + 5, hi);
+    }
+  }
+  __syncthreads();
+  const int lo_min = s_bound[0], hi_max = s_bound[1], g_min = s_bound[2], g_max = s_bound[3];
+  {
+    const int lo_max = s_bound[4], hi_min = s_bound[5];
+    for (int o = warp; o < own; o += THREADS / 32) {
+      const int k0 = (split + o * p.splits) * BK;
+      bool any = false, all = true;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = k0 + e * 32 + lane;
+        const int c = k < p.nk ? __ldg(p.k_code + k) : score::DEAD_KEY;
+        any |= c >= 0 ? (c >= lo_min && c < hi_max) : (c >= g_min && c <= g_max && c != score::DEAD_KEY);
+        all &= c >= 0 && c >= lo_max && c < hi_min;
+      }
+      any = __any_sync(0xffffffffu, any);
+      all = __all_sync(0xffffffffu, all);
+      if (lane == 0 && any) atomicOr(s_vis + (o >> 5), 1u << (o & 31));
+      if (lane == 0 && all) atomicOr(s_full + (o >> 5), 1u << (o & 31));
+    }
+  }
+  __syncthreads();
+  int n = 0;
+  for (int i = 0; i < (own + 31) / 32; ++i) n += __popc(s_vis[i]);
+
+  if (warp == 16) {
+    // ------------------------------ TMA producer ------------------------------
+    if (lane == 0 && n > 0) {
+      mbar_expect_tx(bar_q, TILE_BYTES);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) tma_load_3d(smem_u32(sQ + c * HALF_BYTES), &tm_q, bar_q, c * 64, kvh * G, row0 / G);
+      Walk walk(s_vis);
+      for (int j = 0; j < n; ++j) {
+        const int s = j % STAGES;
+        const int k0 = (split + walk.next() * p.splits) * BK;
+        const uint32_t dst = smem_u32(sKV + s * 2 * TILE_BYTES);
+        if (!mbar_wait_spin(bar_empty + 8 * s, ((j / STAGES) & 1) ^ 1, KID, 10)) break;
+        mbar_expect_tx(bar_kfull + 8 * s, TILE_BYTES);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) tma_load_2d(dst + c * HALF_BYTES, &tm_k, bar_kfull + 8 * s, kvh * HD + c * 64, k0);
+        mbar_expect_tx(bar_vfull + 8 * s, TILE_BYTES);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          tma_load_2d(dst + TILE_BYTES + c * HALF_BYTES, &tm_v, bar_vfull + 8 * s, kvh * HD + c * 64, k0);
+      }
+    }
+  } else if (warp == 17) {
+    // ------------------------------ MMA issuer (whole warp, one elected lane issues) ----
+    if (n > 0) {
+      const bool leader = elect_one();
+      const uint32_t idesc_qk = make_idesc_bf16(128, BK, 0, 0);
+      const uint32_t idesc_pv = make_idesc_bf16(128, HD, 0, 1);
+      auto wait_all = [&](uint32_t bar, uint32_t parity, int detail) {
+        return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, KID, detail));
+      };
+      auto issue_qk = [&](int j) {   // scores of tile j into pipeline j & 1
+        const uint32_t qa = smem_u32(sQ), ka = smem_u32(sKV + (j % STAGES) * 2 * TILE_BYTES);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t off = (k >> 2) * HALF_BYTES + (k & 3) * 32;
+          const uint64_t ad = make_smem_desc_sw128(qa + off, 16, 1024);
+          const uint64_t bd = make_smem_desc_sw128(ka + off, 16, 1024);
+          if (leader) tc_mma_ss(tmem_base + (j & 1) * 128, ad, bd, idesc_qk, k ? 1u : 0u);
+        }
+        if (leader) tc_commit(bar_sfull + 8 * (j & 1));
+      };
+      bool ok = wait_all(bar_q, 0, 20);
+      for (int j = 0; j < 2 && j < n && ok; ++j) {
+        ok = wait_all(bar_kfull + 8 * j, 0, 21);
+        if (ok) {
+          tc_fence_after();
+          issue_qk(j);
+        }
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const int i = j & 1, s = j % STAGES;
+        if (!wait_all(bar_vfull + 8 * s, (j / STAGES) & 1, 22)) break;
+        if (!wait_all(bar_pfull + 8 * i, (j >> 1) & 1, 23)) break;
+        tc_fence_after();
+        const uint32_t va = smem_u32(sKV + s * 2 * TILE_BYTES + TILE_BYTES);
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k) {
+          const uint64_t bd = make_smem_desc_sw128(va + k * 2048, HALF_BYTES, 1024);
+          if (leader) tc_mma_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + k * 8, bd, idesc_pv, (j > 1 || k) ? 1u : 0u);
+        }
+        if (leader) {
+          tc_commit(bar_empty + 8 * s);
+          if (j + 2 >= n) tc_commit(bar_odone + 8 * i);
+        }
+        if (j + 2 < n) {
+          if (!wait_all(bar_kfull + 8 * ((j + 2) % STAGES), ((j + 2) / STAGES) & 1, 24)) break;
+          tc_fence_after();
+          issue_qk(j + 2);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  // ------------------------------ softmax pipelines -------------------------------
+  const int i = warp >> 3;          // pipeline
+  const int sub = (warp >> 2) & 1;  // which 64 keys of a tile (and columns of the accumulator)
+  const int qd = warp & 3;          // TMEM lane quarter
+  const int row = qd * 32 + lane;
+  const uint32_t t_s = tmem_base + ((uint32_t)(qd * 32) << 16) + i * 128;
+  const uint32_t t_o = tmem_base + ((uint32_t)(qd * 32) << 16) + 256 + i * 128;
+  float* xmine = sX + (i * 2 + sub) * 128 + row;
+  const float* xother = sX + (i * 2 + (sub ^ 1)) * 128 + row;
+  float m = -INFINITY, l = 0.f;
+  bool ok = true;
+  if (warp < 16) {
+    const int prow = row0 + row;
+    int lo = 0, hi = 0, grp = 0;
+    [[maybe_unused]] float slope2 = 0.f, qpos = 0.f;
+    if (prow < rows) {
+      const int qi = prow / G;
+      lo = p.q_lo[qi];
+      hi = p.q_hi[qi];
+      grp = p.q_grp[qi];
+      if constexpr ((MOD & score::BIAS) != 0) {
+        slope2 = p.slopes[kvh * G + prow % G] * 1.4426950408889634f;
+        qpos = (float)p.q_pos[qi];
+      }
+    }
+    Walk walk(s_vis);
+    uint32_t r[64];
+    for (int j = 0; j < n; ++j) {
+      const int o = walk.next();
+      if ((j & 1) != i) continue;
+      const int k0 = (split + o * p.splits) * BK + sub * 64;
+      const bool masked = !((s_full[o >> 5] >> (o & 31)) & 1u);
+      bool good = __all_sync(0xffffffffu, mbar_wait_spin(bar_sfull + 8 * i, (j >> 1) & 1, KID, 30));
+      if (good) {
+        tc_fence_after();
+        tmem_ld32(t_s + sub * 64, r);
+        tmem_ld32(t_s + sub * 64 + 32, r + 32);
+        tmem_ld_wait();
+        if (masked) {
+          // this thread's key of the tile: a V row that no row of the CTA can see is cleared (half a row per thread)
+          const int kv = (split + o * p.splits) * BK + row;
+          const int c = kv < p.nk ? __ldg(p.k_code + kv) : score::DEAD_KEY;
+          const bool any = c >= 0 ? (c >= lo_min && c < hi_max) : (c >= g_min && c <= g_max && c != score::DEAD_KEY);
+          if (!any && mbar_wait_spin(bar_vfull + 8 * (j % STAGES), (j / STAGES) & 1, KID, 33)) {
+            uint4* vrow = reinterpret_cast<uint4*>(sKV + (j % STAGES) * 2 * TILE_BYTES + TILE_BYTES + sub * HALF_BYTES + row * 128);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+#pragma unroll
+        for (int e = 0; e < 64; ++e) {
+          float z = __uint_as_float(r[e]);
+          if constexpr ((MOD & score::CAP) != 0) z = score::cap_z(score::cap_r(z, p.mod), p.mod);
+          else z *= p.scale_log2;
+          if constexpr ((MOD & score::BIAS) != 0) {
+            const int k = min(k0 + e, p.nk - 1);   // (a key past the end is masked)
+            z = fmaf(-slope2, fabsf(qpos - (float)__ldg(p.k_pos + k)), z);
+          }
+          r[e] = __float_as_uint(z);
+        }
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            const int c = k0 + e < p.nk ? __ldg(p.k_code + k0 + e) : score::DEAD_KEY;
+            if (!visible(c, lo, hi, grp)) r[e] = 0xff800000u;   // -inf
+          }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+        *xmine = mx;
+      }
+      // the barrier also orders the P stores below after the partner's loads of its score columns
+      if (!named_bar_all(1 + i, 256, good)) { ok = false; break; }
+      const float mx = fmaxf(*xmine, *xother);
+      float alpha = 1.f;   // the reference maximum moves only when the new one is 2^8 larger
+      if (mx > -INFINITY && (m == -INFINITY || mx - m > 8.f)) {
+        alpha = m == -INFINITY ? 0.f : score::exp2_approx(m - mx);
+        m = mx;
+      }
+      l *= alpha;
+      if (__any_sync(0xffffffffu, alpha != 1.f) && j > 1) {
+        uint32_t ro[16];
+#pragma unroll 1
+        for (int c = 4 * sub; c < 4 * sub + 4; ++c) {   // this thread's half of the accumulator columns
+          tmem_ld16(t_o + c * 16, ro);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ro[e] = __float_as_uint(__uint_as_float(ro[e]) * alpha);
+          tmem_st16(t_o + c * 16, ro);
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float p0 = score::exp2_approx(__uint_as_float(r[c * 16 + e]) - ref);
+          const float p1 = score::exp2_approx(__uint_as_float(r[c * 16 + e + 1]) - ref);
+          l += p0 + p1;
+          pk[e >> 1] = pack_bf16x2(p0, p1);
+        }
+        tmem_st8(t_s + sub * 32 + c * 8, pk);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(bar_pfull + 8 * i);
+      // (the exchange slots are rewritten only after this tile's products, which wait for all 256 arrivals above)
+    }
+    if (ok && n > i) ok = mbar_wait_spin(bar_odone + 8 * i, 0, KID, 31);
+  }
+  // ------------------------------ joining the two pipelines ------------------------
+  bool good = !__syncthreads_or(!ok || error_is_set());   // all products done, all tiles consumed: the stages are free
+  float* s_acc = (float*)sKV;      // [128 rows][128 columns] fp32, 16-byte chunks swizzled by row
+  float* s_ml = sX;                // [m1 | l1 of both halves]
+  tc_fence_after();
+  auto chunk_at = [&](int rr, int c) { return s_acc + rr * HD + ((c ^ (rr & 31)) << 2); };   // c: 16-byte chunk 0..31
+  if (good && warp < 16 && i == 1) {
+    uint32_t ro[32];
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      if (n > 1) {
+        tmem_ld32(t_o + sub * 64 + h * 32, ro);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) ro[e] = 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        *reinterpret_cast<uint4*>(chunk_at(row, sub * 16 + h * 8 + e)) = make_uint4(ro[4 * e], ro[4 * e + 1], ro[4 * e + 2], ro[4 * e + 3]);
+    }
+    s_ml[256 + sub * 128 + row] = l;
+    if (sub == 0) s_ml[row] = m;   // (pipeline 0's slots: its own exchange is over)
+  }
+  float m1 = -INFINITY, l1 = 0.f;
+  __syncthreads();
+  if (good && warp < 16 && i == 0) {
+    m1 = s_ml[row];
+    l1 = s_ml[256 + row] + s_ml[384 + row];
+  }
+  __syncthreads();
+  if (good && warp < 16 && i == 0) s_ml[sub * 128 + row] = l;
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f;
+  if (good && warp < 16 && i == 0) {
+    const float l0 = s_ml[row] + s_ml[128 + row];
+    top = fmaxf(m, m1);
+    const float f0 = m == -INFINITY ? 0.f : score::exp2_approx(m - top), f1 = m1 == -INFINITY ? 0.f : score::exp2_approx(m1 - top);
+    sum = f0 * l0 + f1 * l1;
+    const float norm = p.splits == 1 ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
+    const float g0 = f0 * norm, g1 = f1 * norm;
+    uint32_t ro[32];
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      if (n > 0) {
+        tmem_ld32(t_o + sub * 64 + h * 32, ro);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) ro[e] = 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float4* at = reinterpret_cast<float4*>(chunk_at(row, sub * 16 + h * 8 + e));
+        float4 b = *at;
+        b.x = fmaf(g0, __uint_as_float(ro[4 * e]), g1 * b.x);
+        b.y = fmaf(g0, __uint_as_float(ro[4 * e + 1]), g1 * b.y);
+        b.z = fmaf(g0, __uint_as_float(ro[4 * e + 2]), g1 * b.z);
+        b.w = fmaf(g0, __uint_as_float(ro[4 * e + 3]), g1 * b.w);
+        *at = b;
+      }
+    }
+  }
+  __syncthreads();
+  if (good) {
+    // whole rows go out 512 (256) bytes at a time
+    for (int x = tid; x < 128 * (HD / 4); x += THREADS) {
+      const int rr = x / (HD / 4), c = x % (HD / 4), prow = row0 + rr;
+      if (prow >= rows) break;
+      const float4 v = *reinterpret_cast<const float4*>(chunk_at(rr, c));
+      if (p.splits == 1) {
+        const float o4[4] = {v.x, v.y, v.z, v.w};
+        store_row4(p, kvh, G, prow, c * 4, o4);
+      } else {
+        const long long at = ((long long)split * p.nq + prow / G) * p.Hq + kvh * G + prow % G;
+        *reinterpret_cast<float4*>(p.part_o + at * HD + c * 4) = v;
+      }
+    }
+    if (warp < 8 && sub == 0 && row0 + row < rows) {
+      const int prow = row0 + row, qi = prow / G, h = kvh * G + prow % G;
+      if (p.splits == 1)
+        p.lse[(long long)h * p.ld_lse + qi] = sum > 0.f ? top * 0.69314718055994531f + __logf(sum) : -INFINITY;
+      else
+        *reinterpret_cast<float2*>(p.part_ml + (((long long)split * p.nq + qi) * p.Hq + h) * 2) = make_float2(top, sum);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (error_is_set()) {
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 17) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int MOD>
+static cudaError_t launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, cudaStream_t st) {
+  static bool attr_set[64] = {false};   // a function attribute belongs to one device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(few_tiles_kernel<MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  few_tiles_kernel<MOD><<<p.Hkv * p.row_tiles * p.splits, THREADS, SMEM_BYTES, st>>>(tq, tk, tv, p);
+  return cudaGetLastError();
+}
+
+}  // namespace fewt
+
 // One warp per (query row, head): joins the splits.
 __global__ void __launch_bounds__(128) few_rows_join_kernel(const Params p) {
   const int lane = threadIdx.x & 31;
@@ -455,16 +905,22 @@ __global__ void __launch_bounds__(128) few_rows_join_kernel(const Params p) {
 
 struct Plan {
   int wr, row_tiles, splits;
+  bool tiles;   // tcgen05 on 128-row tiles
 };
+constexpr int TILE_ROWS_FROM = 33;   // packed rows
 static Plan plan_of(int nq, int nk, int Hq, int Hkv) {
   Plan pl;
   const int rows = nq * (Hq / Hkv);
   pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
+  pl.tiles = rows >= TILE_ROWS_FROM && 128 % (Hq / Hkv) == 0;
+  if (pl.tiles) pl.wr = 8;
   pl.row_tiles = (rows + 16 * pl.wr - 1) / (16 * pl.wr);
   const int nkt = (nk + BK - 1) / BK;
   int s = tdllm_num_sms() / (Hkv * pl.row_tiles);
   if (s > nkt) s = nkt;
-  pl.splits = s < 1 ? 1 : s;
+  if (s < 1) s = 1;
+  if (pl.tiles && s < (nkt + ROUND - 1) / ROUND) s = (nkt + ROUND - 1) / ROUND;   // one visibility round per CTA
+  pl.splits = s;
   return pl;
 }
 
@@ -540,6 +996,21 @@ extern "C" int tdllm_attn_few_rows(const void* q, const void* k, const void* v, 
   p.mod = score_mod_of(scale, softcap, nullptr, nullptr, nullptr);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
+  if (pl.tiles) {
+    const int G = Hq / Hkv;
+    CUtensorMap tq;
+    const uint64_t dims[3] = {(uint64_t)few::HD, (uint64_t)Hq, (uint64_t)nq};
+    const uint64_t strides[2] = {(uint64_t)few::HD * 2, (uint64_t)ldq * 2};
+    const uint32_t box[3] = {64, (uint32_t)G, (uint32_t)(128 / G)};
+    if (tdllm_host::encode_tmap(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return 3;
+    switch ((softcap > 0.f ? score::CAP : 0) | (slopes ? score::BIAS : 0)) {
+      case 0: e = few::fewt::launch<0>(tq, tk, tv, p, st); break;
+      case score::CAP: e = few::fewt::launch<score::CAP>(tq, tk, tv, p, st); break;
+      case score::BIAS: e = few::fewt::launch<score::BIAS>(tq, tk, tv, p, st); break;
+      default: e = few::fewt::launch<score::CAP | score::BIAS>(tq, tk, tv, p, st); break;
+    }
+  } else
   switch ((softcap > 0.f ? score::CAP : 0) | (slopes ? score::BIAS : 0)) {
     case 0: e = few::launch_wr<0>(pl.wr, tk, tv, p, st); break;
     case score::CAP: e = few::launch_wr<score::CAP>(pl.wr, tk, tv, p, st); break;
