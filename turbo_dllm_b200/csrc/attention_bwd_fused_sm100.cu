@@ -378,34 +378,72 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           tmem_ld16(t_s + 64 + sub * 32 + c * 16, rp);
           tmem_ld_wait();
           if constexpr (MOD != 0) {
-            const bool masked = ent & 1;
             if constexpr ((MOD & score::BIAS) != 0) slope2 = __ldg(p.mod.slope2 + kvh * G + it / n);
+            const int g0 = qrow0 + c * 16;
+            uint32_t hidden = 0u;
+            if (ent & 1) {   // replaced first: a dead row or key may have left NaN in either product
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float pv[2], ds[2];
+              for (int e = 0; e < 16; e += 4) {
+                const int4 lo = __ldg(reinterpret_cast<const int4*>(p.q_lo + g0 + e));
+                const int4 hi = __ldg(reinterpret_cast<const int4*>(p.q_hi + g0 + e));
+                const int4 gr = __ldg(reinterpret_cast<const int4*>(p.q_grp + g0 + e));
+                const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w}, g4[4] = {gr.x, gr.y, gr.z, gr.w};
 #pragma unroll
-              for (int t = 0; t < 2; ++t) {
-                const int g = qrow0 + c * 16 + e + t;
-                float z = __uint_as_float(rs[e + t]), f = 1.f;
-                if constexpr ((MOD & score::CAP) != 0) {
-                  const float r = score::cap_r(z, p.mod);
-                  z = score::cap_z(r, p.mod);
-                  f = score::cap_slope(r);
-                } else {
-                  z *= p.scale_log2;
+                for (int t = 0; t < 4; ++t)
+                  if (!key_visible(kcode, l4[t], h4[t], g4[t])) {
+                    hidden |= 1u << (e + t);
+                    rs[e + t] = 0u;
+                  }
+              }
+            }
+            if constexpr ((MOD & score::CAP) != 0) score::cap_block<16>(rs, p.mod);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const float4 l4 = *reinterpret_cast<const float4*>(sl + c * 16 + e);
+              const float4 d4 = *reinterpret_cast<const float4*>(sd + c * 16 + e);
+              uint64_t z01 = pair_f32(__uint_as_float(rs[e]), __uint_as_float(rs[e + 1]));
+              uint64_t z23 = pair_f32(__uint_as_float(rs[e + 2]), __uint_as_float(rs[e + 3]));
+              uint64_t u01 = fma_f32x2(pair_f32(__uint_as_float(rp[e]), __uint_as_float(rp[e + 1])), score::both(p.scale),
+                                       pair_f32(d4.x, d4.y));
+              uint64_t u23 = fma_f32x2(pair_f32(__uint_as_float(rp[e + 2]), __uint_as_float(rp[e + 3])), score::both(p.scale),
+                                       pair_f32(d4.z, d4.w));
+              if constexpr ((MOD & score::CAP) != 0) {   // dS: times 1 - (z / cap)^2
+                const uint64_t w01 = mul_f32x2(z01, score::both(p.mod.inv_cap2)), w23 = mul_f32x2(z23, score::both(p.mod.inv_cap2));
+                u01 = fma_f32x2(mul_f32x2(u01, w01), mul_f32x2(w01, score::both(-1.f)), u01);
+                u23 = fma_f32x2(mul_f32x2(u23, w23), mul_f32x2(w23, score::both(-1.f)), u23);
+              }
+              if constexpr ((MOD & score::BIAS) != 0) {
+                const float4 qp = __ldg(reinterpret_cast<const float4*>(p.mod.q_pos + g0 + e));
+                if constexpr ((MOD & score::CAP) == 0) {
+                  z01 = mul_f32x2(z01, score::both(p.scale_log2));
+                  z23 = mul_f32x2(z23, score::both(p.scale_log2));
                 }
-                if constexpr ((MOD & score::BIAS) != 0) z = fmaf(-slope2, fabsf(__ldg(p.mod.q_pos + g) - kpos), z);
-                float pr = fast_exp2(z + sl[c * 16 + e + t]);
-                float u = fmaf(__uint_as_float(rp[e + t]), p.scale, sd[c * 16 + e + t]) * (pr * f);
-                if (masked && !key_visible(kcode, __ldg(p.q_lo + g), __ldg(p.q_hi + g), __ldg(p.q_grp + g))) {
-                  pr = 0.f;   // (selected, not multiplied: a dead row or key may have left NaN in either product)
-                  u = 0.f;
-                }
-                pv[t] = pr;
-                ds[t] = u;
+                z01 = score::less_distance(z01, slope2, pair_f32(qp.x, qp.y), score::both(kpos));
+                z23 = score::less_distance(z23, slope2, pair_f32(qp.z, qp.w), score::both(kpos));
+              }
+              if constexpr ((MOD & (score::CAP | score::BIAS)) != 0) {
+                z01 = add_f32x2(z01, pair_f32(l4.x, l4.y));
+                z23 = add_f32x2(z23, pair_f32(l4.z, l4.w));
+              } else {
+                z01 = fma_f32x2(z01, score::both(p.scale_log2), pair_f32(l4.x, l4.y));
+                z23 = fma_f32x2(z23, score::both(p.scale_log2), pair_f32(l4.z, l4.w));
+              }
+              float pv[4], ds[4];
+              unpair_f32(z01, pv[0], pv[1]);
+              unpair_f32(z23, pv[2], pv[3]);
+#pragma unroll
+              for (int t = 0; t < 4; ++t) pv[t] = fast_exp2(pv[t]);
+              unpair_f32(mul_f32x2(pair_f32(pv[0], pv[1]), u01), ds[0], ds[1]);
+              unpair_f32(mul_f32x2(pair_f32(pv[2], pv[3]), u23), ds[2], ds[3]);
+              if (ent & 1) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                  if ((hidden >> (e + t)) & 1u) pv[t] = ds[t] = 0.f;
               }
               pk[c * 8 + (e >> 1)] = pack_bf16x2(pv[0], pv[1]);
+              pk[c * 8 + (e >> 1) + 1] = pack_bf16x2(pv[2], pv[3]);
               dk[c * 8 + (e >> 1)] = pack_bf16x2(ds[0], ds[1]);
+              dk[c * 8 + (e >> 1) + 1] = pack_bf16x2(ds[2], ds[3]);
             }
           } else if (ent & 1) {
 #pragma unroll

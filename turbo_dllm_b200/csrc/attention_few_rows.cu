@@ -262,6 +262,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           }
           float mx[2] = {-INFINITY, -INFINITY};
           uint32_t live[SB * 2];   // bit 0, 1: a row of this warp sees key 2 t4 (+1) of the 8
+          uint32_t seen = 0u;      // this thread's scores: bit 4 n + e
+          uint32_t z[SB * 8];
 #pragma unroll
           for (int n = 0; n < SB * 2; ++n) {
             const int key = b0 * 16 + n * 8 + t4 * 2;
@@ -269,14 +271,23 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             live[n] = 0u;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int x = e >> 1, c = (e & 1) ? c1 : c0;
-              float z = sc[n][e];
-              if constexpr ((MOD & score::CAP) != 0) z = score::cap_z(score::cap_r(z, p.mod), p.mod);
-              else z *= p.scale_log2;
-              if constexpr ((MOD & score::BIAS) != 0) z = fmaf(-slope2[x], fabsf(qpos[x] - kpos[key + (e & 1)]), z);
-              const bool v = visible(c, lo[x], hi[x], grp[x]);
+              const bool v = visible((e & 1) ? c1 : c0, lo[e >> 1], hi[e >> 1], grp[e >> 1]);
               live[n] |= (uint32_t)v << (e & 1);
-              sc[n][e] = v ? z : -INFINITY;
+              seen |= (uint32_t)v << (n * 4 + e);
+              z[n * 4 + e] = v ? __float_as_uint(sc[n][e]) : 0u;
+            }
+          }
+          if constexpr ((MOD & score::CAP) != 0) score::cap_block<SB * 8>(z, p.mod);
+#pragma unroll
+          for (int n = 0; n < SB * 2; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int x = e >> 1;
+              float v = __uint_as_float(z[n * 4 + e]);
+              if constexpr ((MOD & score::CAP) == 0) v *= p.scale_log2;
+              if constexpr ((MOD & score::BIAS) != 0)
+                v = fmaf(-slope2[x], fabsf(qpos[x] - kpos[b0 * 16 + n * 8 + t4 * 2 + (e & 1)]), v);
+              sc[n][e] = ((seen >> (n * 4 + e)) & 1u) ? v : -INFINITY;
               mx[x] = fmaxf(mx[x], sc[n][e]);
             }
           }
@@ -317,14 +328,14 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             uint32_t pf[4], keep[2];
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {   // keys 0-7, 8-15 of the block
-              float* z = sc[b * 2 + hh];
+              float* w = sc[b * 2 + hh];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                z[e] = score::exp2_approx(z[e] - ref[e >> 1]);
-                l[e >> 1] += z[e];
+                w[e] = score::exp2_approx(w[e] - ref[e >> 1]);
+                l[e >> 1] += w[e];
               }
-              pf[hh * 2] = pack_bf16x2(z[0], z[1]);
-              pf[hh * 2 + 1] = pack_bf16x2(z[2], z[3]);
+              pf[hh * 2] = pack_bf16x2(w[0], w[1]);
+              pf[hh * 2 + 1] = pack_bf16x2(w[2], w[3]);
               const uint32_t lv = live[b * 2 + hh];
               keep[hh] = ((lv & 1u) ? 0xffffu : 0u) | ((lv & 2u) ? 0xffff0000u : 0u);
             }
@@ -691,27 +702,31 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           }
           fence_proxy_async_smem();
         }
-#pragma unroll
-        for (int e = 0; e < 64; ++e) {
-          float z = __uint_as_float(r[e]);
-          if constexpr ((MOD & score::CAP) != 0) z = score::cap_z(score::cap_r(z, p.mod), p.mod);
-          else z *= p.scale_log2;
-          if constexpr ((MOD & score::BIAS) != 0) {
-            const int k = min(k0 + e, p.nk - 1);   // (a key past the end is masked)
-            z = fmaf(-slope2, fabsf(qpos - (float)__ldg(p.k_pos + k)), z);
-          }
-          r[e] = __float_as_uint(z);
-        }
+        uint32_t hidden[2] = {0u, 0u};   // masked scores of this thread
         if (masked) {
+          // (a cap makes -inf finite: there masked scores become 0 first and -inf behind the transform)
 #pragma unroll
           for (int e = 0; e < 64; ++e) {
             const int c = k0 + e < p.nk ? __ldg(p.k_code + k0 + e) : score::DEAD_KEY;
-            if (!visible(c, lo, hi, grp)) r[e] = 0xff800000u;   // -inf
+            if (!visible(c, lo, hi, grp)) {
+              r[e] = (MOD & score::CAP) ? 0u : 0xff800000u;
+              hidden[e >> 5] |= 1u << (e & 31);
+            }
           }
+        }
+        score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) {
+          const int k = k0 + e, last = p.nk - 1;   // (a key past the end is masked)
+          return make_float4((float)__ldg(p.k_pos + min(k, last)), (float)__ldg(p.k_pos + min(k + 1, last)),
+                             (float)__ldg(p.k_pos + min(k + 2, last)), (float)__ldg(p.k_pos + min(k + 3, last)));
+        });
+        if ((MOD & score::CAP) && masked) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if ((hidden[e >> 5] >> (e & 31)) & 1u) r[e] = 0xff800000u;
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+        for (int e = 0; e < 64; e += 2) mx = score::max3(mx, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
         *xmine = mx;
       }
       // the barrier also orders the P stores below after the partner's loads of its score columns

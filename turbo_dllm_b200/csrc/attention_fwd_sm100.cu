@@ -310,37 +310,56 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tmem_ld32(t_s + sub * 64, r);
         tmem_ld32(t_s + sub * 64 + 32, r + 32);
         tmem_ld_wait();
-        if constexpr (MOD != 0) {
+        [[maybe_unused]] uint32_t hidden[2] = {0u, 0u};   // MOD: masked scores of this thread
+        if (MOD != 0 && (ent & 1)) {
+          // this thread's key of the tile (and half of its columns): a dead key's V row is zeroed
+          if (__ldg(p.k_code + (ent >> 1) * BKV + row) == score::DEAD_KEY) {
+            if (mbar_wait_spin(bar_vfull + 8 * (j & 1), (j >> 1) & 1, KID, 33)) {
+              uint4* vrow = reinterpret_cast<uint4*>(sV + (j & 1) * TILE_BYTES + sub * HALF_BYTES + row * 128);
 #pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            float z = __uint_as_float(r[e]);
-            if constexpr ((MOD & score::CAP) != 0) z = score::cap_z(score::cap_r(z, p.mod), p.mod);
-            else z *= p.scale_log2;
-            if constexpr ((MOD & score::BIAS) != 0)
-              z = fmaf(-slope2, fabsf(qpos - __ldg(p.mod.k_pos + (ent >> 1) * BKV + sub * 64 + e)), z);
-            r[e] = __float_as_uint(z);
-          }
-          if (ent & 1) {
-            // this thread's key of the tile (and half of its columns): a dead key's V row is zeroed
-            if (__ldg(p.k_code + (ent >> 1) * BKV + row) == score::DEAD_KEY) {
-              if (mbar_wait_spin(bar_vfull + 8 * (j & 1), (j >> 1) & 1, KID, 33)) {
-                uint4* vrow = reinterpret_cast<uint4*>(sV + (j & 1) * TILE_BYTES + sub * HALF_BYTES + row * 128);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
-              }
+              for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
             }
-            fence_proxy_async_smem();
           }
+          fence_proxy_async_smem();
         }
         if (ent & 1) {
           const int lo = __ldg(p.q_lo + grow), hi = __ldg(p.q_hi + grow), grp = __ldg(p.q_grp + grow);
+          if constexpr (MOD == 0) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (!key_visible(__ldg(kc + e), lo, hi, grp)) r[e] = 0xff800000u;  // -inf
+            for (int e = 0; e < 64; ++e)
+              if (!key_visible(__ldg(kc + e), lo, hi, grp)) r[e] = 0xff800000u;  // -inf
+          } else {
+            // (a cap makes -inf finite: there masked scores become 0 first and -inf behind the transform)
+#pragma unroll
+            for (int e = 0; e < 64; e += 4) {
+              const int4 c4 = __ldg(reinterpret_cast<const int4*>(kc + e));
+              const int code[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+              for (int t = 0; t < 4; ++t)
+                if (!key_visible(code[t], lo, hi, grp)) {
+                  r[e + t] = (MOD & score::CAP) ? 0u : 0xff800000u;
+                  hidden[e >> 5] |= 1u << ((e + t) & 31);
+                }
+            }
+          }
+        }
+        if constexpr (MOD != 0) {
+          const float4* kp = reinterpret_cast<const float4*>(p.mod.k_pos + (ent >> 1) * BKV + sub * 64);
+          score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) { return __ldg(kp + e / 4); });
+          if ((MOD & score::CAP) && (ent & 1)) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if ((hidden[e >> 5] >> (e & 31)) & 1u) r[e] = 0xff800000u;
+          }
         }
         float mx = -INFINITY;
+        if constexpr (MOD != 0) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+          for (int e = 0; e < 64; e += 2) mx = score::max3(mx, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+        }
         *xmine = mx;
       }
       // the barrier also orders the P stores below after the partner's loads of its score columns

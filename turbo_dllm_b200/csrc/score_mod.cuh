@@ -6,9 +6,19 @@
 //
 // all in log2 units (z * log2 e), so that a probability is one exp2 of a difference.
 //
-// tanh(x) = 1 - 2 r with r = 1 / (1 + e^(2x)): no cancellation that matters here, since what counts is the absolute
-// error of z (a relative error of the probability): 2^-23 of `cap` at most, also where tanh saturates (e = inf gives
-// r = 0, e = 0 gives r = 1). The derivative of the capped score, 1 - tanh^2, is 4 r (1 - r).
+// What counts is the absolute error of z, which is a relative error of the probability; both forms below keep it under
+// 2^-22 of the cap. The derivative of the capped score is 1 - tanh^2 = 1 - (z / cap)^2.
+//
+//   |x| <= 3/4:  tanh(x) = x Q(x^2), Q of degree 5 with the least largest error there (1e-8; 8e-8 as evaluated): four
+//                fp32 operations a score, two scores to an instruction, and no special-function operation
+//   beyond:      tanh(x) = 1 - 2 r with r = 1 / (1 + 2^y), y = 2 x log2 e clamped to +-60 (r is 0 or 1 to 32 bits there):
+//                2^y = 2^n p(y - n) on the fp32 pipes, n the nearest integer, p of degree 5 with the least largest
+//                relative error on [-1/2, 1/2] (7.5e-8), and two scores share one reciprocal, 1/d0 = d1 / (d0 d1)
+//
+// A warp takes the first form for a whole tile row when all of its scores allow it (a cap of 50 leaves scores up to 37),
+// else the second. With the special-function unit alone (exp2, reciprocal, and the softmax's exp2, at 16 a clock and SM)
+// a 128 x 128 tile takes 3072 clocks, three times its two products. NaN passes through both forms; in the second, what
+// one score of a pair holds reaches the other, so masked scores are replaced BEFORE the pair is formed.
 //
 // MOD & SAFE is set for every transformed kernel: query rows that see no key and keys that no row sees may hold
 // anything (infinities and NaN of uninitialised padding): their rows of an operand tile are overwritten with zeros in
@@ -23,8 +33,12 @@ constexpr int CAP = 1, BIAS = 2, SAFE = 4;
 constexpr int DEAD_KEY = -2147483647 - 1;   // code of a key that no row sees (also of padding behind the last key)
 
 struct Mod {
+  float in1;            // scale / cap
   float in2;            // 2 log2(e) scale / cap
   float cap2;           // cap log2(e)
+  float inv_cap2;       // 1 / cap2
+  float near;           // 3/4 cap / scale: raw products up to here take the polynomial
+  float poly[6];        // cap2 Q
   const float* slope2;  // [Hq] slope_h log2(e)
   const float* q_pos;   // [nq_pad] positions as floats (exact: |position| < 2^24)
   const float* k_pos;   // [nk_pad]
@@ -40,10 +54,106 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// r of tanh = 1 - 2 r for a raw product s
-__device__ __forceinline__ float cap_r(float s, const Mod& m) { return rcp_approx(1.f + exp2_approx(s * m.in2)); }
-__device__ __forceinline__ float cap_z(float r, const Mod& m) { return fmaf(-2.f * m.cap2, r, m.cap2); }
-__device__ __forceinline__ float cap_slope(float r) { return 4.f * r * (1.f - r); }
+__device__ __forceinline__ float clamp60(float y) {   // NaN stays NaN
+  float r;
+  asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, 0fC2700000;\n\tmin.NaN.f32 %0, t, 0f42700000;\n\t}" : "=f"(r) : "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float v) { return pair_f32(v, v); }
+
+// r of tanh = 1 - 2 r for two raw products
+__device__ __forceinline__ void cap_r2(float s0, float s1, const Mod& m, float& r0, float& r1) {
+  float y0, y1;
+  unpair_f32(mul_f32x2(pair_f32(s0, s1), both(m.in2)), y0, y1);
+  const uint64_t y = pair_f32(clamp60(y0), clamp60(y1));
+  const uint64_t t = add_f32x2(y, both(12582912.f));              // 1.5 * 2^23: the low bits hold the integer
+  const uint64_t f = fma_f32x2(add_f32x2(t, both(-12582912.f)), both(-1.f), y);
+  uint64_t e = fma_f32x2(f, both(0.0013276409590616822f), both(0.009675540961325169f));
+  e = fma_f32x2(e, f, both(0.05550713464617729f));
+  e = fma_f32x2(e, f, both(0.24022120237350464f));
+  e = fma_f32x2(e, f, both(0.6931469440460205f));
+  e = fma_f32x2(e, f, both(1.0000001192092896f));
+  float t0, t1, d0, d1;
+  unpair_f32(t, t0, t1);
+  const uint64_t p2 = pair_f32(__int_as_float((__float_as_int(t0) << 23) + 0x3f800000),
+                               __int_as_float((__float_as_int(t1) << 23) + 0x3f800000));
+  unpair_f32(fma_f32x2(e, p2, both(1.f)), d0, d1);
+  const float inv = rcp_approx(d0 * d1);
+  unpair_f32(mul_f32x2(pair_f32(d1, d0), both(inv)), r0, r1);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// N raw products of one thread -> capped scores in log2 units, in place. All lanes of the warp take part.
+template <int N>
+__device__ __forceinline__ void cap_block(uint32_t* s, const Mod& m) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; e += 2) top = max3(top, fabsf(__uint_as_float(s[e])), fabsf(__uint_as_float(s[e + 1])));
+  if (!__any_sync(0xffffffffu, top > m.near)) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const uint64_t x = mul_f32x2(pair_f32(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), both(m.in1));
+      const uint64_t u = mul_f32x2(x, x);
+      uint64_t q = fma_f32x2(u, both(m.poly[5]), both(m.poly[4]));
+      q = fma_f32x2(q, u, both(m.poly[3]));
+      q = fma_f32x2(q, u, both(m.poly[2]));
+      q = fma_f32x2(q, u, both(m.poly[1]));
+      q = fma_f32x2(q, u, both(m.poly[0]));
+      float z0, z1;
+      unpair_f32(mul_f32x2(q, x), z0, z1);
+      s[e] = __float_as_uint(z0);
+      s[e + 1] = __float_as_uint(z1);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      float r0, r1, z0, z1;
+      cap_r2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]), m, r0, r1);
+      unpair_f32(fma_f32x2(pair_f32(r0, r1), both(-2.f * m.cap2), both(m.cap2)), z0, z1);
+      s[e] = __float_as_uint(z0);
+      s[e + 1] = __float_as_uint(z1);
+    }
+  }
+}
+
+// two scores of one head less slope * distance
+__device__ __forceinline__ uint64_t less_distance(uint64_t z, float slope2, uint64_t qp, uint64_t kp) {
+  float d0, d1;
+  unpair_f32(fma_f32x2(kp, both(-1.f), qp), d0, d1);
+  return fma_f32x2(pair_f32(fabsf(d0), fabsf(d1)), both(-slope2), z);
+}
+
+// N raw products of one query row against consecutive keys -> transformed scores in log2 units. kp(e): positions of keys
+// e .. e + 3.
+template <int MOD, int N, class KeyPos>
+__device__ __forceinline__ void transform_row(uint32_t* s, const Mod& m, float scale_log2, float slope2, float qpos, KeyPos kp) {
+  if constexpr ((MOD & CAP) != 0) cap_block<N>(s, m);
+#pragma unroll
+  for (int e = 0; e < N; e += 4) {
+    uint64_t z0 = pair_f32(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+    uint64_t z1 = pair_f32(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+    if constexpr ((MOD & CAP) == 0) {
+      z0 = mul_f32x2(z0, both(scale_log2));
+      z1 = mul_f32x2(z1, both(scale_log2));
+    }
+    if constexpr ((MOD & BIAS) != 0) {
+      const float4 k = kp(e);
+      z0 = less_distance(z0, slope2, both(qpos), pair_f32(k.x, k.y));
+      z1 = less_distance(z1, slope2, both(qpos), pair_f32(k.z, k.w));
+    }
+    float a, b, c, d;
+    unpair_f32(z0, a, b);
+    unpair_f32(z1, c, d);
+    s[e] = __float_as_uint(a);
+    s[e + 1] = __float_as_uint(b);
+    s[e + 2] = __float_as_uint(c);
+    s[e + 3] = __float_as_uint(d);
+  }
+}
 
 }  // namespace score
 }  // namespace tdllm
@@ -52,8 +162,15 @@ static inline tdllm::score::Mod score_mod_of(float scale, float softcap, const f
                                              const float* k_pos) {
   const float log2e = 1.4426950408889634f;
   tdllm::score::Mod m;
-  m.in2 = softcap > 0.f ? 2.f * log2e * scale / softcap : 0.f;
+  static const float q[6] = {0.9999998211860657f, -0.33332470059394836f, 0.13320580124855042f,
+                             -0.053149253129959106f, 0.01923721842467785f, -0.004493444226682186f};
+  const bool cap = softcap > 0.f;
+  m.in1 = cap ? scale / softcap : 0.f;
+  m.in2 = 2.f * log2e * m.in1;
   m.cap2 = softcap * log2e;
+  m.inv_cap2 = cap ? 1.f / m.cap2 : 0.f;
+  m.near = cap ? 0.75f * softcap / fabsf(scale) : 0.f;
+  for (int i = 0; i < 6; ++i) m.poly[i] = m.cap2 * q[i];
   m.slope2 = slope2;
   m.q_pos = q_pos;
   m.k_pos = k_pos;
