@@ -72,7 +72,8 @@ constexpr int OFF_RED = OFF_DS + 2 * DS_BYTES;
 constexpr int OFF_BARS = OFF_RED + 4 * RED_BYTES;
 constexpr int OFF_STAT = OFF_BARS + 512;      // [stage][lse2 64 | delta_s 64] fp32
 // no alignment slack: the kernel checks that its dynamic shared memory starts 1 KiB aligned
-constexpr int SMEM_BYTES = OFF_STAT + STAGES * 128 * 4;
+constexpr int OFF_QPOS = OFF_STAT + STAGES * 128 * 4;   // transformed scores with a distance bias: [stage][64] positions
+constexpr int SMEM_BYTES = OFF_QPOS + STAGES * 64 * 4;
 static_assert(SMEM_BYTES <= 232448, "shared memory budget of one CTA");
 static_assert(OFF_Q + 2 * 65536 <= OFF_RED, "dK/dV staging must not reach the dQ staging rows");
 
@@ -216,7 +217,9 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         const int h = kvh * G + it / n;
         const int qrow = (list[it % n] >> 1) * 128 + b * 64;
         if (!mbar_wait_spin(bar_qempty + 8 * st, ph ^ 1, KID, 10)) break;
-        mbar_expect_tx(bar_qfull + 8 * st, 2 * QS_BYTES + 512);
+        mbar_expect_tx(bar_qfull + 8 * st, 2 * QS_BYTES + 512 + ((MOD & score::BIAS) ? 256 : 0));
+        if constexpr ((MOD & score::BIAS) != 0)
+          bulk_load_1d(smem_u32(smem + OFF_QPOS + st * 256), p.mod.q_pos + qrow, 256, bar_qfull + 8 * st);
         bulk_load_1d(smem_u32(sStat + st * 128), p.lse2 + (size_t)h * p.nq_pad + qrow, 256,
                      bar_qfull + 8 * st);
         bulk_load_1d(smem_u32(sStat + st * 128 + 64), p.delta + (size_t)h * p.nq_pad + qrow, 256,
@@ -413,7 +416,7 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 u23 = fma_f32x2(mul_f32x2(u23, w23), mul_f32x2(w23, score::both(-1.f)), u23);
               }
               if constexpr ((MOD & score::BIAS) != 0) {
-                const float4 qp = __ldg(reinterpret_cast<const float4*>(p.mod.q_pos + g0 + e));
+                const float4 qp = *reinterpret_cast<const float4*>(smem + OFF_QPOS + st * 256 + (sub * 32 + c * 16 + e) * 4);
                 if constexpr ((MOD & score::CAP) == 0) {
                   z01 = mul_f32x2(z01, score::both(p.scale_log2));
                   z23 = mul_f32x2(z23, score::both(p.scale_log2));

@@ -684,6 +684,15 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       if ((j & 1) != i) continue;
       const int k0 = (split + o * p.splits) * BK + sub * 64;
       const bool masked = !((s_full[o >> 5] >> (o & 31)) & 1u);
+      // codes and positions of the 64 keys: two per lane, loaded while the scores are on their way, passed by shuffles
+      int code[2] = {0, 0};
+      [[maybe_unused]] float kpos[2] = {0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int k = k0 + x * 32 + lane;
+        if (masked) code[x] = k < p.nk ? __ldg(p.k_code + k) : score::DEAD_KEY;
+        if constexpr ((MOD & score::BIAS) != 0) kpos[x] = k < p.nk ? (float)__ldg(p.k_pos + k) : 0.f;
+      }
       bool good = __all_sync(0xffffffffu, mbar_wait_spin(bar_sfull + 8 * i, (j >> 1) & 1, KID, 30));
       if (good) {
         tc_fence_after();
@@ -707,17 +716,16 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           // (a cap makes -inf finite: there masked scores become 0 first and -inf behind the transform)
 #pragma unroll
           for (int e = 0; e < 64; ++e) {
-            const int c = k0 + e < p.nk ? __ldg(p.k_code + k0 + e) : score::DEAD_KEY;
-            if (!visible(c, lo, hi, grp)) {
+            if (!visible(__shfl_sync(0xffffffffu, code[e >> 5], e & 31), lo, hi, grp)) {
               r[e] = (MOD & score::CAP) ? 0u : 0xff800000u;
               hidden[e >> 5] |= 1u << (e & 31);
             }
           }
         }
         score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) {
-          const int k = k0 + e, last = p.nk - 1;   // (a key past the end is masked)
-          return make_float4((float)__ldg(p.k_pos + min(k, last)), (float)__ldg(p.k_pos + min(k + 1, last)),
-                             (float)__ldg(p.k_pos + min(k + 2, last)), (float)__ldg(p.k_pos + min(k + 3, last)));
+          const float kp = kpos[e >> 5];
+          return make_float4(__shfl_sync(0xffffffffu, kp, e & 31), __shfl_sync(0xffffffffu, kp, (e + 1) & 31),
+                             __shfl_sync(0xffffffffu, kp, (e + 2) & 31), __shfl_sync(0xffffffffu, kp, (e + 3) & 31));
         });
         if ((MOD & score::CAP) && masked) {
 #pragma unroll

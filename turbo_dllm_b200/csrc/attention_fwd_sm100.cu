@@ -59,6 +59,8 @@ using peer::MAX_PEERS;
 using peer::PULL_ROWS;
 using peer::PullPlan;
 constexpr int SMEM_BYTES = 2 * TILE_BYTES + 2 * KV_STAGES * TILE_BYTES + 512 + 2048 + 1024;   // + barriers + row exchange
+constexpr int META_SLOTS = 4;       // transformed scores: the codes and positions of four tiles' keys, 1 KiB each
+constexpr int SMEM_BYTES_MOD = SMEM_BYTES + META_SLOTS * 1024;
 
 struct FwdParams {
   int nq_pad;          // query rows padded to a multiple of 128
@@ -126,6 +128,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const uint32_t bar_epi = b0 + 120;         // [2] output staged in shared memory
   uint32_t* tmem_slot = (uint32_t*)(bars + 17);
   float* sX = (float*)((uint8_t*)bars + 512);   // [head][column half][128 rows]: row maxima, then row sums
+  // MOD: codes and positions of a tile's keys come into shared memory with its K tile. Slot j & 3 of tile j is free for
+  // tile j + 4: K of that tile waits for the scores of tile j + 2, whose products follow both heads' softmax of tile j.
+  uint8_t* sMeta = (uint8_t*)bars + 512 + 2048;
+  const uint32_t bar_meta = b0 + 144;           // [4]
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -155,6 +161,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_init(bar_pfull + 8 * s, 256);
       mbar_init(bar_odone + 8 * s, 1);
       mbar_init(bar_epi + 8 * s, 256);
+    }
+    if constexpr (MOD != 0) {
+      for (int s = 0; s < META_SLOTS; ++s) mbar_init(bar_meta + 8 * s, 1);
     }
     fence_mbar_init();
   }
@@ -205,6 +214,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         for (int c = 0; c < 2; ++c)
           tma_load_2d(smem_u32(sK + s * TILE_BYTES + c * HALF_BYTES), mk, bar_kfull + 8 * s,
                       kvh * HD + c * 64, kt * BKV);
+        if constexpr (MOD != 0) {
+          const uint32_t bm = bar_meta + 8 * (j % META_SLOTS), dst = smem_u32(sMeta + (j % META_SLOTS) * 1024);
+          mbar_expect_tx(bm, (MOD & score::BIAS) ? 1024 : 512);
+          bulk_load_1d(dst, p.k_code + kt * BKV, 512, bm);
+          if constexpr ((MOD & score::BIAS) != 0) bulk_load_1d(dst + 512, p.mod.k_pos + kt * BKV, 512, bm);
+        }
         if (!mbar_wait_spin(bar_vempty + 8 * s, ph ^ 1, KID, 11)) break;
         mbar_expect_tx(bar_vfull + 8 * s, TILE_BYTES);
 #pragma unroll
@@ -303,8 +318,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       const int ent = list[j];
-      const int* kc = p.k_code + (ent >> 1) * BKV + sub * 64;
+      const int* kc = MOD ? (const int*)(sMeta + (j % META_SLOTS) * 1024) + sub * 64
+                          : p.k_code + (ent >> 1) * BKV + sub * 64;
       bool good = __all_sync(0xffffffffu, mbar_wait_spin(bar_sfull + 8 * i, j & 1, KID, 30));
+      if constexpr (MOD != 0) {
+        if ((ent & 1) || (MOD & score::BIAS))
+          good = __all_sync(0xffffffffu, good && mbar_wait_spin(bar_meta + 8 * (j % META_SLOTS), (j / META_SLOTS) & 1, KID, 34));
+      }
       if (good) {
         tc_fence_after();
         tmem_ld32(t_s + sub * 64, r);
@@ -313,7 +333,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         [[maybe_unused]] uint32_t hidden[2] = {0u, 0u};   // MOD: masked scores of this thread
         if (MOD != 0 && (ent & 1)) {
           // this thread's key of the tile (and half of its columns): a dead key's V row is zeroed
-          if (__ldg(p.k_code + (ent >> 1) * BKV + row) == score::DEAD_KEY) {
+          if ((kc - sub * 64)[row] == score::DEAD_KEY) {
             if (mbar_wait_spin(bar_vfull + 8 * (j & 1), (j >> 1) & 1, KID, 33)) {
               uint4* vrow = reinterpret_cast<uint4*>(sV + (j & 1) * TILE_BYTES + sub * HALF_BYTES + row * 128);
 #pragma unroll
@@ -332,7 +352,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             // (a cap makes -inf finite: there masked scores become 0 first and -inf behind the transform)
 #pragma unroll
             for (int e = 0; e < 64; e += 4) {
-              const int4 c4 = __ldg(reinterpret_cast<const int4*>(kc + e));
+              const int4 c4 = *reinterpret_cast<const int4*>(kc + e);
               const int code[4] = {c4.x, c4.y, c4.z, c4.w};
 #pragma unroll
               for (int t = 0; t < 4; ++t)
@@ -344,8 +364,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         }
         if constexpr (MOD != 0) {
-          const float4* kp = reinterpret_cast<const float4*>(p.mod.k_pos + (ent >> 1) * BKV + sub * 64);
-          score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) { return __ldg(kp + e / 4); });
+          const float4* kp = reinterpret_cast<const float4*>(kc + 128);
+          score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) { return kp[e / 4]; });
           if ((MOD & score::CAP) && (ent & 1)) {
 #pragma unroll
             for (int e = 0; e < 64; ++e)
@@ -509,7 +529,7 @@ static int attn_fwd_launch(const char* who, const void* q, const void* k, const 
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
     cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<false, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         SMEM_BYTES);
+                                         MOD ? SMEM_BYTES_MOD : SMEM_BYTES);
     if (e != cudaSuccess) {
       tdllm_host::set_last_error("%s: cudaFuncSetAttribute: %s", who, cudaGetErrorString(e));
       return 2;
@@ -533,7 +553,7 @@ static int attn_fwd_launch(const char* who, const void* q, const void* k, const 
   PullPlan pl;
   memset(&pl, 0, sizeof(pl));
   const int grid = n_qtiles * Hkv * ((Hq / Hkv + 1) / 2);
-  attn_fwd_kernel<false, MOD><<<grid, THREADS, SMEM_BYTES, stream>>>(tq, tk, tv, to, tk, tv, p, pl);
+  attn_fwd_kernel<false, MOD><<<grid, THREADS, MOD ? SMEM_BYTES_MOD : SMEM_BYTES, stream>>>(tq, tk, tv, to, tk, tv, p, pl);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     tdllm_host::set_last_error("%s launch: %s", who, cudaGetErrorString(e));
