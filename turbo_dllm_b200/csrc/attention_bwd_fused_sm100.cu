@@ -383,22 +383,6 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           if constexpr (MOD != 0) {
             if constexpr ((MOD & score::BIAS) != 0) slope2 = __ldg(p.mod.slope2 + kvh * G + it / n);
             const int g0 = qrow0 + c * 16;
-            uint32_t hidden = 0u;
-            if (ent & 1) {   // replaced first: a dead row or key may have left NaN in either product
-#pragma unroll
-              for (int e = 0; e < 16; e += 4) {
-                const int4 lo = __ldg(reinterpret_cast<const int4*>(p.q_lo + g0 + e));
-                const int4 hi = __ldg(reinterpret_cast<const int4*>(p.q_hi + g0 + e));
-                const int4 gr = __ldg(reinterpret_cast<const int4*>(p.q_grp + g0 + e));
-                const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w}, g4[4] = {gr.x, gr.y, gr.z, gr.w};
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                  if (!key_visible(kcode, l4[t], h4[t], g4[t])) {
-                    hidden |= 1u << (e + t);
-                    rs[e + t] = 0u;
-                  }
-              }
-            }
             if constexpr ((MOD & score::CAP) != 0) score::cap_block<16>(rs, p.mod);
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
@@ -438,10 +422,14 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
               for (int t = 0; t < 4; ++t) pv[t] = fast_exp2(pv[t]);
               unpair_f32(mul_f32x2(pair_f32(pv[0], pv[1]), u01), ds[0], ds[1]);
               unpair_f32(mul_f32x2(pair_f32(pv[2], pv[3]), u23), ds[2], ds[3]);
-              if (ent & 1) {
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                  if ((hidden >> (e + t)) & 1u) pv[t] = ds[t] = 0.f;
+              if (ent & 1) {   // (selected, not multiplied: a dead row or key may have left NaN in either product)
+                const int4 lo = __ldg(reinterpret_cast<const int4*>(p.q_lo + g0 + e));
+                const int4 hi = __ldg(reinterpret_cast<const int4*>(p.q_hi + g0 + e));
+                const int4 gr = __ldg(reinterpret_cast<const int4*>(p.q_grp + g0 + e));
+                if (!score::RowMask(lo.x, hi.x, gr.x).sees(kcode)) pv[0] = ds[0] = 0.f;
+                if (!score::RowMask(lo.y, hi.y, gr.y).sees(kcode)) pv[1] = ds[1] = 0.f;
+                if (!score::RowMask(lo.z, hi.z, gr.z).sees(kcode)) pv[2] = ds[2] = 0.f;
+                if (!score::RowMask(lo.w, hi.w, gr.w).sees(kcode)) pv[3] = ds[3] = 0.f;
               }
               pk[c * 8 + (e >> 1)] = pack_bf16x2(pv[0], pv[1]);
               pk[c * 8 + (e >> 1) + 1] = pack_bf16x2(pv[2], pv[3]);

@@ -78,6 +78,42 @@ __device__ __forceinline__ bool visible(int code, int lo, int hi, int grp) {
   return code >= 0 ? (code >= lo && code < hi) : (code == grp);
 }
 
+// The codes of a tile's keys, four per lane (e * 32 + lane); what lies behind the last key is dead.
+struct Codes {
+  int c[4];
+  __device__ __forceinline__ void load(const Params& p, int k0, int lane) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = k0 + e * 32 + lane;
+      c[e] = k < p.nk ? __ldg(p.k_code + k) : score::DEAD_KEY;
+    }
+  }
+};
+// Bounds over a CTA's rows, in shared memory: lo_min, hi_max (rows with a clean interval), grp_min, grp_max (noisy
+// rows), and over all rows lo_max, hi_min.
+struct Bounds {
+  int v[6];
+  __device__ __forceinline__ void clear() {
+    v[0] = 2147483647; v[1] = -1; v[2] = 0; v[3] = score::DEAD_KEY; v[4] = -2147483647 - 1; v[5] = 2147483647;
+  }
+  __device__ __forceinline__ void add(int lo, int hi, int grp) {
+    if (lo < hi) {
+      atomicMin(v, lo);
+      atomicMax(v + 1, hi);
+    }
+    if (grp < 0) {
+      atomicMin(v + 2, grp);
+      atomicMax(v + 3, grp);
+    }
+    atomicMax(v + 4, lo);
+    atomicMin(v + 5, hi);
+  }
+  __device__ __forceinline__ bool may_see(int c) const {
+    return c >= 0 ? (c >= v[0] && c < v[1]) : (c >= v[2] && c <= v[3] && c != score::DEAD_KEY);
+  }
+  __device__ __forceinline__ bool all_see(int c) const { return c >= 0 && c >= v[4] && c < v[5]; }
+};
+
 // writes one finished row value range: 4 values of row r (packed index) starting at column c
 __device__ __forceinline__ void store_row4(const Params& p, int kvh, int G, int r, int c, const float* v) {
   const int i = r / G, h = kvh * G + r % G;
@@ -98,7 +134,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   float* s_kpos = (float*)(smem + OFF_KPOS);
   float* s_ml = (float*)(smem + OFF_ML);
   uint32_t* s_bits = (uint32_t*)(smem + OFF_BITS);
-  int* s_bound = (int*)(s_bits + ROUND / 32);   // lo_min, hi_max, grp_min, grp_max
+  Bounds* s_bound = (Bounds*)(s_bits + ROUND / 32);
   const uint32_t bar_full = smem_u32(smem + OFF_BARS), bar_empty = bar_full + 8 * STAGES;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -109,33 +145,29 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   const int rows = p.nq * G;             // packed rows of a KV head
   const int row0 = rt * 16 * WR;
   const int nkt = (p.nk + BK - 1) / BK;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int own = split < nkt ? (nkt - split + p.splits - 1) / p.splits : 0;
 
+  // on their way while the barriers are set up: the codes of this warp's first tile and this thread's row's mask
+  Codes first;
+  if (warp < own) first.load(p, (split + warp * p.splits) * BK, lane);
+  const int i1 = min((row0 + 16 * WR - 1) / G, p.nq - 1), i_mine = row0 / G + tid;   // at most 128 query rows
+  int mask_of[3] = {0, 0, 0};
+  if (i_mine <= i1) {
+    mask_of[0] = p.q_lo[i_mine];
+    mask_of[1] = p.q_hi[i_mine];
+    mask_of[2] = p.q_grp[i_mine];
+  }
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 33);
       mbar_init(bar_empty + 8 * s, 8);
     }
     fence_mbar_init();
-    s_bound[0] = 2147483647; s_bound[1] = -1; s_bound[2] = 0; s_bound[3] = score::DEAD_KEY;
+    s_bound->clear();
   }
   __syncthreads();
-  {   // bounds of the rows' masks
-    const int i0 = row0 / G, i1 = min((row0 + 16 * WR - 1) / G, p.nq - 1);
-    for (int i = i0 + tid; i <= i1; i += THREADS) {
-      const int lo = p.q_lo[i], hi = p.q_hi[i], grp = p.q_grp[i];
-      if (lo < hi) {
-        atomicMin(s_bound, lo);
-        atomicMax(s_bound + 1, hi);
-      }
-      if (grp < 0) {
-        atomicMin(s_bound + 2, grp);
-        atomicMax(s_bound + 3, grp);
-      }
-    }
-  }
-  __syncthreads();
-  const int lo_min = s_bound[0], hi_max = s_bound[1], g_min = s_bound[2], g_max = s_bound[3];
+  if (i_mine <= i1) s_bound->add(mask_of[0], mask_of[1], mask_of[2]);
 
   // compute warps: rows and their metadata
   const int wr = warp % WR, kw = warp / WR;
@@ -178,18 +210,14 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   bool ok = true;
   for (int base = 0; base < own; base += ROUND) {
     const int cnt = min(ROUND, own - base);
-    __syncthreads();   // the previous round's bits have been read
+    __syncthreads();   // the previous round's bits have been read; the bounds are complete
     for (int i = tid; i < ROUND / 32; i += THREADS) s_bits[i] = 0u;
     __syncthreads();
+    const Bounds bounds = *s_bound;
     for (int o = warp; o < cnt; o += THREADS / 32) {
-      const int k0 = (split + (base + o) * p.splits) * BK;
-      bool any = false;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = k0 + e * 32 + lane;
-        const int c = k < p.nk ? __ldg(p.k_code + k) : score::DEAD_KEY;
-        any |= c >= 0 ? (c >= lo_min && c < hi_max) : (c >= g_min && c <= g_max && c != score::DEAD_KEY);
-      }
+      if (base + o != warp) first.load(p, (split + (base + o) * p.splits) * BK, lane);
+      const bool any = bounds.may_see(first.c[0]) || bounds.may_see(first.c[1]) || bounds.may_see(first.c[2]) ||
+                       bounds.may_see(first.c[3]);
       if (__any_sync(0xffffffffu, any) && lane == 0) atomicOr(s_bits + (o >> 5), 1u << (o & 31));
     }
     __syncthreads();
@@ -498,7 +526,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   float* sX = (float*)(smem + OFF_X);
   uint32_t* s_vis = (uint32_t*)(smem + OFF_BITS);
   uint32_t* s_full = s_vis + ROUND / 32;
-  int* s_bound = (int*)(smem + OFF_BOUND);   // lo_min, hi_max, grp_min, grp_max, lo_max, hi_min
+  Bounds* s_bound = (Bounds*)(smem + OFF_BOUND);
   const uint32_t b0 = smem_u32(smem + OFF_BARS);
   const uint32_t bar_q = b0, bar_kfull = b0 + 8, bar_vfull = b0 + 32, bar_empty = b0 + 56;   // [3] each
   const uint32_t bar_sfull = b0 + 80, bar_pfull = b0 + 96, bar_odone = b0 + 112;             // [2] each
@@ -512,8 +540,19 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const int rows = p.nq * G;
   const int row0 = rt * 128;
   const int nkt = (p.nk + BK - 1) / BK;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int own = split < nkt ? (nkt - split + p.splits - 1) / p.splits : 0;   // at most ROUND (host)
 
+  // on their way while the barriers are set up: the codes of this warp's first tile and this thread's row's mask
+  Codes first;
+  if (warp < own) first.load(p, (split + warp * p.splits) * BK, lane);
+  const int i1 = min((row0 + 127) / G, p.nq - 1), i_mine = row0 / G + tid;   // at most 128 query rows
+  int mask_of[3] = {0, 0, 0};
+  if (i_mine <= i1) {
+    mask_of[0] = p.q_lo[i_mine];
+    mask_of[1] = p.q_hi[i_mine];
+    mask_of[2] = p.q_grp[i_mine];
+  }
   if (tid == 0) {
     mbar_init(bar_q, 1);
     for (int s = 0; s < STAGES; ++s) {
@@ -527,8 +566,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_init(bar_odone + 8 * s, 1);
     }
     fence_mbar_init();
-    s_bound[0] = 2147483647; s_bound[1] = -1; s_bound[2] = 0; s_bound[3] = score::DEAD_KEY;
-    s_bound[4] = -2147483647 - 1; s_bound[5] = 2147483647;
+    s_bound->clear();
   }
   if (warp == 17) {
     tmem_alloc(smem_u32(tmem_slot), 512);
@@ -539,35 +577,22 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  {   // bounds of the rows' masks
-    const int i0 = row0 / G, i1 = min((row0 + 127) / G, p.nq - 1);
-    for (int i = i0 + tid; i <= i1; i += THREADS) {
-      const int lo = p.q_lo[i], hi = p.q_hi[i], grp = p.q_grp[i];
-      if (lo < hi) {
-        atomicMin(s_bound, lo);
-        atomicMax(s_bound + 1, hi);
-      }
-      if (grp < 0) {
-        atomicMin(s_bound + 2, grp);
-        atomicMax(s_bound + 3, grp);
-      }
-      atomicMax(s_bound + 4, lo);
-      atomicMin(s_bound + 5, hi);
-    }
+  if (i_mine <= i1) s_bound->add(mask_of[0], mask_of[1], mask_of[2]);
+  if (warp == 16 && lane == 0) {   // Q is needed in any case (if no tile is visible, it still has to land before the end)
+    mbar_expect_tx(bar_q, TILE_BYTES);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) tma_load_3d(smem_u32(sQ + c * HALF_BYTES), &tm_q, bar_q, c * 64, kvh * G, row0 / G);
   }
   __syncthreads();
-  const int lo_min = s_bound[0], hi_max = s_bound[1], g_min = s_bound[2], g_max = s_bound[3];
   {
-    const int lo_max = s_bound[4], hi_min = s_bound[5];
+    const Bounds bounds = *s_bound;
     for (int o = warp; o < own; o += THREADS / 32) {
-      const int k0 = (split + o * p.splits) * BK;
+      if (o != warp) first.load(p, (split + o * p.splits) * BK, lane);
       bool any = false, all = true;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int k = k0 + e * 32 + lane;
-        const int c = k < p.nk ? __ldg(p.k_code + k) : score::DEAD_KEY;
-        any |= c >= 0 ? (c >= lo_min && c < hi_max) : (c >= g_min && c <= g_max && c != score::DEAD_KEY);
-        all &= c >= 0 && c >= lo_max && c < hi_min;
+        any |= bounds.may_see(first.c[e]);
+        all &= bounds.all_see(first.c[e]);
       }
       any = __any_sync(0xffffffffu, any);
       all = __all_sync(0xffffffffu, all);
@@ -581,10 +606,8 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 
   if (warp == 16) {
     // ------------------------------ TMA producer ------------------------------
+    if (lane == 0 && n == 0) mbar_wait(bar_q, 0, KID, 11);
     if (lane == 0 && n > 0) {
-      mbar_expect_tx(bar_q, TILE_BYTES);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tma_load_3d(smem_u32(sQ + c * HALF_BYTES), &tm_q, bar_q, c * 64, kvh * G, row0 / G);
       Walk walk(s_vis);
       for (int j = 0; j < n; ++j) {
         const int s = j % STAGES;
@@ -665,13 +688,10 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   bool ok = true;
   if (warp < 16) {
     const int prow = row0 + row;
-    int lo = 0, hi = 0, grp = 0;
+    // (the row's mask is read where a tile needs it: held here it would push the scores out of registers)
+    const int qi = prow < rows ? prow / G : -1;
     [[maybe_unused]] float slope2 = 0.f, qpos = 0.f;
     if (prow < rows) {
-      const int qi = prow / G;
-      lo = p.q_lo[qi];
-      hi = p.q_hi[qi];
-      grp = p.q_grp[qi];
       if constexpr ((MOD & score::BIAS) != 0) {
         slope2 = p.slopes[kvh * G + prow % G] * 1.4426950408889634f;
         qpos = (float)p.q_pos[qi];
@@ -684,14 +704,14 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       if ((j & 1) != i) continue;
       const int k0 = (split + o * p.splits) * BK + sub * 64;
       const bool masked = !((s_full[o >> 5] >> (o & 31)) & 1u);
-      // codes and positions of the 64 keys: two per lane, loaded while the scores are on their way, passed by shuffles
-      int code[2] = {0, 0};
+      // positions of the 64 keys: two per lane, loaded while the scores are on their way, passed by shuffles
       [[maybe_unused]] float kpos[2] = {0.f, 0.f};
+      if constexpr ((MOD & score::BIAS) != 0) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int k = k0 + x * 32 + lane;
-        if (masked) code[x] = k < p.nk ? __ldg(p.k_code + k) : score::DEAD_KEY;
-        if constexpr ((MOD & score::BIAS) != 0) kpos[x] = k < p.nk ? (float)__ldg(p.k_pos + k) : 0.f;
+        for (int x = 0; x < 2; ++x) {
+          const int k = k0 + x * 32 + lane;
+          kpos[x] = k < p.nk ? (float)__ldg(p.k_pos + k) : 0.f;
+        }
       }
       bool good = __all_sync(0xffffffffu, mbar_wait_spin(bar_sfull + 8 * i, (j >> 1) & 1, KID, 30));
       if (good) {
@@ -703,34 +723,38 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           // this thread's key of the tile: a V row that no row of the CTA can see is cleared (half a row per thread)
           const int kv = (split + o * p.splits) * BK + row;
           const int c = kv < p.nk ? __ldg(p.k_code + kv) : score::DEAD_KEY;
-          const bool any = c >= 0 ? (c >= lo_min && c < hi_max) : (c >= g_min && c <= g_max && c != score::DEAD_KEY);
-          if (!any && mbar_wait_spin(bar_vfull + 8 * (j % STAGES), (j / STAGES) & 1, KID, 33)) {
-            uint4* vrow = reinterpret_cast<uint4*>(sKV + (j % STAGES) * 2 * TILE_BYTES + TILE_BYTES + sub * HALF_BYTES + row * 128);
+          const bool none = !s_bound->may_see(c);
+          if (__any_sync(0xffffffffu, none)) {
+            if (none && mbar_wait_spin(bar_vfull + 8 * (j % STAGES), (j / STAGES) & 1, KID, 33)) {
+              uint4* vrow = reinterpret_cast<uint4*>(sKV + (j % STAGES) * 2 * TILE_BYTES + TILE_BYTES + sub * HALF_BYTES + row * 128);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-        }
-        uint32_t hidden[2] = {0u, 0u};   // masked scores of this thread
-        if (masked) {
-          // (a cap makes -inf finite: there masked scores become 0 first and -inf behind the transform)
-#pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            if (!visible(__shfl_sync(0xffffffffu, code[e >> 5], e & 31), lo, hi, grp)) {
-              r[e] = (MOD & score::CAP) ? 0u : 0xff800000u;
-              hidden[e >> 5] |= 1u << (e & 31);
+              for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
             }
+            fence_proxy_async_smem();
           }
         }
         score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) {
           const float kp = kpos[e >> 5];
+          asm volatile("" ::: "memory");
           return make_float4(__shfl_sync(0xffffffffu, kp, e & 31), __shfl_sync(0xffffffffu, kp, (e + 1) & 31),
                              __shfl_sync(0xffffffffu, kp, (e + 2) & 31), __shfl_sync(0xffffffffu, kp, (e + 3) & 31));
         });
-        if ((MOD & score::CAP) && masked) {
+        if (masked) {
+          // (a bit per key first, in a loop that holds one code at a time: the scores keep their registers)
+          const score::RowMask mask(qi < 0 ? 0 : __ldg(p.q_lo + qi), qi < 0 ? 0 : __ldg(p.q_hi + qi), qi < 0 ? 0 : __ldg(p.q_grp + qi));
+          uint32_t hidden[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int k = k0 + x * 32 + lane;
+            const int code = k < p.nk ? __ldg(p.k_code + k) : score::DEAD_KEY;
+            uint32_t h = 0u;
+#pragma unroll 4
+            for (int e = 0; e < 32; ++e) h |= (uint32_t)!mask.sees(__shfl_sync(0xffffffffu, code, e)) << e;
+            hidden[x] = h;
+          }
 #pragma unroll
           for (int e = 0; e < 64; ++e)
-            if ((hidden[e >> 5] >> (e & 31)) & 1u) r[e] = 0xff800000u;
+            if ((hidden[e >> 5] >> (e & 31)) & 1u) r[e] = 0xff800000u;   // -inf
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -893,8 +917,10 @@ static cudaError_t launch(const CUtensorMap& tq, const CUtensorMap& tk, const CU
 
 }  // namespace fewt
 
-// One warp per (query row, head): joins the splits.
+// One warp per (query row, head): joins the splits. Launched while the splits still run; the dependency wait returns when
+// that grid has ended and its results are visible.
 __global__ void __launch_bounds__(128) few_rows_join_kernel(const Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const long long n = (long long)p.nq * p.Hq;
   const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -1042,8 +1068,16 @@ extern "C" int tdllm_attn_few_rows(const void* q, const void* k, const void* v, 
   }
   if (e == cudaSuccess && pl.splits > 1) {
     const long long n = (long long)nq * Hq;
-    few::few_rows_join_kernel<<<(unsigned)((n + 3) / 4), 128, 0, st>>>(p);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((n + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, few::few_rows_join_kernel, p);
   }
   if (e != cudaSuccess) {
     tdllm_host::set_last_error("attn_few_rows launch: %s", cudaGetErrorString(e));

@@ -330,46 +330,36 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tmem_ld32(t_s + sub * 64, r);
         tmem_ld32(t_s + sub * 64 + 32, r + 32);
         tmem_ld_wait();
-        [[maybe_unused]] uint32_t hidden[2] = {0u, 0u};   // MOD: masked scores of this thread
-        if (MOD != 0 && (ent & 1)) {
-          // this thread's key of the tile (and half of its columns): a dead key's V row is zeroed
-          if ((kc - sub * 64)[row] == score::DEAD_KEY) {
-            if (mbar_wait_spin(bar_vfull + 8 * (j & 1), (j >> 1) & 1, KID, 33)) {
-              uint4* vrow = reinterpret_cast<uint4*>(sV + (j & 1) * TILE_BYTES + sub * HALF_BYTES + row * 128);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
-            }
-          }
-          fence_proxy_async_smem();
-        }
-        if (ent & 1) {
-          const int lo = __ldg(p.q_lo + grow), hi = __ldg(p.q_hi + grow), grp = __ldg(p.q_grp + grow);
-          if constexpr (MOD == 0) {
+        if constexpr (MOD == 0) {
+          if (ent & 1) {
+            const int lo = __ldg(p.q_lo + grow), hi = __ldg(p.q_hi + grow), grp = __ldg(p.q_grp + grow);
 #pragma unroll
             for (int e = 0; e < 64; ++e)
               if (!key_visible(__ldg(kc + e), lo, hi, grp)) r[e] = 0xff800000u;  // -inf
-          } else {
-            // (a cap makes -inf finite: there masked scores become 0 first and -inf behind the transform)
+          }
+        } else {
+          const float4* kp = reinterpret_cast<const float4*>(kc + 128);
+          score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) { return kp[e / 4]; });
+          if (ent & 1) {
+            // this thread's key of the tile (and half of its columns): a dead key's V row is zeroed
+            const bool dead = (kc - sub * 64)[row] == score::DEAD_KEY;
+            if (__any_sync(0xffffffffu, dead)) {
+              if (dead && mbar_wait_spin(bar_vfull + 8 * (j & 1), (j >> 1) & 1, KID, 33)) {
+                uint4* vrow = reinterpret_cast<uint4*>(sV + (j & 1) * TILE_BYTES + sub * HALF_BYTES + row * 128);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
+              }
+              fence_proxy_async_smem();
+            }
+            const score::RowMask mask(__ldg(p.q_lo + grow), __ldg(p.q_hi + grow), __ldg(p.q_grp + grow));
 #pragma unroll
             for (int e = 0; e < 64; e += 4) {
               const int4 c4 = *reinterpret_cast<const int4*>(kc + e);
-              const int code[4] = {c4.x, c4.y, c4.z, c4.w};
-#pragma unroll
-              for (int t = 0; t < 4; ++t)
-                if (!key_visible(code[t], lo, hi, grp)) {
-                  r[e + t] = (MOD & score::CAP) ? 0u : 0xff800000u;
-                  hidden[e >> 5] |= 1u << ((e + t) & 31);
-                }
+              if (!mask.sees(c4.x)) r[e] = 0xff800000u;   // -inf
+              if (!mask.sees(c4.y)) r[e + 1] = 0xff800000u;
+              if (!mask.sees(c4.z)) r[e + 2] = 0xff800000u;
+              if (!mask.sees(c4.w)) r[e + 3] = 0xff800000u;
             }
-          }
-        }
-        if constexpr (MOD != 0) {
-          const float4* kp = reinterpret_cast<const float4*>(kc + 128);
-          score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) { return kp[e / 4]; });
-          if ((MOD & score::CAP) && (ent & 1)) {
-#pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if ((hidden[e >> 5] >> (e & 31)) & 1u) r[e] = 0xff800000u;
           }
         }
         float mx = -INFINITY;

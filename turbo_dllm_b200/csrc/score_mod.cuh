@@ -13,12 +13,12 @@
 //                fp32 operations a score, two scores to an instruction, and no special-function operation
 //   beyond:      tanh(x) = 1 - 2 r with r = 1 / (1 + 2^y), y = 2 x log2 e clamped to +-60 (r is 0 or 1 to 32 bits there):
 //                2^y = 2^n p(y - n) on the fp32 pipes, n the nearest integer, p of degree 5 with the least largest
-//                relative error on [-1/2, 1/2] (7.5e-8), and two scores share one reciprocal, 1/d0 = d1 / (d0 d1)
+//                relative error on [-1/2, 1/2] (7.5e-8), and one reciprocal
 //
 // A warp takes the first form for a whole tile row when all of its scores allow it (a cap of 50 leaves scores up to 37),
 // else the second. With the special-function unit alone (exp2, reciprocal, and the softmax's exp2, at 16 a clock and SM)
-// a 128 x 128 tile takes 3072 clocks, three times its two products. NaN passes through both forms; in the second, what
-// one score of a pair holds reaches the other, so masked scores are replaced BEFORE the pair is formed.
+// a 128 x 128 tile takes 3072 clocks, three times its two products. NaN passes through both forms, and nothing crosses
+// from one score to its neighbour, so masked scores, which may hold anything, are replaced behind the transform.
 //
 // MOD & SAFE is set for every transformed kernel: query rows that see no key and keys that no row sees may hold
 // anything (infinities and NaN of uninitialised padding): their rows of an operand tile are overwritten with zeros in
@@ -78,9 +78,21 @@ __device__ __forceinline__ void cap_r2(float s0, float s1, const Mod& m, float& 
   const uint64_t p2 = pair_f32(__int_as_float((__float_as_int(t0) << 23) + 0x3f800000),
                                __int_as_float((__float_as_int(t1) << 23) + 0x3f800000));
   unpair_f32(fma_f32x2(e, p2, both(1.f)), d0, d1);
-  const float inv = rcp_approx(d0 * d1);
-  unpair_f32(mul_f32x2(pair_f32(d1, d0), both(inv)), r0, r1);
+  r0 = rcp_approx(d0);
+  r1 = rcp_approx(d1);
 }
+// A query row's side of the mask: key codes lo .. lo + range - 1, and the noisy block `grp` (a clean row has none: a
+// code that no key carries). One unsigned comparison covers "code >= 0, lo <= code < hi": a negative code is further from
+// lo >= 0 than any range reaches.
+struct RowMask {
+  int lo;
+  unsigned range;
+  int grp;
+  __device__ __forceinline__ RowMask(int lo_, int hi_, int grp_)
+      : lo(lo_), range(hi_ > lo_ ? (unsigned)(hi_ - lo_) : 0u), grp(grp_ < 0 ? grp_ : DEAD_KEY + 1) {}
+  __device__ __forceinline__ bool sees(int code) const { return (unsigned)code - (unsigned)lo < range || code == grp; }
+};
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

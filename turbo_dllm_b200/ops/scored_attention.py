@@ -148,14 +148,15 @@ def _seen_keys(layout: MaskLayout) -> torch.Tensor:
     return torch.where(code >= 0, covered, torch.isin(code, grp[grp < 0]))
 
 
-def _lists(layout: MaskLayout) -> dict:
-    """The layout's tile lists with the codes of keys that no row sees set to DEAD_KEY."""
+def _plan(layout: MaskLayout) -> MaskLayout:
+    """The layout the tile kernels run on: keys that no row sees carry DEAD_KEY, and rows that see no clean key an empty
+    interval behind every coordinate, so that neither widens what a 128-row tile seems to see (a padding row's interval
+    [0, 0) would pull in every tile from the first on)."""
     if "scored" not in layout._cache:
-        L = dict(layout.tile_lists())
-        code = L["k_code"].clone()
-        code[: layout.nk].masked_fill_(~_seen_keys(layout), DEAD_KEY)
-        L["k_code"] = code
-        layout._cache["scored"] = L
+        none = layout.q_hi <= layout.q_lo
+        layout._cache["scored"] = MaskLayout(
+            layout.q_lo.to(torch.int32).masked_fill(none, 2 ** 31 - 1), layout.q_hi.to(torch.int32).masked_fill(none, 0),
+            layout.q_grp, layout.k_code.to(torch.int32).masked_fill(~_seen_keys(layout), DEAD_KEY))
     return layout._cache["scored"]
 
 
@@ -268,7 +269,7 @@ def _forward(q, k, v, layout, transform, scale):
     nk, Hkv, _ = k.shape
     if nq <= FEW_ROWS:
         return _forward_few_rows(q, k, v, layout, transform, scale)
-    L = _lists(layout)
+    L = _plan(layout).tile_lists()
     mod, _kept = _mod_args(transform, L)
     out = torch.empty(nq, Hq, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(Hq, L["nq_pad"], dtype=torch.float32, device=q.device)
@@ -283,8 +284,8 @@ def _forward(q, k, v, layout, transform, scale):
 def _backward(q, k, v, out, dout, lse, layout, transform, scale):
     nq, Hq, D = q.shape
     nk, Hkv, _ = k.shape
-    L = _lists(layout)
-    W = layout.backward_work(backward_chunk_tiles())
+    L = _plan(layout).tile_lists()
+    W = _plan(layout).backward_work(backward_chunk_tiles())
     mod, _kept = _mod_args(transform, L)
     dev = q.device
     dq, dk, dv = torch.empty(nq, Hq, D, dtype=q.dtype, device=dev), torch.empty_like(k, memory_format=torch.contiguous_format), \
