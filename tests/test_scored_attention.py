@@ -18,7 +18,7 @@ FINE = 2.0 ** -14
 
 def exact(q, k, v, layout, tr, scale, dout=None):
     """The definition in 64 bits, head by head, and the largest error a kernel may show in each output: P and dS are
-    rounded to bf16 as operands of the next product, out enters the row sum dO.out rounded, every result is rounded."""
+    rounded to bf16 as operands of the next product, out enters the row sum dO.out as two bf16 terms, every result is rounded."""
     nq, Hq, _ = q.shape
     Hkv = k.shape[1]
     G = Hq // Hkv
@@ -62,7 +62,8 @@ def exact(q, k, v, layout, tr, scale, dout=None):
         res["dq"][:, h] = scale * (ds @ kh)
         res["dk"][:, h // G] += scale * (ds.t() @ qh)
         res["dv"][:, h // G] += p.t() @ do
-        edelta = (do.abs() * eo).sum(-1, keepdim=True)
+        # out is P.V with rounded P; its own rounding is kept apart (to 2^-17 of it)
+        edelta = (do.abs() * ((HALF + FINE) * a + FINE * o.abs())).sum(-1, keepdim=True)
         eds = HALF * ds.abs() + p * f * edelta + p * (f + FINE) * FINE * (dp.abs() + delta.abs())
         eds = eds + HALF * eds
         tol["dq"][:, h] += scale * (eds @ kh.abs())
@@ -282,7 +283,8 @@ def step_layout(caches, new, device="cuda", capacity=None, window=None):
                                                ([1000], 100, 2, 2), ([300, 200], 64, 8, 1), ([5], 40, 16, 1)])
 def test_few_rows(kind, caches, new, Hq, Hkv):
     L, qpos, kpos = step_layout(caches, new)
-    run_case(*_operands(L.nq, L.nk, Hq, Hkv, 8), L, transform_for(kind, Hq, qpos, kpos, "cuda"))
+    for backward in (False, True):
+        run_case(*_operands(L.nq, L.nk, Hq, Hkv, 8), L, transform_for(kind, Hq, qpos, kpos, "cuda"), backward=backward)
 
 
 @pytest.mark.gpu
@@ -293,9 +295,10 @@ def test_few_rows_against_caches_with_junk_behind_their_lengths(new, Hq):
     dead = L.k_code == DEAD_KEY
     k[dead] = float("nan")
     v[dead] = float("inf")
-    run_case(q, k, v, L, transform_for("both", Hq, qpos, kpos, "cuda"))
+    for backward in (False, True):
+        run_case(q, k, v, L, transform_for("both", Hq, qpos, kpos, "cuda"), backward=backward)
     L, qpos, kpos = step_layout([3000], new, window=300)
-    run_case(*_operands(L.nq, L.nk, Hq, 2, 9), L, transform_for("cap", Hq, qpos, kpos, "cuda"))
+    run_case(*_operands(L.nq, L.nk, Hq, 2, 9), L, transform_for("cap", Hq, qpos, kpos, "cuda"), backward=False)
 
 
 @pytest.mark.gpu

@@ -137,7 +137,8 @@ int tdllm_attn_merge_bwd(const void* go, const void* out, const float* lse, cons
 // As tdllm_attn_fwd / tdllm_attn_bwd_fused, on scores cap*tanh(scale*q.k/cap) - slope_h*|q_pos - k_pos|. softcap 0: no
 // cap; slope2 null: no bias, else [Hq] slopes times log2(e), with positions as floats padded to nq_pad / nk_pad.
 // Contents of query rows and keys that take part in no visible pair do not matter (keys: code -2^31).
-int tdllm_attn_fwd_scored(const void* q, const void* k, const void* v, void* o, float* lse, int nq, int nk, int Hq,
+// o_rest (null: not wanted): what rounding took from o, [nq, Hq*128] packed; the backward pass's row sums take it in.
+int tdllm_attn_fwd_scored(const void* q, const void* k, const void* v, void* o, void* o_rest, float* lse, int nq, int nk, int Hq,
                           int Hkv, long long ldq, long long ldk, long long ldv, long long ldo, const int* q_lo,
                           const int* q_hi, const int* q_grp, const int* k_code, const int* tile_ptr,
                           const int* tile_idx, const int* order, int n_qtiles, float scale, float softcap,
@@ -149,7 +150,7 @@ int tdllm_attn_few_rows(const void* q, const void* k, const void* v, void* o, fl
                         int Hq, int Hkv, long long ldq, long long ldk, long long ldv, long long ldo, long long ld_lse,
                         const int* q_lo, const int* q_hi, const int* q_grp, const int* k_code, float scale,
                         float softcap, const float* slopes, const int* q_pos, const int* k_pos, void* stream);
-int tdllm_attn_bwd_scored(const void* q, const void* k, const void* v, const void* o, const void* dout, void* dq,
+int tdllm_attn_bwd_scored(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout, void* dq,
                           void* dk, void* dv, const float* lse, float* delta, float* acc, int nq, int nk, int Hq,
                           int Hkv, long long ldq, long long ldk, long long ldv, long long ldo, long long lddo,
                           long long lddq, long long lddk, long long lddv, const int* q_lo, const int* q_hi,

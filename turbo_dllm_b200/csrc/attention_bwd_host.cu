@@ -49,7 +49,7 @@ extern "C" int tdllm_attn_bwd(const void* q, const void* k, const void* v, const
   {
     const long long items = (long long)nq_pad * Hq;
     attn_dq::attn_delta_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(
-        (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
+        (const __nv_bfloat16*)o, nullptr, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
         nq, nq_pad, Hq, ldo, lddo);
   }
   CUtensorMap tq, tdo, tk, tv, tk64, tv64, tdq, tdk, tdv;
@@ -115,7 +115,7 @@ __global__ void acc_cast_kernel(const float* __restrict__ acc, __nv_bfloat16* __
 // c*n_ktiles + kt lists the chunk's query tiles that see the key tile (w_ptr has one entry per item
 // plus one); `w_order` names the non-empty items, chunk by chunk.
 template <int MOD>
-static int attn_bwd_fused_launch(const char* who, const void* q, const void* k, const void* v, const void* o,
+static int attn_bwd_fused_launch(const char* who, const void* q, const void* k, const void* v, const void* o, const void* o_rest,
                                  const void* dout, void* dq, void* dk, void* dv, const float* lse,
                                  float* delta, float* acc, int nq, int nk, int Hq, int Hkv,
                                  long long ldq, long long ldk, long long ldv, long long ldo,
@@ -161,7 +161,7 @@ static int attn_bwd_fused_launch(const char* who, const void* q, const void* k, 
   {
     const long long items = (long long)nq_pad * Hq;
     attn_dq::attn_delta_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(
-        (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
+        (const __nv_bfloat16*)o, (const __nv_bfloat16*)o_rest, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
         nq, nq_pad, Hq, ldo, lddo);
   }
   CUtensorMap tq, tdo, tk, tv, tdk, tdv, tacc;
@@ -227,13 +227,13 @@ extern "C" int tdllm_attn_bwd_fused(const void* q, const void* k, const void* v,
                                     float scale, void* stream) {
   score::Mod mod;
   memset(&mod, 0, sizeof(mod));
-  return attn_bwd_fused_launch<0>("attn_bwd_fused", q, k, v, o, dout, dq, dk, dv, lse, delta, acc, nq, nk, Hq, Hkv, ldq,
+  return attn_bwd_fused_launch<0>("attn_bwd_fused", q, k, v, o, nullptr, dout, dq, dk, dv, lse, delta, acc, nq, nk, Hq, Hkv, ldq,
                                   ldk, ldv, ldo, lddo, lddq, lddk, lddv, q_lo, q_hi, q_grp, k_code, w_ptr, w_idx, w_order,
                                   n_work, n_qtiles, n_ktiles, scale, mod, stream);
 }
 
 // The same for transformed scores (arguments as in tdllm_attn_fwd_scored).
-extern "C" int tdllm_attn_bwd_scored(const void* q, const void* k, const void* v, const void* o, const void* dout,
+extern "C" int tdllm_attn_bwd_scored(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout,
                                      void* dq, void* dk, void* dv, const float* lse, float* delta, float* acc, int nq,
                                      int nk, int Hq, int Hkv, long long ldq, long long ldk, long long ldv, long long ldo,
                                      long long lddo, long long lddq, long long lddk, long long lddv, const int* q_lo,
@@ -243,7 +243,7 @@ extern "C" int tdllm_attn_bwd_scored(const void* q, const void* k, const void* v
                                      const float* k_pos, void* stream) {
   const score::Mod mod = score_mod_of(scale, softcap, slope2, q_pos, k_pos);
 #define TD_SCORED_BWD(M)                                                                                               \
-  return attn_bwd_fused_launch<score::SAFE | (M)>("attn_bwd_scored", q, k, v, o, dout, dq, dk, dv, lse, delta, acc,    \
+  return attn_bwd_fused_launch<score::SAFE | (M)>("attn_bwd_scored", q, k, v, o, o_rest, dout, dq, dk, dv, lse, delta, acc,    \
                                                   nq, nk, Hq, Hkv, ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv, q_lo,   \
                                                   q_hi, q_grp, k_code, w_ptr, w_idx, w_order, n_work, n_qtiles,        \
                                                   n_ktiles, scale, mod, stream)
@@ -314,7 +314,7 @@ extern "C" int tdllm_attn_bwd_fused_csbp(
   {
     const long long items = (long long)nq_pad * Hq;
     attn_dq::attn_delta_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(
-        (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
+        (const __nv_bfloat16*)o, nullptr, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
         nq, nq_pad, Hq, ldo, lddo);
   }
   float* my_dk = (float*)acc_dk[rank];

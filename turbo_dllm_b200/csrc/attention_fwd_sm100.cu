@@ -25,7 +25,11 @@
 //
 // Transformed scores (template argument MOD, score_mod.cuh): a tanh cap and / or a bias by distance, applied to the
 // scores right after they leave TMEM, in log2 units; the row maximum, the lazy rescale and the exponentials then work
-// on the transformed values. Keys that no row sees have their V row overwritten with zeros before P.V reads the tile.
+// on the transformed values. Keys that no row sees have their V row overwritten with zeros before P.V reads the tile. On
+// request (training) the bf16 rounding error of the output goes out as a second bf16 tensor, and the output is divided by
+// the sum of the ROUNDED probabilities, so that for a row with few keys the roundings cancel: the backward pass takes its
+// row sums dO.O from both tensors. From the rounded output alone they cost dQ and dK as much accuracy as the rounding of
+// dS does. The stored lse is that of the unrounded sum.
 //
 // Context-sharded form (template argument CSBP): key tiles [0, nlt) are this rank's own rows and are read
 // in place; key tiles [nlt, nlt + nrt) are clean K|V rows owned by the peers of the context-parallel group.
@@ -314,6 +318,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
     float m_used = -INFINITY;  // max the stored probabilities are relative to (raw score units; log2 units if MOD)
     float l = 0.f;             // this thread's share of the row sum
+    [[maybe_unused]] float lr = 0.f;   // the same of the rounded probabilities (MOD & REST)
     uint32_t r[64];
     bool ok = true;
     for (int j = 0; j < n; ++j) {
@@ -383,6 +388,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         m_used = mx;
       }
       l *= alpha;
+      if constexpr ((MOD & score::REST) != 0) lr *= alpha;
       if (__any_sync(0xffffffffu, alpha != 1.f) && j > 0) {
         uint32_t ro[16];
 #pragma unroll 1
@@ -406,6 +412,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           l += p0 + p1;
           pk[e >> 1] = pack_bf16x2(p0, p1);
         }
+        if constexpr ((MOD & score::REST) != 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lr += __uint_as_float(pk[e] << 16) + __uint_as_float(pk[e] & 0xffff0000u);
+        }
         tmem_st8(t_s + sub * 32 + c * 8, pk);
       }
       tmem_st_wait();
@@ -420,7 +430,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (ok) {
       l += *xother;
       tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      float inv = l > 0.f ? 1.f / l : 0.f;
+      if constexpr ((MOD & score::REST) != 0) {   // (a second exchange through the same slots)
+        named_bar_sync(1 + i, 256);
+        *xmine = lr;
+        named_bar_sync(1 + i, 256);
+        lr += *xother;
+        inv = lr > 0.f ? 1.f / lr : 0.f;
+      }
       uint8_t* st = sQ + i * TILE_BYTES;
       uint32_t ro[32];
 #pragma unroll 1
@@ -442,6 +459,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                                __uint_as_float(ro[8 * v + 2 * e + 1]) * inv);
           *reinterpret_cast<uint4*>(half + sw128_offset(row, (c & 1) * 4 + v)) =
               make_uint4(a[0], a[1], a[2], a[3]);
+          if constexpr ((MOD & score::REST) != 0) {   // staged over the K tiles, whose last products are done
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&a[e]));
+              a[e] = pack_bf16x2(__uint_as_float(ro[8 * v + 2 * e]) * inv - hi.x,
+                                 __uint_as_float(ro[8 * v + 2 * e + 1]) * inv - hi.y);
+            }
+            *reinterpret_cast<uint4*>(sK + i * TILE_BYTES + (c >> 1) * HALF_BYTES + sw128_offset(row, (c & 1) * 4 + v)) =
+                make_uint4(a[0], a[1], a[2], a[3]);
+          }
         }
       }
       if (sub == 0)
@@ -453,6 +480,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
           for (int c = 0; c < 2; ++c)
             tma_store_2d(&tm_o, smem_u32(st + c * HALF_BYTES), min(h0 + i, h_last) * HD + c * 64, qt * BQ);
+          if constexpr ((MOD & score::REST) != 0) {   // (the context-sharded form's remote K map is free here)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              tma_store_2d(&tm_kr, smem_u32(sK + i * TILE_BYTES + c * HALF_BYTES), min(h0 + i, h_last) * HD + c * 64, qt * BQ);
+          }
           tma_store_commit();
           tma_store_wait_all();
         }
@@ -505,7 +537,7 @@ static int attn_fwd_check(const char* who, int Hq, int Hkv, const long long* lds
 
 // One-GPU launch, plain (MOD == 0) or with transformed scores.
 template <int MOD>
-static int attn_fwd_launch(const char* who, const void* q, const void* k, const void* v, void* o, float* lse, int nq,
+static int attn_fwd_launch(const char* who, const void* q, const void* k, const void* v, void* o, void* o_rest, float* lse, int nq,
                            int nk, int Hq, int Hkv, long long ldq, long long ldk, long long ldv, long long ldo,
                            const int* q_lo, const int* q_hi, const int* q_grp, const int* k_code, const int* tile_ptr,
                            const int* tile_idx, const int* order, int n_qtiles, float scale, const score::Mod& mod,
@@ -531,6 +563,8 @@ static int attn_fwd_launch(const char* who, const void* q, const void* k, const 
   if (tdllm_host::encode_rows_tmap(&tk, k, (long long)Hkv * HD, nk, ldk, 128)) return 3;
   if (tdllm_host::encode_rows_tmap(&tv, v, (long long)Hkv * HD, nk, ldv, 128)) return 3;
   if (tdllm_host::encode_rows_tmap(&to, o, (long long)Hq * HD, nq, ldo, 128)) return 3;
+  CUtensorMap tor = to;
+  if (o_rest && tdllm_host::encode_rows_tmap(&tor, o_rest, (long long)Hq * HD, nq, (long long)Hq * HD, 128)) return 3;
   FwdParams p;
   p.nq_pad = n_qtiles * BQ;
   p.Hq = Hq; p.Hkv = Hkv;
@@ -543,7 +577,7 @@ static int attn_fwd_launch(const char* who, const void* q, const void* k, const 
   PullPlan pl;
   memset(&pl, 0, sizeof(pl));
   const int grid = n_qtiles * Hkv * ((Hq / Hkv + 1) / 2);
-  attn_fwd_kernel<false, MOD><<<grid, THREADS, MOD ? SMEM_BYTES_MOD : SMEM_BYTES, stream>>>(tq, tk, tv, to, tk, tv, p, pl);
+  attn_fwd_kernel<false, MOD><<<grid, THREADS, MOD ? SMEM_BYTES_MOD : SMEM_BYTES, stream>>>(tq, tk, tv, to, tor, tv, p, pl);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     tdllm_host::set_last_error("%s launch: %s", who, cudaGetErrorString(e));
@@ -563,13 +597,14 @@ extern "C" int tdllm_attn_fwd(const void* q, const void* k, const void* v, void*
   if (nq <= 0) return 0;
   score::Mod mod;
   memset(&mod, 0, sizeof(mod));
-  return attn_fwd_launch<0>("attn_fwd", q, k, v, o, lse, nq, nk, Hq, Hkv, ldq, ldk, ldv, ldo, q_lo, q_hi, q_grp, k_code,
+  return attn_fwd_launch<0>("attn_fwd", q, k, v, o, nullptr, lse, nq, nk, Hq, Hkv, ldq, ldk, ldv, ldo, q_lo, q_hi, q_grp, k_code,
                             tile_ptr, tile_idx, order, n_qtiles, scale, mod, (cudaStream_t)stream);
 }
 
 // The same with transformed scores (score_mod.cuh). softcap 0 = none; slope2 null = no bias, else [Hq] slopes times
-// log2(e) with q_pos / k_pos, positions as floats padded to nq_pad / nk_pad.
-extern "C" int tdllm_attn_fwd_scored(const void* q, const void* k, const void* v, void* o, float* lse, int nq, int nk,
+// log2(e) with q_pos / k_pos, positions as floats padded to nq_pad / nk_pad. o_rest: null, or [nq, Hq*128] (packed) for
+// what rounding took from o.
+extern "C" int tdllm_attn_fwd_scored(const void* q, const void* k, const void* v, void* o, void* o_rest, float* lse, int nq, int nk,
                                      int Hq, int Hkv, long long ldq, long long ldk, long long ldv, long long ldo,
                                      const int* q_lo, const int* q_hi, const int* q_grp, const int* k_code,
                                      const int* tile_ptr, const int* tile_idx, const int* order, int n_qtiles,
@@ -579,13 +614,17 @@ extern "C" int tdllm_attn_fwd_scored(const void* q, const void* k, const void* v
   const score::Mod mod = score_mod_of(scale, softcap, slope2, q_pos, k_pos);
   cudaStream_t st = (cudaStream_t)stream;
 #define TD_SCORED_FWD(M)                                                                                              \
-  return attn_fwd_launch<score::SAFE | (M)>("attn_fwd_scored", q, k, v, o, lse, nq, nk, Hq, Hkv, ldq, ldk, ldv, ldo,  \
+  return attn_fwd_launch<score::SAFE | (M)>("attn_fwd_scored", q, k, v, o, o_rest, lse, nq, nk, Hq, Hkv, ldq, ldk, ldv, ldo,  \
                                             q_lo, q_hi, q_grp, k_code, tile_ptr, tile_idx, order, n_qtiles, scale, mod, st)
-  switch ((softcap > 0.f ? score::CAP : 0) | (slope2 ? score::BIAS : 0)) {
+  switch ((softcap > 0.f ? score::CAP : 0) | (slope2 ? score::BIAS : 0) | (o_rest ? score::REST : 0)) {
     case 0: TD_SCORED_FWD(0);
     case score::CAP: TD_SCORED_FWD(score::CAP);
     case score::BIAS: TD_SCORED_FWD(score::BIAS);
-    default: TD_SCORED_FWD(score::CAP | score::BIAS);
+    case score::CAP | score::BIAS: TD_SCORED_FWD(score::CAP | score::BIAS);
+    case score::REST: TD_SCORED_FWD(score::REST);
+    case score::REST | score::CAP: TD_SCORED_FWD(score::REST | score::CAP);
+    case score::REST | score::BIAS: TD_SCORED_FWD(score::REST | score::BIAS);
+    default: TD_SCORED_FWD(score::REST | score::CAP | score::BIAS);
   }
 #undef TD_SCORED_FWD
 }

@@ -29,7 +29,7 @@
 namespace tdllm {
 namespace score {
 
-constexpr int CAP = 1, BIAS = 2, SAFE = 4;
+constexpr int CAP = 1, BIAS = 2, SAFE = 4, REST = 8;   // REST: the forward form whose output a backward pass will use
 constexpr int DEAD_KEY = -2147483647 - 1;   // code of a key that no row sees (also of padding behind the last key)
 
 struct Mod {

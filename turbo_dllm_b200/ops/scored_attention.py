@@ -34,13 +34,13 @@ from ._util import ptr
 from .attention import TILE, MaskLayout, backward_chunk_tiles, backward_mode
 
 native.register_signatures({
-    "tdllm_attn_fwd_scored": (native.c_int, [native.c_void_p] * 5 + [native.c_int] * 4 + [native.c_ll] * 4
+    "tdllm_attn_fwd_scored": (native.c_int, [native.c_void_p] * 6 + [native.c_int] * 4 + [native.c_ll] * 4
                               + [native.c_void_p] * 7 + [native.c_int, native.c_float, native.c_float]
                               + [native.c_void_p] * 4),
     "tdllm_attn_few_rows_scratch": (native.c_ll, [native.c_int] * 4),
     "tdllm_attn_few_rows": (native.c_int, [native.c_void_p] * 6 + [native.c_int] * 4 + [native.c_ll] * 5
                             + [native.c_void_p] * 4 + [native.c_float] * 2 + [native.c_void_p] * 4),
-    "tdllm_attn_bwd_scored": (native.c_int, [native.c_void_p] * 11 + [native.c_int] * 4 + [native.c_ll] * 8
+    "tdllm_attn_bwd_scored": (native.c_int, [native.c_void_p] * 12 + [native.c_int] * 4 + [native.c_ll] * 8
                               + [native.c_void_p] * 7 + [native.c_int, native.c_int, native.c_int, native.c_float,
                                                          native.c_float] + [native.c_void_p] * 4),
 })
@@ -48,7 +48,9 @@ native.register_signatures({
 DEAD_KEY = -(2 ** 31)      # key code that no query row matches
 MAX_POSITION = 1 << 24     # distances are taken between positions held as floats
 LOG2E = 1.4426950408889634
-# Up to this many query rows the forward splits the keys over the GPU instead of giving a CTA a 128-row query tile
+# Up to this many query rows a forward without gradients splits the keys over the GPU instead of giving a CTA a 128-row
+# query tile. B200, 32 / 8 heads, scores capped: 1 row x 20000 keys 24 us against 490, 32 x 32768 45 against 797,
+# 128 x 1024 20 against 36, 32 x 300 15.4 against 18.3
 FEW_ROWS = 128
 
 
@@ -264,24 +266,26 @@ def _forward_few_rows(q, k, v, layout, transform, scale):
     return out, lse
 
 
-def _forward(q, k, v, layout, transform, scale):
+def _forward(q, k, v, layout, transform, scale, for_backward=False):
+    """(out, lse [Hq, nq padded to 128], what rounding took from out where a backward pass will want it)."""
     nq, Hq, D = q.shape
     nk, Hkv, _ = k.shape
-    if nq <= FEW_ROWS:
-        return _forward_few_rows(q, k, v, layout, transform, scale)
+    if nq <= FEW_ROWS and not for_backward:
+        return (*_forward_few_rows(q, k, v, layout, transform, scale), None)
     L = _plan(layout).tile_lists()
     mod, _kept = _mod_args(transform, L)
     out = torch.empty(nq, Hq, D, dtype=q.dtype, device=q.device)
+    rest = torch.empty_like(out) if for_backward else None
     lse = torch.empty(Hq, L["nq_pad"], dtype=torch.float32, device=q.device)
     rc = native.lib().tdllm_attn_fwd_scored(
-        ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v),
+        ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(lse), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v),
         out.stride(0), ptr(L["q_lo"]), ptr(L["q_hi"]), ptr(L["q_grp"]), ptr(L["k_code"]), ptr(L["f_ptr"]), ptr(L["f_idx"]),
         ptr(L["f_order"]), L["nqt"], float(scale), *mod, _stream(q))
     native.check(rc, "attn_fwd_scored")
-    return out, lse
+    return out, lse, rest
 
 
-def _backward(q, k, v, out, dout, lse, layout, transform, scale):
+def _backward(q, k, v, out, rest, dout, lse, layout, transform, scale):
     nq, Hq, D = q.shape
     nk, Hkv, _ = k.shape
     L = _plan(layout).tile_lists()
@@ -294,7 +298,7 @@ def _backward(q, k, v, out, dout, lse, layout, transform, scale):
     # (allocated per call: two streams, or two captured graphs, must not add into one accumulator)
     acc = torch.empty(L["nq_pad"] * Hq * D + 2 * L["nk_pad"] * Hkv * D, dtype=torch.float32, device=dev)
     rc = native.lib().tdllm_attn_bwd_scored(
-        ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(lse), ptr(delta), ptr(acc),
+        ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(lse), ptr(delta), ptr(acc),
         nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v), _row_stride(out), _row_stride(dout),
         dq.stride(0), dk.stride(0), dv.stride(0), ptr(L["q_lo"]), ptr(L["q_hi"]), ptr(L["q_grp"]), ptr(L["k_code"]),
         ptr(W["w_ptr"]), ptr(W["w_idx"]), ptr(W["w_order"]), W["n_work"], L["nqt"], L["nkt"], float(scale), *mod, _stream(q))
@@ -307,8 +311,8 @@ class _ScoredAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, layout, transform, scale):
         with torch.cuda.device(q.device):
             q, k, v = _operand(q), _operand(k), _operand(v)
-            out, lse = _forward(q, k, v, layout, transform, scale)
-        ctx.save_for_backward(q, k, v, out, lse)
+            out, lse, rest = _forward(q, k, v, layout, transform, scale, for_backward=True)
+        ctx.save_for_backward(q, k, v, out, rest, lse)
         ctx.layout, ctx.transform, ctx.scale = layout, transform, scale
         lse = lse[:, : q.shape[0]]
         ctx.mark_non_differentiable(lse)
@@ -317,9 +321,9 @@ class _ScoredAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _dlse):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, rest, lse = ctx.saved_tensors
         with torch.cuda.device(q.device):
-            grads = _backward(q, k, v, out, _operand(dout), lse, ctx.layout, ctx.transform, ctx.scale)
+            grads = _backward(q, k, v, out, rest, _operand(dout), lse, ctx.layout, ctx.transform, ctx.scale)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
 
 
@@ -348,6 +352,6 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
         lse = torch.full((q.shape[1], q.shape[0]), float("-inf"), dtype=torch.float32, device=q.device)
     else:
         with torch.cuda.device(q.device):
-            out, lse = _forward(_operand(q), _operand(k), _operand(v), layout, transform, scale)
+            out, lse, _ = _forward(_operand(q), _operand(k), _operand(v), layout, transform, scale)
             lse = lse[:, : q.shape[0]]
     return (out, lse) if return_lse else out
