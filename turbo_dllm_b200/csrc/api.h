@@ -85,11 +85,11 @@ int tdllm_swiglu_bwd(const void* dy, const void* gu, void* dgu, long long rows, 
 // Norms behind and in front of a block (sandwich_norm.cu): h = a res + g rms(x) w_post, y = rms(h) w_pre. dtype 0 bf16,
 // 1 fp16, 2 fp32; gate_kind 0 none, 1 [H], 2 [rows, H]; rstd [2][rows] for backward, or null. Backward: dy / dh may be null
 // (no gradient there), and the sums dw_post, dw_pre, dgate_sum (gate_kind 1) where they are not wanted; scratch holds
-// tdllm_sandwich_norm_parts(rows) * 2 * H floats.
+// tdllm_sandwich_norm_parts(rows, H) * 2 * H floats.
 int tdllm_sandwich_norm_fwd(const void* x, const void* res, const void* w_post, const void* w_pre, const void* gate,
                             void* y, void* h, float* rstd, long long ldx, long long ldres, long long ldgate, int rows,
                             int H, int gate_kind, int dtype, float a, float eps, void* stream);
-int tdllm_sandwich_norm_parts(int rows);
+int tdllm_sandwich_norm_parts(int rows, int H);
 int tdllm_sandwich_norm_bwd(const void* x, const void* res, const void* w_post, const void* w_pre, const void* gate,
                             const void* dy, const void* dh, const float* rstd, void* dx, void* dres, void* dgate,
                             void* dw_post, void* dw_pre, void* dgate_sum, int post_fp32, int post_acc, int pre_fp32,

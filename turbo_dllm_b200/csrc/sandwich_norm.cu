@@ -13,14 +13,21 @@
 // Everything is 32-bit between the loads and the stores; y is formed from h before h is rounded, and the backward pass
 // recomputes h from x and res, which it needs anyway, instead of reading the rounded h.
 //
-// Bound by memory: x, res (g) in and h, y out; dy, dh, x, res (g) in and dx, dres (dg) out. One group of threads owns a
-// row and keeps it in registers: forward passes over a row once. The backward pass needs two row sums, the second of
-// which depends on the first; it is split into
+// Bound by memory: x, res (g) in and h, y out; dy, dh, x, res (g) in and dx, dres (dg) out. A block owns rows that are
+// gridDim.x apart and keeps a ring of them in shared memory, filled by bulk copies two or more rows ahead, so the copies
+// run while a row's sums are joined and its results are stored; the passes over a row read shared memory. (Rows loaded
+// into registers, one ahead, reached 3.4 TB/s forward and 2.9 TB/s backward at 16384 x 4096 bf16; see the end of this
+// comment for the ring.) The backward pass needs two row sums, the second of which depends on the first; it is split into
 //   sum du u = sum g w_post u (dh + dt / rms(h)) - mean(dt t) / rms(h) * sum g w_post u t
-// so that all three sums are taken together in one reduction. The sums over rows stay in registers while a block walks
-// its rows, and one partial row per block goes to memory; a second kernel adds the partial rows in a fixed order, so
-// results repeat bit for bit. For a channel gate (or none) both dw_post = g * A and dg = w_post * A follow from the one
-// sum A = sum_rows d * u.
+// so that all three sums are taken together in one reduction. The sums over rows stay in registers, one partial row per
+// block goes to memory, and a second kernel adds the partial rows in a fixed order, so results repeat bit for bit. For a
+// channel gate (or none) both dw_post = g * A and dg = w_post * A follow from the one sum A = sum_rows d * u.
+//
+// Any width goes in 16-byte lines: with V values to a line, a row that starts s values behind a 16-byte boundary is cut
+// into units [V c - s, V c - s + V). Whole lines are bulk-copied to the same shift in shared memory; the ragged values at
+// both ends are loaded by a few threads, a row ahead of the copies that need them, and stored value by value. The number
+// of blocks is a multiple of V, so s is the same for all rows of a block. All row operands have to be shifted alike (the
+// caller copies one that is not).
 #include "common.cuh"
 #include "vec_io.cuh"
 #include "api.h"
@@ -29,21 +36,32 @@ namespace tdllm {
 namespace sandwich {
 
 enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_FULL = 2 };
+constexpr int KID = 14;
+constexpr int MAX_H = 16384;
+constexpr int MAX_THREADS = 512;
+constexpr int MOST_THREADS = 544;   // a shifted row of the largest width has one unit more than 512 threads hold
+constexpr int MAX_STAGES = 6;
+constexpr int HEADER = 512;         // barriers and the reduction's slots, in front of the ring
 
 struct Args {
   const void *x, *res, *w_post, *w_pre, *gate;
   long long ldx, ldres, ldgate;   // row strides in elements
   int rows, H, gate_kind;
   float a, eps;
+  int stages, line_bytes;         // ring: rows, bytes of one tensor's row
 };
 
-// sum of N values over the threads of a row (a warp, or the whole block); every thread gets the sums
+// sum of N values over the block; every thread gets the sums
 template <int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float* red, int tpr) {
+__device__ __forceinline__ void row_sum(float (&v)[N], float* red) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-  if (tpr == 32) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = tpr >> 5;
+  const int nw = blockDim.x >> 5;
+  if (nw == 1) {
+    __syncwarp();
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __syncthreads();   // the previous sums have been read
   if (lane == 0) {
 #pragma unroll
@@ -54,188 +72,466 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int tpr) {
   for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < nw ? red[i * 32 + lane] : 0.f);
 }
 
-// tpr threads per row (32: a warp, several rows per block; else the whole block), NV vectors of V values per thread
-template <class T, int V, int NV>
-__global__ void __launch_bounds__(1024) fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h,
-                                                   float* __restrict__ rstd, int tpr) {
-  __shared__ float red[32];
-  const int rpb = blockDim.x / tpr;
-  const long long row = (long long)blockIdx.x * rpb + threadIdx.x / tpr;
-  const int t = threadIdx.x % tpr;
-  if (row >= p.rows) return;   // (a whole warp, or the whole block)
-  const T* x = (const T*)p.x + row * p.ldx;
-  const T* res = (const T*)p.res + row * p.ldres;
-  const T* wq = (const T*)p.w_post;
-  const T* wp = (const T*)p.w_pre;
-  const T* gate = (const T*)p.gate + (p.gate_kind == GATE_FULL ? row * p.ldgate : 0);
-  float xv[NV][V], rv[NV][V];
-  float ss[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (t + i * tpr) * V;
-    if (c < p.H) {
-      vio::load<T, V>(x + c, xv[i]);
-      vio::load<T, V>(res + c, rv[i]);
-#pragma unroll
-      for (int j = 0; j < V; ++j) ss[0] += xv[i][j] * xv[i][j];
+// The ring of rows of NB tensors. Rows too wide for two stages (RING false) are read from global memory in each pass
+// instead; the second pass finds them in L2.
+template <class T, int V, int NB, bool RING, bool SHIFT>
+struct Ring {
+  const T* base[NB];      // null: absent, reads as zeros (the slot was cleared)
+  long long ld[NB];
+  uint8_t* smem;          // [stage][tensor][line_bytes]
+  uint32_t bars;
+  int stages, line_bytes, H, shift;
+  T ragged;               // this thread's ragged value of the row that is being brought in
+  int rag_tensor, rag_e;  // whose, and which value; -1: none
+
+  __device__ __forceinline__ void setup(uint8_t* sm, const Args& p) {
+    smem = sm + HEADER;
+    bars = smem_u32(sm);
+    stages = p.stages;
+    line_bytes = p.line_bytes;
+    H = p.H;
+    // row r of every tensor starts (r * H) values behind a 16-byte boundary (strides differ from H by whole lines)
+    shift = SHIFT ? (int)(((long long)blockIdx.x * p.H) % V) : 0;
+    rag_tensor = -1;
+    rag_e = 0;
+    if (!RING) return;
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < stages; ++s) mbar_init(bars + 8 * s, 1);
+      fence_mbar_init();
     }
-  }
-  row_sum(ss, red, tpr);
-  const float r1 = rsqrtf(ss[0] / (float)p.H + p.eps);
-  ss[0] = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (t + i * tpr) * V;
-    if (c < p.H) {
-      float w[V], g[V];
-      vio::load<T, V>(wq + c, w);
-      if (p.gate_kind) vio::load<T, V>(gate + c, g);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float b = xv[i][j] * r1 * w[j];
-        if (p.gate_kind) b *= g[j];
-        rv[i][j] = fmaf(p.a, rv[i][j], b);
-        ss[0] += rv[i][j] * rv[i][j];
+    if (!SHIFT) return;
+    const int head = shift ? V - shift : 0, tail = (H + shift) % V;   // ragged values in front and behind
+    // threads 0 .. 2 V - 1 of every group of 2 V take one tensor
+    const int b = threadIdx.x / (2 * V), k = threadIdx.x % (2 * V);
+    if (b < NB) {
+      if (k < V) {
+        if (k < head && k < H) { rag_tensor = b; rag_e = k; }
+      } else if (k - V < tail && H + shift >= V) {   // (a row within one line has its values in the head part only)
+        rag_tensor = b;
+        rag_e = H - tail + (k - V);
       }
-      vio::store<T, V>(h + row * p.H + c, rv[i]);
+      if (shift == 0 && H < V && k < H) { rag_tensor = b; rag_e = k; }
     }
   }
-  row_sum(ss, red, tpr);
-  const float r2 = rsqrtf(ss[0] / (float)p.H + p.eps);
+  __device__ __forceinline__ T* slot(int s, int b) const { return (T*)(smem + ((size_t)s * NB + b) * line_bytes); }
+  // absent tensors read as zeros
+  __device__ __forceinline__ void clear_absent() {
+    if (!RING) return;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (t + i * tpr) * V;
-    if (c < p.H) {
-      float w[V];
-      vio::load<T, V>(wp + c, w);
+    for (int b = 0; b < NB; ++b)
+      if (!base[b])
+        for (int s = 0; s < stages; ++s)
+          for (int i = threadIdx.x; i < line_bytes / 16; i += blockDim.x)
+            reinterpret_cast<uint4*>(slot(s, b))[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  // thread 0: whole lines of a row into a stage
+  __device__ __forceinline__ void bring(int s, long long row) {
+    if (!RING) return;
+    const int first = shift ? 1 : 0, last = (H + shift) / V;   // whole lines
+    const uint32_t bytes = last > first ? (uint32_t)(last - first) * 16u : 0u;
+    uint32_t total = 0;
 #pragma unroll
-      for (int j = 0; j < V; ++j) w[j] *= rv[i][j] * r2;
-      vio::store<T, V>(y + row * p.H + c, w);
+    for (int b = 0; b < NB; ++b)
+      if (base[b]) total += bytes;
+    mbar_expect_tx(bars + 8 * s, total);
+    if (!bytes) return;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (base[b]) bulk_load_1d(smem_u32(slot(s, b)) + first * 16, base[b] + row * ld[b] + first * V - shift, bytes, bars + 8 * s);
+  }
+  __device__ __forceinline__ void load_ragged(long long row) {
+    if (!SHIFT || rag_tensor < 0) return;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (b == rag_tensor && base[b]) ragged = base[b][row * ld[b] + rag_e];
+  }
+  __device__ __forceinline__ void store_ragged(int s) {
+    if (!SHIFT || rag_tensor < 0) return;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (b == rag_tensor && base[b]) slot(s, b)[shift + rag_e] = ragged;
+  }
+  __device__ __forceinline__ void wait(int s, uint32_t parity) const {
+    if (RING) mbar_wait(bars + 8 * s, parity, KID, s);
+  }
+  // line c of a tensor's row (values e ..) as pairs, zeros outside the row
+  __device__ __forceinline__ void read(int s, int b, long long row, int c, int e, bool whole, uint64_t* f) const {
+    vio::Raw<T, V> r;
+    if (RING) {
+      r = vio::load_raw<T, V>(slot(s, b) + c * V);
+      if (SHIFT && !whole) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (e + j < 0 || e + j >= H) r.v[j] = vio::from_f<T>(0.f);
+      }
+    } else {
+      const T* at = base[b] ? base[b] + row * ld[b] : nullptr;
+      if (at && whole) {
+        r = vio::load_raw<T, V>(at + e);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) r.v[j] = (at && e + j >= 0 && e + j < H) ? at[e + j] : vio::from_f<T>(0.f);
+      }
+    }
+    vio::to_pairs<T, V>(r, f);
+  }
+};
+
+// How a thread's units lie in its rows: unit i of NV covers the values from e[i] on, line c[i] of shared memory
+template <int V, int NV, bool SHIFT>
+struct Units {
+  int c[NV], e[NV];
+  bool live[NV], whole[NV];
+  __device__ __forceinline__ Units(int shift, int H) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      c[i] = threadIdx.x + i * blockDim.x;
+      e[i] = c[i] * V - (SHIFT ? shift : 0);
+      live[i] = e[i] < H && (!SHIFT || e[i] + V > 0);
+      whole[i] = SHIFT ? e[i] >= 0 && e[i] + V <= H : live[i];
     }
   }
-  if (t == 0 && rstd) {
-    rstd[row] = r1;
-    rstd[p.rows + row] = r2;
+};
+template <class T, int V>
+__device__ __forceinline__ vio::Raw<T, V> weight_unit(const T* w, int e, int H, float absent) {
+  vio::Raw<T, V> r;
+#pragma unroll
+  for (int j = 0; j < V; ++j) r.v[j] = (w && e + j >= 0 && e + j < H) ? w[e + j] : vio::from_f<T>(absent);
+  return r;
+}
+template <class T, int V, bool SHIFT>
+__device__ __forceinline__ void store_unit(T* row, int e, bool whole, int H, const uint64_t* f) {
+  const vio::Raw<T, V> r = vio::from_pairs<T, V>(f);
+  if (!SHIFT || whole) {
+    *reinterpret_cast<vio::Raw<T, V>*>(row + e) = r;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (e + j >= 0 && e + j < H) row[e + j] = r.v[j];
   }
 }
 
-// part: [gridDim.x * rows per block][2][H]: the two row sums of each row walker
-template <class T, int V, int NV>
-__global__ void __launch_bounds__(1024) bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh,
-                                                   const float* __restrict__ rstd, T* __restrict__ dx,
-                                                   T* __restrict__ dres, T* __restrict__ dgate,
-                                                   float* __restrict__ part, int tpr) {
-  __shared__ float red[3 * 32];
-  const int rpb = blockDim.x / tpr;
-  const long long walker = (long long)blockIdx.x * rpb + threadIdx.x / tpr;
-  const long long walkers = (long long)gridDim.x * rpb;
-  const int t = threadIdx.x % tpr;
+// The rows a block walks: row index of its n-th row is blockIdx.x + n * gridDim.x.
+// SHIFT: the width is no multiple of V. GATE: see Args.
+template <class T, int V, int NV, bool SHIFT, int GATE>
+__global__ void __launch_bounds__(NV > 2 ? MOST_THREADS : MAX_THREADS, NV > 2 ? 1 : 2)
+fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h, float* __restrict__ rstd) {
+  constexpr bool FULL = GATE == GATE_FULL;
+  constexpr int NB = FULL ? 3 : 2;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* red = (float*)(smem + 64);
+  constexpr bool RING = NV == 2;
+  Ring<T, V, NB, RING, SHIFT> ring;
+  ring.base[0] = (const T*)p.x;
+  ring.base[1] = (const T*)p.res;
+  ring.ld[0] = p.ldx;
+  ring.ld[1] = p.ldres;
+  if constexpr (FULL) {
+    ring.base[2] = (const T*)p.gate;
+    ring.ld[2] = p.ldgate;
+  }
+  ring.setup(smem, p);
+  const Units<V, NV, SHIFT> un(ring.shift, p.H);
+  const T* gate = GATE == GATE_CHANNEL ? (const T*)p.gate : nullptr;
+  const long long step = gridDim.x;
+  const int n = (int)((p.rows - (long long)blockIdx.x + step - 1) / step);   // rows of this block
+  const int S = p.stages;
+  // weights: of an even width straight from L1, of a shifted one from a copy behind the ring that is shifted like the rows
+  constexpr bool copied = SHIFT;
+  T* s_w = (T*)(smem + HEADER + (RING ? (size_t)S * NB * p.line_bytes : 0));   // [w_post, w_pre, channel gate][line_bytes]
+  if constexpr (copied) {
+    const T* w[3] = {(const T*)p.w_post, (const T*)p.w_pre, gate};
+#pragma unroll
+    for (int b = 0; b < 3; ++b)
+      for (int i = threadIdx.x; i < p.line_bytes / (int)sizeof(T); i += blockDim.x) {
+        const int c = i - ring.shift;
+        s_w[b * (p.line_bytes / (int)sizeof(T)) + i] = w[b] && c >= 0 && c < p.H ? w[b][c] : vio::from_f<T>(0.f);
+      }
+  }
+  constexpr int P = V / 2;
+  auto weight = [&](int b, const T* w, int i, uint64_t* f) {
+    if constexpr (copied) vio::to_pairs<T, V>(vio::load_raw<T, V>(s_w + b * (p.line_bytes / (int)sizeof(T)) + un.c[i] * V), f);
+    else vio::to_pairs<T, V>(vio::load_raw<T, V>(w + un.e[i]), f);
+  };
+  __syncthreads();
+  for (int k = 0; RING && k < S - 1 && k < n; ++k) {
+    if (threadIdx.x == 0) ring.bring(k, blockIdx.x + k * step);
+    ring.load_ragged(blockIdx.x + k * step);
+    ring.store_ragged(k);
+  }
+  __syncthreads();
+  int s = 0;
+  uint32_t parity = 0;
+  bool pending = false;   // a ragged value waits for its stage
+  int pending_stage = 0;
+  for (int k = 0; k < n; ++k) {
+    const long long row = blockIdx.x + k * step;
+    if (pending) {
+      // into the stage of the row S - 2 ahead: with more than two stages a block barrier lies before its reader
+      ring.store_ragged(pending_stage);
+      if (S == 2 && copied) __syncthreads();
+    }
+    ring.wait(s, parity);
+    uint64_t hv[NV][P], sq = 0ull;
+    float ss[1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (un.live[i]) {
+        ring.read(s, 0, row, un.c[i], un.e[i], un.whole[i], hv[i]);
+#pragma unroll
+        for (int j = 0; j < P; ++j) sq = fma_f32x2(hv[i][j], hv[i][j], sq);
+      }
+    }
+    ss[0] = vio::sum_of(sq);
+    row_sum(ss, red);
+    // every thread is past the previous row: its stage takes the row S - 1 ahead
+    const int sn = s ? s - 1 : S - 1;
+    pending = RING && k + S - 1 < n;
+    if (pending) {
+      if (threadIdx.x == 0) ring.bring(sn, row + (S - 1) * step);
+      ring.load_ragged(row + (S - 1) * step);
+      pending_stage = sn;
+    }
+    const float r1 = rsqrtf(ss[0] / (float)p.H + p.eps);
+    sq = 0ull;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!un.live[i]) continue;
+      uint64_t w[P], v[P];
+      weight(0, (const T*)p.w_post, i, w);
+      if constexpr (GATE != GATE_NONE) {
+        if constexpr (FULL) ring.read(s, NB - 1, row, un.c[i], un.e[i], un.whole[i], v);
+        else weight(2, gate, i, v);
+#pragma unroll
+        for (int j = 0; j < P; ++j) w[j] = mul_f32x2(w[j], v[j]);
+      }
+      ring.read(s, 1, row, un.c[i], un.e[i], un.whole[i], v);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const uint64_t b = mul_f32x2(mul_f32x2(hv[i][j], vio::twice(r1)), w[j]);
+        hv[i][j] = fma_f32x2(vio::twice(p.a), v[j], b);
+        sq = fma_f32x2(hv[i][j], hv[i][j], sq);
+      }
+      store_unit<T, V, SHIFT>(h + row * p.H, un.e[i], un.whole[i], p.H, hv[i]);
+    }
+    ss[0] = vio::sum_of(sq);
+    row_sum(ss, red);
+    const float r2 = rsqrtf(ss[0] / (float)p.H + p.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!un.live[i]) continue;
+      uint64_t w[P];
+      weight(1, (const T*)p.w_pre, i, w);
+#pragma unroll
+      for (int j = 0; j < P; ++j) w[j] = mul_f32x2(w[j], mul_f32x2(hv[i][j], vio::twice(r2)));
+      store_unit<T, V, SHIFT>(y + row * p.H, un.e[i], un.whole[i], p.H, w);
+    }
+    if (threadIdx.x == 0 && rstd) {
+      rstd[row] = r1;
+      rstd[p.rows + row] = r2;
+    }
+    if (++s == S) {
+      s = 0;
+      parity ^= 1;
+    }
+  }
+}
+
+// part: [blocks][2][H]: the two row sums of each block
+template <class T, int V, int NV, bool SHIFT, int GATE>
+__global__ void __launch_bounds__(NV > 2 ? MOST_THREADS : MAX_THREADS, 1)
+bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, const float* __restrict__ rstd,
+           T* __restrict__ dx, T* __restrict__ dres, T* __restrict__ dgate, float* __restrict__ part) {
+  constexpr bool FULL = GATE == GATE_FULL;
+  constexpr int NB = FULL ? 5 : 4;
+  constexpr bool HELD = NV <= 2;   // weights in registers; wider rows read them again (they stay in L1 and L2)
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* red = (float*)(smem + 64);
+  constexpr bool RING = NV == 2;
+  Ring<T, V, NB, RING, SHIFT> ring;
+  ring.base[0] = (const T*)p.x;
+  ring.base[1] = (const T*)p.res;
+  ring.base[2] = dy;
+  ring.base[3] = dh;
+  ring.ld[0] = p.ldx;
+  ring.ld[1] = p.ldres;
+  ring.ld[2] = ring.ld[3] = p.H;
+  if constexpr (FULL) {
+    ring.base[4] = (const T*)p.gate;
+    ring.ld[4] = p.ldgate;
+  }
+  ring.setup(smem, p);
+  const Units<V, NV, SHIFT> un(ring.shift, p.H);
   const T* wq = (const T*)p.w_post;
   const T* wp = (const T*)p.w_pre;
+  const T* gate = GATE == GATE_CHANNEL ? (const T*)p.gate : nullptr;
+  const long long step = gridDim.x;
+  const int n = (int)((p.rows - (long long)blockIdx.x + step - 1) / step);
+  ring.clear_absent();
+  __syncthreads();
+  const int S = p.stages;
+  for (int k = 0; RING && k < S - 1 && k < n; ++k) {
+    if (threadIdx.x == 0) ring.bring(k, blockIdx.x + k * step);
+    ring.load_ragged(blockIdx.x + k * step);
+    ring.store_ragged(k);
+  }
+  constexpr int P = V / 2;
+  // held: g w_post (w_post alone for a full gate) as floats, w_pre as it came
+  uint64_t gwh[HELD ? NV : 1][P];
+  vio::Raw<T, V> hp[HELD ? NV : 1];
+  auto gated = [&](int i, uint64_t* gw) {   // w_post, times a channel gate
+    vio::to_pairs<T, V>(weight_unit<T, V>(wq, un.e[i], p.H, 0.f), gw);
+    if constexpr (GATE == GATE_CHANNEL) {
+      uint64_t g[P];
+      vio::to_pairs<T, V>(weight_unit<T, V>(gate, un.e[i], p.H, 0.f), g);
+#pragma unroll
+      for (int j = 0; j < P; ++j) gw[j] = mul_f32x2(gw[j], g[j]);
+    }
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      gated(i, gwh[i]);
+      hp[i] = weight_unit<T, V>(wp, un.e[i], p.H, 0.f);
+    }
+  }
+  __syncthreads();
   const float inv_h = 1.f / (float)p.H;
-  float sum_post[NV][V], sum_pre[NV][V];
+  uint64_t sum_post[NV][P], sum_pre[NV][P];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum_post[i][j] = sum_pre[i][j] = 0.f;
-  for (long long row = walker; row < p.rows; row += walkers) {
-    const T* x = (const T*)p.x + row * p.ldx;
-    const T* res = (const T*)p.res + row * p.ldres;
-    const T* gate = (const T*)p.gate + (p.gate_kind == GATE_FULL ? row * p.ldgate : 0);
-    const float r1 = rstd[row], r2 = rstd[p.rows + row];
-    float u[NV][V], tt[NV][V], dt[NV][V], dd[NV][V], gw[NV][V];
-    float s[3] = {0.f, 0.f, 0.f};
+    for (int j = 0; j < P; ++j) sum_post[i][j] = sum_pre[i][j] = 0ull;
+  auto staged = [&](int s, long long row, int b, int i, uint64_t* f) {
+    ring.read(s, b, row, un.c[i], un.e[i], un.whole[i], f);
+  };
+  auto weights = [&](int i, int s, long long row, uint64_t* gw, uint64_t* q) {   // g w_post and w_pre
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) gw[j] = gwh[i][j];
+      vio::to_pairs<T, V>(hp[i], q);
+    } else {
+      gated(i, gw);
+      vio::to_pairs<T, V>(weight_unit<T, V>(wp, un.e[i], p.H, 0.f), q);
+    }
+    if constexpr (FULL) {
+      uint64_t g[P];
+      staged(s, row, NB - 1, i, g);
+#pragma unroll
+      for (int j = 0; j < P; ++j) gw[j] = mul_f32x2(gw[j], g[j]);
+    }
+  };
+  int s = 0;
+  uint32_t parity = 0;
+  bool pending = false;
+  int pending_stage = 0;
+  float n1 = n > 0 ? rstd[blockIdx.x] : 0.f, n2 = n > 0 ? rstd[p.rows + blockIdx.x] : 0.f;
+  for (int k = 0; k < n; ++k) {
+    const long long row = blockIdx.x + k * step;
+    if (pending) {
+      ring.store_ragged(pending_stage);   // (as in the forward kernel)
+      if (SHIFT && S == 2) __syncthreads();
+    }
+    const float r1 = n1, r2 = n2;
+    if (k + 1 < n) {
+      n1 = rstd[row + step];
+      n2 = rstd[p.rows + row + step];
+    }
+    ring.wait(s, parity);
+    uint64_t s0 = 0ull, s1 = 0ull, s2 = 0ull;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * tpr) * V;
-      if (c < p.H) {
-        vio::load<T, V>(x + c, u[i]);
-        vio::load<T, V>(res + c, tt[i]);
-        vio::load<T, V>(wq + c, gw[i]);
-        if (p.gate_kind) {
-          float g[V];
-          vio::load<T, V>(gate + c, g);
+      if (!un.live[i]) continue;
+      uint64_t gw[P], q[P], u[P], t[P], dt[P], d[P];
+      weights(i, s, row, gw, q);
+      staged(s, row, 0, i, u);
+      staged(s, row, 1, i, t);
+      staged(s, row, 2, i, dt);
+      staged(s, row, 3, i, d);
 #pragma unroll
-          for (int j = 0; j < V; ++j) gw[i][j] *= g[j];
-        }
-        if (dy) {
-          float w[V];
-          vio::load<T, V>(dy + row * p.H + c, dt[i]);
-          vio::load<T, V>(wp + c, w);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            u[i][j] *= r1;
-            tt[i][j] = r2 * fmaf(p.a, tt[i][j], u[i][j] * gw[i][j]);
-            sum_pre[i][j] += dt[i][j] * tt[i][j];
-            dt[i][j] *= w[j];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            u[i][j] *= r1;
-            tt[i][j] = r2 * fmaf(p.a, tt[i][j], u[i][j] * gw[i][j]);
-            dt[i][j] = 0.f;
-          }
-        }
-        if (dh) {
-          vio::load<T, V>(dh + row * p.H + c, dd[i]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) dd[i][j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          dd[i][j] = fmaf(r2, dt[i][j], dd[i][j]);
-          s[0] += dt[i][j] * tt[i][j];
-          s[1] += gw[i][j] * u[i][j] * dd[i][j];
-          s[2] += gw[i][j] * u[i][j] * tt[i][j];
-        }
+      for (int j = 0; j < P; ++j) {
+        const uint64_t b = mul_f32x2(mul_f32x2(u[j], vio::twice(r1)), gw[j]);
+        t[j] = mul_f32x2(vio::twice(r2), fma_f32x2(vio::twice(p.a), t[j], b));
+        sum_pre[i][j] = fma_f32x2(dt[j], t[j], sum_pre[i][j]);
+        dt[j] = mul_f32x2(dt[j], q[j]);
+        d[j] = fma_f32x2(vio::twice(r2), dt[j], d[j]);
+        s0 = fma_f32x2(dt[j], t[j], s0);
+        s1 = fma_f32x2(b, d[j], s1);
+        s2 = fma_f32x2(b, t[j], s2);
       }
     }
-    row_sum(s, red, tpr);
-    const float m1 = s[0] * inv_h * r2;
-    const float m2 = (s[1] - m1 * s[2]) * inv_h;
+    float sums[3] = {vio::sum_of(s0), vio::sum_of(s1), vio::sum_of(s2)};
+    row_sum(sums, red);
+    const int sn = s ? s - 1 : S - 1;
+    pending = RING && k + S - 1 < n;
+    if (pending) {
+      if (threadIdx.x == 0) ring.bring(sn, row + (S - 1) * step);
+      ring.load_ragged(row + (S - 1) * step);
+      pending_stage = sn;
+    }
+    const float m1 = sums[0] * inv_h * r2;
+    const float m2 = (sums[1] - m1 * sums[2]) * inv_h;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * tpr) * V;
-      if (c < p.H) {
-        float o[V];
+      if (!un.live[i]) continue;
+      uint64_t gw[P], q[P], u[P], t[P], d[P];
+      weights(i, s, row, gw, q);
+      staged(s, row, 2, i, t);
+      staged(s, row, 3, i, d);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          dd[i][j] = fmaf(-tt[i][j], m1, dd[i][j]);
-          o[j] = p.a * dd[i][j];
-        }
-        vio::store<T, V>(dres + row * p.H + c, o);
+      for (int j = 0; j < P; ++j) d[j] = fma_f32x2(vio::twice(r2), mul_f32x2(t[j], q[j]), d[j]);
+      staged(s, row, 0, i, u);
+      staged(s, row, 1, i, t);
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = r1 * fmaf(-u[i][j], m2, dd[i][j] * gw[i][j]);
-        vio::store<T, V>(dx + row * p.H + c, o);
-        if (p.gate_kind == GATE_FULL) {
-          float w[V], g[V];
-          vio::load<T, V>(wq + c, w);
-          vio::load<T, V>(gate + c, g);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float du = dd[i][j] * u[i][j];
-            o[j] = du * w[j];
-            sum_post[i][j] += du * g[j];
-          }
-          vio::store<T, V>(dgate + row * p.H + c, o);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) sum_post[i][j] += dd[i][j] * u[i][j];
-        }
+      for (int j = 0; j < P; ++j) {
+        u[j] = mul_f32x2(u[j], vio::twice(r1));
+        t[j] = mul_f32x2(vio::twice(r2), fma_f32x2(vio::twice(p.a), t[j], mul_f32x2(u[j], gw[j])));
+        d[j] = fma_f32x2(t[j], vio::twice(-m1), d[j]);
+        q[j] = mul_f32x2(vio::twice(p.a), d[j]);
       }
+      store_unit<T, V, SHIFT>(dres + row * p.H, un.e[i], un.whole[i], p.H, q);
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        q[j] = mul_f32x2(vio::twice(r1), fma_f32x2(u[j], vio::twice(-m2), mul_f32x2(d[j], gw[j])));
+      store_unit<T, V, SHIFT>(dx + row * p.H, un.e[i], un.whole[i], p.H, q);
+      if constexpr (FULL) {
+        uint64_t g[P];
+        staged(s, row, NB - 1, i, g);
+        if constexpr (HELD) {
+#pragma unroll
+          for (int j = 0; j < P; ++j) gw[j] = gwh[i][j];
+        } else {
+          gated(i, gw);
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          u[j] = mul_f32x2(u[j], d[j]);
+          q[j] = mul_f32x2(gw[j], u[j]);
+          sum_post[i][j] = fma_f32x2(u[j], g[j], sum_post[i][j]);
+        }
+        store_unit<T, V, SHIFT>(dgate + row * p.H, un.e[i], un.whole[i], p.H, q);
+      } else {
+#pragma unroll
+        for (int j = 0; j < P; ++j) sum_post[i][j] = fma_f32x2(u[j], d[j], sum_post[i][j]);
+      }
+    }
+    if (++s == S) {
+      s = 0;
+      parity ^= 1;
     }
   }
-  float* mine = part + walker * 2 * p.H;
+  float* mine = part + (long long)blockIdx.x * 2 * p.H;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (t + i * tpr) * V;
-    if (c < p.H) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        mine[c + j] = sum_post[i][j];
-        mine[p.H + c + j] = sum_pre[i][j];
+    for (int j = 0; j < V; ++j) {
+      const int c = un.e[i] + j;
+      float a[2], b[2];
+      unpair_f32(sum_post[i][j / 2], a[0], a[1]);
+      unpair_f32(sum_pre[i][j / 2], b[0], b[1]);
+      if (c >= 0 && c < p.H) {
+        mine[c] = a[j & 1];
+        mine[p.H + c] = b[j & 1];
       }
     }
   }
@@ -258,16 +554,19 @@ __device__ __forceinline__ void put(const Out& o, int c, float v) {
   }
 }
 
-// Column sums of the partial rows: 32 columns x 8 row lanes per block.
+// Column sums of the partial rows: 32 columns x 32 row lanes per block. Launched while the partial sums are still being
+// made; the dependency wait returns when they are complete and visible.
 template <class T>
-__global__ void __launch_bounds__(256) finish_kernel(const float* __restrict__ part, int parts, const Args p, Out dw_post,
-                                                     Out dw_pre, Out dgate) {
-  __shared__ float sm[2][8][33];
+__global__ void __launch_bounds__(1024) finish_kernel(const float* __restrict__ part, int parts, const Args p, Out dw_post,
+                                                      Out dw_pre, Out dgate) {
+  __shared__ float sm[2][32][33];
   const int lane = threadIdx.x & 31, lanes = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float s0 = 0.f, s1 = 0.f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (c < p.H) {
-    for (int r = lanes; r < parts; r += 8) {
+#pragma unroll 4
+    for (int r = lanes; r < parts; r += 32) {
       s0 += part[(size_t)r * 2 * p.H + c];
       s1 += part[(size_t)r * 2 * p.H + p.H + c];
     }
@@ -275,38 +574,51 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* __restrict__ p
   sm[0][lanes][lane] = s0;
   sm[1][lanes][lane] = s1;
   __syncthreads();
-  if (lanes || c >= p.H) return;
-  s0 = s1 = 0.f;
+  if (lanes > 1) return;   // warp 0 joins the first sum, warp 1 the second
+  float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    s0 += sm[0][i][lane];
-    s1 += sm[1][i][lane];
+  for (int i = 0; i < 32; ++i) s += sm[lanes][i][lane];
+  if (c >= p.H) return;
+  if (lanes == 1) {
+    put<T>(dw_pre, c, s);
+    return;
   }
-  put<T>(dw_pre, c, s1);
   if (p.gate_kind == GATE_CHANNEL) {
-    put<T>(dgate, c, s0 * vio::to_f(((const T*)p.w_post)[c]));
-    s0 *= vio::to_f(((const T*)p.gate)[c]);
+    put<T>(dgate, c, s * vio::to_f(((const T*)p.w_post)[c]));
+    s *= vio::to_f(((const T*)p.gate)[c]);
   }
-  put<T>(dw_post, c, s0);
+  put<T>(dw_post, c, s);
 }
 
-constexpr int MAX_H = 16384;
-
-// threads per row and vectors per thread; a width that does not fill 16-byte vectors goes value by value
+// Units per thread, threads, blocks and the ring.
 struct Shape {
-  int v, nv, tpr;
+  int nv, threads, stages, grid, line_bytes;
+  size_t smem;
 };
-static Shape shape_of(int H, int per16, bool vectors) {
+static Shape shape_of(int rows, int H, int elem, int tensors, bool backward) {
   Shape s;
-  s.v = vectors ? per16 : 1;
-  const int units = (H + s.v - 1) / s.v;
-  const int want = vectors ? 1 : 4;   // units per thread before the row gets more threads
-  int tpr = 32;
-  while (tpr < 1024 && tpr * want < units) tpr *= 2;
-  s.tpr = tpr;
-  int nv = 1;
-  while (nv * tpr < units) nv *= 2;
-  s.nv = nv;
+  const int V = 16 / elem;
+  const int units = H % V ? (H + V - 1 + V - 1) / V : H / V;   // room for any shift
+  s.nv = 2;
+  while (s.nv * MAX_THREADS < units && s.nv < 32 / V) s.nv *= 2;   // 32 values per thread at most
+  s.threads = ((units + s.nv - 1) / s.nv + 31) / 32 * 32;
+  if (s.threads < 2 * V * tensors && H % V) s.threads = (2 * V * tensors + 31) / 32 * 32;   // one thread per ragged value
+  s.line_bytes = units * 16;
+  const bool ring = s.nv == 2;
+  const size_t row = ring ? (size_t)tensors * s.line_bytes : 0;
+  const size_t extra = HEADER + (!backward && (H % V || !ring) ? (size_t)3 * s.line_bytes : 0);
+  const size_t budget = 227 * 1024;
+  int resident = (backward || s.nv > 2 ? 512 : 1024) / s.threads;   // by the kernels' registers
+  if (resident < 1) resident = 1;
+  if (resident > 16) resident = 16;
+  // three rows per block; fewer blocks on an SM where they would not fit (the widest ring has 80 KiB rows: two fit)
+  while (resident > 1 && resident * (3 * row + extra + 1024) > budget) --resident;
+  s.stages = ring ? (int)((budget / resident - extra - 1024) / row) : 1;
+  if (s.stages > 4) s.stages = 4;
+  s.smem = extra + s.stages * row;
+  const int most = (tdllm_num_sms() * resident + 7) / 8 * 8;   // a multiple of the values in a line: one shift per block
+  const int need = (rows + 7) / 8 * 8;
+  s.grid = need < most ? need : most;
   return s;
 }
 
@@ -315,35 +627,41 @@ static Shape shape_of(int H, int per16, bool vectors) {
 
 using namespace tdllm;
 
-static bool sandwich_vectors(int elem, int H, const long long* lds, int nld, const void* const* ptrs, int n) {
-  const int per16 = 16 / elem;
-  if (H % per16) return false;
+// All row operands shifted alike: the same place in a 16-byte line and row strides that differ by whole lines.
+static bool sandwich_alike(int elem, int H, const long long* lds, int nld, const void* const* ptrs, int n) {
   for (int i = 0; i < nld; ++i)
-    if (lds[i] % per16) return false;
+    if (((lds[i] - H) * elem) % 16) return false;
   for (int i = 0; i < n; ++i)
     if ((uintptr_t)ptrs[i] % 16) return false;
   return true;
 }
 
-#define SANDWICH_NV(T, V, BODY)                         \
-  switch (s.nv) {                                       \
-    case 1: { constexpr int NV = 1; BODY(T, V, NV); break; }   \
-    case 2: { constexpr int NV = 2; BODY(T, V, NV); break; }   \
-    case 4: { constexpr int NV = 4; BODY(T, V, NV); break; }   \
-    case 8: { constexpr int NV = 8; BODY(T, V, NV); break; }   \
-    default: { constexpr int NV = 16; BODY(T, V, NV); break; } \
-  }
-#define SANDWICH_DISPATCH(BODY)                                                              \
-  if (dtype == 0) {                                                                          \
-    if (vec) { if (s.nv == 1) { BODY(__nv_bfloat16, 8, 1); } else { BODY(__nv_bfloat16, 8, 2); } } \
-    else SANDWICH_NV(__nv_bfloat16, 1, BODY)                                                 \
-  } else if (dtype == 1) {                                                                   \
-    if (vec) { if (s.nv == 1) { BODY(__half, 8, 1); } else { BODY(__half, 8, 2); } }         \
-    else SANDWICH_NV(__half, 1, BODY)                                                        \
-  } else {                                                                                   \
-    if (vec) { if (s.nv == 1) { BODY(float, 4, 1); } else if (s.nv == 2) { BODY(float, 4, 2); } else { BODY(float, 4, 4); } } \
-    else SANDWICH_NV(float, 1, BODY)                                                         \
-  }
+template <class K>
+static cudaError_t sandwich_smem(K kernel, size_t bytes) {
+  return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
+}
+
+#define SANDWICH_GATE(T, V, NV, SHIFT, BODY)                                   \
+  if (gate_kind == GATE_NONE) { BODY(T, V, NV, SHIFT, GATE_NONE); }            \
+  else if (gate_kind == GATE_CHANNEL) { BODY(T, V, NV, SHIFT, GATE_CHANNEL); } \
+  else { BODY(T, V, NV, SHIFT, GATE_FULL); }
+// (rows too wide for the ring: one form for aligned and shifted widths)
+#define SANDWICH_TYPE(T, V, BODY)                                              \
+  if (s.nv == 2 && H % V == 0) { SANDWICH_GATE(T, V, 2, false, BODY) }         \
+  else if (s.nv == 2) { SANDWICH_GATE(T, V, 2, true, BODY) }                   \
+  else if (s.nv == 4) { SANDWICH_GATE(T, V, 4, true, BODY) }                   \
+  else if constexpr (V == 4) { SANDWICH_GATE(T, V, 8, true, BODY) }
+#define SANDWICH_DISPATCH(BODY)                                                \
+  if (dtype == 0) { SANDWICH_TYPE(__nv_bfloat16, 8, BODY) }                    \
+  else if (dtype == 1) { SANDWICH_TYPE(__half, 8, BODY) }                      \
+  else { SANDWICH_TYPE(float, 4, BODY) }
+
+// a ring of fewer than two rows would wait for a row that nobody brings
+static int sandwich_ring(const char* who, const sandwich::Shape& s) {
+  if (s.nv == 2 ? s.stages >= 2 && s.stages <= sandwich::MAX_STAGES : s.stages == 1) return 0;
+  tdllm_host::set_last_error("%s: %d stages", who, s.stages);
+  return 1;
+}
 
 static int sandwich_check(const char* who, int rows, int H, int gate_kind, int dtype) {
   if (rows < 0 || H < 1 || H > sandwich::MAX_H || gate_kind < 0 || gate_kind > 2 || dtype < 0 || dtype > 2) {
@@ -363,17 +681,26 @@ extern "C" int tdllm_sandwich_norm_fwd(const void* x, const void* res, const voi
   if (sandwich_check("sandwich_norm_fwd", rows, H, gate_kind, dtype)) return 1;
   if (rows == 0) return 0;
   const int elem = dtype == 2 ? 4 : 2;
-  const long long lds[3] = {ldx, ldres, gate_kind == GATE_FULL ? ldgate : 0};
-  const void* ptrs[7] = {x, res, w_post, w_pre, gate, y, h};
-  const bool vec = sandwich_vectors(elem, H, lds, 3, ptrs, 7);
-  const Shape s = shape_of(H, 16 / elem, vec);
-  const Args p = {x, res, w_post, w_pre, gate, ldx, ldres, ldgate, rows, H, gate_kind, a, eps};
-  const int rpb = s.tpr == 32 ? 4 : 1;
-  const unsigned grid = (unsigned)(((long long)rows + rpb - 1) / rpb);
-#define FWD(T, V, NV) fwd_kernel<T, V, NV><<<grid, s.tpr * rpb, 0, (cudaStream_t)stream>>>(p, (T*)y, (T*)h, rstd, s.tpr)
+  const long long lds[3] = {ldx, ldres, gate_kind == GATE_FULL ? ldgate : H};
+  const void* ptrs[5] = {x, res, y, h, gate_kind == GATE_FULL ? gate : nullptr};
+  if (!sandwich_alike(elem, H, lds, 3, ptrs, 5)) {
+    tdllm_host::set_last_error("sandwich_norm_fwd: rows must start on 16 bytes and lie H values plus whole 16 bytes apart");
+    return 1;
+  }
+  const Shape s = shape_of(rows, H, elem, gate_kind == GATE_FULL ? 3 : 2, false);
+  if (sandwich_ring("sandwich_norm_fwd", s)) return 1;
+  const Args p = {x, res, w_post, w_pre, gate, ldx, ldres, ldgate, rows, H, gate_kind, a, eps, s.stages, s.line_bytes};
+  cudaError_t e = cudaErrorInvalidValue;
+#define FWD(T, V, NV, SHIFT, GATE)                                                             \
+  do {                                                                                  \
+    auto k = fwd_kernel<T, V, NV, SHIFT, GATE>;                                                \
+    e = sandwich_smem(k, s.smem);                                                       \
+    if (e == cudaSuccess)                                                               \
+      k<<<s.grid, s.threads, s.smem, (cudaStream_t)stream>>>(p, (T*)y, (T*)h, rstd);    \
+  } while (0)
   SANDWICH_DISPATCH(FWD)
 #undef FWD
-  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     tdllm_host::set_last_error("sandwich_norm_fwd launch: %s", cudaGetErrorString(e));
     return 4;
@@ -381,10 +708,17 @@ extern "C" int tdllm_sandwich_norm_fwd(const void* x, const void* res, const voi
   return 0;
 }
 
-// rows of partial sums that tdllm_sandwich_norm_bwd writes: the caller's scratch holds parts * 2 * H floats
-extern "C" int tdllm_sandwich_norm_parts(int rows) {
-  const int most = 2 * tdllm_num_sms();
-  return rows < most ? (rows + 3) / 4 * 4 : most * 4;
+// rows of partial sums that tdllm_sandwich_norm_bwd may write: the caller's scratch holds parts * 2 * H floats
+extern "C" int tdllm_sandwich_norm_parts(int rows, int H) {
+  using namespace tdllm::sandwich;
+  if (rows <= 0 || H < 1) return 0;
+  int most = 0;
+  for (int elem = 2; elem <= 4; elem += 2)      // either type, either kind of gate
+    for (int tensors = 4; tensors <= 5; ++tensors) {
+      const Shape s = shape_of(rows, H, elem, tensors, true);
+      if (s.grid > most) most = s.grid;
+    }
+  return most;
 }
 
 // dy / dh null: no gradient comes in there. dw_post, dw_pre, dgate_sum (a channel gate's gradient) may be null;
@@ -398,29 +732,47 @@ extern "C" int tdllm_sandwich_norm_bwd(const void* x, const void* res, const voi
   using namespace tdllm::sandwich;
   if (sandwich_check("sandwich_norm_bwd", rows, H, gate_kind, dtype)) return 1;
   const int elem = dtype == 2 ? 4 : 2;
-  const long long lds[3] = {ldx, ldres, gate_kind == GATE_FULL ? ldgate : 0};
-  const void* ptrs[10] = {x, res, w_post, w_pre, gate, dy, dh, dx, dres, dgate};
-  const bool vec = sandwich_vectors(elem, H, lds, 3, ptrs, 10);
-  const Shape s = shape_of(H, 16 / elem, vec);
-  const Args p = {x, res, w_post, w_pre, gate, ldx, ldres, ldgate, rows, H, gate_kind, a, 0.f};
-  const int rpb = s.tpr == 32 ? 4 : 1;
-  const int most = 2 * tdllm_num_sms();
-  int grid = (rows + rpb - 1) / rpb;
-  if (grid > most) grid = most;
+  const long long lds[3] = {ldx, ldres, gate_kind == GATE_FULL ? ldgate : H};
+  const void* ptrs[8] = {x, res, dx, dres, dy, dh, gate_kind == GATE_FULL ? gate : nullptr, gate_kind == GATE_FULL ? dgate : nullptr};
+  if (!sandwich_alike(elem, H, lds, 3, ptrs, 8)) {
+    tdllm_host::set_last_error("sandwich_norm_bwd: rows must start on 16 bytes and lie H values plus whole 16 bytes apart");
+    return 1;
+  }
+  const Shape s = shape_of(rows, H, elem, gate_kind == GATE_FULL ? 5 : 4, true);
+  if (sandwich_ring("sandwich_norm_bwd", s)) return 1;
+  const Args p = {x, res, w_post, w_pre, gate, ldx, ldres, ldgate, rows, H, gate_kind, a, 0.f, s.stages, s.line_bytes};
   cudaStream_t st = (cudaStream_t)stream;
-  if (grid > 0) {
-#define BWD(T, V, NV)                                                                                              \
-  bwd_kernel<T, V, NV><<<grid, s.tpr * rpb, 0, st>>>(p, (const T*)dy, (const T*)dh, rstd, (T*)dx, (T*)dres, (T*)dgate, \
-                                                     scratch, s.tpr)
+  cudaError_t e = cudaSuccess;
+  if (rows > 0) {
+    e = cudaErrorInvalidValue;
+#define BWD(T, V, NV, SHIFT, GATE)                                                                                              \
+  do {                                                                                                                   \
+    auto k = bwd_kernel<T, V, NV, SHIFT, GATE>;                                                                                 \
+    e = sandwich_smem(k, s.smem);                                                                                        \
+    if (e == cudaSuccess)                                                                                                \
+      k<<<s.grid, s.threads, s.smem, st>>>(p, (const T*)dy, (const T*)dh, rstd, (T*)dx, (T*)dres, (T*)dgate, scratch);   \
+  } while (0)
     SANDWICH_DISPATCH(BWD)
 #undef BWD
+    if (e == cudaSuccess) e = cudaGetLastError();
   }
-  const Out op = {dw_post, post_fp32, post_acc}, oq = {dw_pre, pre_fp32, pre_acc}, og = {dgate_sum, gate_fp32, gate_acc};
-  const int blocks = (H + 31) / 32, parts = grid * rpb;
-  if (dtype == 0) finish_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(scratch, parts, p, op, oq, og);
-  else if (dtype == 1) finish_kernel<__half><<<blocks, 256, 0, st>>>(scratch, parts, p, op, oq, og);
-  else finish_kernel<float><<<blocks, 256, 0, st>>>(scratch, parts, p, op, oq, og);
-  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) {
+    const Out op = {dw_post, post_fp32, post_acc}, oq = {dw_pre, pre_fp32, pre_acc}, og = {dgate_sum, gate_fp32, gate_acc};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((H + 31) / 32);
+    cfg.blockDim = dim3(1024);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = rows > 0 ? 1 : 0;
+    const int parts = rows > 0 ? s.grid : 0;
+    const float* sc = scratch;
+    if (dtype == 0) e = cudaLaunchKernelEx(&cfg, finish_kernel<__nv_bfloat16>, sc, parts, p, op, oq, og);
+    else if (dtype == 1) e = cudaLaunchKernelEx(&cfg, finish_kernel<__half>, sc, parts, p, op, oq, og);
+    else e = cudaLaunchKernelEx(&cfg, finish_kernel<float>, sc, parts, p, op, oq, og);
+  }
   if (e != cudaSuccess) {
     tdllm_host::set_last_error("sandwich_norm_bwd launch: %s", cudaGetErrorString(e));
     return 4;

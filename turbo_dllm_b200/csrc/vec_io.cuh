@@ -1,5 +1,8 @@
 // 16-byte vectors of bf16, fp16 or fp32 values as 32-bit floats, for the bandwidth-bound kernels that take all three.
+// Values are handled as pairs of floats in one 64-bit register: one instruction unpacks each value (none for fp32), one
+// rounds and packs two, and the packed fp32 instructions do two values of arithmetic.
 #pragma once
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
@@ -39,6 +42,49 @@ __device__ __forceinline__ void store(T* p, const float* f) {
 #pragma unroll
   for (int i = 0; i < N; ++i) r.v[i] = from_f<T>(f[i]);
   *reinterpret_cast<Raw<T, N>*>(p) = r;
+}
+
+// N values (a whole 16-byte vector) <-> N / 2 pairs of floats
+template <class T, int N>
+__device__ __forceinline__ void to_pairs(const Raw<T, N>& r, uint64_t* p) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      p[i] = pair_f32(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      p[i] = pair_f32(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(u + i));
+      p[i] = pair_f32(f.x, f.y);
+    }
+  }
+}
+template <class T, int N>
+__device__ __forceinline__ Raw<T, N> from_pairs(const uint64_t* p) {
+  Raw<T, N> r;
+  uint32_t* u = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    float a, b;
+    unpair_f32(p[i], a, b);
+    if constexpr (sizeof(T) == 4) {
+      u[2 * i] = __float_as_uint(a);
+      u[2 * i + 1] = __float_as_uint(b);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      u[i] = pack_bf16x2(a, b);
+    } else {
+      const __half2 h = __floats2half2_rn(a, b);
+      u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return r;
+}
+__device__ __forceinline__ uint64_t twice(float v) { return pair_f32(v, v); }
+__device__ __forceinline__ float sum_of(uint64_t p) {
+  float a, b;
+  unpair_f32(p, a, b);
+  return a + b;
 }
 
 }  // namespace vio

@@ -15,7 +15,7 @@ from ._util import dtype_code, grad_sink, mark_grad_written, on_device, ptr, scr
 native.register_signatures({
     "tdllm_sandwich_norm_fwd": (native.c_int, [native.c_void_p] * 8 + [native.c_ll] * 3 + [native.c_int] * 4
                                 + [native.c_float] * 2 + [native.c_void_p]),
-    "tdllm_sandwich_norm_parts": (native.c_int, [native.c_int]),
+    "tdllm_sandwich_norm_parts": (native.c_int, [native.c_int] * 2),
     "tdllm_sandwich_norm_bwd": (native.c_int, [native.c_void_p] * 14 + [native.c_int] * 6 + [native.c_void_p]
                                 + [native.c_ll] * 3 + [native.c_int] * 4 + [native.c_float, native.c_void_p]),
 })
@@ -104,9 +104,15 @@ GATE_NONE, GATE_CHANNEL, GATE_FULL = 0, 1, 2
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    """[rows, H] view with unit inner stride (a copy only where the tensor has none)."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+    """[rows, H] with unit inner stride, rows that start on 16 bytes and lie H values plus whole 16 bytes apart: what the
+    kernels ask of every row operand. A view where the tensor is like that, else a copy."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    H, size = t.shape[1], t.element_size()
+    if (t.stride(1) == 1 or H == 1) and t.data_ptr() % 16 == 0 \
+            and (t.shape[0] <= 1 or (t.stride(0) - H) * size % 16 == 0):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
 
 
 def _sandwich_forward(x, res, w_post, w_pre, gate, res_scale, eps, want_stats):
@@ -116,10 +122,19 @@ def _sandwich_forward(x, res, w_post, w_pre, gate, res_scale, eps, want_stats):
     stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if want_stats else None
     with on_device(x):
         native.check(native.lib().tdllm_sandwich_norm_fwd(
-            ptr(x), ptr(res), ptr(w_post), ptr(w_pre), ptr(gate), ptr(y), ptr(h), ptr(stats), x.stride(0), res.stride(0),
-            gate.stride(0) if kind == GATE_FULL else 0, rows, H, kind, dtype_code(x), res_scale, eps, stream()),
+            ptr(x), ptr(res), ptr(w_post), ptr(w_pre), ptr(gate), ptr(y), ptr(h), ptr(stats), _row_stride(x), _row_stride(res),
+            _row_stride(gate) if kind == GATE_FULL else H, rows, H, kind, dtype_code(x), res_scale, eps, stream()),
             "sandwich_norm_fwd")
     return y, h, stats
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]      # (a single row's stride may be anything)
+
+
+def _packed(t: torch.Tensor, rows: int, H: int) -> torch.Tensor:
+    t = t.reshape(rows, H).contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 class _SandwichNorm(torch.autograd.Function):
@@ -141,8 +156,8 @@ class _SandwichNorm(torch.autograd.Function):
         res_scale, shape = ctx.meta
         rows, H = x.shape
         kind = GATE_NONE if gate is None else GATE_CHANNEL if gate.dim() == 1 else GATE_FULL
-        dy = None if dy is None else dy.reshape(rows, H).contiguous()
-        dh = None if dh is None else dh.reshape(rows, H).contiguous()
+        dy = None if dy is None else _packed(dy, rows, H)
+        dh = None if dh is None else _packed(dh, rows, H)
         dx, dres = torch.empty(rows, H, dtype=x.dtype, device=x.device), torch.empty(rows, H, dtype=x.dtype, device=x.device)
         dgate = torch.empty(rows, H, dtype=x.dtype, device=x.device) if kind == GATE_FULL else None
         # vectors that own a slice of the flat gradient buffer are written (or added) there, the others are returned
@@ -161,11 +176,11 @@ class _SandwichNorm(torch.autograd.Function):
         with on_device(x):
             lib = native.lib()
             # (allocated per call: streams and captured graphs do not share it)
-            part = torch.empty(lib.tdllm_sandwich_norm_parts(rows) * 2 * H, dtype=torch.float32, device=x.device)
+            part = torch.empty(lib.tdllm_sandwich_norm_parts(rows, H) * 2 * H, dtype=torch.float32, device=x.device)
             native.check(lib.tdllm_sandwich_norm_bwd(
                 ptr(x), ptr(res), ptr(w_post), ptr(w_pre), ptr(gate), ptr(dy), ptr(dh), ptr(stats), ptr(dx), ptr(dres),
-                ptr(dgate), *(ptr(t) for t in targets), *flags, ptr(part), x.stride(0), res.stride(0),
-                gate.stride(0) if kind == GATE_FULL else 0, rows, H, kind, dtype_code(x), res_scale, stream()),
+                ptr(dgate), *(ptr(t) for t in targets), *flags, ptr(part), _row_stride(x), _row_stride(res),
+                _row_stride(gate) if kind == GATE_FULL else H, rows, H, kind, dtype_code(x), res_scale, stream()),
                 "sandwich_norm_bwd")
         for ref in written:
             mark_grad_written(ref)
