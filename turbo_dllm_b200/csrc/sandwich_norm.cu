@@ -24,10 +24,10 @@
 // channel gate (or none) both dw_post = g * A and dg = w_post * A follow from the one sum A = sum_rows d * u.
 //
 // Any width goes in 16-byte lines: with V values to a line, a row that starts s values behind a 16-byte boundary is cut
-// into units [V c - s, V c - s + V). Whole lines are bulk-copied to the same shift in shared memory; the ragged values at
-// both ends are loaded by a few threads, a row ahead of the copies that need them, and stored value by value. The number
-// of blocks is a multiple of V, so s is the same for all rows of a block. All row operands have to be shifted alike (the
-// caller copies one that is not).
+// into units [V c - s, V c - s + V). Its lines are bulk-copied as they are, the neighbours' values at both ends included,
+// and what lies outside the row is masked off when a line is read; only behind the tensors' last row, where no neighbour
+// is, the last values come one by one. Ragged lines are stored value by value. The number of blocks is a multiple of V, so
+// s is the same for all rows of a block. All row operands have to be shifted alike (the caller copies one that is not).
 #include "common.cuh"
 #include "vec_io.cuh"
 #include "api.h"
@@ -72,8 +72,8 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red) {
   for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < nw ? red[i * 32 + lane] : 0.f);
 }
 
-// The ring of rows of NB tensors. Rows too wide for two stages (RING false) are read from global memory in each pass
-// instead; the second pass finds them in L2.
+// The ring of rows of NB tensors. RING false (rows too wide for two stages, or no more than one row per block): rows are
+// read from global memory in each pass; the second pass finds them in L2.
 template <class T, int V, int NB, bool RING, bool SHIFT>
 struct Ring {
   const T* base[NB];      // null: absent, reads as zeros (the slot was cleared)
@@ -81,9 +81,7 @@ struct Ring {
   uint8_t* smem;          // [stage][tensor][line_bytes]
   uint32_t bars;
   int stages, line_bytes, H, shift;
-  T ragged;               // this thread's ragged value of the row that is being brought in
-  int rag_tensor, rag_e;  // whose, and which value; -1: none
-
+  long long last;         // the tensors' last row
   __device__ __forceinline__ void setup(uint8_t* sm, const Args& p) {
     smem = sm + HEADER;
     bars = smem_u32(sm);
@@ -92,25 +90,10 @@ struct Ring {
     H = p.H;
     // row r of every tensor starts (r * H) values behind a 16-byte boundary (strides differ from H by whole lines)
     shift = SHIFT ? (int)(((long long)blockIdx.x * p.H) % V) : 0;
-    rag_tensor = -1;
-    rag_e = 0;
-    if (!RING) return;
-    if (threadIdx.x == 0) {
+    last = p.rows - 1;
+    if (RING && threadIdx.x == 0) {
       for (int s = 0; s < stages; ++s) mbar_init(bars + 8 * s, 1);
       fence_mbar_init();
-    }
-    if (!SHIFT) return;
-    const int head = shift ? V - shift : 0, tail = (H + shift) % V;   // ragged values in front and behind
-    // threads 0 .. 2 V - 1 of every group of 2 V take one tensor
-    const int b = threadIdx.x / (2 * V), k = threadIdx.x % (2 * V);
-    if (b < NB) {
-      if (k < V) {
-        if (k < head && k < H) { rag_tensor = b; rag_e = k; }
-      } else if (k - V < tail && H + shift >= V) {   // (a row within one line has its values in the head part only)
-        rag_tensor = b;
-        rag_e = H - tail + (k - V);
-      }
-      if (shift == 0 && H < V && k < H) { rag_tensor = b; rag_e = k; }
     }
   }
   __device__ __forceinline__ T* slot(int s, int b) const { return (T*)(smem + ((size_t)s * NB + b) * line_bytes); }
@@ -124,64 +107,59 @@ struct Ring {
           for (int i = threadIdx.x; i < line_bytes / 16; i += blockDim.x)
             reinterpret_cast<uint4*>(slot(s, b))[i] = make_uint4(0u, 0u, 0u, 0u);
   }
-  // thread 0: whole lines of a row into a stage
+  // all threads: a row's lines into a stage (one thread copies; the last row's last values go in by themselves, and the
+  // caller puts a block barrier between this and their use)
   __device__ __forceinline__ void bring(int s, long long row) {
     if (!RING) return;
-    const int first = shift ? 1 : 0, last = (H + shift) / V;   // whole lines
-    const uint32_t bytes = last > first ? (uint32_t)(last - first) * 16u : 0u;
-    uint32_t total = 0;
+    const int tail = SHIFT && row == last ? (H + shift) % V : 0;
+    if (threadIdx.x == 0) {
+      const int lines = SHIFT ? (tail ? (H + shift) / V : (H + shift + V - 1) / V) : H / V;
+      uint32_t total = 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (base[b]) total += bytes;
-    mbar_expect_tx(bars + 8 * s, total);
-    if (!bytes) return;
+      for (int b = 0; b < NB; ++b)
+        if (base[b]) total += lines * 16;
+      mbar_expect_tx(bars + 8 * s, total);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (base[b]) bulk_load_1d(smem_u32(slot(s, b)) + first * 16, base[b] + row * ld[b] + first * V - shift, bytes, bars + 8 * s);
-  }
-  __device__ __forceinline__ void load_ragged(long long row) {
-    if (!SHIFT || rag_tensor < 0) return;
+      for (int b = 0; b < NB; ++b)
+        if (base[b] && lines)
+          bulk_load_1d(smem_u32(slot(s, b)), base[b] + row * ld[b] - shift, lines * 16, bars + 8 * s);
+    }
+    if (tail && (int)threadIdx.x < tail) {
+      const int e = H - tail + threadIdx.x;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (b == rag_tensor && base[b]) ragged = base[b][row * ld[b] + rag_e];
-  }
-  __device__ __forceinline__ void store_ragged(int s) {
-    if (!SHIFT || rag_tensor < 0) return;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-      if (b == rag_tensor && base[b]) slot(s, b)[shift + rag_e] = ragged;
+      for (int b = 0; b < NB; ++b)
+        if (base[b] && e >= 0) slot(s, b)[shift + e] = base[b][row * ld[b] + e];
+    }
   }
   __device__ __forceinline__ void wait(int s, uint32_t parity) const {
     if (RING) mbar_wait(bars + 8 * s, parity, KID, s);
   }
-  // line c of a tensor's row (values e ..) as pairs, zeros outside the row
-  __device__ __forceinline__ void read(int s, int b, long long row, int c, int e, bool whole, uint64_t* f) const {
-    vio::Raw<T, V> r;
+  // line c of a tensor's row (values e ..) as pairs, zeros outside the row; keep: the bits of the line that are the row's
+  __device__ __forceinline__ void read(int s, int b, long long row, int c, int e, bool whole, const uint4& keep, uint64_t* f) const {
     if (RING) {
-      r = vio::load_raw<T, V>(slot(s, b) + c * V);
-      if (SHIFT && !whole) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (e + j < 0 || e + j >= H) r.v[j] = vio::from_f<T>(0.f);
+      vio::Raw<T, V> r = vio::load_raw<T, V>(slot(s, b) + c * V);
+      if (SHIFT) {
+        uint4* u = reinterpret_cast<uint4*>(&r);
+        u->x &= keep.x;
+        u->y &= keep.y;
+        u->z &= keep.z;
+        u->w &= keep.w;
       }
+      vio::to_pairs<T, V>(r, f);
     } else {
       const T* at = base[b] ? base[b] + row * ld[b] : nullptr;
-      if (at && whole) {
-        r = vio::load_raw<T, V>(at + e);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) r.v[j] = (at && e + j >= 0 && e + j < H) ? at[e + j] : vio::from_f<T>(0.f);
-      }
+      if (at && whole) vio::to_pairs<T, V>(vio::load_raw<T, V>(at + e), f);
+      else vio::load_pairs_each<T, V>(at, e, H, f);
     }
-    vio::to_pairs<T, V>(r, f);
   }
 };
 
 // How a thread's units lie in its rows: unit i of NV covers the values from e[i] on, line c[i] of shared memory
-template <int V, int NV, bool SHIFT>
+template <int V, int NV, bool RING, bool SHIFT>
 struct Units {
   int c[NV], e[NV];
   bool live[NV], whole[NV];
+  uint4 keep[NV];
   __device__ __forceinline__ Units(int shift, int H) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -189,38 +167,57 @@ struct Units {
       e[i] = c[i] * V - (SHIFT ? shift : 0);
       live[i] = e[i] < H && (!SHIFT || e[i] + V > 0);
       whole[i] = SHIFT ? e[i] >= 0 && e[i] + V <= H : live[i];
+      if (RING && SHIFT) {
+        uint32_t m[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          m[w] = 0u;
+#pragma unroll
+          for (int j = 0; j < V / 4; ++j) {   // one 32-bit value or two 16-bit values to a word
+            const int at = e[i] + w * (V / 4) + j;
+            if (at >= 0 && at < H) m[w] |= V == 4 ? 0xffffffffu : 0xffffu << (16 * j);
+          }
+        }
+        keep[i] = make_uint4(m[0], m[1], m[2], m[3]);
+      }
     }
   }
 };
+// values e .. e + V - 1 of a weight vector
 template <class T, int V>
-__device__ __forceinline__ vio::Raw<T, V> weight_unit(const T* w, int e, int H, float absent) {
-  vio::Raw<T, V> r;
+__device__ __forceinline__ void weight_unit(const T* w, int e, int H, uint64_t* f) {
+  if (e >= 0 && e + V <= H && (uintptr_t)(w + e) % 16 == 0) vio::to_pairs<T, V>(vio::load_raw<T, V>(w + e), f);
+  else vio::load_pairs_each<T, V>(w, e, H, f);
+}
+// a block's copies of the weights, shifted like its rows: [w_post, w_pre, channel gate][line_bytes]
+template <class T>
+__device__ __forceinline__ void copy_weights(T* sm, const T* post, const T* pre, const T* gate, int line, int shift, int H) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) r.v[j] = (w && e + j >= 0 && e + j < H) ? w[e + j] : vio::from_f<T>(absent);
-  return r;
+  for (int b = 0; b < 3; ++b) {
+    const T* w = b == 0 ? post : b == 1 ? pre : gate;
+    if (!w) continue;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < line; i += blockDim.x) {
+      const int c = i - shift;
+      sm[b * line + i] = c >= 0 && c < H ? w[c] : vio::from_f<T>(0.f);
+    }
+  }
 }
 template <class T, int V, bool SHIFT>
 __device__ __forceinline__ void store_unit(T* row, int e, bool whole, int H, const uint64_t* f) {
-  const vio::Raw<T, V> r = vio::from_pairs<T, V>(f);
-  if (!SHIFT || whole) {
-    *reinterpret_cast<vio::Raw<T, V>*>(row + e) = r;
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (e + j >= 0 && e + j < H) row[e + j] = r.v[j];
-  }
+  if (!SHIFT || whole) *reinterpret_cast<vio::Raw<T, V>*>(row + e) = vio::from_pairs<T, V>(f);
+  else vio::store_pairs_each<T, V>(row, e, H, f);
 }
 
 // The rows a block walks: row index of its n-th row is blockIdx.x + n * gridDim.x.
-// SHIFT: the width is no multiple of V. GATE: see Args.
-template <class T, int V, int NV, bool SHIFT, int GATE>
-__global__ void __launch_bounds__(NV > 2 ? MOST_THREADS : MAX_THREADS, NV > 2 ? 1 : 2)
+// SHIFT: the width may be no multiple of V. GATE: see Args. RING: see Ring.
+template <class T, int V, int NV, bool RING, bool SHIFT, int GATE>
+__global__ void __launch_bounds__(NV > 2 ? MOST_THREADS : MAX_THREADS, RING ? 2 : 1)
 fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h, float* __restrict__ rstd) {
   constexpr bool FULL = GATE == GATE_FULL;
   constexpr int NB = FULL ? 3 : 2;
   extern __shared__ __align__(128) uint8_t smem[];
   float* red = (float*)(smem + 64);
-  constexpr bool RING = NV == 2;
   Ring<T, V, NB, RING, SHIFT> ring;
   ring.base[0] = (const T*)p.x;
   ring.base[1] = (const T*)p.res;
@@ -231,53 +228,54 @@ fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h, float* __restrict
     ring.ld[2] = p.ldgate;
   }
   ring.setup(smem, p);
-  const Units<V, NV, SHIFT> un(ring.shift, p.H);
+  const Units<V, NV, RING, SHIFT> un(ring.shift, p.H);
   const T* gate = GATE == GATE_CHANNEL ? (const T*)p.gate : nullptr;
   const long long step = gridDim.x;
   const int n = (int)((p.rows - (long long)blockIdx.x + step - 1) / step);   // rows of this block
   const int S = p.stages;
-  // weights: of an even width straight from L1, of a shifted one from a copy behind the ring that is shifted like the rows
-  constexpr bool copied = SHIFT;
-  T* s_w = (T*)(smem + HEADER + (RING ? (size_t)S * NB * p.line_bytes : 0));   // [w_post, w_pre, channel gate][line_bytes]
-  if constexpr (copied) {
-    const T* w[3] = {(const T*)p.w_post, (const T*)p.w_pre, gate};
-#pragma unroll
-    for (int b = 0; b < 3; ++b)
-      for (int i = threadIdx.x; i < p.line_bytes / (int)sizeof(T); i += blockDim.x) {
-        const int c = i - ring.shift;
-        s_w[b * (p.line_bytes / (int)sizeof(T)) + i] = w[b] && c >= 0 && c < p.H ? w[b][c] : vio::from_f<T>(0.f);
-      }
-  }
+  // weights: with one row per block in registers, loaded beside the row; of an aligned width straight from L1; else from a
+  // copy behind the ring that is shifted like the rows
+  constexpr bool HELD = !RING && NV == 2, COPIED = !HELD && SHIFT;
   constexpr int P = V / 2;
+  T* s_w = (T*)(smem + HEADER + (RING ? (size_t)S * NB * p.line_bytes : 0));
+  const int line = p.line_bytes / (int)sizeof(T);
+  vio::Raw<T, V> held[3][HELD ? NV : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint64_t f[P];
+      weight_unit<T, V>((const T*)p.w_post, un.e[i], p.H, f);
+      held[0][i] = vio::from_pairs<T, V>(f);   // (exact: the values came as T)
+      weight_unit<T, V>((const T*)p.w_pre, un.e[i], p.H, f);
+      held[1][i] = vio::from_pairs<T, V>(f);
+      if constexpr (GATE == GATE_CHANNEL) {
+        weight_unit<T, V>(gate, un.e[i], p.H, f);
+        held[2][i] = vio::from_pairs<T, V>(f);
+      }
+    }
+  }
   auto weight = [&](int b, const T* w, int i, uint64_t* f) {
-    if constexpr (copied) vio::to_pairs<T, V>(vio::load_raw<T, V>(s_w + b * (p.line_bytes / (int)sizeof(T)) + un.c[i] * V), f);
+    if constexpr (HELD) vio::to_pairs<T, V>(held[b][i], f);
+    else if constexpr (COPIED) vio::to_pairs<T, V>(vio::load_raw<T, V>(s_w + b * line + un.c[i] * V), f);
     else vio::to_pairs<T, V>(vio::load_raw<T, V>(w + un.e[i]), f);
   };
   __syncthreads();
   for (int k = 0; RING && k < S - 1 && k < n; ++k) {
-    if (threadIdx.x == 0) ring.bring(k, blockIdx.x + k * step);
-    ring.load_ragged(blockIdx.x + k * step);
-    ring.store_ragged(k);
+    ring.bring(k, blockIdx.x + k * step);
   }
+  if constexpr (COPIED) copy_weights<T>(s_w, (const T*)p.w_post, (const T*)p.w_pre, gate, line, ring.shift, p.H);
   __syncthreads();
   int s = 0;
   uint32_t parity = 0;
-  bool pending = false;   // a ragged value waits for its stage
-  int pending_stage = 0;
   for (int k = 0; k < n; ++k) {
     const long long row = blockIdx.x + k * step;
-    if (pending) {
-      // into the stage of the row S - 2 ahead: with more than two stages a block barrier lies before its reader
-      ring.store_ragged(pending_stage);
-      if (S == 2 && copied) __syncthreads();
-    }
     ring.wait(s, parity);
     uint64_t hv[NV][P], sq = 0ull;
     float ss[1];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (un.live[i]) {
-        ring.read(s, 0, row, un.c[i], un.e[i], un.whole[i], hv[i]);
+        ring.read(s, 0, row, un.c[i], un.e[i], un.whole[i], un.keep[i], hv[i]);
 #pragma unroll
         for (int j = 0; j < P; ++j) sq = fma_f32x2(hv[i][j], hv[i][j], sq);
       }
@@ -286,12 +284,7 @@ fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h, float* __restrict
     row_sum(ss, red);
     // every thread is past the previous row: its stage takes the row S - 1 ahead
     const int sn = s ? s - 1 : S - 1;
-    pending = RING && k + S - 1 < n;
-    if (pending) {
-      if (threadIdx.x == 0) ring.bring(sn, row + (S - 1) * step);
-      ring.load_ragged(row + (S - 1) * step);
-      pending_stage = sn;
-    }
+    if (RING && k + S - 1 < n) ring.bring(sn, row + (S - 1) * step);
     const float r1 = rsqrtf(ss[0] / (float)p.H + p.eps);
     sq = 0ull;
 #pragma unroll
@@ -300,12 +293,12 @@ fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h, float* __restrict
       uint64_t w[P], v[P];
       weight(0, (const T*)p.w_post, i, w);
       if constexpr (GATE != GATE_NONE) {
-        if constexpr (FULL) ring.read(s, NB - 1, row, un.c[i], un.e[i], un.whole[i], v);
+        if constexpr (FULL) ring.read(s, NB - 1, row, un.c[i], un.e[i], un.whole[i], un.keep[i], v);
         else weight(2, gate, i, v);
 #pragma unroll
         for (int j = 0; j < P; ++j) w[j] = mul_f32x2(w[j], v[j]);
       }
-      ring.read(s, 1, row, un.c[i], un.e[i], un.whole[i], v);
+      ring.read(s, 1, row, un.c[i], un.e[i], un.whole[i], un.keep[i], v);
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         const uint64_t b = mul_f32x2(mul_f32x2(hv[i][j], vio::twice(r1)), w[j]);
@@ -338,16 +331,15 @@ fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h, float* __restrict
 }
 
 // part: [blocks][2][H]: the two row sums of each block
-template <class T, int V, int NV, bool SHIFT, int GATE>
+template <class T, int V, int NV, bool RING, bool SHIFT, int GATE>
 __global__ void __launch_bounds__(NV > 2 ? MOST_THREADS : MAX_THREADS, 1)
 bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, const float* __restrict__ rstd,
            T* __restrict__ dx, T* __restrict__ dres, T* __restrict__ dgate, float* __restrict__ part) {
   constexpr bool FULL = GATE == GATE_FULL;
   constexpr int NB = FULL ? 5 : 4;
-  constexpr bool HELD = NV <= 2;   // weights in registers; wider rows read them again (they stay in L1 and L2)
+  constexpr bool HELD = NV == 2;   // weights in registers
   extern __shared__ __align__(128) uint8_t smem[];
   float* red = (float*)(smem + 64);
-  constexpr bool RING = NV == 2;
   Ring<T, V, NB, RING, SHIFT> ring;
   ring.base[0] = (const T*)p.x;
   ring.base[1] = (const T*)p.res;
@@ -361,7 +353,7 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
     ring.ld[4] = p.ldgate;
   }
   ring.setup(smem, p);
-  const Units<V, NV, SHIFT> un(ring.shift, p.H);
+  const Units<V, NV, RING, SHIFT> un(ring.shift, p.H);
   const T* wq = (const T*)p.w_post;
   const T* wp = (const T*)p.w_pre;
   const T* gate = GATE == GATE_CHANNEL ? (const T*)p.gate : nullptr;
@@ -371,19 +363,24 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
   __syncthreads();
   const int S = p.stages;
   for (int k = 0; RING && k < S - 1 && k < n; ++k) {
-    if (threadIdx.x == 0) ring.bring(k, blockIdx.x + k * step);
-    ring.load_ragged(blockIdx.x + k * step);
-    ring.store_ragged(k);
+    ring.bring(k, blockIdx.x + k * step);
   }
   constexpr int P = V / 2;
-  // held: g w_post (w_post alone for a full gate) as floats, w_pre as it came
+  // held: g w_post (w_post alone for a full gate) as floats, w_pre as it came; wider rows read copies in shared memory
   uint64_t gwh[HELD ? NV : 1][P];
   vio::Raw<T, V> hp[HELD ? NV : 1];
+  T* s_w = (T*)(smem + HEADER + (RING ? (size_t)S * NB * p.line_bytes : 0));
+  const int line = p.line_bytes / (int)sizeof(T);
+  if constexpr (!HELD) copy_weights<T>(s_w, wq, wp, gate, line, ring.shift, p.H);
+  auto weight = [&](int b, const T* w, int i, uint64_t* f) {
+    if constexpr (HELD) weight_unit<T, V>(w, un.e[i], p.H, f);
+    else vio::to_pairs<T, V>(vio::load_raw<T, V>(s_w + b * line + un.c[i] * V), f);
+  };
   auto gated = [&](int i, uint64_t* gw) {   // w_post, times a channel gate
-    vio::to_pairs<T, V>(weight_unit<T, V>(wq, un.e[i], p.H, 0.f), gw);
+    weight(0, wq, i, gw);
     if constexpr (GATE == GATE_CHANNEL) {
       uint64_t g[P];
-      vio::to_pairs<T, V>(weight_unit<T, V>(gate, un.e[i], p.H, 0.f), g);
+      weight(2, gate, i, g);
 #pragma unroll
       for (int j = 0; j < P; ++j) gw[j] = mul_f32x2(gw[j], g[j]);
     }
@@ -392,7 +389,9 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       gated(i, gwh[i]);
-      hp[i] = weight_unit<T, V>(wp, un.e[i], p.H, 0.f);
+      uint64_t f[P];
+      weight(1, wp, i, f);
+      hp[i] = vio::from_pairs<T, V>(f);
     }
   }
   __syncthreads();
@@ -403,7 +402,7 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
 #pragma unroll
     for (int j = 0; j < P; ++j) sum_post[i][j] = sum_pre[i][j] = 0ull;
   auto staged = [&](int s, long long row, int b, int i, uint64_t* f) {
-    ring.read(s, b, row, un.c[i], un.e[i], un.whole[i], f);
+    ring.read(s, b, row, un.c[i], un.e[i], un.whole[i], un.keep[i], f);
   };
   auto weights = [&](int i, int s, long long row, uint64_t* gw, uint64_t* q) {   // g w_post and w_pre
     if constexpr (HELD) {
@@ -412,7 +411,7 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
       vio::to_pairs<T, V>(hp[i], q);
     } else {
       gated(i, gw);
-      vio::to_pairs<T, V>(weight_unit<T, V>(wp, un.e[i], p.H, 0.f), q);
+      weight(1, wp, i, q);
     }
     if constexpr (FULL) {
       uint64_t g[P];
@@ -423,15 +422,9 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
   };
   int s = 0;
   uint32_t parity = 0;
-  bool pending = false;
-  int pending_stage = 0;
   float n1 = n > 0 ? rstd[blockIdx.x] : 0.f, n2 = n > 0 ? rstd[p.rows + blockIdx.x] : 0.f;
   for (int k = 0; k < n; ++k) {
     const long long row = blockIdx.x + k * step;
-    if (pending) {
-      ring.store_ragged(pending_stage);   // (as in the forward kernel)
-      if (SHIFT && S == 2) __syncthreads();
-    }
     const float r1 = n1, r2 = n2;
     if (k + 1 < n) {
       n1 = rstd[row + step];
@@ -463,12 +456,7 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
     float sums[3] = {vio::sum_of(s0), vio::sum_of(s1), vio::sum_of(s2)};
     row_sum(sums, red);
     const int sn = s ? s - 1 : S - 1;
-    pending = RING && k + S - 1 < n;
-    if (pending) {
-      if (threadIdx.x == 0) ring.bring(sn, row + (S - 1) * step);
-      ring.load_ragged(row + (S - 1) * step);
-      pending_stage = sn;
-    }
+    if (RING && k + S - 1 < n) ring.bring(sn, row + (S - 1) * step);
     const float m1 = sums[0] * inv_h * r2;
     const float m2 = (sums[1] - m1 * sums[2]) * inv_h;
 #pragma unroll
@@ -515,6 +503,8 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
         for (int j = 0; j < P; ++j) sum_post[i][j] = fma_f32x2(u[j], d[j], sum_post[i][j]);
       }
     }
+    // the tensors' last row may have had values put in by themselves: a barrier before they are read
+    if (RING && SHIFT && row + (S - 1) * step == p.rows - 1) __syncthreads();
     if (++s == S) {
       s = 0;
       parity ^= 1;
@@ -592,7 +582,7 @@ __global__ void __launch_bounds__(1024) finish_kernel(const float* __restrict__ 
 
 // Units per thread, threads, blocks and the ring.
 struct Shape {
-  int nv, threads, stages, grid, line_bytes;
+  int nv, ring, threads, stages, grid, line_bytes;
   size_t smem;
 };
 static Shape shape_of(int rows, int H, int elem, int tensors, bool backward) {
@@ -602,23 +592,34 @@ static Shape shape_of(int rows, int H, int elem, int tensors, bool backward) {
   s.nv = 2;
   while (s.nv * MAX_THREADS < units && s.nv < 32 / V) s.nv *= 2;   // 32 values per thread at most
   s.threads = ((units + s.nv - 1) / s.nv + 31) / 32 * 32;
-  if (s.threads < 2 * V * tensors && H % V) s.threads = (2 * V * tensors + 31) / 32 * 32;   // one thread per ragged value
   s.line_bytes = units * 16;
-  const bool ring = s.nv == 2;
-  const size_t row = ring ? (size_t)tensors * s.line_bytes : 0;
-  const size_t extra = HEADER + (!backward && (H % V || !ring) ? (size_t)3 * s.line_bytes : 0);
-  const size_t budget = 227 * 1024;
+  const int sms = tdllm_num_sms();
   int resident = (backward || s.nv > 2 ? 512 : 1024) / s.threads;   // by the kernels' registers
   if (resident < 1) resident = 1;
   if (resident > 16) resident = 16;
-  // three rows per block; fewer blocks on an SM where they would not fit (the widest ring has 80 KiB rows: two fit)
-  while (resident > 1 && resident * (3 * row + extra + 1024) > budget) --resident;
-  s.stages = ring ? (int)((budget / resident - extra - 1024) / row) : 1;
-  if (s.stages > 4) s.stages = 4;
-  s.smem = extra + s.stages * row;
-  const int most = (tdllm_num_sms() * resident + 7) / 8 * 8;   // a multiple of the values in a line: one shift per block
-  const int need = (rows + 7) / 8 * 8;
-  s.grid = need < most ? need : most;
+  const size_t row = (size_t)tensors * s.line_bytes;
+  const size_t weights = (size_t)3 * s.line_bytes, budget = 227 * 1024;
+  // a multiple of the values in a line: one shift per block
+  auto blocks = [&](int most) { return most < rows ? (most + 7) / 8 * 8 : (rows + 7) / 8 * 8; };
+  s.ring = s.nv == 2;
+  if (s.ring) {
+    const size_t extra = HEADER + (!backward && H % V ? weights : 0);
+    // three rows per block; fewer blocks on an SM where they would not fit (the widest ring has 80 KiB rows: two fit)
+    while (resident > 1 && resident * (3 * row + extra + 1024) > budget) --resident;
+    s.stages = (int)((budget / resident - extra - 1024) / row);
+    if (s.stages > 4) s.stages = 4;
+    s.smem = extra + s.stages * row;
+    int most = sms * resident;
+    // backward: a block's partial sums are two rows of floats; keep them under a sixth of what its own rows move
+    if (backward && most > rows * elem / 16) most = rows * elem / 16 > sms ? rows * elem / 16 : sms;
+    s.grid = blocks(most);
+    if (s.grid >= rows) s.ring = 0;   // one row per block: nothing to bring in ahead
+  }
+  if (!s.ring) {
+    s.stages = 1;
+    s.smem = HEADER + (s.nv > 2 ? weights : 0);
+    if (s.nv > 2) s.grid = blocks(sms);
+  }
   return s;
 }
 
@@ -641,16 +642,17 @@ static cudaError_t sandwich_smem(K kernel, size_t bytes) {
   return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
 }
 
-#define SANDWICH_GATE(T, V, NV, SHIFT, BODY)                                   \
-  if (gate_kind == GATE_NONE) { BODY(T, V, NV, SHIFT, GATE_NONE); }            \
-  else if (gate_kind == GATE_CHANNEL) { BODY(T, V, NV, SHIFT, GATE_CHANNEL); } \
-  else { BODY(T, V, NV, SHIFT, GATE_FULL); }
-// (rows too wide for the ring: one form for aligned and shifted widths)
-#define SANDWICH_TYPE(T, V, BODY)                                              \
-  if (s.nv == 2 && H % V == 0) { SANDWICH_GATE(T, V, 2, false, BODY) }         \
-  else if (s.nv == 2) { SANDWICH_GATE(T, V, 2, true, BODY) }                   \
-  else if (s.nv == 4) { SANDWICH_GATE(T, V, 4, true, BODY) }                   \
-  else if constexpr (V == 4) { SANDWICH_GATE(T, V, 8, true, BODY) }
+#define SANDWICH_GATE(T, V, NV, RING, SHIFT, BODY)                                   \
+  if (gate_kind == GATE_NONE) { BODY(T, V, NV, RING, SHIFT, GATE_NONE); }            \
+  else if (gate_kind == GATE_CHANNEL) { BODY(T, V, NV, RING, SHIFT, GATE_CHANNEL); } \
+  else { BODY(T, V, NV, RING, SHIFT, GATE_FULL); }
+// (without the ring: one form for aligned and shifted widths)
+#define SANDWICH_TYPE(T, V, BODY)                                                     \
+  if (s.ring && H % V == 0) { SANDWICH_GATE(T, V, 2, true, false, BODY) }             \
+  else if (s.ring) { SANDWICH_GATE(T, V, 2, true, true, BODY) }                       \
+  else if (s.nv == 2) { SANDWICH_GATE(T, V, 2, false, true, BODY) }                   \
+  else if (s.nv == 4) { SANDWICH_GATE(T, V, 4, false, true, BODY) }                   \
+  else if constexpr (V == 4) { SANDWICH_GATE(T, V, 8, false, true, BODY) }
 #define SANDWICH_DISPATCH(BODY)                                                \
   if (dtype == 0) { SANDWICH_TYPE(__nv_bfloat16, 8, BODY) }                    \
   else if (dtype == 1) { SANDWICH_TYPE(__half, 8, BODY) }                      \
@@ -658,7 +660,7 @@ static cudaError_t sandwich_smem(K kernel, size_t bytes) {
 
 // a ring of fewer than two rows would wait for a row that nobody brings
 static int sandwich_ring(const char* who, const sandwich::Shape& s) {
-  if (s.nv == 2 ? s.stages >= 2 && s.stages <= sandwich::MAX_STAGES : s.stages == 1) return 0;
+  if (s.ring ? s.stages >= 2 && s.stages <= sandwich::MAX_STAGES : s.stages == 1) return 0;
   tdllm_host::set_last_error("%s: %d stages", who, s.stages);
   return 1;
 }
@@ -691,9 +693,9 @@ extern "C" int tdllm_sandwich_norm_fwd(const void* x, const void* res, const voi
   if (sandwich_ring("sandwich_norm_fwd", s)) return 1;
   const Args p = {x, res, w_post, w_pre, gate, ldx, ldres, ldgate, rows, H, gate_kind, a, eps, s.stages, s.line_bytes};
   cudaError_t e = cudaErrorInvalidValue;
-#define FWD(T, V, NV, SHIFT, GATE)                                                             \
+#define FWD(T, V, NV, RING, SHIFT, GATE)                                                             \
   do {                                                                                  \
-    auto k = fwd_kernel<T, V, NV, SHIFT, GATE>;                                                \
+    auto k = fwd_kernel<T, V, NV, RING, SHIFT, GATE>;                                                \
     e = sandwich_smem(k, s.smem);                                                       \
     if (e == cudaSuccess)                                                               \
       k<<<s.grid, s.threads, s.smem, (cudaStream_t)stream>>>(p, (T*)y, (T*)h, rstd);    \
@@ -745,9 +747,9 @@ extern "C" int tdllm_sandwich_norm_bwd(const void* x, const void* res, const voi
   cudaError_t e = cudaSuccess;
   if (rows > 0) {
     e = cudaErrorInvalidValue;
-#define BWD(T, V, NV, SHIFT, GATE)                                                                                              \
+#define BWD(T, V, NV, RING, SHIFT, GATE)                                                                                              \
   do {                                                                                                                   \
-    auto k = bwd_kernel<T, V, NV, SHIFT, GATE>;                                                                                 \
+    auto k = bwd_kernel<T, V, NV, RING, SHIFT, GATE>;                                                                                 \
     e = sandwich_smem(k, s.smem);                                                                                        \
     if (e == cudaSuccess)                                                                                                \
       k<<<s.grid, s.threads, s.smem, st>>>(p, (const T*)dy, (const T*)dh, rstd, (T*)dx, (T*)dres, (T*)dgate, scratch);   \

@@ -80,6 +80,36 @@ __device__ __forceinline__ Raw<T, N> from_pairs(const uint64_t* p) {
   }
   return r;
 }
+// values outside [0, H) of the N that start at e become zero
+template <int N>
+__device__ __forceinline__ void trim_pairs(uint64_t* p, int e, int H) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    float a, b;
+    unpair_f32(p[i], a, b);
+    p[i] = pair_f32(e + 2 * i >= 0 && e + 2 * i < H ? a : 0.f, e + 2 * i + 1 >= 0 && e + 2 * i + 1 < H ? b : 0.f);
+  }
+}
+// the same N values by single accesses, those outside [0, H) left out (read as zero)
+template <class T, int N>
+__device__ __forceinline__ void load_pairs_each(const T* row, int e, int H, uint64_t* p) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const int c = e + 2 * i;
+    p[i] = pair_f32(row && c >= 0 && c < H ? to_f(row[c]) : 0.f, row && c + 1 >= 0 && c + 1 < H ? to_f(row[c + 1]) : 0.f);
+  }
+}
+template <class T, int N>
+__device__ __forceinline__ void store_pairs_each(T* row, int e, int H, const uint64_t* p) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const int c = e + 2 * i;
+    float a, b;
+    unpair_f32(p[i], a, b);
+    if (c >= 0 && c < H) row[c] = from_f<T>(a);
+    if (c + 1 >= 0 && c + 1 < H) row[c + 1] = from_f<T>(b);
+  }
+}
 __device__ __forceinline__ uint64_t twice(float v) { return pair_f32(v, v); }
 __device__ __forceinline__ float sum_of(uint64_t p) {
   float a, b;
