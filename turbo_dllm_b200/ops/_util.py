@@ -38,11 +38,25 @@ def dtype_code(t: torch.Tensor) -> int | None:
     return _DTYPE_CODES.get(t.dtype)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(t: torch.Tensor):
-    """Makes the tensor's device the current one for a launch on it (and for `stream()`)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    """Makes the tensor's device the current one for a launch on it."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        return _HERE
     return torch.cuda.device(t.device)
+
+
+def stream_of(t: torch.Tensor) -> int:
+    """The current stream of the tensor's device."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def refuse_twice(what: str) -> None:
+    """For a backward pass made of kernels: with create_graph its results would silently carry no graph."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} cannot be differentiated twice")
 
 
 def grad_sink(param: torch.Tensor):

@@ -9,7 +9,8 @@ from __future__ import annotations
 import torch
 
 from ..kernels import native
-from ._util import dtype_code, grad_sink, mark_grad_written, on_device, ptr, scratch, stream, use_native
+from ._util import (dtype_code, grad_sink, mark_grad_written, on_device, ptr, refuse_twice, scratch, stream, stream_of,
+                    use_native)
 
 
 native.register_signatures({
@@ -48,7 +49,7 @@ class _RMSNorm(torch.autograd.Function):
         ctx.has_res = has_res
         ctx.shape = x.shape
         if has_res:
-            return y.view(x.shape), h.view(x.shape)
+            return (y, h) if x.dim() == 2 else (y.view(x.shape), h.view(x.shape))
         return y.view(x.shape)
 
     @staticmethod
@@ -101,6 +102,7 @@ def sandwich_norm_reference(x, res, w_post, w_pre, gate=None, res_scale: float =
 
 
 GATE_NONE, GATE_CHANNEL, GATE_FULL = 0, 1, 2
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
@@ -108,23 +110,25 @@ def _rows2d(t: torch.Tensor) -> torch.Tensor:
     kernels ask of every row operand. A view where the tensor is like that, else a copy."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    H, size = t.shape[1], t.element_size()
-    if (t.stride(1) == 1 or H == 1) and t.data_ptr() % 16 == 0 \
-            and (t.shape[0] <= 1 or (t.stride(0) - H) * size % 16 == 0):
+    if t.is_contiguous():
+        return t if t.data_ptr() % 16 == 0 else t.clone()
+    H = t.shape[1]
+    if (t.stride(1) == 1 or H == 1) and t.data_ptr() % 16 == 0 and (t.stride(0) - H) * t.element_size() % 16 == 0:
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t.contiguous()
 
 
 def _sandwich_forward(x, res, w_post, w_pre, gate, res_scale, eps, want_stats):
     kind = GATE_NONE if gate is None else GATE_CHANNEL if gate.dim() == 1 else GATE_FULL
     rows, H = x.shape
-    y, h = torch.empty(rows, H, dtype=x.dtype, device=x.device), torch.empty(rows, H, dtype=x.dtype, device=x.device)
-    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if want_stats else None
+    dtype, dev = x.dtype, x.device
+    y, h = torch.empty((rows, H), dtype=dtype, device=dev), torch.empty((rows, H), dtype=dtype, device=dev)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=dev) if want_stats else None
     with on_device(x):
         native.check(native.lib().tdllm_sandwich_norm_fwd(
-            ptr(x), ptr(res), ptr(w_post), ptr(w_pre), ptr(gate), ptr(y), ptr(h), ptr(stats), _row_stride(x), _row_stride(res),
-            _row_stride(gate) if kind == GATE_FULL else H, rows, H, kind, dtype_code(x), res_scale, eps, stream()),
-            "sandwich_norm_fwd")
+            x.data_ptr(), res.data_ptr(), w_post.data_ptr(), w_pre.data_ptr(), ptr(gate), y.data_ptr(), h.data_ptr(), ptr(stats),
+            _row_stride(x), _row_stride(res), _row_stride(gate) if kind == GATE_FULL else H, rows, H, kind, _DTYPES[dtype],
+            res_scale, eps, stream_of(x)), "sandwich_norm_fwd")
     return y, h, stats
 
 
@@ -133,7 +137,9 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _packed(t: torch.Tensor, rows: int, H: int) -> torch.Tensor:
-    t = t.reshape(rows, H).contiguous()
+    if t.dim() != 2:
+        t = t.reshape(rows, H)
+    t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -147,19 +153,20 @@ class _SandwichNorm(torch.autograd.Function):
         ctx.refs = (w_post, w_pre, gate if gate is not None and gate.dim() == 1 else None)
         ctx.meta = (res_scale, x.shape)
         ctx.set_materialize_grads(False)
-        return y.view(x.shape), h.view(x.shape)
+        return (y, h) if x.dim() == 2 else (y.view(x.shape), h.view(x.shape))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh):
+        refuse_twice("sandwich_norm")
         x, res, w_post, w_pre, gate, stats = ctx.saved_tensors
         res_scale, shape = ctx.meta
         rows, H = x.shape
         kind = GATE_NONE if gate is None else GATE_CHANNEL if gate.dim() == 1 else GATE_FULL
         dy = None if dy is None else _packed(dy, rows, H)
         dh = None if dh is None else _packed(dh, rows, H)
-        dx, dres = torch.empty(rows, H, dtype=x.dtype, device=x.device), torch.empty(rows, H, dtype=x.dtype, device=x.device)
-        dgate = torch.empty(rows, H, dtype=x.dtype, device=x.device) if kind == GATE_FULL else None
+        dtype, dev = x.dtype, x.device
+        dx, dres = torch.empty((rows, H), dtype=dtype, device=dev), torch.empty((rows, H), dtype=dtype, device=dev)
+        dgate = torch.empty((rows, H), dtype=dtype, device=dev) if kind == GATE_FULL else None
         # vectors that own a slice of the flat gradient buffer are written (or added) there, the others are returned
         targets, flags, returned, written = [], [], [], []
         for vec, ref, need in zip((w_post, w_pre, gate if kind == GATE_CHANNEL else None), ctx.refs, ctx.needs_input_grad[2:5]):
@@ -176,16 +183,20 @@ class _SandwichNorm(torch.autograd.Function):
         with on_device(x):
             lib = native.lib()
             # (allocated per call: streams and captured graphs do not share it)
-            part = torch.empty(lib.tdllm_sandwich_norm_parts(rows, H) * 2 * H, dtype=torch.float32, device=x.device)
+            part = torch.empty((lib.tdllm_sandwich_norm_parts(rows, H) * 2 * H,), dtype=torch.float32, device=dev)
             native.check(lib.tdllm_sandwich_norm_bwd(
-                ptr(x), ptr(res), ptr(w_post), ptr(w_pre), ptr(gate), ptr(dy), ptr(dh), ptr(stats), ptr(dx), ptr(dres),
-                ptr(dgate), *(ptr(t) for t in targets), *flags, ptr(part), _row_stride(x), _row_stride(res),
-                _row_stride(gate) if kind == GATE_FULL else H, rows, H, kind, dtype_code(x), res_scale, stream()),
+                x.data_ptr(), res.data_ptr(), w_post.data_ptr(), w_pre.data_ptr(), ptr(gate), ptr(dy), ptr(dh),
+                stats.data_ptr(), dx.data_ptr(), dres.data_ptr(), ptr(dgate), *(ptr(t) for t in targets), *flags, ptr(part), _row_stride(x), _row_stride(res),
+                _row_stride(gate) if kind == GATE_FULL else H, rows, H, kind, _DTYPES[dtype], res_scale, stream_of(x)),
                 "sandwich_norm_bwd")
         for ref in written:
             mark_grad_written(ref)
-        return (dx.view(shape), dres.view(shape), returned[0], returned[1],
-                dgate.view(shape) if kind == GATE_FULL else returned[2], None, None)
+        if kind != GATE_FULL:
+            dgate = returned[2]
+        if len(shape) != 2:
+            dx, dres = dx.view(shape), dres.view(shape)
+            dgate = dgate.view(shape) if kind == GATE_FULL else dgate
+        return dx, dres, returned[0], returned[1], dgate, None, None
 
 
 def sandwich_norm(x: torch.Tensor, res: torch.Tensor, w_post: torch.Tensor, w_pre: torch.Tensor, *,
@@ -204,9 +215,11 @@ def sandwich_norm(x: torch.Tensor, res: torch.Tensor, w_post: torch.Tensor, w_pr
         raise ValueError(f"w_post and w_pre must be vectors of {H} values")
     if gate is not None and gate.shape != (H,) and gate.shape != x.shape:
         raise ValueError(f"gate must be a vector of {H} values or have x's shape, got {tuple(gate.shape)}")
-    given = [t for t in (res, w_post, w_pre, gate) if t is not None]
-    if any(t.dtype != x.dtype or t.device != x.device for t in given):
-        raise ValueError("x, res, the weights and the gate must share dtype and device")
+    dtype, dev, grad = x.dtype, x.device, x.requires_grad
+    for t in (res, w_post, w_pre) if gate is None else (res, w_post, w_pre, gate):
+        if t.dtype != dtype or t.device != dev:
+            raise ValueError("x, res, the weights and the gate must share dtype and device")
+        grad = grad or t.requires_grad
     if dtype_code(x) is None:
         return sandwich_norm_reference(x, res, w_post, w_pre, gate, res_scale, eps)
     if H > SANDWICH_MAX_WIDTH:
@@ -214,7 +227,7 @@ def sandwich_norm(x: torch.Tensor, res: torch.Tensor, w_post: torch.Tensor, w_pr
     w_post, w_pre = w_post.contiguous(), w_pre.contiguous()
     if gate is not None and gate.dim() == 1:
         gate = gate.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *given)):
+    if grad and torch.is_grad_enabled():
         return _SandwichNorm.apply(x, res, w_post, w_pre, gate, float(res_scale), float(eps))
     g2 = gate if gate is None or gate.dim() == 1 else _rows2d(gate)
     y, h, _ = _sandwich_forward(_rows2d(x), _rows2d(res), w_post, w_pre, g2, float(res_scale), float(eps), False)

@@ -20,7 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from ..kernels import native
-from ._util import dtype_code, on_device, ptr, stream
+from ._util import dtype_code, on_device, refuse_twice, stream_of
 
 native.register_signatures({
     "tdllm_rotary": (native.c_int, [native.c_void_p] * 4 + [native.c_int] * 4 + [native.c_ll] * 2 + [native.c_int] * 2
@@ -107,14 +107,16 @@ def rotary_reference(x, positions, freqs, pairs: str = "half", scale: float = 1.
 
 def _turn(x, positions, freqs, half: int, scale: float, back: bool):
     rows, H, D = x.shape
-    if x.stride(2) != 1:
+    ld_row, ld_head, inner = x.stride()
+    if inner != 1:
         x = x.contiguous()
-    out = torch.empty(rows, H, D, dtype=x.dtype, device=x.device)
-    if out.numel():
+        ld_row, ld_head = H * D, D
+    out = torch.empty((rows, H, D), dtype=x.dtype, device=x.device)
+    if rows and H:
         with on_device(x):
             native.check(native.lib().tdllm_rotary(
-                ptr(x), ptr(out), ptr(positions), ptr(freqs), rows, H, D, 2 * freqs.shape[0], x.stride(0), x.stride(1), half,
-                dtype_code(x), float(scale), -1.0 if back else 1.0, stream()), "rotary")
+                x.data_ptr(), out.data_ptr(), positions.data_ptr(), freqs.data_ptr(), rows, H, D, 2 * freqs.shape[0], ld_row,
+                ld_head, half, dtype_code(x), scale, -1.0 if back else 1.0, stream_of(x)), "rotary")
     return out
 
 
@@ -126,8 +128,8 @@ class _Rotary(torch.autograd.Function):
         return _turn(x, positions, freqs, half, scale, False)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        refuse_twice("rotary")
         positions, freqs = ctx.saved_tensors
         return _turn(dout, positions, freqs, *ctx.meta, True), None, None, None, None
 

@@ -30,7 +30,7 @@ from dataclasses import dataclass, field
 import torch
 
 from ..kernels import native
-from ._util import ptr
+from ._util import on_device, ptr, refuse_twice, stream_of
 from .attention import TILE, MaskLayout, backward_chunk_tiles, backward_mode
 
 native.register_signatures({
@@ -226,10 +226,6 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]     # (a single row's stride may be anything)
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
 def _mod_args(transform: ScoreTransform | None, L: dict):
     """(softcap, slope2, q_pos, k_pos) of a launch and the tensors behind the pointers."""
     if transform is None:
@@ -241,7 +237,7 @@ def _mod_args(transform: ScoreTransform | None, L: dict):
 
 
 def _int32(t: torch.Tensor) -> torch.Tensor:
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def _forward_few_rows(q, k, v, layout, transform, scale):
@@ -261,7 +257,7 @@ def _forward_few_rows(q, k, v, layout, transform, scale):
     rc = lib.tdllm_attn_few_rows(
         ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(part), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k),
         _row_stride(v), out.stride(0), TILE, *(ptr(t) for t in meta), float(scale),
-        0.0 if transform is None else float(transform.softcap), *(ptr(t) for t in bias), _stream(q))
+        0.0 if transform is None else float(transform.softcap), *(ptr(t) for t in bias), stream_of(q))
     native.check(rc, "attn_few_rows" if part is None else "attn_few_rows_split")
     return out, lse
 
@@ -280,7 +276,7 @@ def _forward(q, k, v, layout, transform, scale, for_backward=False):
     rc = native.lib().tdllm_attn_fwd_scored(
         ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(lse), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v),
         out.stride(0), ptr(L["q_lo"]), ptr(L["q_hi"]), ptr(L["q_grp"]), ptr(L["k_code"]), ptr(L["f_ptr"]), ptr(L["f_idx"]),
-        ptr(L["f_order"]), L["nqt"], float(scale), *mod, _stream(q))
+        ptr(L["f_order"]), L["nqt"], float(scale), *mod, stream_of(q))
     native.check(rc, "attn_fwd_scored")
     return out, lse, rest
 
@@ -301,7 +297,7 @@ def _backward(q, k, v, out, rest, dout, lse, layout, transform, scale):
         ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(lse), ptr(delta), ptr(acc),
         nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v), _row_stride(out), _row_stride(dout),
         dq.stride(0), dk.stride(0), dv.stride(0), ptr(L["q_lo"]), ptr(L["q_hi"]), ptr(L["q_grp"]), ptr(L["k_code"]),
-        ptr(W["w_ptr"]), ptr(W["w_idx"]), ptr(W["w_order"]), W["n_work"], L["nqt"], L["nkt"], float(scale), *mod, _stream(q))
+        ptr(W["w_ptr"]), ptr(W["w_idx"]), ptr(W["w_order"]), W["n_work"], L["nqt"], L["nkt"], float(scale), *mod, stream_of(q))
     native.check(rc, "attn_bwd_scored")
     return dq, dk, dv
 
@@ -309,7 +305,7 @@ def _backward(q, k, v, out, rest, dout, lse, layout, transform, scale):
 class _ScoredAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, layout, transform, scale):
-        with torch.cuda.device(q.device):
+        with on_device(q):
             q, k, v = _operand(q), _operand(k), _operand(v)
             out, lse, rest = _forward(q, k, v, layout, transform, scale, for_backward=True)
         ctx.save_for_backward(q, k, v, out, rest, lse)
@@ -319,10 +315,10 @@ class _ScoredAttention(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _dlse):
+        refuse_twice("scored attention")
         q, k, v, out, rest, lse = ctx.saved_tensors
-        with torch.cuda.device(q.device):
+        with on_device(q):
             grads = _backward(q, k, v, out, rest, _operand(dout), lse, ctx.layout, ctx.transform, ctx.scale)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
 
@@ -351,7 +347,7 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.full((q.shape[1], q.shape[0]), float("-inf"), dtype=torch.float32, device=q.device)
     else:
-        with torch.cuda.device(q.device):
+        with on_device(q):
             out, lse, _ = _forward(_operand(q), _operand(k), _operand(v), layout, transform, scale)
             lse = lse[:, : q.shape[0]]
     return (out, lse) if return_lse else out
