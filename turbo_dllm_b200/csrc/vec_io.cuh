@@ -18,9 +18,9 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
 
-// N consecutive values of T: one 16-byte access when N fills it, else value by value
+// N (a power of two) consecutive values of T in one access of at most 16 bytes, aligned to its size
 template <class T, int N>
-struct alignas(N * sizeof(T) == 16 ? 16 : sizeof(T)) Raw {
+struct alignas(N * sizeof(T)) Raw {
   T v[N];
 };
 template <class T, int N>
