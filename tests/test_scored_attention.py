@@ -371,6 +371,77 @@ def test_strides_and_alignment():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("make", [lambda: document_layout([300, 0, 77], prefix=[40, 0, 0], rows=400, device="cuda"),
+                                  lambda: blocks(640, 32, window=200)[0], lambda: step_layout([70, 900, 0], 60, capacity=1000)[0],
+                                  lambda: document_layout([1], device="cuda")])
+def test_plan_matches_the_dense_mask(make):
+    """Every visible pair lies in a listed tile, tiles without a mask are fully visible, lists are complete and in order."""
+    import ctypes
+
+    from turbo_dllm_b200.ops import scored_attention as sa
+
+    L = make()
+    P = sa._plan(L)
+    off = (ctypes.c_longlong * 11)()
+    from turbo_dllm_b200.kernels import native
+
+    chunk = P["chunk"]
+    native.lib().tdllm_attn_plan_size(L.nq, L.nk, chunk, off)
+    buf = P["buf"].cpu().tolist()
+    nqt, nkt = P["nqt"], P["nkt"]
+    m = torch.zeros(nqt * 128, nkt * 128, dtype=torch.bool)
+    m[: L.nq, : L.nk] = L.dense_mask().cpu()
+    any_ = m.view(nqt, 128, nkt, 128).any(3).any(1)
+    real = torch.arange(nqt * 128) < L.nq
+    all_ = (m | ~real[:, None]).view(nqt, 128, nkt, 128).all(3).all(1)
+    part = lambda i, n: buf[off[i]: off[i] + n]   # noqa: E731
+    f_ptr, f_order = part(4, nqt + 1), part(6, nqt)
+    lists = [buf[off[5] + f_ptr[i]: off[5] + f_ptr[i + 1]] for i in range(nqt)]
+    for i, l in enumerate(lists):
+        tiles = [e >> 1 for e in l]
+        assert tiles == sorted(set(tiles)) and set(any_[i].nonzero().flatten().tolist()) <= set(tiles)
+        assert all(bool(all_[i, e >> 1]) for e in l if not e & 1)
+    assert sorted(f_order) == list(range(nqt)) and all(len(lists[a]) >= len(lists[b]) for a, b in zip(f_order, f_order[1:]))
+    nch = (nqt + chunk - 1) // chunk
+    w_ptr, w_order = part(7, nch * nkt + 1), part(9, nch * nkt)
+    back = {(e >> 1, it % nkt, e & 1) for it in range(nch * nkt) for e in buf[off[8] + w_ptr[it]: off[8] + w_ptr[it + 1]]}
+    assert back == {(i, e >> 1, e & 1) for i, l in enumerate(lists) for e in l}
+    assert all((e >> 1) // chunk == it // nkt for it in range(nch * nkt) for e in buf[off[8] + w_ptr[it]: off[8] + w_ptr[it + 1]])
+    assert sorted(w_order) == list(range(nch * nkt))
+
+
+@pytest.mark.gpu
+def test_a_layout_that_is_written_to_and_a_plan_built_inside_a_capture():
+    q, k, v = _operands(300, 300, 4, 2, 13)
+    L = document_layout([300], device="cuda")
+    tr = ScoreTransform(20.0)
+    scored_attention(q, k, v, L, tr)
+    M = document_layout([100, 200], device="cuda")
+    for a, b in ((L.q_lo, M.q_lo), (L.q_hi, M.q_hi)):
+        a.copy_(b)
+    want = scored_attention(q, k, v, M, tr)
+    assert torch.equal(scored_attention(q, k, v, L, tr), want)
+    torch.cuda.synchronize()
+    fresh = document_layout([100, 200], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = scored_attention(q, k, v, fresh, tr)
+    # nothing of a capture is kept outside of it: its lists exist only once it has run
+    assert "scored" not in fresh._cache and torch.equal(scored_attention(q, k, v, fresh, tr), want)
+    graph.replay()
+    assert torch.equal(held, want)
+    # a graph that was captured with a layout's lists goes on using them when the layout moves on
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = scored_attention(q, k, v, fresh, tr)
+    fresh.q_hi.copy_(document_layout([300], device="cuda").q_hi)
+    scored_attention(q, k, v, fresh, tr)
+    junk = [torch.full((4096,), 7, dtype=torch.int32, device="cuda") for _ in range(64)]
+    graph.replay()
+    assert torch.equal(held, want) and len(junk) == 64
+
+
+@pytest.mark.gpu
 def test_empty_operands_and_other_types():
     e = torch.empty(0, 4, D, dtype=torch.bfloat16, device="cuda")
     L = document_layout([], device="cuda")

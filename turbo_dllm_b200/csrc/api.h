@@ -134,6 +134,11 @@ int tdllm_attn_merge_bwd(const void* go, const void* out, const float* lse, cons
                          void* stream);
 
 // ---- attention with transformed scores (score_mod.cuh) ----------------------
+// Tile lists of a mask on the device (attention_plan.cu): one buffer of tdllm_attn_plan_size ints, whose parts begin at
+// `offsets` [11]: q_lo, q_hi, q_grp, k_code (padded to whole tiles), f_ptr, f_idx, f_order, w_ptr, w_idx, w_order, scratch.
+long long tdllm_attn_plan_size(int nq, int nk, int chunk, long long* offsets);
+int tdllm_attn_plan(const int* q_lo, const int* q_hi, const int* q_grp, const int* k_code, int nq, int nk, int chunk,
+                    int* buf, void* stream);
 // As tdllm_attn_fwd / tdllm_attn_bwd_fused, on scores cap*tanh(scale*q.k/cap) - slope_h*|q_pos - k_pos|. softcap 0: no
 // cap; slope2 null: no bias, else [Hq] slopes times log2(e), with positions as floats padded to nq_pad / nk_pad.
 // Contents of query rows and keys that take part in no visible pair do not matter (keys: code -2^31).

@@ -167,6 +167,7 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   const int list_begin = p.tile_ptr[work];
   const int n = p.tile_ptr[work + 1] - list_begin;
   const int* list = p.tile_idx + list_begin;
+  if (MOD != 0 && n == 0) return;   // (the device-built lists keep their empty items; the whole CTA leaves)
   const int items = G * n;   // (query head, query tile) pairs
   const int U = 2 * items;   // 64-query units
 

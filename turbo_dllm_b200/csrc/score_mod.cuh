@@ -82,14 +82,14 @@ __device__ __forceinline__ void cap_r2(float s0, float s1, const Mod& m, float& 
   r1 = rcp_approx(d1);
 }
 // A query row's side of the mask: key codes lo .. lo + range - 1, and the noisy block `grp` (a clean row has none: a
-// code that no key carries). One unsigned comparison covers "code >= 0, lo <= code < hi": a negative code is further from
-// lo >= 0 than any range reaches.
+// code that no key carries). One unsigned comparison covers "code >= 0, lo <= code < hi": with lo raised to 0 at least, a
+// negative code is further from it than any range reaches.
 struct RowMask {
   int lo;
   unsigned range;
   int grp;
   __device__ __forceinline__ RowMask(int lo_, int hi_, int grp_)
-      : lo(lo_), range(hi_ > lo_ ? (unsigned)(hi_ - lo_) : 0u), grp(grp_ < 0 ? grp_ : DEAD_KEY + 1) {}
+      : lo(max(lo_, 0)), range(hi_ > max(lo_, 0) ? (unsigned)(hi_ - max(lo_, 0)) : 0u), grp(grp_ < 0 ? grp_ : DEAD_KEY + 1) {}
   __device__ __forceinline__ bool sees(int code) const { return (unsigned)code - (unsigned)lo < range || code == grp; }
 };
 

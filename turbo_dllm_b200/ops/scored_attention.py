@@ -20,7 +20,9 @@ The block-diffusion masks come from `block_diffusion_layout`; `document_layout` 
 a prefix that is read in both directions). On CUDA bf16 tensors with head width 128 the tcgen05 kernels run
 (`csrc/attention_fwd_sm100.cu`, `csrc/attention_bwd_fused_sm100.cu` with the transforms of `csrc/score_mod.cuh`);
 everything else takes `scored_attention_reference`. A layout's tile lists and a transform's padded positions are built on
-first use, which synchronises: run a call once before it is captured into a CUDA graph.
+first use and again when one of their tensors has been written to. A captured graph uses the lists that its layout and
+transform had then (or builds its own at every replay, if they had none): keep both objects as long as the graph. The form
+for few query rows has no lists and follows its tensors.
 """
 from __future__ import annotations
 
@@ -37,6 +39,8 @@ native.register_signatures({
     "tdllm_attn_fwd_scored": (native.c_int, [native.c_void_p] * 6 + [native.c_int] * 4 + [native.c_ll] * 4
                               + [native.c_void_p] * 7 + [native.c_int, native.c_float, native.c_float]
                               + [native.c_void_p] * 4),
+    "tdllm_attn_plan_size": (native.c_ll, [native.c_int] * 3 + [native.c_void_p]),
+    "tdllm_attn_plan": (native.c_int, [native.c_void_p] * 4 + [native.c_int] * 3 + [native.c_void_p] * 2),
     "tdllm_attn_few_rows_scratch": (native.c_ll, [native.c_int] * 4),
     "tdllm_attn_few_rows": (native.c_int, [native.c_void_p] * 6 + [native.c_int] * 4 + [native.c_ll] * 5
                             + [native.c_void_p] * 4 + [native.c_float] * 2 + [native.c_void_p] * 4),
@@ -52,6 +56,28 @@ LOG2E = 1.4426950408889634
 # query tile. B200, 32 / 8 heads, scores capped: 1 row x 20000 keys 24 us against 490, 32 x 32768 45 against 797,
 # 128 x 1024 20 against 36, 32 x 300 15.4 against 18.3
 FEW_ROWS = 128
+
+
+def _version(t: torch.Tensor) -> int:
+    return 0 if t.is_inference() else t._version
+
+
+def _kept(cache: dict, name: str, key, like: torch.Tensor, build):
+    """cache[name] if it was made for `key`, else what `build` makes on `like`'s device. What is made eagerly is complete on
+    return, so that any stream may use it; what is made while a graph is captured belongs to that graph and is not kept.
+    What a capture uses stays with its owner as long as that lives, also when a newer one takes its place."""
+    hit = cache.get(name)
+    capturing = like.is_cuda and torch.cuda.is_current_stream_capturing()
+    if hit is not None and hit[0] == key:
+        if capturing:
+            cache.setdefault(name + "_captured", []).append(hit[1])
+        return hit[1]
+    made = build()
+    if not capturing:
+        if like.is_cuda:
+            torch.cuda.current_stream(like.device).synchronize()
+        cache[name] = (key, made)
+    return made
 
 
 @dataclass(frozen=True, eq=False)
@@ -90,19 +116,19 @@ class ScoreTransform:
     def _padded(self, nq_pad: int, nk_pad: int):
         """(slopes * log2 e, q_pos, k_pos) as the kernels read them: floats, positions padded with zeros. Rebuilt when
         one of the tensors has been written to since."""
-        version = (self.slopes._version, self.q_pos._version, self.k_pos._version, nq_pad, nk_pad)
-        hit = self._cache.get("padded")
-        if hit is not None and hit[0] == version:
-            return hit[1]
+        version = (_version(self.slopes), _version(self.q_pos), _version(self.k_pos), nq_pad, nk_pad)
+        return _kept(self._cache, "padded", version, self.slopes, lambda: self._pad(nq_pad, nk_pad))
+
+    def _pad(self, nq_pad: int, nk_pad: int):
         out = [(self.slopes * LOG2E).contiguous()]
         for t, n in ((self.q_pos, nq_pad), (self.k_pos, nk_pad)):
-            if t.numel() and int(t.abs().max()) >= MAX_POSITION:
+            # (the check waits for the device, which a capture may not)
+            if t.numel() and not (t.is_cuda and torch.cuda.is_current_stream_capturing()) and int(t.abs().max()) >= MAX_POSITION:
                 raise ValueError(f"positions of the distance bias must lie within +-{MAX_POSITION}")
             f = torch.zeros(n, dtype=torch.float32, device=t.device)
             f[: t.shape[0]] = t
             out.append(f)
-        self._cache["padded"] = (version, tuple(out))
-        return self._cache["padded"][1]
+        return tuple(out)
 
 
 def document_layout(lengths, *, prefix=None, rows: int | None = None, causal: bool = True, device="cpu") -> MaskLayout:
@@ -141,25 +167,52 @@ def document_positions(lengths, *, rows: int | None = None, device="cpu") -> tor
 
 
 def _seen_keys(layout: MaskLayout) -> torch.Tensor:
-    """[nk] bool: keys that some query row sees."""
+    """[nk] bool: keys that some query row sees. (Sorts and searches only: no size that the host would wait for.)"""
+    never = 1 << 40
     lo, hi, grp, code = (t.long() for t in (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code))
+    if lo.numel() == 0:
+        return torch.zeros_like(code, dtype=torch.bool)
     real = hi > lo
-    starts, stops = torch.sort(lo[real]).values, torch.sort(hi[real]).values
+    starts = torch.sort(lo.masked_fill(~real, never)).values
+    stops = torch.sort(hi.masked_fill(~real, never)).values
+    groups = torch.sort(grp.masked_fill(grp >= 0, never)).values
     # intervals that contain c: those that start at or before it minus those that have ended by then
     covered = torch.searchsorted(starts, code, right=True) > torch.searchsorted(stops, code, right=True)
-    return torch.where(code >= 0, covered, torch.isin(code, grp[grp < 0]))
+    noisy = torch.searchsorted(groups, code, right=True) > torch.searchsorted(groups, code)
+    return torch.where(code >= 0, covered, noisy)
 
 
-def _plan(layout: MaskLayout) -> MaskLayout:
-    """The layout the tile kernels run on: keys that no row sees carry DEAD_KEY, and rows that see no clean key an empty
-    interval behind every coordinate, so that neither widens what a 128-row tile seems to see (a padding row's interval
-    [0, 0) would pull in every tile from the first on)."""
-    if "scored" not in layout._cache:
-        none = layout.q_hi <= layout.q_lo
-        layout._cache["scored"] = MaskLayout(
-            layout.q_lo.to(torch.int32).masked_fill(none, 2 ** 31 - 1), layout.q_hi.to(torch.int32).masked_fill(none, 0),
-            layout.q_grp, layout.k_code.to(torch.int32).masked_fill(~_seen_keys(layout), DEAD_KEY))
-    return layout._cache["scored"]
+_PLAN_PARTS = ("q_lo", "q_hi", "q_grp", "k_code", "f_ptr", "f_idx", "f_order", "w_ptr", "w_idx", "w_order")
+
+
+def _plan(layout: MaskLayout) -> dict:
+    """Device pointers of the layout's tile lists (`csrc/attention_plan.cu`) and the buffer they lie in. Kept with the
+    layout, and built anew when one of its tensors has been written to."""
+    parts = (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code)
+    chunk = backward_chunk_tiles()
+    nq, nk = layout.nq, layout.nk
+    nqt, nkt = (nq + TILE - 1) // TILE, (nk + TILE - 1) // TILE
+    chunk = max(1, min(chunk, nqt)) if chunk > 0 else nqt
+    key = (chunk, *(_version(t) for t in parts))
+    return _kept(layout._cache, "scored", key, layout.q_lo, lambda: _build_plan(layout, chunk, nqt, nkt))
+
+
+def _build_plan(layout: MaskLayout, chunk: int, nqt: int, nkt: int) -> dict:
+    lib = native.lib()
+    nq, nk = layout.nq, layout.nk
+    offsets = (native.c_ll * 11)()
+    size = lib.tdllm_attn_plan_size(nq, nk, chunk, offsets)
+    if size < 0:
+        raise native.NativeKernelError(f"{nq} rows x {nk} keys have too many tiles for a plan")
+    lo, hi, grp, code = (_int32(t) for t in (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code))
+    code = code.masked_fill(~_seen_keys(layout), DEAD_KEY)
+    buf = torch.empty(size, dtype=torch.int32, device=lo.device)
+    native.check(lib.tdllm_attn_plan(ptr(lo), ptr(hi), ptr(grp), ptr(code), nq, nk, chunk, ptr(buf), stream_of(buf)), "attn_plan")
+    base = buf.data_ptr()
+    plan = {n: base + 4 * offsets[i] for i, n in enumerate(_PLAN_PARTS)}
+    plan.update(chunk=chunk, buf=buf, nqt=nqt, nkt=nkt, nq_pad=nqt * TILE, nk_pad=nkt * TILE,
+                n_work=(nqt + chunk - 1) // chunk * nkt)
+    return plan
 
 
 def scored_attention_reference(q, k, v, layout: MaskLayout, transform: ScoreTransform | None = None,
@@ -268,15 +321,14 @@ def _forward(q, k, v, layout, transform, scale, for_backward=False):
     nk, Hkv, _ = k.shape
     if nq <= FEW_ROWS and not for_backward:
         return (*_forward_few_rows(q, k, v, layout, transform, scale), None)
-    L = _plan(layout).tile_lists()
+    L = _plan(layout)
     mod, _kept = _mod_args(transform, L)
     out = torch.empty(nq, Hq, D, dtype=q.dtype, device=q.device)
     rest = torch.empty_like(out) if for_backward else None
     lse = torch.empty(Hq, L["nq_pad"], dtype=torch.float32, device=q.device)
     rc = native.lib().tdllm_attn_fwd_scored(
         ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(lse), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v),
-        out.stride(0), ptr(L["q_lo"]), ptr(L["q_hi"]), ptr(L["q_grp"]), ptr(L["k_code"]), ptr(L["f_ptr"]), ptr(L["f_idx"]),
-        ptr(L["f_order"]), L["nqt"], float(scale), *mod, stream_of(q))
+        out.stride(0), L["q_lo"], L["q_hi"], L["q_grp"], L["k_code"], L["f_ptr"], L["f_idx"], L["f_order"], L["nqt"], float(scale), *mod, stream_of(q))
     native.check(rc, "attn_fwd_scored")
     return out, lse, rest
 
@@ -284,8 +336,7 @@ def _forward(q, k, v, layout, transform, scale, for_backward=False):
 def _backward(q, k, v, out, rest, dout, lse, layout, transform, scale):
     nq, Hq, D = q.shape
     nk, Hkv, _ = k.shape
-    L = _plan(layout).tile_lists()
-    W = _plan(layout).backward_work(backward_chunk_tiles())
+    L = _plan(layout)
     mod, _kept = _mod_args(transform, L)
     dev = q.device
     dq, dk, dv = torch.empty(nq, Hq, D, dtype=q.dtype, device=dev), torch.empty_like(k, memory_format=torch.contiguous_format), \
@@ -296,8 +347,8 @@ def _backward(q, k, v, out, rest, dout, lse, layout, transform, scale):
     rc = native.lib().tdllm_attn_bwd_scored(
         ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(lse), ptr(delta), ptr(acc),
         nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v), _row_stride(out), _row_stride(dout),
-        dq.stride(0), dk.stride(0), dv.stride(0), ptr(L["q_lo"]), ptr(L["q_hi"]), ptr(L["q_grp"]), ptr(L["k_code"]),
-        ptr(W["w_ptr"]), ptr(W["w_idx"]), ptr(W["w_order"]), W["n_work"], L["nqt"], L["nkt"], float(scale), *mod, stream_of(q))
+        dq.stride(0), dk.stride(0), dv.stride(0), L["q_lo"], L["q_hi"], L["q_grp"], L["k_code"], L["w_ptr"], L["w_idx"],
+        L["w_order"], L["n_work"], L["nqt"], L["nkt"], float(scale), *mod, stream_of(q))
     native.check(rc, "attn_bwd_scored")
     return dq, dk, dv
 
