@@ -327,8 +327,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 // delta_s = −scale · sum_d dO·O and lse2 = −lse·log2(e), with lse2 = −inf for rows that saw no key
 // (and for padding rows) so that exp2(x + lse2) is exactly 0 there.
 // One warp per (row, head). Output layout: delta_s [Hq, nq_pad], lse2 [Hq, nq_pad].
-// o_rest, where given: what rounding took from o ([nq, Hq*128], packed).
-__global__ void attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_rest,
+__global__ void attn_delta_kernel(const __nv_bfloat16* __restrict__ o,
                                   const __nv_bfloat16* __restrict__ dout,
                                   const float* __restrict__ lse, float* __restrict__ delta,
                                   float* __restrict__ lse2, float scale,
@@ -347,15 +346,6 @@ __global__ void attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __n
     for (int e = 0; e < 2; ++e) {
       const float2 x = __bfloat1622float2(a2[e]), y = __bfloat1622float2(b2[e]);
       s += x.x * y.x + x.y * y.y;
-    }
-    if (o_rest) {
-      const uint2 r = *reinterpret_cast<const uint2*>(o_rest + ((size_t)row * Hq + h) * HD + lane * 4);
-      const __nv_bfloat162* r2 = reinterpret_cast<const __nv_bfloat162*>(&r);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float2 x = __bfloat1622float2(r2[e]), y = __bfloat1622float2(b2[e]);
-        s += x.x * y.x + x.y * y.y;
-      }
     }
   }
   s = warp_sum(s);

@@ -49,7 +49,7 @@ extern "C" int tdllm_attn_bwd(const void* q, const void* k, const void* v, const
   {
     const long long items = (long long)nq_pad * Hq;
     attn_dq::attn_delta_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(
-        (const __nv_bfloat16*)o, nullptr, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
+        (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
         nq, nq_pad, Hq, ldo, lddo);
   }
   CUtensorMap tq, tdo, tk, tv, tk64, tv64, tdq, tdk, tdv;
@@ -95,6 +95,58 @@ extern "C" int tdllm_attn_bwd(const void* q, const void* k, const void* v, const
 }
 
 namespace tdllm {
+// Row statistics of the transformed-score backward, as attn_delta_kernel's: half a warp per (row, head) and 16-byte loads
+// of dO, out and what rounding took from out. 8192 rows x 32 heads: 201 MB in 39 us (a warp per head and 8-byte loads
+// took 63 us).
+__global__ void __launch_bounds__(256) scored_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_rest,
+                                                           const __nv_bfloat16* __restrict__ dout, const float* __restrict__ lse,
+                                                           float* __restrict__ delta, float* __restrict__ lse2, float scale,
+                                                           int nq, int nq_pad, int Hq, long long ldo, long long lddo) {
+  const int lane = threadIdx.x & 15;
+  const long long item = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (item >= (long long)nq_pad * Hq) return;   // (whole halves of a warp)
+  const int row = (int)(item / Hq), h = (int)(item % Hq);
+  float s = 0.f;
+  if (row < nq) {
+    const uint4 a = *reinterpret_cast<const uint4*>(o + (size_t)row * ldo + h * 128 + lane * 8);
+    const uint4 r = *reinterpret_cast<const uint4*>(o_rest + ((size_t)row * Hq + h) * 128 + lane * 8);
+    const uint4 b = *reinterpret_cast<const uint4*>(dout + (size_t)row * lddo + h * 128 + lane * 8);
+    const uint32_t av[4] = {a.x, a.y, a.z, a.w}, rv[4] = {r.x, r.y, r.z, r.w}, bv[4] = {b.x, b.y, b.z, b.w};
+    float rest = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y0 = __uint_as_float(bv[e] << 16), y1 = __uint_as_float(bv[e] & 0xffff0000u);
+      s = fmaf(__uint_as_float(av[e] << 16), y0, fmaf(__uint_as_float(av[e] & 0xffff0000u), y1, s));
+      rest = fmaf(__uint_as_float(rv[e] << 16), y0, fmaf(__uint_as_float(rv[e] & 0xffff0000u), y1, rest));
+    }
+    s += rest;
+  }
+  const unsigned half = 0xffffu << (threadIdx.x & 16);
+#pragma unroll
+  for (int m = 8; m > 0; m >>= 1) s += __shfl_xor_sync(half, s, m);
+  if (lane == 0) {
+    const size_t at = (size_t)h * nq_pad + row;
+    const float l = row < nq ? lse[at] : -INFINITY;
+    delta[at] = -s * scale;
+    lse2[at] = l > -INFINITY ? -l * 1.4426950408889634f : -INFINITY;
+  }
+}
+
+// The three fp32 accumulators -> bf16, eight values per thread, in one launch (whole rows of 128-value heads, packed).
+__global__ void __launch_bounds__(256) scored_cast_kernel(const float* __restrict__ dq_acc, const float* __restrict__ dk_acc,
+                                                          const float* __restrict__ dv_acc, __nv_bfloat16* __restrict__ dq,
+                                                          __nv_bfloat16* __restrict__ dk, __nv_bfloat16* __restrict__ dv,
+                                                          long long q8, long long k8) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= q8 + 2 * k8) return;
+  const long long at = i < q8 ? i : i < q8 + k8 ? i - q8 : i - q8 - k8;
+  const float* src = (i < q8 ? dq_acc : i < q8 + k8 ? dk_acc : dv_acc) + at * 8;
+  __nv_bfloat16* dst = (i < q8 ? dq : i < q8 + k8 ? dk : dv) + at * 8;
+  const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+  *reinterpret_cast<uint4*>(dst) =
+      make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+}
+
 // fp32 [rows, cols] accumulator -> bf16 rows of a (possibly wider) destination
 __global__ void acc_cast_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ out, int rows,
                                 int cols, long long ld_out) {
@@ -158,10 +210,19 @@ static int attn_bwd_fused_launch(const char* who, const void* q, const void* k, 
   float* dk_acc = dq_acc + (size_t)nq_pad * qc;
   float* dv_acc = dk_acc + (size_t)nk_pad * kc;
   cudaMemsetAsync(acc, 0, ((size_t)nq_pad * qc + 2 * (size_t)nk_pad * kc) * sizeof(float), s);
-  {
+  if constexpr (MOD != 0) {
+    if (!o_rest || lddq != qc || lddk != kc || lddv != kc || ((uintptr_t)o_rest % 16)) {
+      tdllm_host::set_last_error("%s: needs the output's rest and packed gradients", who);
+      return 1;
+    }
+    const long long items = (long long)nq_pad * Hq;
+    scored_delta_kernel<<<(unsigned)((items + 15) / 16), 256, 0, s>>>(
+        (const __nv_bfloat16*)o, (const __nv_bfloat16*)o_rest, (const __nv_bfloat16*)dout, lse, delta,
+        delta + (size_t)Hq * nq_pad, scale, nq, nq_pad, Hq, ldo, lddo);
+  } else {
     const long long items = (long long)nq_pad * Hq;
     attn_dq::attn_delta_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(
-        (const __nv_bfloat16*)o, (const __nv_bfloat16*)o_rest, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
+        (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
         nq, nq_pad, Hq, ldo, lddo);
   }
   CUtensorMap tq, tdo, tk, tv, tdk, tdv, tacc;
@@ -201,7 +262,11 @@ static int attn_bwd_fused_launch(const char* who, const void* q, const void* k, 
     attn_fused::attn_bwd_fused_kernel<false, MOD><<<n_work * Hkv, attn_fused::THREADS, attn_fused::SMEM_BYTES, s>>>(
         tq, tdo, tk, tv, tdk, tdv, tacc, tk, tv, p, pp);
   }
-  {
+  if constexpr (MOD != 0) {
+    const long long q8 = (long long)nq * (qc / 8), k8 = (long long)nk * (kc / 8);
+    scored_cast_kernel<<<(unsigned)((q8 + 2 * k8 + 255) / 256), 256, 0, s>>>(
+        dq_acc, dk_acc, dv_acc, (__nv_bfloat16*)dq, (__nv_bfloat16*)dk, (__nv_bfloat16*)dv, q8, k8);
+  } else {
     const long long n4 = (long long)nq * (qc / 4);
     acc_cast_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, s>>>(dq_acc, (__nv_bfloat16*)dq, nq, (int)qc, lddq);
     const long long k4 = (long long)nk * (kc / 4);
@@ -314,7 +379,7 @@ extern "C" int tdllm_attn_bwd_fused_csbp(
   {
     const long long items = (long long)nq_pad * Hq;
     attn_dq::attn_delta_kernel<<<(unsigned)((items + 7) / 8), 256, 0, s>>>(
-        (const __nv_bfloat16*)o, nullptr, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
+        (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, lse, delta, delta + (size_t)Hq * nq_pad, scale,
         nq, nq_pad, Hq, ldo, lddo);
   }
   float* my_dk = (float*)acc_dk[rank];
