@@ -442,6 +442,30 @@ def test_a_layout_that_is_written_to_and_a_plan_built_inside_a_capture():
 
 
 @pytest.mark.gpu
+def test_a_layout_that_dies_while_another_stream_uses_its_lists():
+    """The lists were allocated on the default stream; their memory must not go to a tensor there while the side stream
+    still has the kernels that read them in front of it."""
+    q, k, v = _operands(2000, 2000, 4, 2, 17)
+    tr = ScoreTransform(20.0)
+    want = scored_attention(q, k, v, document_layout([700, 1300], device="cuda"), tr)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        L = document_layout([700, 1300], device="cuda")
+        scored_attention(q, k, v, L, tr)
+        side.wait_stream(torch.cuda.current_stream())
+        busy = torch.randn(6000, 6000, device="cuda")
+        with torch.cuda.stream(side):
+            for _ in range(8):
+                busy = busy @ busy * 1e-3
+            got = scored_attention(q, k, v, L, tr)
+        size = L._cache["scored"][1][0][0].numel()
+        del L
+        junk = [torch.zeros(size, dtype=torch.int32, device="cuda") for _ in range(8)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and len(junk) == 8
+
+
+@pytest.mark.gpu
 def test_empty_operands_and_other_types():
     e = torch.empty(0, 4, D, dtype=torch.bfloat16, device="cuda")
     L = document_layout([], device="cuda")

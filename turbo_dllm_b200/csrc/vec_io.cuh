@@ -27,22 +27,6 @@ template <class T, int N>
 __device__ __forceinline__ Raw<T, N> load_raw(const T* p) {
   return *reinterpret_cast<const Raw<T, N>*>(p);
 }
-template <class T, int N>
-__device__ __forceinline__ void unpack(const Raw<T, N>& r, float* f) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = to_f(r.v[i]);
-}
-template <class T, int N>
-__device__ __forceinline__ void load(const T* p, float* f) {
-  unpack<T, N>(load_raw<T, N>(p), f);
-}
-template <class T, int N>
-__device__ __forceinline__ void store(T* p, const float* f) {
-  Raw<T, N> r;
-#pragma unroll
-  for (int i = 0; i < N; ++i) r.v[i] = from_f<T>(f[i]);
-  *reinterpret_cast<Raw<T, N>*>(p) = r;
-}
 
 // N values (a whole 16-byte vector) <-> N / 2 pairs of floats
 template <class T, int N>

@@ -231,4 +231,4 @@ def sandwich_norm(x: torch.Tensor, res: torch.Tensor, w_post: torch.Tensor, w_pr
         return _SandwichNorm.apply(x, res, w_post, w_pre, gate, float(res_scale), float(eps))
     g2 = gate if gate is None or gate.dim() == 1 else _rows2d(gate)
     y, h, _ = _sandwich_forward(_rows2d(x), _rows2d(res), w_post, w_pre, g2, float(res_scale), float(eps), False)
-    return y.view(x.shape), h.view(x.shape)
+    return (y, h) if x.dim() == 2 else (y.view(x.shape), h.view(x.shape))

@@ -63,20 +63,27 @@ def _version(t: torch.Tensor) -> int:
 
 
 def _kept(cache: dict, name: str, key, like: torch.Tensor, build):
-    """cache[name] if it was made for `key`, else what `build` makes on `like`'s device. What is made eagerly is complete on
-    return, so that any stream may use it; what is made while a graph is captured belongs to that graph and is not kept.
-    What a capture uses stays with its owner as long as that lives, also when a newer one takes its place."""
+    """cache[name] if it was made for `key`, else what `build` makes on `like`'s device: (tensors, what goes with them). What
+    is made eagerly is complete on return, so that any stream may use it, and its memory is not given away before those
+    streams are done; what is made while a graph is captured belongs to that graph and is not kept. What a capture uses
+    stays with its owner as long as that lives, also when a newer one takes its place."""
     hit = cache.get(name)
-    capturing = like.is_cuda and torch.cuda.is_current_stream_capturing()
+    if not like.is_cuda:
+        if hit is None or hit[0] != key:
+            cache[name] = hit = (key, build(), None)
+        return hit[1]
+    capturing = torch.cuda.is_current_stream_capturing()
     if hit is not None and hit[0] == key:
         if capturing:
             cache.setdefault(name + "_captured", []).append(hit[1])
+        elif hit[2] != stream_of(like):
+            for t in hit[1][0]:
+                t.record_stream(torch.cuda.current_stream(like.device))
         return hit[1]
     made = build()
     if not capturing:
-        if like.is_cuda:
-            torch.cuda.current_stream(like.device).synchronize()
-        cache[name] = (key, made)
+        torch.cuda.current_stream(like.device).synchronize()
+        cache[name] = (key, made, stream_of(like))
     return made
 
 
@@ -117,7 +124,7 @@ class ScoreTransform:
         """(slopes * log2 e, q_pos, k_pos) as the kernels read them: floats, positions padded with zeros. Rebuilt when
         one of the tensors has been written to since."""
         version = (_version(self.slopes), _version(self.q_pos), _version(self.k_pos), nq_pad, nk_pad)
-        return _kept(self._cache, "padded", version, self.slopes, lambda: self._pad(nq_pad, nk_pad))
+        return _kept(self._cache, "padded", version, self.slopes, lambda: (self._pad(nq_pad, nk_pad),))[0]
 
     def _pad(self, nq_pad: int, nk_pad: int):
         out = [(self.slopes * LOG2E).contiguous()]
@@ -186,7 +193,7 @@ _PLAN_PARTS = ("q_lo", "q_hi", "q_grp", "k_code", "f_ptr", "f_idx", "f_order", "
 
 
 def _plan(layout: MaskLayout) -> dict:
-    """Device pointers of the layout's tile lists (`csrc/attention_plan.cu`) and the buffer they lie in. Kept with the
+    """Device pointers of the layout's tile lists (`csrc/attention_plan.cu`) with the buffer they lie in. Kept with the
     layout, and built anew when one of its tensors has been written to."""
     parts = (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code)
     chunk = backward_chunk_tiles()
@@ -194,10 +201,10 @@ def _plan(layout: MaskLayout) -> dict:
     nqt, nkt = (nq + TILE - 1) // TILE, (nk + TILE - 1) // TILE
     chunk = max(1, min(chunk, nqt)) if chunk > 0 else nqt
     key = (chunk, *(_version(t) for t in parts))
-    return _kept(layout._cache, "scored", key, layout.q_lo, lambda: _build_plan(layout, chunk, nqt, nkt))
+    return _kept(layout._cache, "scored", key, layout.q_lo, lambda: _build_plan(layout, chunk, nqt, nkt))[1]
 
 
-def _build_plan(layout: MaskLayout, chunk: int, nqt: int, nkt: int) -> dict:
+def _build_plan(layout: MaskLayout, chunk: int, nqt: int, nkt: int):
     lib = native.lib()
     nq, nk = layout.nq, layout.nk
     offsets = (native.c_ll * 11)()
@@ -212,7 +219,7 @@ def _build_plan(layout: MaskLayout, chunk: int, nqt: int, nkt: int) -> dict:
     plan = {n: base + 4 * offsets[i] for i, n in enumerate(_PLAN_PARTS)}
     plan.update(chunk=chunk, buf=buf, nqt=nqt, nkt=nkt, nq_pad=nqt * TILE, nk_pad=nkt * TILE,
                 n_work=(nqt + chunk - 1) // chunk * nkt)
-    return plan
+    return (buf,), plan
 
 
 def scored_attention_reference(q, k, v, layout: MaskLayout, transform: ScoreTransform | None = None,
@@ -251,11 +258,11 @@ def _check(q, k, v, layout: MaskLayout, transform: ScoreTransform | None) -> Non
         raise ValueError(f"{q.shape[1]} query heads do not divide over {k.shape[1]} KV heads")
     if not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
         raise ValueError("q, k and v must share dtype and device")
-    meta = (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code)
-    if layout.nq != q.shape[0] or layout.nk != k.shape[0] or layout.q_hi.shape != layout.q_lo.shape \
-            or layout.q_grp.shape != layout.q_lo.shape:
+    lo, hi, grp, code = layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code
+    rows, dev = lo.shape, q.device
+    if rows[0] != q.shape[0] or code.shape[0] != k.shape[0] or hi.shape != rows or grp.shape != rows:
         raise ValueError(f"the layout describes {layout.nq} query rows and {layout.nk} keys, got {q.shape[0]} and {k.shape[0]}")
-    if any(t.device != q.device for t in meta):
+    if lo.device != dev or hi.device != dev or grp.device != dev or code.device != dev:
         raise ValueError(f"the layout must lie on {q.device}")
     if transform is not None and transform.biased:
         if transform.slopes.shape[0] != q.shape[1]:
@@ -268,15 +275,17 @@ def _check(q, k, v, layout: MaskLayout, transform: ScoreTransform | None) -> Non
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """[n, H, 128] rows the tensor maps can address: packed heads, 16-byte aligned base and row stride."""
-    n, H, D = t.shape
-    if t.stride(2) == 1 and (H == 1 or t.stride(1) == D) and t.data_ptr() % 16 == 0 \
-            and (n == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= H * D)):
+    if t.is_contiguous():
+        return t if t.data_ptr() % 16 == 0 else t.clone()
+    (n, H, D), (row, head, inner) = t.shape, t.stride()
+    if inner == 1 and (H == 1 or head == D) and t.data_ptr() % 16 == 0 and (n == 1 or (row % 8 == 0 and row >= H * D)):
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t.contiguous()
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]     # (a single row's stride may be anything)
+    n, H, D = t.shape
+    return t.stride(0) if n > 1 else H * D     # (a single row's stride may be anything)
 
 
 def _mod_args(transform: ScoreTransform | None, L: dict):
@@ -294,35 +303,33 @@ def _int32(t: torch.Tensor) -> torch.Tensor:
 
 
 def _forward_few_rows(q, k, v, layout, transform, scale):
-    """(out, lse [Hq, rows padded to 128]) with the keys split over CTAs. Reads the layout's and the transform's own
+    """(out, lse [Hq, nq]) with the keys split over CTAs. Reads the layout's and the transform's own
     tensors at run time: nothing is built or cached, so a captured graph follows what is written to them."""
     nq, Hq, D = q.shape
     nk, Hkv, _ = k.shape
     lib = native.lib()
-    out = torch.empty(nq, Hq, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(Hq, TILE, dtype=torch.float32, device=q.device)
+    dev = q.device
+    out = torch.empty((nq, Hq, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((Hq, nq), dtype=torch.float32, device=dev)
     n = lib.tdllm_attn_few_rows_scratch(nq, nk, Hq, Hkv)
-    part = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    part = torch.empty((n,), dtype=torch.float32, device=dev) if n else None
     meta = [_int32(t) for t in (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code)]
-    bias = [None] * 3
+    bias = (None, None, None)
     if transform is not None and transform.biased:
         bias = [transform.slopes.contiguous(), _int32(transform.q_pos), _int32(transform.k_pos)]
     rc = lib.tdllm_attn_few_rows(
         ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(part), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k),
-        _row_stride(v), out.stride(0), TILE, *(ptr(t) for t in meta), float(scale),
-        0.0 if transform is None else float(transform.softcap), *(ptr(t) for t in bias), stream_of(q))
+        _row_stride(v), Hq * D, nq, *[t.data_ptr() for t in meta], float(scale),
+        0.0 if transform is None else float(transform.softcap), *[ptr(t) for t in bias], stream_of(q))
     native.check(rc, "attn_few_rows" if part is None else "attn_few_rows_split")
     return out, lse
 
 
-def _forward(q, k, v, layout, transform, scale, for_backward=False):
-    """(out, lse [Hq, nq padded to 128], what rounding took from out where a backward pass will want it)."""
+def _forward(q, k, v, L, mod, scale, for_backward=False):
+    """(out, lse [Hq, nq padded to 128], what rounding took from out where a backward pass will want it) by the tile lists
+    of `_plan` and the arguments of `_mod_args`."""
     nq, Hq, D = q.shape
     nk, Hkv, _ = k.shape
-    if nq <= FEW_ROWS and not for_backward:
-        return (*_forward_few_rows(q, k, v, layout, transform, scale), None)
-    L = _plan(layout)
-    mod, _kept = _mod_args(transform, L)
     out = torch.empty(nq, Hq, D, dtype=q.dtype, device=q.device)
     rest = torch.empty_like(out) if for_backward else None
     lse = torch.empty(Hq, L["nq_pad"], dtype=torch.float32, device=q.device)
@@ -333,19 +340,18 @@ def _forward(q, k, v, layout, transform, scale, for_backward=False):
     return out, lse, rest
 
 
-def _backward(q, k, v, out, rest, dout, lse, layout, transform, scale):
+def _backward(q, k, v, out, rest, dout, lse, L, mod, scale):
     nq, Hq, D = q.shape
     nk, Hkv, _ = k.shape
-    L = _plan(layout)
-    mod, _kept = _mod_args(transform, L)
     dev = q.device
     dq, dk, dv = torch.empty(nq, Hq, D, dtype=q.dtype, device=dev), torch.empty_like(k, memory_format=torch.contiguous_format), \
         torch.empty_like(v, memory_format=torch.contiguous_format)
-    delta = torch.empty(2, Hq, L["nq_pad"], dtype=torch.float32, device=dev)
-    # (allocated per call: two streams, or two captured graphs, must not add into one accumulator)
-    acc = torch.empty(L["nq_pad"] * Hq * D + 2 * L["nk_pad"] * Hkv * D, dtype=torch.float32, device=dev)
+    # row statistics [2, Hq, nq_pad], then the accumulators (allocated per call: two streams, or two captured graphs, must
+    # not add into one accumulator)
+    stats = 2 * Hq * L["nq_pad"]
+    work = torch.empty((stats + L["nq_pad"] * Hq * D + 2 * L["nk_pad"] * Hkv * D,), dtype=torch.float32, device=dev)
     rc = native.lib().tdllm_attn_bwd_scored(
-        ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(lse), ptr(delta), ptr(acc),
+        ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(lse), ptr(work), ptr(work) + 4 * stats,
         nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v), _row_stride(out), _row_stride(dout),
         dq.stride(0), dk.stride(0), dv.stride(0), L["q_lo"], L["q_hi"], L["q_grp"], L["k_code"], L["w_ptr"], L["w_idx"],
         L["w_order"], L["n_work"], L["nqt"], L["nkt"], float(scale), *mod, stream_of(q))
@@ -358,9 +364,12 @@ class _ScoredAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, layout, transform, scale):
         with on_device(q):
             q, k, v = _operand(q), _operand(k), _operand(v)
-            out, lse, rest = _forward(q, k, v, layout, transform, scale, for_backward=True)
+            # (the backward pass goes by the lists and positions of the forward pass, whatever is written to them since)
+            ctx.L = _plan(layout)
+            ctx.mod, ctx.behind_mod = _mod_args(transform, ctx.L)
+            out, lse, rest = _forward(q, k, v, ctx.L, ctx.mod, scale, for_backward=True)
         ctx.save_for_backward(q, k, v, out, rest, lse)
-        ctx.layout, ctx.transform, ctx.scale = layout, transform, scale
+        ctx.scale = scale
         lse = lse[:, : q.shape[0]]
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -370,7 +379,7 @@ class _ScoredAttention(torch.autograd.Function):
         refuse_twice("scored attention")
         q, k, v, out, rest, lse = ctx.saved_tensors
         with on_device(q):
-            grads = _backward(q, k, v, out, rest, _operand(dout), lse, ctx.layout, ctx.transform, ctx.scale)
+            grads = _backward(q, k, v, out, rest, _operand(dout), lse, ctx.L, ctx.mod, ctx.scale)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
 
 
@@ -399,6 +408,12 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
         lse = torch.full((q.shape[1], q.shape[0]), float("-inf"), dtype=torch.float32, device=q.device)
     else:
         with on_device(q):
-            out, lse, _ = _forward(_operand(q), _operand(k), _operand(v), layout, transform, scale)
-            lse = lse[:, : q.shape[0]]
+            q, k, v = _operand(q), _operand(k), _operand(v)
+            if q.shape[0] <= FEW_ROWS:
+                out, lse = _forward_few_rows(q, k, v, layout, transform, scale)
+            else:
+                L = _plan(layout)
+                mod, _behind = _mod_args(transform, L)
+                out, lse, _ = _forward(q, k, v, L, mod, scale)
+                lse = lse[:, : q.shape[0]]
     return (out, lse) if return_lse else out
