@@ -684,16 +684,17 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const uint32_t t_o = tmem_base + ((uint32_t)(qd * 32) << 16) + 256 + i * 128;
   float* xmine = sX + (i * 2 + sub) * 128 + row;
   const float* xother = sX + (i * 2 + (sub ^ 1)) * 128 + row;
+  const float scl = (MOD & score::CAP) != 0 ? 1.f : p.scale_log2;   // capped scores already are in log2 units
   float m = -INFINITY, l = 0.f;
   bool ok = true;
   if (warp < 16) {
     const int prow = row0 + row;
     // (the row's mask is read where a tile needs it: held here it would push the scores out of registers)
     const int qi = prow < rows ? prow / G : -1;
-    [[maybe_unused]] float slope2 = 0.f, qpos = 0.f;
+    [[maybe_unused]] float slope = 0.f, qpos = 0.f;
     if (prow < rows) {
       if constexpr ((MOD & score::BIAS) != 0) {
-        slope2 = p.slopes[kvh * G + prow % G] * 1.4426950408889634f;
+        slope = p.slopes[kvh * G + prow % G] * 1.4426950408889634f / scl;
         qpos = (float)p.q_pos[qi];
       }
     }
@@ -733,7 +734,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             fence_proxy_async_smem();
           }
         }
-        score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) {
+        score::transform_row<MOD>(r, p.mod, slope, qpos, make_float2(kpos[0], kpos[1]), [&](int e) {
           const float kp = kpos[e >> 5];
           asm volatile("" ::: "memory");
           return make_float4(__shfl_sync(0xffffffffu, kp, e & 31), __shfl_sync(0xffffffffu, kp, (e + 1) & 31),
@@ -765,8 +766,8 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       if (!named_bar_all(1 + i, 256, good)) { ok = false; break; }
       const float mx = fmaxf(*xmine, *xother);
       float alpha = 1.f;   // the reference maximum moves only when the new one is 2^8 larger
-      if (mx > -INFINITY && (m == -INFINITY || mx - m > 8.f)) {
-        alpha = m == -INFINITY ? 0.f : score::exp2_approx(m - mx);
+      if (mx > -INFINITY && (m == -INFINITY || (mx - m) * scl > 8.f)) {
+        alpha = m == -INFINITY ? 0.f : score::exp2_approx((m - mx) * scl);
         m = mx;
       }
       l *= alpha;
@@ -781,14 +782,14 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           tmem_st16(t_o + c * 16, ro);
         }
       }
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = m == -INFINITY ? 0.f : m * scl;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t pk[8];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-          const float p0 = score::exp2_approx(__uint_as_float(r[c * 16 + e]) - ref);
-          const float p1 = score::exp2_approx(__uint_as_float(r[c * 16 + e + 1]) - ref);
+          const float p0 = score::exp2_approx(fmaf(__uint_as_float(r[c * 16 + e]), scl, -ref));
+          const float p1 = score::exp2_approx(fmaf(__uint_as_float(r[c * 16 + e + 1]), scl, -ref));
           l += p0 + p1;
           pk[e >> 1] = pack_bf16x2(p0, p1);
         }
@@ -799,6 +800,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       mbar_arrive(bar_pfull + 8 * i);
       // (the exchange slots are rewritten only after this tile's products, which wait for all 256 arrivals above)
     }
+    m *= scl;   // (log2 units from here on)
     if (ok && n > i) ok = mbar_wait_spin(bar_odone + 8 * i, 0, KID, 31);
   }
   // ------------------------------ joining the two pipelines ------------------------

@@ -310,13 +310,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint32_t t_o = tmem_base + ((uint32_t)(qd * 32) << 16) + 256 + i * 128;
     float* xmine = sX + (i * 2 + sub) * 128 + row;
     const float* xother = sX + (i * 2 + (sub ^ 1)) * 128 + row;
-    const float scl = MOD ? 1.f : p.scale_log2;   // transformed scores already are in log2 units
-    [[maybe_unused]] float slope2 = 0.f, qpos = 0.f;
+    constexpr bool LOG2 = (MOD & score::CAP) != 0;   // capped scores already are in log2 units
+    const float scl = LOG2 ? 1.f : p.scale_log2;
+    [[maybe_unused]] float slope = 0.f, qpos = 0.f;
     if constexpr ((MOD & score::BIAS) != 0) {
-      slope2 = p.mod.slope2[min(h0 + i, h_last)];
+      slope = p.mod.slope2[min(h0 + i, h_last)];
+      if constexpr (!LOG2) slope /= scl;
       qpos = p.mod.q_pos[grow];
     }
-    float m_used = -INFINITY;  // max the stored probabilities are relative to (raw score units; log2 units if MOD)
+    float m_used = -INFINITY;  // max the stored probabilities are relative to (raw score units; log2 units if capped)
     float l = 0.f;             // this thread's share of the row sum
     [[maybe_unused]] float lr = 0.f;   // the same of the rounded probabilities (MOD & REST)
     uint32_t r[64];
@@ -343,8 +345,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               if (!key_visible(__ldg(kc + e), lo, hi, grp)) r[e] = 0xff800000u;  // -inf
           }
         } else {
-          const float4* kp = reinterpret_cast<const float4*>(kc + 128);
-          score::transform_row<MOD, 64>(r, p.mod, p.scale_log2, slope2, qpos, [&](int e) { return kp[e / 4]; });
+          const float* kp = reinterpret_cast<const float*>(kc + 128);
+          float2 own = make_float2(0.f, 0.f);
+          if constexpr ((MOD & score::BIAS) != 0) own = make_float2(kp[lane], kp[32 + lane]);
+          score::transform_row<MOD>(r, p.mod, slope, qpos, own,
+                                    [&](int e) { return *reinterpret_cast<const float4*>(kp + e); });
           if (ent & 1) {
             // this thread's key of the tile (and half of its columns): a dead key's V row is zeroed
             const bool dead = (kc - sub * 64)[row] == score::DEAD_KEY;
@@ -472,7 +477,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       if (sub == 0)
-        p.lse[(size_t)min(h0 + i, h_last) * p.nq_pad + grow] = l > 0.f ? m_used * (MOD ? 0.69314718055994531f : p.scale) + __logf(l) : -INFINITY;
+        p.lse[(size_t)min(h0 + i, h_last) * p.nq_pad + grow] = l > 0.f ? m_used * (LOG2 ? 0.69314718055994531f : p.scale) + __logf(l) : -INFINITY;
       fence_proxy_async_smem();
       mbar_arrive(bar_epi + 8 * i);
       if (row == 0 && sub == 0) {

@@ -33,12 +33,11 @@ constexpr int CAP = 1, BIAS = 2, SAFE = 4, REST = 8;   // REST: the forward form
 constexpr int DEAD_KEY = -2147483647 - 1;   // code of a key that no row sees (also of padding behind the last key)
 
 struct Mod {
-  float in1;            // scale / cap
   float in2;            // 2 log2(e) scale / cap
   float cap2;           // cap log2(e)
   float inv_cap2;       // 1 / cap2
-  float near;           // 3/4 cap / scale: raw products up to here take the polynomial
-  float poly[6];        // cap2 Q
+  float near4, near6;   // 3/8 and 3/4 cap / scale: raw products up to here take the polynomials
+  float poly4[4], poly6[6];   // z / s in powers of s^2
   const float* slope2;  // [Hq] slope_h log2(e)
   const float* q_pos;   // [nq_pad] positions as floats (exact: |position| < 2^24)
   const float* k_pos;   // [nk_pad]
@@ -99,27 +98,33 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// z = s P(s^2), two scores to an instruction
+template <int N, int C>
+__device__ __forceinline__ void cap_poly(uint32_t* s, const float* c) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    const uint64_t x = pair_f32(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+    const uint64_t u = mul_f32x2(x, x);
+    uint64_t q = both(c[C - 1]);
+#pragma unroll
+    for (int i = C - 2; i >= 0; --i) q = fma_f32x2(q, u, both(c[i]));
+    float z0, z1;
+    unpair_f32(mul_f32x2(q, x), z0, z1);
+    s[e] = __float_as_uint(z0);
+    s[e + 1] = __float_as_uint(z1);
+  }
+}
+
 // N raw products of one thread -> capped scores in log2 units, in place. All lanes of the warp take part.
 template <int N>
 __device__ __forceinline__ void cap_block(uint32_t* s, const Mod& m) {
   float top = 0.f;
 #pragma unroll
   for (int e = 0; e < N; e += 2) top = max3(top, fabsf(__uint_as_float(s[e])), fabsf(__uint_as_float(s[e + 1])));
-  if (!__any_sync(0xffffffffu, top > m.near)) {
-#pragma unroll
-    for (int e = 0; e < N; e += 2) {
-      const uint64_t x = mul_f32x2(pair_f32(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), both(m.in1));
-      const uint64_t u = mul_f32x2(x, x);
-      uint64_t q = fma_f32x2(u, both(m.poly[5]), both(m.poly[4]));
-      q = fma_f32x2(q, u, both(m.poly[3]));
-      q = fma_f32x2(q, u, both(m.poly[2]));
-      q = fma_f32x2(q, u, both(m.poly[1]));
-      q = fma_f32x2(q, u, both(m.poly[0]));
-      float z0, z1;
-      unpair_f32(mul_f32x2(q, x), z0, z1);
-      s[e] = __float_as_uint(z0);
-      s[e + 1] = __float_as_uint(z1);
-    }
+  if (!__any_sync(0xffffffffu, top > m.near4)) {
+    cap_poly<N, 4>(s, m.poly4);
+  } else if (!__any_sync(0xffffffffu, top > m.near6)) {
+    cap_poly<N, 6>(s, m.poly6);
   } else {
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
@@ -139,31 +144,34 @@ __device__ __forceinline__ uint64_t less_distance(uint64_t z, float slope2, uint
   return fma_f32x2(pair_f32(fabsf(d0), fabsf(d1)), both(-slope2), z);
 }
 
-// N raw products of one query row against consecutive keys -> transformed scores in log2 units. kp(e): positions of keys
-// e .. e + 3.
-template <int MOD, int N, class KeyPos>
-__device__ __forceinline__ void transform_row(uint32_t* s, const Mod& m, float scale_log2, float slope2, float qpos, KeyPos kp) {
+// The 64 raw products of one query row against consecutive keys -> transformed scores: in log2 units where they are capped,
+// else still without the scale, which the exponent's subtraction applies; `slope` is in the same units. All lanes of the
+// warp take part, with the same keys: `own` are the positions of keys lane and 32 + lane, kp(e) those of keys e .. e + 3.
+//
+// Positions mostly rise by one from key to key, and away from the diagonal all of a warp's rows lie behind all of the keys
+// (or in front of them): then |distance| = +-(d0 - e), and no position is loaded and no absolute value taken.
+template <int MOD, class KeyPos>
+__device__ __forceinline__ void transform_row(uint32_t* s, const Mod& m, float slope, float qpos, float2 own, KeyPos kp) {
+  constexpr int N = 64;
   if constexpr ((MOD & CAP) != 0) cap_block<N>(s, m);
+  if constexpr ((MOD & BIAS) != 0) {
+    const int lane = threadIdx.x & 31;
+    const float k0 = __shfl_sync(0xffffffffu, own.x, 0), d0 = qpos - k0;
+    const bool plain = own.x == k0 + lane && own.y == k0 + (32 + lane) && (d0 >= N - 1 || d0 <= 0.f);
+    if (__all_sync(0xffffffffu, plain)) {
+      const float f = d0 > 0.f ? -slope : slope;
 #pragma unroll
-  for (int e = 0; e < N; e += 4) {
-    uint64_t z0 = pair_f32(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-    uint64_t z1 = pair_f32(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
-    if constexpr ((MOD & CAP) == 0) {
-      z0 = mul_f32x2(z0, both(scale_log2));
-      z1 = mul_f32x2(z1, both(scale_log2));
+      for (int e = 0; e < N; ++e) s[e] = __float_as_uint(fmaf(f, d0 - e, __uint_as_float(s[e])));
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; e += 4) {
+        const float4 k = kp(e);
+        s[e] = __float_as_uint(fmaf(-slope, fabsf(qpos - k.x), __uint_as_float(s[e])));
+        s[e + 1] = __float_as_uint(fmaf(-slope, fabsf(qpos - k.y), __uint_as_float(s[e + 1])));
+        s[e + 2] = __float_as_uint(fmaf(-slope, fabsf(qpos - k.z), __uint_as_float(s[e + 2])));
+        s[e + 3] = __float_as_uint(fmaf(-slope, fabsf(qpos - k.w), __uint_as_float(s[e + 3])));
+      }
     }
-    if constexpr ((MOD & BIAS) != 0) {
-      const float4 k = kp(e);
-      z0 = less_distance(z0, slope2, both(qpos), pair_f32(k.x, k.y));
-      z1 = less_distance(z1, slope2, both(qpos), pair_f32(k.z, k.w));
-    }
-    float a, b, c, d;
-    unpair_f32(z0, a, b);
-    unpair_f32(z1, c, d);
-    s[e] = __float_as_uint(a);
-    s[e + 1] = __float_as_uint(b);
-    s[e + 2] = __float_as_uint(c);
-    s[e + 3] = __float_as_uint(d);
   }
 }
 
@@ -174,15 +182,26 @@ static inline tdllm::score::Mod score_mod_of(float scale, float softcap, const f
                                              const float* k_pos) {
   const float log2e = 1.4426950408889634f;
   tdllm::score::Mod m;
-  static const float q[6] = {0.9999998211860657f, -0.33332470059394836f, 0.13320580124855042f,
+  static const float q6[6] = {0.9999998211860657f, -0.33332470059394836f, 0.13320580124855042f,
                              -0.053149253129959106f, 0.01923721842467785f, -0.004493444226682186f};
   const bool cap = softcap > 0.f;
-  m.in1 = cap ? scale / softcap : 0.f;
-  m.in2 = 2.f * log2e * m.in1;
+  const double in1 = cap ? (double)scale / softcap : 0.;
+  m.in2 = (float)(2. * log2e * in1);
   m.cap2 = softcap * log2e;
   m.inv_cap2 = cap ? 1.f / m.cap2 : 0.f;
-  m.near = cap ? 0.75f * softcap / fabsf(scale) : 0.f;
-  for (int i = 0; i < 6; ++i) m.poly[i] = m.cap2 * q[i];
+  // (a form one of whose coefficients is not an ordinary number of 32 bits is never taken)
+  auto powers = [&](const float* c, int n, float* out) {
+    bool fine = cap;
+    double f = m.cap2 * in1;
+    for (int i = 0; i < n; ++i, f *= in1 * in1) {
+      out[i] = (float)(f * c[i]);
+      fine = fine && fabs(f * c[i]) > 1.2e-38 && fabs(f * c[i]) < 3.0e38;
+    }
+    return fine;
+  };
+  static const float q4[4] = {0.9999997615814209f, -0.3333083987236023f, 0.1326839178800583f, -0.04761846736073494f};
+  m.near4 = powers(q4, 4, m.poly4) ? (float)(0.375 / fabs(in1)) : -1.f;
+  m.near6 = powers(q6, 6, m.poly6) ? (float)(0.75 / fabs(in1)) : -1.f;
   m.slope2 = slope2;
   m.q_pos = q_pos;
   m.k_pos = k_pos;

@@ -391,6 +391,8 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
     tiles by fp32 adds whose order is not fixed, as in `block_attention`'s one-pass backward."""
     _check(q, k, v, layout, transform)
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if not 1e-20 <= scale < math.inf:      # (the row maximum is taken before the scale is applied)
+        raise ValueError(f"scale must be a positive number, got {scale}")
     if not q.is_cuda or q.dtype != torch.bfloat16:
         out, lse = scored_attention_reference(q, k, v, layout, transform, scale)
         return (out, lse.detach()) if return_lse else out
