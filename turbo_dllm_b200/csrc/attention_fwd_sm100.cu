@@ -136,6 +136,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   // tile j + 4: K of that tile waits for the scores of tile j + 2, whose products follow both heads' softmax of tile j.
   uint8_t* sMeta = (uint8_t*)bars + 512 + 2048;
   const uint32_t bar_meta = b0 + 144;           // [4]
+  // MOD: P_i is handed over in two halves (keys 0-31 and 64-95 first), so that the product starts under the exponentials
+  const uint32_t bar_phalf = b0 + 176;          // [2]
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -168,6 +170,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
     if constexpr (MOD != 0) {
       for (int s = 0; s < META_SLOTS; ++s) mbar_init(bar_meta + 8 * s, 1);
+      for (int s = 0; s < 2; ++s) mbar_init(bar_phalf + 8 * s, 256);
     }
     fence_mbar_init();
   }
@@ -268,10 +271,22 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (!wait_all(bar_vfull + 8 * s, ph, 22)) break;
         const uint32_t va = smem_u32(sV + s * TILE_BYTES);
         for (int i = 0; i < 2; ++i) {
+          if constexpr (MOD != 0) {
+            if (!wait_all(bar_phalf + 8 * i, j & 1, 25)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const int k = (h & 1) + (h >> 1) * 4;
+              const uint64_t bd = make_smem_desc_sw128(va + k * 2048, HALF_BYTES, 1024);
+              if (leader)
+                tc_mma_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + k * 8, bd, idesc_pv, (j | k) ? 1u : 0u);
+            }
+          }
           if (!wait_all(bar_pfull + 8 * i, j & 1, 23)) { ok = false; break; }
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < BKV / 16; ++k) {
+            if (MOD != 0 && (k & 2) == 0) continue;
             const uint64_t bd = make_smem_desc_sw128(va + k * 2048, HALF_BYTES, 1024);
             if (leader)
               tc_mma_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + k * 8, bd, idesc_pv, (j | k) ? 1u : 0u);
@@ -422,6 +437,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           for (int e = 0; e < 8; ++e) lr += __uint_as_float(pk[e] << 16) + __uint_as_float(pk[e] & 0xffff0000u);
         }
         tmem_st8(t_s + sub * 32 + c * 8, pk);
+        if constexpr (MOD != 0) {
+          if (c == 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(bar_phalf + 8 * i);
+          }
+        }
       }
       tmem_st_wait();
       tc_fence_before();
