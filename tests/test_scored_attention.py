@@ -171,6 +171,9 @@ def test_refusals():
         scored_attention(q, k, k, L, ScoreTransform(0.0, s, pos[:5], pos))
     with pytest.raises(ValueError, match="divide"):
         scored_attention(q[:, :3], k, k, L)
+    for bad in (0.0, -0.1, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            scored_attention(q, k, k, L, scale=bad)
     with pytest.raises(ValueError, match="layout describes"):
         scored_attention(q[:5], k, k, L)
     with pytest.raises(ValueError, match="share"):
@@ -463,6 +466,26 @@ def test_a_layout_that_dies_while_another_stream_uses_its_lists():
         junk = [torch.zeros(size, dtype=torch.int32, device="cuda") for _ in range(8)]
         torch.cuda.synchronize()
         assert torch.equal(got, want) and len(junk) == 8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e-3, 0.7, 8.0, 300.0, 1e5])
+@pytest.mark.parametrize("gain", [0.3, 6.0])
+def test_caps_of_every_size(cap, gain):
+    """Small and large scores against the cap take different forms of the tanh, and very small or large caps leave one whose
+    coefficients 32 bits do not hold: whatever is taken, the row maximum's probability is right to the usual tolerance."""
+    q, k, v = (t * gain for t in _operands(200, 200, 4, 2, 23))
+    L, tr = document_layout([150, 50], device="cuda"), ScoreTransform(cap)
+    want, lse = scored_attention_reference(q.double(), k.double(), v.double(), L, tr)
+    for rows in (200, 40):
+        M = MaskLayout(L.q_lo[:rows], L.q_hi[:rows], L.q_grp[:rows], L.k_code)
+        out, got = scored_attention(q[:rows], k, v, M, tr, return_lse=True)
+        # z is known to 2^-20 of the cap and 2^-22 of itself (a score of up to 600 here)
+        tol = 2.0 ** -20 * min(cap, 600.0) + 2.0 ** -21 * min(cap, 600.0) + 2.0 ** -18
+        assert float((got.double() - lse[:, :rows]).abs().max()) <= tol
+        # probabilities are off by half a step (2^-8) and by tol, the output by half a step
+        size = scored_attention_reference(q.double(), k.double(), v.double().abs(), L, tr)[0][:rows]
+        assert bool(((out.double() - want[:rows]).abs() <= 2.0 ** -8 * want[:rows].abs() + (2.0 ** -8 + 4 * tol) * size).all())
 
 
 @pytest.mark.gpu

