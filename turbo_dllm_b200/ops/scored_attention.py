@@ -27,6 +27,7 @@ for few query rows has no lists and follows its tensors.
 from __future__ import annotations
 
 import math
+import os
 from dataclasses import dataclass, field
 
 import torch
@@ -56,6 +57,11 @@ LOG2E = 1.4426950408889634
 # query tile. B200, 32 / 8 heads, scores capped: 1 row x 20000 keys 24 us against 490, 32 x 32768 45 against 797,
 # 128 x 1024 20 against 36, 32 x 300 15.4 against 18.3
 FEW_ROWS = 128
+# The backward pass has an item of work per (key tile, chunk of query tiles, KV head). Where the key tiles and heads alone are
+# few, shorter chunks make about this many items, 2.5 to each SM. B200, forward and backward in us, one chunk against the
+# chunks of this rule: 500 rows, 16 / 8 heads 68 / 50, 2000 rows, 4 / 1 heads 273 / 98, 2000 rows, 16 / 8 heads 191 / 155, 3000
+# rows, 16 / 8 heads 276 / 255; from 300 items on one chunk is as good (5000 rows, 16 / 8 heads 533, two chunks 545).
+BACKWARD_ITEMS = 370
 
 
 def _version(t: torch.Tensor) -> int:
@@ -192,16 +198,23 @@ def _seen_keys(layout: MaskLayout) -> torch.Tensor:
 _PLAN_PARTS = ("q_lo", "q_hi", "q_grp", "k_code", "f_ptr", "f_idx", "f_order", "w_ptr", "w_idx", "w_order")
 
 
-def _plan(layout: MaskLayout) -> dict:
+def _chunk_tiles(nqt: int, nkt: int, Hkv: int) -> int:
+    chunk = backward_chunk_tiles()
+    chunk = min(chunk, nqt) if chunk > 0 else nqt
+    if "TDLLM_ATTN_BWD_CHUNK" not in os.environ:
+        pieces = max(1, round(BACKWARD_ITEMS / (nkt * Hkv)))
+        chunk = min(chunk, (nqt + pieces - 1) // pieces)
+    return chunk
+
+
+def _plan(layout: MaskLayout, Hkv: int) -> dict:
     """Device pointers of the layout's tile lists (`csrc/attention_plan.cu`) with the buffer they lie in. Kept with the
     layout, and built anew when one of its tensors has been written to."""
     parts = (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code)
-    chunk = backward_chunk_tiles()
-    nq, nk = layout.nq, layout.nk
-    nqt, nkt = (nq + TILE - 1) // TILE, (nk + TILE - 1) // TILE
-    chunk = max(1, min(chunk, nqt)) if chunk > 0 else nqt
-    key = (chunk, *(_version(t) for t in parts))
-    return _kept(layout._cache, "scored", key, layout.q_lo, lambda: _build_plan(layout, chunk, nqt, nkt))[1]
+    nqt, nkt = (layout.nq + TILE - 1) // TILE, (layout.nk + TILE - 1) // TILE
+    chunk = _chunk_tiles(nqt, nkt, Hkv)
+    key = tuple(_version(t) for t in parts)
+    return _kept(layout._cache, f"scored_{chunk}", key, layout.q_lo, lambda: _build_plan(layout, chunk, nqt, nkt))[1]
 
 
 def _build_plan(layout: MaskLayout, chunk: int, nqt: int, nkt: int):
@@ -365,7 +378,7 @@ class _ScoredAttention(torch.autograd.Function):
         with on_device(q):
             q, k, v = _operand(q), _operand(k), _operand(v)
             # (the backward pass goes by the lists and positions of the forward pass, whatever is written to them since)
-            ctx.L = _plan(layout)
+            ctx.L = _plan(layout, k.shape[1])
             ctx.mod, ctx.behind_mod = _mod_args(transform, ctx.L)
             out, lse, rest = _forward(q, k, v, ctx.L, ctx.mod, scale, for_backward=True)
         ctx.save_for_backward(q, k, v, out, rest, lse)
@@ -387,8 +400,8 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
                      transform: ScoreTransform | None = None, *, scale: float | None = None, return_lse: bool = False):
     """q [nq, Hq, D], k / v [nk, Hkv, D] -> out [nq, Hq, D] (and lse [Hq, nq] float32, without gradient).
 
-    Operands may be views of a packed projection (packed heads, any row stride). The gradient of dQ is summed over key
-    tiles by fp32 adds whose order is not fixed, as in `block_attention`'s one-pass backward."""
+    Operands may be views of a packed projection (packed heads, any row stride). Gradients are summed over tiles by
+    fp32 adds whose order is not fixed, as in `block_attention`'s one-pass backward."""
     _check(q, k, v, layout, transform)
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if not 1e-20 <= scale < math.inf:      # (the row maximum is taken before the scale is applied)
@@ -414,7 +427,7 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
             if q.shape[0] <= FEW_ROWS:
                 out, lse = _forward_few_rows(q, k, v, layout, transform, scale)
             else:
-                L = _plan(layout)
+                L = _plan(layout, k.shape[1])
                 mod, _behind = _mod_args(transform, L)
                 out, lse, _ = _forward(q, k, v, L, mod, scale)
                 lse = lse[:, : q.shape[0]]
