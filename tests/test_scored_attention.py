@@ -210,14 +210,24 @@ def _operands(nq, nk, Hq, Hkv, seed, packed=False, gain=2.0):
     return (r(nq, Hq, D) * gain).bfloat16(), r(nk, Hkv, D).bfloat16(), r(nk, Hkv, D).bfloat16()
 
 
+@pytest.fixture
+def listed(monkeypatch):
+    """Forward passes without gradients go by tile lists, whatever their size."""
+    from turbo_dllm_b200.ops import scored_attention as sa
+
+    monkeypatch.setattr(sa, "_few", lambda *a: False)
+
+
 def run_case(q, k, v, layout, tr, backward=True, seed=3):
+    """Forward (and backward) against 64 bits; the forward pass without gradients in both of its forms, too."""
     from turbo_dllm_b200.kernels import native
+    from turbo_dllm_b200.ops import scored_attention as sa
 
     scale = 1.0 / math.sqrt(D)
     q, k, v = (t.detach().requires_grad_(backward) for t in (q, k, v))
     out, lse = scored_attention(q, k, v, layout, tr, return_lse=True)
     dout = torch.randn(out.shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").bfloat16()
-    got = {"out": out, "lse": lse}
+    got = {"out": out.detach(), "lse": lse}
     if backward:
         got.update(zip(("dq", "dk", "dv"), torch.autograd.grad(out, [q, k, v], dout)))
     torch.cuda.synchronize()
@@ -225,6 +235,14 @@ def run_case(q, k, v, layout, tr, backward=True, seed=3):
     want, tol = exact(q, k, v, layout, tr, scale, dout if backward else None)
     for n, t in got.items():
         near(t, want[n], tol[n], n)
+    for few in (True, False):
+        with pytest.MonkeyPatch.context() as mp, torch.no_grad():
+            mp.setattr(sa, "_few", lambda *a: few)
+            out, lse = scored_attention(q, k, v, layout, tr, return_lse=True)
+        torch.cuda.synchronize()
+        native.raise_on_device_error()
+        near(out, want["out"], tol["out"], "out")
+        near(lse, want["lse"], tol["lse"], "lse")
     return got
 
 
@@ -283,7 +301,8 @@ def step_layout(caches, new, device="cuda", capacity=None, window=None):
 @pytest.mark.parametrize("caches,new,Hq,Hkv", [([1], 1, 1, 1), ([0], 1, 4, 2), ([5000], 1, 8, 2), ([700, 0, 1300], 1, 12, 4),
                                                ([300, 129], 32, 8, 2), ([4000], 32, 4, 1), ([260, 1, 513], 17, 6, 2),
                                                ([130], 128, 3, 1), ([2000], 5, 16, 2),
-                                               ([1000], 100, 2, 2), ([300, 200], 64, 8, 1), ([5], 40, 16, 1)])
+                                               ([1000], 100, 2, 2), ([300, 200], 64, 8, 1), ([5], 40, 16, 1),
+                                               ([900], 300, 8, 2), ([500, 31], 137, 4, 4), ([600], 140, 6, 2)])
 def test_few_rows(kind, caches, new, Hq, Hkv):
     L, qpos, kpos = step_layout(caches, new)
     for backward in (False, True):
@@ -415,7 +434,7 @@ def test_plan_matches_the_dense_mask(make, Hkv):
 
 
 @pytest.mark.gpu
-def test_a_layout_that_is_written_to_and_a_plan_built_inside_a_capture():
+def test_a_layout_that_is_written_to_and_a_plan_built_inside_a_capture(listed):
     q, k, v = _operands(300, 300, 4, 2, 13)
     L = document_layout([300], device="cuda")
     tr = ScoreTransform(20.0)
@@ -446,7 +465,7 @@ def test_a_layout_that_is_written_to_and_a_plan_built_inside_a_capture():
 
 
 @pytest.mark.gpu
-def test_a_layout_that_dies_while_another_stream_uses_its_lists():
+def test_a_layout_that_dies_while_another_stream_uses_its_lists(listed):
     """The lists were allocated on the default stream; their memory must not go to a tensor there while the side stream
     still has the kernels that read them in front of it."""
     q, k, v = _operands(2000, 2000, 4, 2, 17)
@@ -507,6 +526,14 @@ def test_empty_operands_and_other_types():
 
     with pytest.raises(NativeKernelError, match="head_dim"):
         scored_attention(x.bfloat16(), x.bfloat16(), x.bfloat16(), L)
+
+
+@pytest.mark.parametrize("heads,nq,nk,few", [((32, 8), 128, 1, True), ((32, 8), 129, 256, False), ((32, 8), 512, 512, True),
+                                             ((32, 8), 577, 4096, False), ((8, 8), 2304, 2304, True), ((12, 4), 129, 4096, False)])
+def test_which_form_a_forward_pass_takes(heads, nq, nk, few):
+    from turbo_dllm_b200.ops import scored_attention as sa
+
+    assert sa._few(nq, nk, *heads) is few
 
 
 @pytest.mark.gpu

@@ -1,5 +1,5 @@
-// Attention of a few new rows (one token, one block of new tokens, a batch of either) against a long cache, head width
-// 128, with the score transforms and the declarative mask of the tile kernels. Forward only.
+// Attention of a few new rows (one token, one block of new tokens, a batch of either, a piece of a prompt) against a long
+// cache, head width 128, with the score transforms and the declarative mask of the tile kernels. Forward only.
 //
 // A call reads K and V once and does little with them, so it is bound by memory as long as every SM pulls: the keys are
 // split over CTAs. The G query heads of a KV head and the query rows are packed into one row axis (row r = query r / G,

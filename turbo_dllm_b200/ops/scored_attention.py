@@ -53,10 +53,13 @@ native.register_signatures({
 DEAD_KEY = -(2 ** 31)      # key code that no query row matches
 MAX_POSITION = 1 << 24     # distances are taken between positions held as floats
 LOG2E = 1.4426950408889634
-# Up to this many query rows a forward without gradients splits the keys over the GPU instead of giving a CTA a 128-row
-# query tile. B200, 32 / 8 heads, scores capped: 1 row x 20000 keys 24 us against 490, 32 x 32768 45 against 797,
-# 128 x 1024 20 against 36, 32 x 300 15.4 against 18.3
+# A forward without gradients packs the query heads of a KV head into rows and splits the keys over the GPU (`_few`), instead
+# of giving a CTA the whole list of a 128-row query tile, for up to FEW_ROWS query rows, and for as many as one 128-row tile
+# of packed rows per SM holds. B200, scores capped, us (split / listed): 32 / 8 heads: 1 row x 20000 keys 23 / 485, 32 x 32768
+# 41 / 797, 128 x 1024 19 / 36, 512 x 512 21 / 22, 512 x 8192 114 / 188, 1024 x 8192 (two packed tiles per SM) 241 / 208; 16 / 8
+# heads: 1024 x 1024 26 / 32, 1024 x 32768 387 / 689; two key tiles: 200 x 200 20 / 16
 FEW_ROWS = 128
+SMS = 148
 # The backward pass has an item of work per (key tile, chunk of query tiles, KV head). Where the key tiles and heads alone are
 # few, shorter chunks make about this many items, 2.5 to each SM. B200, forward and backward in us, one chunk against the
 # chunks of this rule: 500 rows, 16 / 8 heads 68 / 50, 2000 rows, 4 / 1 heads 273 / 98, 2000 rows, 16 / 8 heads 191 / 155, 3000
@@ -311,6 +314,13 @@ def _mod_args(transform: ScoreTransform | None, L: dict):
     return (float(transform.softcap), *(ptr(t) for t in kept)), kept
 
 
+def _few(nq: int, nk: int, Hq: int, Hkv: int) -> bool:
+    if nq <= FEW_ROWS:
+        return True
+    G = Hq // Hkv      # (group sizes that do not divide a tile have the form for up to 128 packed rows only)
+    return TILE % G == 0 and nk > 2 * TILE and (nq * G + TILE - 1) // TILE * Hkv <= SMS
+
+
 def _int32(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
@@ -424,7 +434,7 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
     else:
         with on_device(q):
             q, k, v = _operand(q), _operand(k), _operand(v)
-            if q.shape[0] <= FEW_ROWS:
+            if _few(q.shape[0], k.shape[0], q.shape[1], k.shape[1]):
                 out, lse = _forward_few_rows(q, k, v, layout, transform, scale)
             else:
                 L = _plan(layout, k.shape[1])
