@@ -173,6 +173,16 @@ def test_gradients_go_to_the_flat_buffers():
                 assert leaves[n].grad is None and leaves[n].grad_acc
                 # (two roundings to bf16 apart: the plain result's and, for the second step, the buffer's)
                 assert torch.allclose(leaves[n].main_grad.float(), step * plain[n].float(), rtol=2.0 ** -6, atol=2.0 ** -8), (n, step)
+    # one parameter in all three places
+    w = t["w_post"].detach().requires_grad_()
+    w.main_grad, w.grad_acc = torch.full((512,), 7.0, device="cuda"), False
+    same = run({**t, "w_post": w.detach(), "w_pre": w.detach(), "gate": w.detach()}, dy, dh)
+    y, h = sandwich_norm(t["x"], t["res"], w, w, gate=w, res_scale=0.9, eps=EPS)
+    torch.autograd.backward([y, h], [dy, dh])
+    total = sum(same[n].double() for n in ("w_post", "w_pre", "gate"))
+    size = sum(same[n].double().abs() for n in ("w_post", "w_pre", "gate"))
+    # (the separate gradients come rounded to bf16, the buffer holds 32 bits)
+    assert bool(((w.main_grad.double() - total).abs() <= 2.0 ** -8 * size + 2.0 ** -20).all())
     from turbo_dllm_b200.kernels.native import NativeKernelError
 
     leaves["w_post"].main_grad = torch.zeros(512, dtype=torch.float16, device="cuda")

@@ -168,11 +168,14 @@ class _SandwichNorm(torch.autograd.Function):
         dx, dres = torch.empty((rows, H), dtype=dtype, device=dev), torch.empty((rows, H), dtype=dtype, device=dev)
         dgate = torch.empty((rows, H), dtype=dtype, device=dev) if kind == GATE_FULL else None
         # vectors that own a slice of the flat gradient buffer are written (or added) there, the others are returned
-        targets, flags, returned, written = [], [], [], []
+        targets, flags, returned, written, again = [], [], [], [], []
         for vec, ref, need in zip((w_post, w_pre, gate if kind == GATE_CHANNEL else None), ctx.refs, ctx.needs_input_grad[2:5]):
             sink, acc = (None, False) if vec is None or not need else grad_sink(ref)
             if sink is not None and sink.dtype not in (torch.float32, x.dtype):
                 raise native.NativeKernelError(f"gradient buffer of {sink.dtype} for a {x.dtype} parameter")
+            if sink is not None and any(ref is r for r in written):   # one parameter in two places: added behind the kernel
+                again.append((sink, torch.empty_like(sink)))
+                sink, acc = again[-1][1], False
             grad = torch.empty_like(vec) if vec is not None and need and sink is None else None
             to = sink if sink is not None else grad
             targets.append(to)
@@ -189,6 +192,8 @@ class _SandwichNorm(torch.autograd.Function):
                 stats.data_ptr(), dx.data_ptr(), dres.data_ptr(), ptr(dgate), *(ptr(t) for t in targets), *flags, ptr(part), _row_stride(x), _row_stride(res),
                 _row_stride(gate) if kind == GATE_FULL else H, rows, H, kind, _DTYPES[dtype], res_scale, stream_of(x)),
                 "sandwich_norm_bwd")
+        for sink, more in again:
+            sink.add_(more)
         for ref in written:
             mark_grad_written(ref)
         if kind != GATE_FULL:
