@@ -171,6 +171,8 @@ def test_refusals():
         scored_attention(q, k, k, L, ScoreTransform(0.0, s, pos[:5], pos))
     with pytest.raises(ValueError, match="divide"):
         scored_attention(q[:, :3], k, k, L)
+    with pytest.raises(ValueError, match="divide"):
+        scored_attention(q[:, :0], k, k, L)
     for bad in (0.0, -0.1, float("nan"), float("inf")):
         with pytest.raises(ValueError, match="scale"):
             scored_attention(q, k, k, L, scale=bad)
@@ -462,6 +464,19 @@ def test_a_layout_that_is_written_to_and_a_plan_built_inside_a_capture(listed):
     junk = [torch.full((4096,), 7, dtype=torch.int32, device="cuda") for _ in range(64)]
     graph.replay()
     assert torch.equal(held, want) and len(junk) == 64
+
+
+@pytest.mark.gpu
+def test_layouts_of_inference_mode_are_followed(listed):
+    q, k, v = _operands(300, 300, 4, 2, 19)
+    want = scored_attention(q, k, v, document_layout([300], device="cuda"))
+    with torch.inference_mode():
+        L = document_layout([100, 200], device="cuda")
+        scored_attention(q, k, v, L)
+        M = document_layout([300], device="cuda")
+        L.q_lo.copy_(M.q_lo)
+        L.q_hi.copy_(M.q_hi)
+        assert torch.equal(scored_attention(q, k, v, L), want)
 
 
 @pytest.mark.gpu

@@ -1046,7 +1046,7 @@ using namespace tdllm;
 
 // floats of scratch that tdllm_attn_few_rows needs (0: the keys are not split)
 extern "C" long long tdllm_attn_few_rows_scratch(int nq, int nk, int Hq, int Hkv) {
-  if (nq <= 0 || nk <= 0 || Hkv <= 0 || Hq % Hkv) return 0;
+  if (nq <= 0 || nk <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv) return 0;
   const few::Plan pl = few::plan_of(nq, nk, Hq, Hkv);
   return pl.splits > 1 ? (long long)pl.splits * nq * Hq * (few::HD + 2) : 0;
 }
@@ -1059,7 +1059,7 @@ extern "C" int tdllm_attn_few_rows(const void* q, const void* k, const void* v, 
                                    const int* k_code, float scale, float softcap, const float* slopes, const int* q_pos,
                                    const int* k_pos, void* stream) {
   if (nq <= 0 || nk <= 0) return 0;
-  if (Hkv <= 0 || Hq % Hkv) {
+  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv) {
     tdllm_host::set_last_error("attn_few_rows: %d query heads do not divide over %d KV heads", Hq, Hkv);
     return 1;
   }

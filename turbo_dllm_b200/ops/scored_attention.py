@@ -20,7 +20,8 @@ The block-diffusion masks come from `block_diffusion_layout`; `document_layout` 
 a prefix that is read in both directions). On CUDA bf16 tensors with head width 128 the tcgen05 kernels run
 (`csrc/attention_fwd_sm100.cu`, `csrc/attention_bwd_fused_sm100.cu` with the transforms of `csrc/score_mod.cuh`);
 everything else takes `scored_attention_reference`. A layout's tile lists and a transform's padded positions are built on
-first use and again when one of their tensors has been written to. A captured graph uses the lists that its layout and
+first use and again when one of their tensors has been written to (in every call where the tensors were made in inference
+mode, which does not count writes). A captured graph uses the lists that its layout and
 transform had then (or builds its own at every replay, if they had none): keep both objects as long as the graph. The form
 for few query rows has no lists and follows its tensors.
 """
@@ -67,15 +68,19 @@ SMS = 148
 BACKWARD_ITEMS = 370
 
 
-def _version(t: torch.Tensor) -> int:
-    return 0 if t.is_inference() else t._version
+def _version(t: torch.Tensor) -> int | None:
+    """None: a tensor of inference mode, which does not say when it has been written to."""
+    return None if t.is_inference() else t._version
 
 
 def _kept(cache: dict, name: str, key, like: torch.Tensor, build):
     """cache[name] if it was made for `key`, else what `build` makes on `like`'s device: (tensors, what goes with them). What
     is made eagerly is complete on return, so that any stream may use it, and its memory is not given away before those
-    streams are done; what is made while a graph is captured belongs to that graph and is not kept. What a capture uses
-    stays with its owner as long as that lives, also when a newer one takes its place."""
+    streams are done; what is made while a graph is captured belongs to that graph and is not kept, nor is what a key with
+    None in it asks for. What a capture uses stays with its owner as long as that lives, also when a newer one takes its
+    place."""
+    if None in key:
+        return build()
     hit = cache.get(name)
     if not like.is_cuda:
         if hit is None or hit[0] != key:
@@ -270,7 +275,7 @@ def scored_attention_reference(q, k, v, layout: MaskLayout, transform: ScoreTran
 def _check(q, k, v, layout: MaskLayout, transform: ScoreTransform | None) -> None:
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
         raise ValueError(f"need q [nq, Hq, D] and k, v [nk, Hkv, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+    if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError(f"{q.shape[1]} query heads do not divide over {k.shape[1]} KV heads")
     if not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
         raise ValueError("q, k and v must share dtype and device")
