@@ -389,7 +389,7 @@ def _backward(q, k, v, out, rest, dout, lse, L, mod, scale):
 
 class _ScoredAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, layout, transform, scale):
+    def forward(ctx, q, k, v, layout, transform, scale, want_lse):
         with on_device(q):
             q, k, v = _operand(q), _operand(k), _operand(v)
             # (the backward pass goes by the lists and positions of the forward pass, whatever is written to them since)
@@ -398,17 +398,23 @@ class _ScoredAttention(torch.autograd.Function):
             out, lse, rest = _forward(q, k, v, ctx.L, ctx.mod, scale, for_backward=True)
         ctx.save_for_backward(q, k, v, out, rest, lse)
         ctx.scale = scale
-        lse = lse[:, : q.shape[0]]
+        ctx.set_materialize_grads(False)
+        if not want_lse:
+            return out, None
+        if lse.shape[1] != q.shape[0]:
+            lse = lse[:, : q.shape[0]]
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
     def backward(ctx, dout, _dlse):
         refuse_twice("scored attention")
+        if dout is None:
+            return (None,) * 7
         q, k, v, out, rest, lse = ctx.saved_tensors
         with on_device(q):
             grads = _backward(q, k, v, out, rest, _operand(dout), lse, ctx.L, ctx.mod, ctx.scale)
-        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None)
 
 
 def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: MaskLayout,
@@ -432,7 +438,7 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
         if q.shape[0] == 0 or k.shape[0] == 0:
             out, lse = scored_attention_reference(q, k, v, layout, transform, scale)
         else:
-            out, lse = _ScoredAttention.apply(q, k, v, layout, transform, scale)
+            out, lse = _ScoredAttention.apply(q, k, v, layout, transform, scale, return_lse)
     elif q.shape[0] == 0 or k.shape[0] == 0:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.full((q.shape[1], q.shape[0]), float("-inf"), dtype=torch.float32, device=q.device)
