@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from turbo_dllm_b200.ops.attention import MaskLayout, block_diffusion_layout
-from turbo_dllm_b200.ops.scored_attention import (DEAD_KEY, ScoreTransform, _seen_keys, document_layout, document_positions,
+from turbo_dllm_b200.ops.scored_attention import (DEAD_KEY, ScoreTransform, document_layout, document_positions,
                                                   scored_attention, scored_attention_reference)
 
 D = 128
@@ -104,20 +104,6 @@ def test_document_layout_masks():
     assert torch.equal(full, torch.block_diag(torch.ones(3, 3), torch.ones(5, 5)).bool())
     assert document_positions([3, 0, 5], rows=11).tolist() == [0, 1, 2, 0, 1, 2, 3, 4, 0, 0, 0]
     assert document_layout([]).nq == 0
-
-
-@pytest.mark.parametrize("seed", range(4))
-def test_seen_keys_match_the_dense_mask(seed):
-    g = torch.Generator().manual_seed(seed)
-    lo = torch.randint(0, 60, (23,), generator=g)
-    hi = lo + torch.randint(-5, 20, (23,), generator=g)
-    grp = -torch.randint(0, 6, (23,), generator=g)
-    code = torch.randint(-8, 80, (57,), generator=g)
-    code[5] = DEAD_KEY
-    L = MaskLayout(*(t.to(torch.int32) for t in (lo, hi, grp, code)))
-    want = L.dense_mask().any(0)
-    # a query of grp 0 sees no noisy key: codes are negative there
-    assert torch.equal(_seen_keys(L), want)
 
 
 @pytest.mark.parametrize("kind", ["none", "cap", "smallcap", "bias", "both"])
@@ -394,10 +380,22 @@ def test_strides_and_alignment():
     assert torch.isfinite(dq).all()
 
 
+def scattered_layout(seed, nq, nk):
+    """Intervals, blocks and codes in no order; some rows see nothing, some keys are seen by none."""
+    g = torch.Generator().manual_seed(seed)
+    lo = torch.randint(0, 60, (nq,), generator=g)
+    hi = lo + torch.randint(-5, 20, (nq,), generator=g)
+    grp = -torch.randint(0, 6, (nq,), generator=g)
+    code = torch.randint(-8, 90, (nk,), generator=g)
+    code[5] = DEAD_KEY
+    return MaskLayout(*(t.to(torch.int32).cuda() for t in (lo, hi, grp, code)))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("make", [lambda: document_layout([300, 0, 77], prefix=[40, 0, 0], rows=400, device="cuda"),
                                   lambda: blocks(640, 32, window=200)[0], lambda: step_layout([70, 900, 0], 60, capacity=1000)[0],
-                                  lambda: document_layout([1], device="cuda")])
+                                  lambda: document_layout([1], device="cuda"),
+                                  *(lambda seed=seed, n=n: scattered_layout(seed, *n) for seed in (0, 1) for n in ((23, 57), (500, 700)))])
 @pytest.mark.parametrize("Hkv", [1, 8, 64])
 def test_plan_matches_the_dense_mask(make, Hkv):
     """Every visible pair lies in a listed tile, tiles without a mask are fully visible, lists are complete and in order."""
@@ -416,6 +414,9 @@ def test_plan_matches_the_dense_mask(make, Hkv):
     nqt, nkt = P["nqt"], P["nkt"]
     m = torch.zeros(nqt * 128, nkt * 128, dtype=torch.bool)
     m[: L.nq, : L.nk] = L.dense_mask().cpu()
+    # keys that no row sees come in as dead
+    codes = torch.where(m.any(0)[: L.nk], L.k_code.cpu(), torch.full((), DEAD_KEY, dtype=torch.int32)).tolist()
+    assert buf[off[3]: off[3] + L.nk] == codes and set(buf[off[3] + L.nk: off[3] + nkt * 128]) <= {DEAD_KEY}
     any_ = m.view(nqt, 128, nkt, 128).any(3).any(1)
     real = torch.arange(nqt * 128) < L.nq
     all_ = (m | ~real[:, None]).view(nqt, 128, nkt, 128).all(3).all(1)

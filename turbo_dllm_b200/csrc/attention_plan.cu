@@ -3,12 +3,13 @@
 // only the device knows, so a plan can be built inside a captured graph.
 //
 // Rows that see no clean key get an empty interval behind every coordinate, so that they do not widen what their tile
-// seems to see; keys that no row sees come in with code DEAD_KEY. Per tile:
+// seems to see; keys that no row sees get the code DEAD_KEY. Per tile:
 //   queries   lo_min, hi_max (rows with an interval), lo_max, hi_min (all rows), grp_min, grp_max (noisy rows)
 //   keys      c_min, c_max (clean), n_min, n_max (noisy), all_clean
 // A pair of tiles is visited if the clean or the noisy ranges meet, and needs no mask if every row's interval holds all
 // of the keys. Lists are in tile order; `order` has the longest lists first (ties: lowest tile), so results and their
-// launch order repeat. The work is a few comparisons per pair of tiles.
+// launch order repeat. The work is a few comparisons per pair of tiles: the first pass on a new layout of 5000 rows takes
+// 0.3 ms longer than the next one, most of it on the host (1.7 ms with lists built there).
 #include "common.cuh"
 #include "score_mod.cuh"
 #include "api.h"
@@ -42,34 +43,22 @@ __device__ __forceinline__ int red_min(int v, int* sm) {
 }
 __device__ __forceinline__ int red_max(int v, int* sm) { return ~red_min(~v, sm); }
 
-// one block per tile: padded copies and the tile's bounds
-__global__ void __launch_bounds__(TILE) stat_kernel(const Args a) {
+// one block per query tile: padded copies and the tile's bounds
+__global__ void __launch_bounds__(TILE) query_kernel(const Args a) {
   __shared__ int sm[4];
-  const int t = threadIdx.x;
-  if ((int)blockIdx.x < a.nqt) {
-    const int at = blockIdx.x * TILE + t;
-    const bool real = at < a.nq;
-    int lo = real ? max(a.q_lo[at], 0) : 0, hi = real ? a.q_hi[at] : 0;
-    const int grp = real ? a.q_grp[at] : 0;
-    const bool sees = hi > lo;
-    if (!sees) { lo = BIG; hi = 0; }
-    a.lo[at] = lo;
-    a.hi[at] = hi;
-    a.grp[at] = grp;
-    const int lo_min = red_min(sees ? lo : BIG, sm), hi_max = red_max(sees ? hi : -1, sm);
-    const int lo_max = red_max(real ? lo : -BIG, sm), hi_min = red_min(real ? hi : BIG, sm);
-    const int g_min = red_min(grp < 0 ? grp : 0, sm), g_max = red_max(grp < 0 ? grp : -BIG - 1, sm);
-    if (t == 0) a.qs[blockIdx.x] = {lo_min, hi_max, lo_max, hi_min, g_min, g_max};
-  } else {
-    const int k = blockIdx.x - a.nqt, at = k * TILE + t;
-    const int c = at < a.nk ? a.k_code[at] : score::DEAD_KEY;
-    a.code[at] = c;
-    const bool clean = c >= 0, noisy = c < 0 && c != score::DEAD_KEY;
-    const int c_min = red_min(clean ? c : BIG, sm), c_max = red_max(clean ? c : -1, sm);
-    const int n_min = red_min(noisy ? c : 0, sm), n_max = red_max(noisy ? c : -BIG - 1, sm);
-    const int all = red_min(clean ? 1 : 0, sm);
-    if (t == 0) a.ks[k] = {c_min, c_max, n_min, n_max, all, 0};
-  }
+  const int at = blockIdx.x * TILE + threadIdx.x;
+  const bool real = at < a.nq;
+  int lo = real ? max(a.q_lo[at], 0) : 0, hi = real ? a.q_hi[at] : 0;
+  const int grp = real ? a.q_grp[at] : 0;
+  const bool sees = hi > lo;
+  if (!sees) { lo = BIG; hi = 0; }
+  a.lo[at] = lo;
+  a.hi[at] = hi;
+  a.grp[at] = grp;
+  const int lo_min = red_min(sees ? lo : BIG, sm), hi_max = red_max(sees ? hi : -1, sm);
+  const int lo_max = red_max(real ? lo : -BIG, sm), hi_min = red_min(real ? hi : BIG, sm);
+  const int g_min = red_min(grp < 0 ? grp : 0, sm), g_max = red_max(grp < 0 ? grp : -BIG - 1, sm);
+  if (threadIdx.x == 0) a.qs[blockIdx.x] = {lo_min, hi_max, lo_max, hi_min, g_min, g_max};
 }
 
 __device__ __forceinline__ bool meets(const QStat& q, const KStat& k) {
@@ -77,6 +66,43 @@ __device__ __forceinline__ bool meets(const QStat& q, const KStat& k) {
 }
 __device__ __forceinline__ bool whole(const QStat& q, const KStat& k) {
   return k.all_clean && k.c_max < q.hi_min && k.c_min >= q.lo_max;
+}
+
+__device__ __forceinline__ KStat key_stat(int c, int* sm) {
+  const bool clean = c >= 0, noisy = c < 0 && c != score::DEAD_KEY;
+  KStat s;
+  s.c_min = red_min(clean ? c : BIG, sm);
+  s.c_max = red_max(clean ? c : -1, sm);
+  s.n_min = red_min(noisy ? c : 0, sm);
+  s.n_max = red_max(noisy ? c : -BIG - 1, sm);
+  s.all_clean = red_min(clean ? 1 : 0, sm);
+  s.pad = 0;
+  return s;
+}
+
+// one block per key tile: the codes, those of keys that no row sees replaced by DEAD_KEY, and the tile's bounds. The rows of
+// the query tiles that may see the tile are tried until every key has been seen (mostly in the first tile).
+__global__ void __launch_bounds__(TILE) key_kernel(const Args a) {
+  __shared__ int sm[4];
+  __shared__ int4 rows[TILE];
+  const int t = threadIdx.x, at = blockIdx.x * TILE + t;
+  const int c = at < a.nk ? a.k_code[at] : score::DEAD_KEY;
+  const KStat all = key_stat(c, sm);
+  bool seen = false;
+  for (int q = 0; q < a.nqt; ++q) {
+    if (!meets(a.qs[q], all)) continue;
+    if (__syncthreads_and(seen || c == score::DEAD_KEY)) break;
+    rows[t] = make_int4(a.lo[q * TILE + t], a.hi[q * TILE + t], a.grp[q * TILE + t], 0);
+    __syncthreads();
+    for (int e = 0; e < TILE && !seen; ++e) {
+      const int4 r = rows[e];
+      seen = c >= 0 ? c >= r.x && c < r.y : c == r.z;
+    }
+  }
+  const int code = seen ? c : score::DEAD_KEY;
+  a.code[at] = code;
+  const KStat s = key_stat(code, sm);
+  if (t == 0) a.ks[blockIdx.x] = s;
 }
 
 // one warp per list, forward lists first: FILL false counts, FILL true writes the entries (tile * 2 + needs a mask)
@@ -208,7 +234,8 @@ extern "C" int tdllm_attn_plan(const int* q_lo, const int* q_hi, const int* q_gr
   a.w_count = work + (a.nqt + 63) / 64 * 64;
   cudaStream_t st = (cudaStream_t)stream;
   const int lists = a.nqt + a.nch * a.nkt;
-  plan::stat_kernel<<<a.nqt + a.nkt, 128, 0, st>>>(a);
+  plan::query_kernel<<<a.nqt, 128, 0, st>>>(a);
+  plan::key_kernel<<<a.nkt, 128, 0, st>>>(a);
   plan::list_kernel<false><<<(lists + 7) / 8, 256, 0, st>>>(a);
   plan::scan_kernel<<<2, 1024, 0, st>>>(a);
   plan::list_kernel<true><<<(lists + 7) / 8, 256, 0, st>>>(a);

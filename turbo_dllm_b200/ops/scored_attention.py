@@ -187,22 +187,6 @@ def document_positions(lengths, *, rows: int | None = None, device="cpu") -> tor
     return pos.to(device)
 
 
-def _seen_keys(layout: MaskLayout) -> torch.Tensor:
-    """[nk] bool: keys that some query row sees. (Sorts and searches only: no size that the host would wait for.)"""
-    never = 1 << 40
-    lo, hi, grp, code = (t.long() for t in (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code))
-    if lo.numel() == 0:
-        return torch.zeros_like(code, dtype=torch.bool)
-    real = hi > lo
-    starts = torch.sort(lo.masked_fill(~real, never)).values
-    stops = torch.sort(hi.masked_fill(~real, never)).values
-    groups = torch.sort(grp.masked_fill(grp >= 0, never)).values
-    # intervals that contain c: those that start at or before it minus those that have ended by then
-    covered = torch.searchsorted(starts, code, right=True) > torch.searchsorted(stops, code, right=True)
-    noisy = torch.searchsorted(groups, code, right=True) > torch.searchsorted(groups, code)
-    return torch.where(code >= 0, covered, noisy)
-
-
 _PLAN_PARTS = ("q_lo", "q_hi", "q_grp", "k_code", "f_ptr", "f_idx", "f_order", "w_ptr", "w_idx", "w_order")
 
 
@@ -233,7 +217,6 @@ def _build_plan(layout: MaskLayout, chunk: int, nqt: int, nkt: int):
     if size < 0:
         raise native.NativeKernelError(f"{nq} rows x {nk} keys have too many tiles for a plan")
     lo, hi, grp, code = (_int32(t) for t in (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code))
-    code = code.masked_fill(~_seen_keys(layout), DEAD_KEY)
     buf = torch.empty(size, dtype=torch.int32, device=lo.device)
     native.check(lib.tdllm_attn_plan(ptr(lo), ptr(hi), ptr(grp), ptr(code), nq, nk, chunk, ptr(buf), stream_of(buf)), "attn_plan")
     base = buf.data_ptr()
