@@ -570,3 +570,61 @@ def test_another_stream_and_a_captured_graph():
     q.copy_(q.flip(0))
     graph.replay()
     assert torch.equal(held, scored_attention(q, k, v, L, tr))
+
+
+@pytest.mark.gpu
+def test_threads_share_a_layout(listed):
+    import threading
+
+    L, tr = document_layout([400, 200], device="cuda"), ScoreTransform(20.0)
+    q, k, v = _operands(600, 600, 8, 2, 29)
+    want = scored_attention(q, k, v, document_layout([400, 200], device="cuda"), tr)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            for _ in range(10):
+                out = scored_attention(q, k, v, L, tr)
+                side.synchronize()
+                wrong.extend([] if torch.equal(out, want) else [1])
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
+def test_two_captured_training_steps_replay_at_once():
+    L, tr = document_layout([400, 200], device="cuda"), ScoreTransform(20.0)
+    leaves = [t.requires_grad_() for t in _operands(600, 600, 8, 2, 31)]
+    dout = torch.randn(600, 8, D, device="cuda").bfloat16()
+
+    def step():
+        out = scored_attention(*leaves, L, tr)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(step())
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for got in held:
+        assert torch.equal(got[0], want[0])
+        for a, b in zip(got[1:], want[1:]):    # (sums in another order: a step of the type)
+            assert float((a.double() - b.double()).norm()) <= HALF * float(b.double().norm())

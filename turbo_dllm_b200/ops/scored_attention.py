@@ -23,7 +23,8 @@ everything else takes `scored_attention_reference`. A layout's tile lists and a 
 first use and again when one of their tensors has been written to (in every call where the tensors were made in inference
 mode, which does not count writes). A captured graph uses the lists that its layout and
 transform had then (or builds its own at every replay, if they had none): keep both objects as long as the graph. The form
-for few query rows has no lists and follows its tensors.
+for few query rows has no lists and follows its tensors. Before a training step is captured, let go of eager autograd graphs
+over the same leaves: torch adds into a leaf on the stream of the oldest graph that is alive, which a capture may not use.
 """
 from __future__ import annotations
 
