@@ -18,7 +18,7 @@
 //
 // A warp takes the first form that all the scores of its tile row allow (a cap of 50 leaves scores up to 18, then 37).
 // With the special-function unit alone (exp2, reciprocal, and the softmax's exp2, at 16 a clock and SM) a 128 x 128 tile
-// takes 3072 clocks, three times its two products. Measured over the whole forward pass of 5000 rows, 16 / 8 heads, two
+// takes three times as long as its two products. Measured over the whole forward pass of 5000 rows, 16 / 8 heads, two
 // documents with a prefix: 129 us without a transform, 160 with a cap, 173 with a bias, 201 with both (187, 195 and 244
 // with degree 5 throughout, a loaded position and an absolute value for every score).
 // NaN passes through all forms, and nothing crosses from one score to its neighbour, so masked scores, which may hold

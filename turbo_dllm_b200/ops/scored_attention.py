@@ -347,7 +347,8 @@ def _forward(q, k, v, L, mod, scale, for_backward=False):
     lse = torch.empty(Hq, L["nq_pad"], dtype=torch.float32, device=q.device)
     rc = native.lib().tdllm_attn_fwd_scored(
         ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(lse), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v),
-        out.stride(0), L["q_lo"], L["q_hi"], L["q_grp"], L["k_code"], L["f_ptr"], L["f_idx"], L["f_order"], L["nqt"], float(scale), *mod, stream_of(q))
+        out.stride(0), L["q_lo"], L["q_hi"], L["q_grp"], L["k_code"], L["f_ptr"], L["f_idx"], L["f_order"], L["nqt"],
+        float(scale), *mod, stream_of(q))
     native.check(rc, "attn_fwd_scored")
     return out, lse, rest
 
@@ -363,7 +364,8 @@ def _backward(q, k, v, out, rest, dout, lse, L, mod, scale):
     stats = 2 * Hq * L["nq_pad"]
     work = torch.empty((stats + L["nq_pad"] * Hq * D + 2 * L["nk_pad"] * Hkv * D,), dtype=torch.float32, device=dev)
     rc = native.lib().tdllm_attn_bwd_scored(
-        ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(lse), ptr(work), ptr(work) + 4 * stats,
+        ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(lse), ptr(work),
+        ptr(work) + 4 * stats,
         nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k), _row_stride(v), _row_stride(out), _row_stride(dout),
         dq.stride(0), dk.stride(0), dv.stride(0), L["q_lo"], L["q_hi"], L["q_grp"], L["k_code"], L["w_ptr"], L["w_idx"],
         L["w_order"], L["n_work"], L["nqt"], L["nkt"], float(scale), *mod, stream_of(q))
