@@ -187,6 +187,22 @@ def test_padded_positions_follow_the_tensors():
     assert tr._padded(128, 128)[1][4] == 9
 
 
+def test_changed_copies_have_their_own_lists_and_positions():
+    import dataclasses
+
+    pos = torch.arange(5)
+    tr = ScoreTransform(0.0, torch.ones(2), pos, pos)
+    tr._padded(128, 128)
+    new = dataclasses.replace(tr, k_pos=pos + 7, slopes=torch.full((2,), 3.0))
+    slopes, q_pos, k_pos = new._padded(128, 128)
+    assert k_pos[:5].tolist() == [7, 8, 9, 10, 11] and q_pos[:5].tolist() == [0, 1, 2, 3, 4]
+    assert torch.allclose(slopes, torch.full((2,), 3.0 * math.log2(math.e)))
+    assert tr._padded(128, 128)[2][:5].tolist() == [0, 1, 2, 3, 4]
+    L = document_layout([3, 2])
+    L._cache["mark"] = 1
+    assert dataclasses.replace(L, q_hi=L.q_hi + 1)._cache == {}
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 def _operands(nq, nk, Hq, Hkv, seed, packed=False, gain=2.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -465,6 +481,27 @@ def test_a_layout_that_is_written_to_and_a_plan_built_inside_a_capture(listed):
     junk = [torch.full((4096,), 7, dtype=torch.int32, device="cuda") for _ in range(64)]
     graph.replay()
     assert torch.equal(held, want) and len(junk) == 64
+
+
+@pytest.mark.gpu
+def test_changed_copies_and_assigned_tensors_are_followed(listed):
+    """A replaced layout or transform, and a layout with a new tensor in one of its fields, whose version counters are those of
+    the tensors before them: the results of objects made from nothing."""
+    import dataclasses
+
+    q, k, v = _operands(300, 300, 4, 2, 14)
+    pos = torch.arange(300, device="cuda", dtype=torch.int32)
+    one, two = document_layout([300], device="cuda"), document_layout([100, 200], device="cuda")
+    tr = transform_for("bias", 4, pos, pos, "cuda")
+    other = transform_for("bias", 4, pos, pos * 3, "cuda")
+    first = scored_attention(q, k, v, one, tr)
+    want = scored_attention(q, k, v, two, ScoreTransform(0.0, other.slopes, other.q_pos, other.k_pos))
+    L = dataclasses.replace(one, q_lo=two.q_lo, q_hi=two.q_hi)
+    assert torch.equal(scored_attention(q, k, v, L, dataclasses.replace(tr, k_pos=other.k_pos)), want)
+    out = scored_attention(q.detach().requires_grad_(), k, v, L, tr)
+    assert torch.equal(out[100], v[100].repeat_interleave(2, 0))      # (the second document's first row sees itself alone)
+    one.q_lo, one.q_hi = two.q_lo.clone(), two.q_hi.clone()
+    assert not torch.equal(first, want) and torch.equal(scored_attention(q, k, v, one, other), want)
 
 
 @pytest.mark.gpu

@@ -44,7 +44,7 @@ class MaskLayout:
     q_hi: torch.Tensor
     q_grp: torch.Tensor
     k_code: torch.Tensor
-    _cache: dict = field(default_factory=dict, repr=False)
+    _cache: dict = field(default_factory=dict, init=False, repr=False)      # (a replaced copy begins with its own)
 
     @property
     def nq(self) -> int:

@@ -74,21 +74,25 @@ def _version(t: torch.Tensor) -> int | None:
     return None if t.is_inference() else t._version
 
 
-def _kept(cache: dict, name: str, key, like: torch.Tensor, build):
-    """cache[name] if it was made for `key`, else what `build` makes on `like`'s device: (tensors, what goes with them). What
+def _kept(cache: dict, name: str, sources: tuple, sizes: tuple, build):
+    """cache[name] if it was made from these very tensors as they are now and for these sizes, else what `build` makes on their
+    device: (tensors, what goes with them). An entry holds its tensors, so that another tensor cannot pass for one of them. What
     is made eagerly is complete on return, so that any stream may use it, and its memory is not given away before those
-    streams are done; what is made while a graph is captured belongs to that graph and is not kept, nor is what a key with
-    None in it asks for. What a capture uses stays with its owner as long as that lives, also when a newer one takes its
+    streams are done; what is made while a graph is captured belongs to that graph and is not kept, nor is what is made from
+    tensors of inference mode. What a capture uses stays with its owner as long as that lives, also when a newer one takes its
     place."""
+    like, key = sources[0], (*(_version(t) for t in sources), *sizes)
     if None in key:
         return build()
     hit = cache.get(name)
+    if hit is not None and (hit[0] != key or any(a is not b for a, b in zip(hit[3], sources))):
+        hit = None
     if not like.is_cuda:
-        if hit is None or hit[0] != key:
-            cache[name] = hit = (key, build(), None)
+        if hit is None:
+            cache[name] = hit = (key, build(), None, sources)
         return hit[1]
     capturing = torch.cuda.is_current_stream_capturing()
-    if hit is not None and hit[0] == key:
+    if hit is not None:
         if capturing:
             cache.setdefault(name + "_captured", []).append(hit[1])
         elif hit[2] != stream_of(like):
@@ -98,7 +102,7 @@ def _kept(cache: dict, name: str, key, like: torch.Tensor, build):
     made = build()
     if not capturing:
         torch.cuda.current_stream(like.device).synchronize()
-        cache[name] = (key, made, stream_of(like))
+        cache[name] = (key, made, stream_of(like), sources)
     return made
 
 
@@ -113,7 +117,7 @@ class ScoreTransform:
     slopes: torch.Tensor | None = None
     q_pos: torch.Tensor | None = None
     k_pos: torch.Tensor | None = None
-    _cache: dict = field(default_factory=dict, repr=False)
+    _cache: dict = field(default_factory=dict, init=False, repr=False)      # (a replaced copy begins with its own)
 
     def __post_init__(self):
         if not (math.isfinite(self.softcap) and self.softcap >= 0.0):
@@ -138,8 +142,8 @@ class ScoreTransform:
     def _padded(self, nq_pad: int, nk_pad: int):
         """(slopes * log2 e, q_pos, k_pos) as the kernels read them: floats, positions padded with zeros. Rebuilt when
         one of the tensors has been written to since."""
-        version = (_version(self.slopes), _version(self.q_pos), _version(self.k_pos), nq_pad, nk_pad)
-        return _kept(self._cache, "padded", version, self.slopes, lambda: (self._pad(nq_pad, nk_pad),))[0]
+        return _kept(self._cache, "padded", (self.slopes, self.q_pos, self.k_pos), (nq_pad, nk_pad),
+                     lambda: (self._pad(nq_pad, nk_pad),))[0]
 
     def _pad(self, nq_pad: int, nk_pad: int):
         out = [(self.slopes * LOG2E).contiguous()]
@@ -202,12 +206,11 @@ def _chunk_tiles(nqt: int, nkt: int, Hkv: int) -> int:
 
 def _plan(layout: MaskLayout, Hkv: int) -> dict:
     """Device pointers of the layout's tile lists (`csrc/attention_plan.cu`) with the buffer they lie in. Kept with the
-    layout, and built anew when one of its tensors has been written to."""
+    layout, and built anew when one of its tensors has been written to or another one assigned."""
     parts = (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code)
     nqt, nkt = (layout.nq + TILE - 1) // TILE, (layout.nk + TILE - 1) // TILE
     chunk = _chunk_tiles(nqt, nkt, Hkv)
-    key = tuple(_version(t) for t in parts)
-    return _kept(layout._cache, f"scored_{chunk}", key, layout.q_lo, lambda: _build_plan(layout, chunk, nqt, nkt))[1]
+    return _kept(layout._cache, f"scored_{chunk}", parts, (), lambda: _build_plan(layout, chunk, nqt, nkt))[1]
 
 
 def _build_plan(layout: MaskLayout, chunk: int, nqt: int, nkt: int):
