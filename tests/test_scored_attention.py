@@ -203,6 +203,23 @@ def test_changed_copies_have_their_own_lists_and_positions():
     assert dataclasses.replace(L, q_hi=L.q_hi + 1)._cache == {}
 
 
+@pytest.mark.parametrize("way", ["copy", "deepcopy", "pickle"])
+def test_copies_keep_nothing_that_was_built(way):
+    """What is kept holds addresses of one process's device memory, which a copy does not own."""
+    import copy
+    import pickle
+
+    make = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda t: pickle.loads(pickle.dumps(t))}[way]
+    L, pos = document_layout([3, 2]), torch.arange(5)
+    tr = ScoreTransform(2.0, torch.ones(2), pos, pos + 1)
+    lists = L.tile_lists()
+    tr._padded(128, 128)
+    M, ts = make(L), make(tr)
+    assert M._cache == {} and ts._cache == {} and L._cache["lists"] is lists and "padded" in tr._cache
+    assert torch.equal(M.dense_mask(), L.dense_mask()) and ts.softcap == 2.0 and torch.equal(ts.k_pos, tr.k_pos)
+    assert M.tile_lists()["f_idx"].tolist() == lists["f_idx"].tolist()
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 def _operands(nq, nk, Hq, Hkv, seed, packed=False, gain=2.0):
     g = torch.Generator(device="cuda").manual_seed(seed)

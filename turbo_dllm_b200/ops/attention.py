@@ -46,6 +46,10 @@ class MaskLayout:
     k_code: torch.Tensor
     _cache: dict = field(default_factory=dict, init=False, repr=False)      # (a replaced copy begins with its own)
 
+    def __getstate__(self):
+        """Copies and pickles without what was built, which holds addresses of this object's buffers."""
+        return {**self.__dict__, "_cache": {}}
+
     @property
     def nq(self) -> int:
         return int(self.q_lo.shape[0])

@@ -135,6 +135,10 @@ class ScoreTransform:
             if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"{name} must be a vector of int32 or int64")
 
+    def __getstate__(self):
+        """Copies and pickles without what was built."""
+        return {**self.__dict__, "_cache": {}}
+
     @property
     def biased(self) -> bool:
         return self.slopes is not None
