@@ -389,6 +389,25 @@ def test_contents_of_dead_rows_do_not_matter(junk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["none", "cap", "both"])
+@pytest.mark.parametrize("masked", ["0" * 11, "1" * 11, "10000100010", "0001111011110", "01", "1000", "00000001", "0110" * 6])
+def test_key_tiles_with_and_without_a_mask_in_turn(kind, masked):
+    """Codes come into shared memory for the tiles that need them only; a tile after one without still reads its own. One dead
+    key with junk in each masked tile, at another place each time."""
+    n, nq = 128 * len(masked), 200
+    code = torch.arange(n, dtype=torch.int32)
+    for t, c in enumerate(masked):
+        if c == "1":
+            code[128 * t + (37 * t + 5) % 128] = DEAD_KEY
+    z = torch.zeros(nq, dtype=torch.int32, device="cuda")
+    L = MaskLayout(z, z + n, z, code.cuda())
+    q, k, v = _operands(nq, n, 4, 2, 16)
+    k[L.k_code == DEAD_KEY], v[L.k_code == DEAD_KEY] = float("nan"), float("nan")
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    run_case(q, k, v, L, transform_for(kind, 4, pos[:nq] if n >= nq else pos.new_zeros(nq), pos, "cuda"))
+
+
+@pytest.mark.gpu
 def test_masks_that_leave_every_row_empty():
     z = torch.zeros(70, dtype=torch.int32, device="cuda")
     L = MaskLayout(z, z, z, z + 5)

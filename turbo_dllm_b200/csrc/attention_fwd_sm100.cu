@@ -204,7 +204,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (int j = 0; j < n; ++j) {
         const int s = j & 1;
         const uint32_t ph = (j >> 1) & 1;
-        int kt = list[j] >> 1;
+        const int ent = list[j];
+        int kt = ent >> 1;
         const CUtensorMap* mk = &tm_k;
         const CUtensorMap* mv = &tm_v;
         if (CSBP && kt >= pl.nlt) {
@@ -222,9 +223,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           tma_load_2d(smem_u32(sK + s * TILE_BYTES + c * HALF_BYTES), mk, bar_kfull + 8 * s,
                       kvh * HD + c * 64, kt * BKV);
         if constexpr (MOD != 0) {
+          // (only what the softmax warps will wait for: nothing may be on its way when the slot is used again or the CTA
+          // ends. Without bytes to expect, the barrier's phase is over at once, and the tiles keep their count.)
           const uint32_t bm = bar_meta + 8 * (j % META_SLOTS), dst = smem_u32(sMeta + (j % META_SLOTS) * 1024);
-          mbar_expect_tx(bm, (MOD & score::BIAS) ? 1024 : 512);
-          bulk_load_1d(dst, p.k_code + kt * BKV, 512, bm);
+          const bool codes = ent & 1;
+          mbar_expect_tx(bm, (codes ? 512 : 0) + ((MOD & score::BIAS) ? 512 : 0));
+          if (codes) bulk_load_1d(dst, p.k_code + kt * BKV, 512, bm);
           if constexpr ((MOD & score::BIAS) != 0) bulk_load_1d(dst + 512, p.mod.k_pos + kt * BKV, 512, bm);
         }
         if (!mbar_wait_spin(bar_vempty + 8 * s, ph ^ 1, KID, 11)) break;
