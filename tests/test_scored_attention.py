@@ -345,6 +345,30 @@ def test_few_rows_against_caches_with_junk_behind_their_lengths(new, Hq):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("junk", [float("nan"), float("inf")])
+@pytest.mark.parametrize("kind", ["none", "both"])
+@pytest.mark.parametrize("caches,new,Hq,window", [([100] * 4, 9, 8, None), ([100, 250, 0, 180], 32, 8, None),
+                                                  ([120, 256, 200], 20, 6, 60), ([30, 700], 3, 16, 20)])
+def test_junk_in_unseen_cache_slots_between_seen_ones(caches, new, Hq, window, kind, junk):
+    """Slots behind a sequence's length, or in front of its window, with running codes that no row sees: between the codes
+    that the sequences before and behind it see. And unused noisy groups between used ones."""
+    cap = max(caches) + 30
+    L, qpos, kpos = step_layout(caches, new, capacity=cap, window=window)
+    seqs, span = len(caches), 1 << 20
+    at = torch.arange(cap, dtype=torch.int32, device="cuda")
+    slots = (torch.arange(seqs, dtype=torch.int32, device="cuda")[:, None] * span + at[None]).reshape(-1)
+    # (groups 1, 3, 5, ... used; a key of each even one in between)
+    L = MaskLayout(L.q_lo, L.q_hi, 2 * L.q_grp, torch.cat([slots, 2 * L.k_code[seqs * cap:], -1 - 2 * torch.arange(
+        1, seqs + 1, dtype=torch.int32, device="cuda")]))
+    kpos = torch.cat([kpos, torch.zeros(seqs, dtype=torch.int32, device="cuda")])
+    unseen = ~L.dense_mask().any(0)
+    assert int(unseen[: seqs * cap].sum()) >= 30 * seqs and bool(unseen[-seqs:].all())
+    q, k, v = _operands(L.nq, L.nk, Hq, 2, 15)
+    k[unseen], v[unseen] = junk, -junk
+    run_case(q, k, v, L, transform_for(kind, Hq, qpos, kpos, "cuda"), backward=False)
+
+
+@pytest.mark.gpu
 def test_few_rows_over_more_tiles_than_one_round():
     """148 KV heads leave one split of the keys, whose 1095 tiles exceed the 1024 of one visibility round."""
     L, qpos, kpos = step_layout([140000], 1)

@@ -476,8 +476,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 // exponentials of one tile overlap the products of the next; the two accumulators are joined at the end like two splits.
 //   warps 0-15 softmax, warp 16 TMA (Q once: a 3-D box of 128 / G rows x G heads lands as packed rows; K and V, three
 //   stages), warp 17 issues the MMAs.  TMEM: S0 [0,128) S1 [128,256) O0 [256,384) O1 [384,512), P over S as bf16.
-// Tiles that every row sees whole skip the mask; in the others, V rows that no row of the CTA can see are overwritten
-// with zeros.
+// Tiles that every row sees whole skip the mask; in the others, V rows of keys that none of the CTA's rows sees (an OR over
+// its rows, per key: the bounds' hull also holds unused cache slots between two sequences) are overwritten with zeros.
 namespace fewt {
 
 constexpr int KID = 13;
@@ -488,8 +488,9 @@ constexpr int OFF_X = OFF_STAGE + STAGES * 2 * TILE_BYTES;        // row exchang
 constexpr int OFF_BITS = OFF_X + 2048;                            // visible tiles, then fully visible tiles
 constexpr int OFF_BOUND = OFF_BITS + 2 * ROUND / 8;
 constexpr int OFF_BARS = OFF_BOUND + 32;
+constexpr int OFF_SEEN = OFF_BARS + 256;                          // keys seen: [pipeline][lane quarter][128 bits]
 // no alignment slack: the kernel checks that its dynamic shared memory starts 1 KiB aligned
-constexpr int SMEM_BYTES = OFF_BARS + 256;
+constexpr int SMEM_BYTES = OFF_SEEN + 2 * 4 * 16;
 static_assert(SMEM_BYTES <= 232448, "shared memory budget of one CTA");
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -540,6 +541,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const uint32_t bar_q = b0, bar_kfull = b0 + 8, bar_vfull = b0 + 32, bar_empty = b0 + 56;   // [3] each
   const uint32_t bar_sfull = b0 + 80, bar_pfull = b0 + 96, bar_odone = b0 + 112;             // [2] each
   uint32_t* tmem_slot = (uint32_t*)(smem + OFF_BARS + 128);
+  uint32_t* s_seen = (uint32_t*)(smem + OFF_SEEN);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.Hq / p.Hkv;
@@ -734,20 +736,6 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tmem_ld32(t_s + sub * 64, r);
         tmem_ld32(t_s + sub * 64 + 32, r + 32);
         tmem_ld_wait();
-        if (masked) {
-          // this thread's key of the tile: a V row that no row of the CTA can see is cleared (half a row per thread)
-          const int kv = (split + o * p.splits) * BK + row;
-          const int c = kv < p.nk ? __ldg(p.k_code + kv) : score::DEAD_KEY;
-          const bool none = !s_bound->may_see(c);
-          if (__any_sync(0xffffffffu, none)) {
-            if (none && mbar_wait_spin(bar_vfull + 8 * (j % STAGES), (j / STAGES) & 1, KID, 33)) {
-              uint4* vrow = reinterpret_cast<uint4*>(sKV + (j % STAGES) * 2 * TILE_BYTES + TILE_BYTES + sub * HALF_BYTES + row * 128);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_proxy_async_smem();
-          }
-        }
         score::transform_row<MOD>(r, p.mod, slope, qpos, make_float2(kpos[0], kpos[1]), [&](int e) {
           const float kp = kpos[e >> 5];
           asm volatile("" ::: "memory");
@@ -766,6 +754,8 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll 4
             for (int e = 0; e < 32; ++e) h |= (uint32_t)!mask.sees(__shfl_sync(0xffffffffu, code, e)) << e;
             hidden[x] = h;
+            const uint32_t some = __reduce_or_sync(0xffffffffu, ~h);   // the keys that a row of this warp sees
+            if (lane == 0) s_seen[(i * 4 + qd) * 4 + sub * 2 + x] = some;
           }
 #pragma unroll
           for (int e = 0; e < 64; ++e)
@@ -778,6 +768,19 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       }
       // the barrier also orders the P stores below after the partner's loads of its score columns
       if (!named_bar_all(1 + i, 256, good)) { ok = false; break; }
+      if (masked) {
+        // this thread's key of the tile: a V row that no row of the CTA sees is cleared (half a row per thread)
+        const uint32_t* w = s_seen + i * 16 + qd;   // key `row`: word qd of the four lane quarters
+        const bool none = !(((w[0] | w[4] | w[8] | w[12]) >> lane) & 1u);
+        if (__any_sync(0xffffffffu, none)) {
+          if (none && mbar_wait_spin(bar_vfull + 8 * (j % STAGES), (j / STAGES) & 1, KID, 33)) {
+            uint4* vrow = reinterpret_cast<uint4*>(sKV + (j % STAGES) * 2 * TILE_BYTES + TILE_BYTES + sub * HALF_BYTES + row * 128);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+      }
       const float mx = fmaxf(*xmine, *xother);
       float alpha = 1.f;   // the reference maximum moves only when the new one is 2^8 larger
       if (mx > -INFINITY && (m == -INFINITY || (mx - m) * scl > 8.f)) {
