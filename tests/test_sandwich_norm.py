@@ -158,6 +158,29 @@ def test_strides_and_empty_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,H", [(torch.bfloat16, 4096), (torch.float16, 264), (torch.float32, 516), (torch.bfloat16, 12288)])
+@pytest.mark.parametrize("gate", [None, "channel", "full"])
+@pytest.mark.parametrize("off", [1, 3])
+@pytest.mark.parametrize("rows", [40, 4000])
+def test_weights_that_start_anywhere(dtype, H, gate, off, rows):
+    """Vectors that are slices of a flat buffer, `off` values behind a 16-byte boundary, with and without more rows than blocks."""
+    rows = min(rows, (1 << 24) // H)
+    t, dy, dh = operands(rows, H, gate, dtype, "cuda", rows + H)
+    want, tol = exact(t["x"], t["res"], t["w_post"], t["w_pre"], t.get("gate"), 0.9, dy, dh)
+    for n in ("w_post", "w_pre", "gate"):
+        if n in t and t[n].dim() == 1:
+            flat = torch.full((H + 16,), float("nan"), dtype=dtype, device="cuda")
+            flat[off: off + H] = t[n]
+            t[n] = flat[off: off + H]
+            assert t[n].is_contiguous() and t[n].data_ptr() % 16
+    got = run(t, dy, dh)
+    for n in got:
+        near(got[n], want[n], tol[n], n)
+    y, h = sandwich_norm(t["x"], t["res"], t["w_post"], t["w_pre"], gate=t.get("gate"), res_scale=0.9, eps=EPS)
+    assert torch.equal(y, got["y"]) and torch.equal(h, got["h"])
+
+
+@pytest.mark.gpu
 def test_gradients_go_to_the_flat_buffers():
     t, dy, dh = operands(60, 512, "channel", torch.bfloat16, "cuda")
     plain = run(t, dy, dh)

@@ -211,7 +211,7 @@ __device__ __forceinline__ void store_unit(T* row, int e, bool whole, int H, con
 }
 
 // The rows a block walks: row index of its n-th row is blockIdx.x + n * gridDim.x.
-// SHIFT: the width may be no multiple of V. GATE: see Args. RING: see Ring.
+// SHIFT: the width may be no multiple of V, and the weights need no alignment. GATE: see Args. RING: see Ring.
 template <class T, int V, int NV, bool RING, bool SHIFT, int GATE>
 __global__ void __launch_bounds__(NV > 2 ? MOST_THREADS : MAX_THREADS, RING ? 2 : 1)
 fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h, float* __restrict__ rstd) {
@@ -581,14 +581,15 @@ __global__ void __launch_bounds__(1024) finish_kernel(const float* __restrict__ 
   put<T>(dw_post, c, s);
 }
 
-// Units per thread, threads, blocks and the ring.
+// Units per thread, threads, blocks and the ring. shift: rows or (forward) weights that lines of 16 bytes do not fit.
 struct Shape {
-  int nv, ring, threads, stages, grid, line_bytes;
+  int nv, ring, shift, threads, stages, grid, line_bytes;
   size_t smem;
 };
-static Shape shape_of(int rows, int H, int elem, int tensors, bool backward) {
+static Shape shape_of(int rows, int H, int elem, int tensors, bool backward, bool weights_fit = true) {
   Shape s;
   const int V = 16 / elem;
+  s.shift = H % V != 0 || !weights_fit;
   const int units = H % V ? (H + V - 1 + V - 1) / V : H / V;   // room for any shift
   s.nv = 2;
   while (s.nv * MAX_THREADS < units && s.nv < 32 / V) s.nv *= 2;   // 32 values per thread at most
@@ -604,7 +605,7 @@ static Shape shape_of(int rows, int H, int elem, int tensors, bool backward) {
   auto blocks = [&](int most) { return most < rows ? (most + 7) / 8 * 8 : (rows + 7) / 8 * 8; };
   s.ring = s.nv == 2;
   if (s.ring) {
-    const size_t extra = HEADER + (!backward && H % V ? weights : 0);
+    const size_t extra = HEADER + (!backward && s.shift ? weights : 0);
     // three rows per block; fewer blocks on an SM where they would not fit (the widest ring has 80 KiB rows: two fit)
     while (resident > 1 && resident * (3 * row + extra + 1024) > budget) --resident;
     s.stages = (int)((budget / resident - extra - 1024) / row);
@@ -647,9 +648,9 @@ static cudaError_t sandwich_smem(K kernel, size_t bytes) {
   if (gate_kind == GATE_NONE) { BODY(T, V, NV, RING, SHIFT, GATE_NONE); }            \
   else if (gate_kind == GATE_CHANNEL) { BODY(T, V, NV, RING, SHIFT, GATE_CHANNEL); } \
   else { BODY(T, V, NV, RING, SHIFT, GATE_FULL); }
-// (without the ring: one form for aligned and shifted widths)
+// (without the ring: one form for aligned and shifted widths; the shifted form also serves aligned widths, with a shift of 0)
 #define SANDWICH_TYPE(T, V, BODY)                                                     \
-  if (s.ring && H % V == 0) { SANDWICH_GATE(T, V, 2, true, false, BODY) }             \
+  if (s.ring && !s.shift) { SANDWICH_GATE(T, V, 2, true, false, BODY) }               \
   else if (s.ring) { SANDWICH_GATE(T, V, 2, true, true, BODY) }                       \
   else if (s.nv == 2) { SANDWICH_GATE(T, V, 2, false, true, BODY) }                   \
   else if (s.nv == 4) { SANDWICH_GATE(T, V, 4, false, true, BODY) }                   \
@@ -690,7 +691,9 @@ extern "C" int tdllm_sandwich_norm_fwd(const void* x, const void* res, const voi
     tdllm_host::set_last_error("sandwich_norm_fwd: rows must start on 16 bytes and lie H values plus whole 16 bytes apart");
     return 1;
   }
-  const Shape s = shape_of(rows, H, elem, gate_kind == GATE_FULL ? 3 : 2, false);
+  // weights that do not start on 16 bytes (a slice of a flat buffer) are copied value by value, as for widths of no whole lines
+  const uintptr_t vectors = (uintptr_t)w_post | (uintptr_t)w_pre | (gate_kind == GATE_CHANNEL ? (uintptr_t)gate : 0);
+  const Shape s = shape_of(rows, H, elem, gate_kind == GATE_FULL ? 3 : 2, false, vectors % 16 == 0);
   if (sandwich_ring("sandwich_norm_fwd", s)) return 1;
   const Args p = {x, res, w_post, w_pre, gate, ldx, ldres, ldgate, rows, H, gate_kind, a, eps, s.stages, s.line_bytes};
   cudaError_t e = cudaErrorInvalidValue;
