@@ -218,6 +218,34 @@ def test_gradients_go_to_the_flat_buffers():
 
 
 @pytest.mark.gpu
+def test_threads_with_rows_of_different_widths():
+    """Widths of one kernel that need different amounts of shared memory, launched from several threads at once."""
+    import threading
+
+    cases = [operands(600, H, "full", torch.bfloat16, "cuda", H) for H in (4096, 4608, 5120, 6144)]
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(mine, expected):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    y, h = sandwich_norm(mine["x"], mine["res"], mine["w_post"], mine["w_pre"], gate=mine["gate"], res_scale=0.9, eps=EPS)
+                torch.cuda.current_stream().synchronize()
+                wrong.extend([] if torch.equal(y, expected["y"]) and torch.equal(h, expected["h"]) else ["result"])
+        except Exception as e:   # noqa: BLE001 (a thread's exception is not pytest's)
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(c[0], w)) for c, w in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
 def test_two_captured_graphs_side_by_side():
     t, dy, dh = operands(300, 512, None, torch.bfloat16, "cuda")
     u, ey, eh = operands(300, 512, None, torch.bfloat16, "cuda", seed=5)

@@ -42,6 +42,7 @@ constexpr int MAX_H = 16384;
 constexpr int MAX_THREADS = 512;
 constexpr int MOST_THREADS = 544;   // a shifted row of the largest width has one unit more than 512 threads hold
 constexpr int MAX_STAGES = 6;
+constexpr int BUDGET = 227 * 1024;  // shared memory of a block at most
 constexpr int HEADER = 512;         // barriers and the reduction's slots, in front of the ring
 
 struct Args {
@@ -600,7 +601,7 @@ static Shape shape_of(int rows, int H, int elem, int tensors, bool backward, boo
   if (resident < 1) resident = 1;
   if (resident > 16) resident = 16;
   const size_t row = (size_t)tensors * s.line_bytes;
-  const size_t weights = (size_t)3 * s.line_bytes, budget = 227 * 1024;
+  const size_t weights = (size_t)3 * s.line_bytes, budget = BUDGET;
   // a multiple of the values in a line: one shift per block
   auto blocks = [&](int most) { return most < rows ? (most + 7) / 8 * 8 : (rows + 7) / 8 * 8; };
   s.ring = s.nv == 2;
@@ -639,9 +640,17 @@ static bool sandwich_alike(int elem, int H, const long long* lds, int nld, const
   return true;
 }
 
+// The limit is a property of the kernel and the device that all host threads share: it is set once, to the most that any width
+// takes, so that no thread lowers it between another's setting and its launch. `done`: the instantiation's own flags.
 template <class K>
-static cudaError_t sandwich_smem(K kernel, size_t bytes) {
-  return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
+static cudaError_t sandwich_smem(K kernel, size_t bytes, bool (&done)[64]) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sandwich::BUDGET);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  return e;
 }
 
 #define SANDWICH_GATE(T, V, NV, RING, SHIFT, BODY)                                   \
@@ -699,8 +708,9 @@ extern "C" int tdllm_sandwich_norm_fwd(const void* x, const void* res, const voi
   cudaError_t e = cudaErrorInvalidValue;
 #define FWD(T, V, NV, RING, SHIFT, GATE)                                                             \
   do {                                                                                  \
-    auto k = fwd_kernel<T, V, NV, RING, SHIFT, GATE>;                                                \
-    e = sandwich_smem(k, s.smem);                                                       \
+    static bool done[64] = {false};                                                     \
+    auto k = fwd_kernel<T, V, NV, RING, SHIFT, GATE>;                                   \
+    e = sandwich_smem(k, s.smem, done);                                                 \
     if (e == cudaSuccess)                                                               \
       k<<<s.grid, s.threads, s.smem, (cudaStream_t)stream>>>(p, (T*)y, (T*)h, rstd);    \
   } while (0)
@@ -753,8 +763,9 @@ extern "C" int tdllm_sandwich_norm_bwd(const void* x, const void* res, const voi
     e = cudaErrorInvalidValue;
 #define BWD(T, V, NV, RING, SHIFT, GATE)                                                                                              \
   do {                                                                                                                   \
-    auto k = bwd_kernel<T, V, NV, RING, SHIFT, GATE>;                                                                                 \
-    e = sandwich_smem(k, s.smem);                                                                                        \
+    static bool done[64] = {false};                                                                                      \
+    auto k = bwd_kernel<T, V, NV, RING, SHIFT, GATE>;                                                                    \
+    e = sandwich_smem(k, s.smem, done);                                                                                  \
     if (e == cudaSuccess)                                                                                                \
       k<<<s.grid, s.threads, s.smem, st>>>(p, (const T*)dy, (const T*)dh, rstd, (T*)dx, (T*)dres, (T*)dgate, scratch);   \
   } while (0)
