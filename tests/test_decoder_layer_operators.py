@@ -204,3 +204,39 @@ def test_the_split_backward_is_refused(monkeypatch):
         scored_attention(x, x, x, layout)
     with torch.no_grad():
         assert scored_attention(x, x, x, layout).shape == x.shape
+
+
+def test_tangents_are_refused_where_kernels_run_and_nowhere_else():
+    from torch.autograd import forward_ad
+
+    from turbo_dllm_b200.ops._util import refuse_tangents
+
+    x, t = torch.randn(4, 1, 128), torch.randn(4, 1, 128)
+    freqs = frequencies("cpu")
+    refuse_tangents("this", x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, t)
+        refuse_tangents("this", x, None)
+        with pytest.raises(NotImplementedError, match="this has no forward-mode"):
+            refuse_tangents("this", x, None, dual)
+        # (the reference, which the CPU takes, has the derivative: the rotation is linear)
+        turned = forward_ad.unpack_dual(rotary(dual, torch.arange(4), freqs)).tangent
+    assert torch.equal(turned, rotary(t, torch.arange(4), freqs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["rotary", "attention", "norm"])
+def test_tangents_are_refused_on_the_gpu(which):
+    from torch.autograd import forward_ad
+
+    x = torch.randn(4, 1, 128, device="cuda").bfloat16()
+    w, freqs, pos = torch.ones(128, device="cuda").bfloat16(), frequencies("cuda"), torch.arange(4, device="cuda")
+    L = document_layout([4], device="cuda")
+    call, places = {"rotary": (lambda t: rotary(t[0], pos, freqs), 1),
+                    "attention": (lambda t: scored_attention(*t, L, ScoreTransform(5.0)), 3),
+                    "norm": (lambda t: sandwich_norm(t[0], t[1], w, w, gate=t[2]), 3)}[which]
+    with forward_ad.dual_level():
+        call([x] * 3)
+        for at in range(places):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call([forward_ad.make_dual(x, x) if i == at else x for i in range(3)])

@@ -4,6 +4,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from ..kernels import native
 
@@ -57,6 +58,13 @@ def refuse_twice(what: str) -> None:
     """For a backward pass made of kernels: with create_graph its results would silently carry no graph."""
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} cannot be differentiated twice")
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """For a call of kernels outside of an autograd function, which would drop a forward-mode tangent (a dual tensor does not
+    require a gradient)."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def grad_sink(param: torch.Tensor):

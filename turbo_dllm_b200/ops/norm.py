@@ -9,8 +9,8 @@ from __future__ import annotations
 import torch
 
 from ..kernels import native
-from ._util import (dtype_code, grad_sink, mark_grad_written, on_device, ptr, refuse_twice, scratch, stream, stream_of,
-                    use_native)
+from ._util import (dtype_code, grad_sink, mark_grad_written, on_device, ptr, refuse_tangents, refuse_twice, scratch, stream,
+                    stream_of, use_native)
 
 
 native.register_signatures({
@@ -227,6 +227,7 @@ def sandwich_norm(x: torch.Tensor, res: torch.Tensor, w_post: torch.Tensor, w_pr
         grad = grad or t.requires_grad
     if dtype_code(x) is None:
         return sandwich_norm_reference(x, res, w_post, w_pre, gate, res_scale, eps)
+    refuse_tangents("sandwich_norm", x, res, w_post, w_pre, gate)
     if H > SANDWICH_MAX_WIDTH:
         raise native.NativeKernelError(f"sandwich_norm kernels take widths up to {SANDWICH_MAX_WIDTH}, got {H}")
     w_post, w_pre = w_post.contiguous(), w_pre.contiguous()

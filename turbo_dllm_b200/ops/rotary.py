@@ -20,7 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from ..kernels import native
-from ._util import dtype_code, on_device, refuse_twice, stream_of
+from ._util import dtype_code, on_device, refuse_tangents, refuse_twice, stream_of
 
 native.register_signatures({
     "tdllm_rotary": (native.c_int, [native.c_void_p] * 4 + [native.c_int] * 4 + [native.c_ll] * 2 + [native.c_int] * 2
@@ -150,6 +150,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, pai
         raise ValueError(f"positions and freqs must lie on {x.device}")
     if dtype_code(x) is None:
         return rotary_reference(x, positions, freqs, pairs, scale)
+    refuse_tangents("rotary", x, freqs)
     if positions.dtype != torch.int32:
         positions = positions.to(torch.int32)
     positions, freqs = positions.contiguous(), freqs.contiguous()

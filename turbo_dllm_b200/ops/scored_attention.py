@@ -35,7 +35,7 @@ from dataclasses import dataclass, field
 import torch
 
 from ..kernels import native
-from ._util import on_device, ptr, refuse_twice, stream_of
+from ._util import on_device, ptr, refuse_tangents, refuse_twice, stream_of
 from .attention import TILE, MaskLayout, backward_chunk_tiles, backward_mode
 
 native.register_signatures({
@@ -425,6 +425,7 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
         return (out, lse.detach()) if return_lse else out
     if q.shape[2] != 128:
         raise native.NativeKernelError("scored attention on bf16 CUDA tensors is built for head_dim 128 (no silent fallback)")
+    refuse_tangents("scored attention", q, k, v, None if transform is None else transform.slopes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if backward_mode() == "split":
             raise native.NativeKernelError("scored attention has the one-pass backward only; unset TDLLM_ATTN_BWD=split")
