@@ -92,6 +92,15 @@ def test_refusals():
         rotary(x, pos, f, pairs="quarter")
 
 
+def test_frequencies_that_want_a_gradient_are_refused():
+    f = rotary_frequencies(8, 1e4)[0].requires_grad_()
+    x, pos = torch.randn(3, 2, 8), torch.arange(3)
+    with pytest.raises(ValueError, match="no gradient"):
+        rotary(x, pos, f)
+    with torch.no_grad():
+        assert torch.equal(rotary(x, pos, f), rotary(x, pos, f.detach()))
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])

@@ -137,13 +137,16 @@ class _Rotary(torch.autograd.Function):
 def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, pairs: str = "half",
            scale: float = 1.0) -> torch.Tensor:
     """x [rows, H, D] (any row and head stride, e.g. the query and key heads of a packed projection) -> [rows, H, D].
-    positions [rows] int32 or int64 (within int32), freqs [n / 2] float32 with n <= D, from `rotary_frequencies`."""
+    positions [rows] int32 or int64 (within int32), freqs [n / 2] float32 with n <= D, from `rotary_frequencies`
+    (constants: they get no gradient)."""
     if x.dim() != 3 or positions.shape != x.shape[:1]:
         raise ValueError(f"need x [rows, H, D] and one position per row, got {tuple(x.shape)} and {tuple(positions.shape)}")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be int32 or int64")
     if freqs.dim() != 1 or freqs.dtype != torch.float32 or not 1 <= freqs.shape[0] <= x.shape[2] // 2:
         raise ValueError(f"freqs must be a float32 vector of 1 to {x.shape[2] // 2} values")
+    if freqs.requires_grad and torch.is_grad_enabled():
+        raise ValueError("freqs are constants of the rotation and get no gradient; detach them")
     if pairs not in PAIRS:
         raise ValueError(f"pairs must be one of {PAIRS}, got {pairs!r}")
     if positions.device != x.device or freqs.device != x.device:
