@@ -399,6 +399,36 @@ def test_few_rows_graph_follows_the_metadata():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Hq", [4, 6, 32])
+@pytest.mark.parametrize("kind", ["none", "cap", "bias"])
+@pytest.mark.parametrize("rows", [100, 160])
+def test_a_row_whose_scores_are_nan_says_so(rows, kind, Hq):
+    """A query row of NaN that does see keys: NaN out, log-sum-exp and gradients, not those of a row without keys (which a
+    merge of partial results would leave out). The other rows keep theirs."""
+    from turbo_dllm_b200.ops import scored_attention as sa
+
+    bad = 37
+    L, pos = document_layout([rows], device="cuda"), document_positions([rows], device="cuda")
+    tr = transform_for(kind, Hq, pos, pos, "cuda")
+    q, k, v = _operands(rows, rows, Hq, 2, 18)
+    spoilt = q.clone()
+    spoilt[bad] = float("nan")
+    rest = torch.arange(rows, device="cuda") != bad
+    for few in (True, False):
+        with pytest.MonkeyPatch.context() as mp:
+            mp.setattr(sa, "_few", lambda *a: few)
+            want, want_lse = scored_attention(q, k, v, L, tr, return_lse=True)
+            out, lse = scored_attention(spoilt, k, v, L, tr, return_lse=True)
+        assert bool(out[bad].isnan().all()) and bool(lse[:, bad].isnan().all())
+        assert torch.equal(out[rest], want[rest]) and torch.equal(lse[:, rest], want_lse[:, rest])
+    leaves = [t.requires_grad_() for t in (spoilt, k, v)]
+    out, lse = scored_attention(*leaves, L, tr, return_lse=True)
+    dq, dk, dv = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert bool(out[bad].isnan().all()) and bool(lse[:, bad].isnan().all()) and bool(dq[bad].isnan().all())
+    assert not bool(dq[rest].isnan().any()) and bool(dv[:bad + 1].isnan().all()) and not bool(dv[bad + 1:].isnan().any())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("junk", [float("nan"), float("inf"), -3.0e38])
 def test_contents_of_dead_rows_do_not_matter(junk):
     lens, rows = [90, 130], 300

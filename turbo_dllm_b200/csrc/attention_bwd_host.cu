@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(256) scored_delta_kernel(const __nv_bfloat16* 
     const size_t at = (size_t)h * nq_pad + row;
     const float l = row < nq ? lse[at] : -INFINITY;
     delta[at] = -s * scale;
-    lse2[at] = l > -INFINITY ? -l * 1.4426950408889634f : -INFINITY;
+    lse2[at] = l != -INFINITY ? -l * 1.4426950408889634f : -INFINITY;   // (NaN goes on to the gradients)
   }
 }
 

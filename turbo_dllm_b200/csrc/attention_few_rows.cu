@@ -119,6 +119,11 @@ struct Bounds {
   __device__ __forceinline__ bool all_see(int c) const { return c >= 0 && c >= v[4] && c < v[5]; }
 };
 
+// a row's log-sum-exp from its maximum (log2 units) and sum: -inf for a row that sees nothing, NaN for one with NaN scores
+__device__ __forceinline__ float lse_of(float top, float sum) {
+  return sum == 0.f ? -INFINITY : top * 0.69314718055994531f + __logf(sum);
+}
+
 // writes one finished row value range: 4 values of row r (packed index) starting at column c
 __device__ __forceinline__ void store_row4(const Params& p, int kvh, int G, int r, int c, const float* v) {
   const int i = r / G, h = kvh * G + r % G;
@@ -438,18 +443,17 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 #pragma unroll
     for (int k = 0; k < KW; ++k) top = fmaxf(top, s_ml[(k * WR + r / 16) * 16 + r % 16]);
     float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (top > -INFINITY) {
+    const float ref = top > -INFINITY ? top : 0.f;
 #pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        const int w = k * WR + r / 16;
-        const float f = score::exp2_approx(s_ml[w * 16 + r % 16] - top);   // (-inf - top: 0)
-        sum += f * s_ml[128 + w * 16 + r % 16];
-        const float4 a = *reinterpret_cast<const float4*>(s_acc + (w * 16 + r % 16) * HD + c);
-        v[0] += f * a.x;
-        v[1] += f * a.y;
-        v[2] += f * a.z;
-        v[3] += f * a.w;
-      }
+    for (int k = 0; k < KW; ++k) {
+      const int w = k * WR + r / 16;
+      const float f = score::exp2_approx(s_ml[w * 16 + r % 16] - ref);   // (-inf: 0; times NaN sums: NaN)
+      sum += f * s_ml[128 + w * 16 + r % 16];
+      const float4 a = *reinterpret_cast<const float4*>(s_acc + (w * 16 + r % 16) * HD + c);
+      v[0] += f * a.x;
+      v[1] += f * a.y;
+      v[2] += f * a.z;
+      v[3] += f * a.w;
     }
     const long long out_row = (long long)(row / G) * p.Hq + kvh * G + row % G;
     if (p.splits == 1) {
@@ -457,9 +461,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] *= inv;
       store_row4(p, kvh, G, row, c, v);
-      if (c == 0)
-        p.lse[(long long)(kvh * G + row % G) * p.ld_lse + row / G] =
-            sum > 0.f ? top * 0.69314718055994531f + __logf(sum) : -INFINITY;
+      if (c == 0) p.lse[(long long)(kvh * G + row % G) * p.ld_lse + row / G] = lse_of(ref, sum);
     } else {
       const long long at = (long long)split * p.nq * p.Hq + out_row;
       *reinterpret_cast<float4*>(p.part_o + at * HD + c) = make_float4(v[0], v[1], v[2], v[3]);
@@ -901,7 +903,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     if (warp < 8 && sub == 0 && row0 + row < rows) {
       const int prow = row0 + row, qi = prow / G, h = kvh * G + prow % G;
       if (p.splits == 1)
-        p.lse[(long long)h * p.ld_lse + qi] = sum > 0.f ? top * 0.69314718055994531f + __logf(sum) : -INFINITY;
+        p.lse[(long long)h * p.ld_lse + qi] = lse_of(top, sum);
       else
         *reinterpret_cast<float2*>(p.part_ml + (((long long)split * p.nq + qi) * p.Hq + h) * 2) = make_float2(top, sum);
     }
@@ -991,8 +993,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) few_rows_join_kernel(const Param
   w.x = pack_bf16x2(v.x * inv, v.y * inv);
   w.y = pack_bf16x2(v.z * inv, v.w * inv);
   *reinterpret_cast<uint2*>(p.o + (long long)i * p.ldo + h * HD + lane * 4) = w;
-  if (lane == 0)
-    p.lse[(long long)h * p.ld_lse + i] = sum > 0.f ? top * 0.69314718055994531f + __logf(sum) : -INFINITY;
+  if (lane == 0) p.lse[(long long)h * p.ld_lse + i] = lse_of(ref, sum);
 }
 
 struct Plan {

@@ -502,8 +502,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         }
       }
+      // (MOD: NaN scores give NaN; a row that sees nothing has l = 0)
+      const bool sees = MOD != 0 ? l != 0.f : l > 0.f;
       if (sub == 0)
-        p.lse[(size_t)min(h0 + i, h_last) * p.nq_pad + grow] = l > 0.f ? m_used * (LOG2 ? 0.69314718055994531f : p.scale) + __logf(l) : -INFINITY;
+        p.lse[(size_t)min(h0 + i, h_last) * p.nq_pad + grow] = sees ? m_used * (LOG2 ? 0.69314718055994531f : p.scale) + __logf(l) : -INFINITY;
       fence_proxy_async_smem();
       mbar_arrive(bar_epi + 8 * i);
       if (row == 0 && sub == 0) {
