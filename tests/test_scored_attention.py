@@ -179,6 +179,25 @@ def test_refusals():
         ScoreTransform(0.0, s, far, pos)._padded(128, 128)
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_positions_at_the_limit(dtype):
+    lim = 1 << 24
+    pos = torch.zeros(4, dtype=dtype)
+    ends = [lim, -lim, torch.iinfo(dtype).min, torch.iinfo(dtype).max]
+    for bad in ends:
+        far = pos.clone()
+        far[2] = bad
+        with pytest.raises(ValueError, match="positions"):
+            ScoreTransform(0.0, torch.ones(2), pos, far)._padded(128, 128)
+    near_ = torch.tensor([lim - 1, 1 - lim, 0, 7], dtype=dtype)
+    assert ScoreTransform(0.0, torch.ones(2), pos, near_)._padded(128, 128)[2][:4].tolist() == near_.tolist()
+    # the reference holds any difference: 2^24 + 1 and 2^24 are one apart
+    x = torch.randn(2, 2, 8)
+    L = document_layout([2])
+    tr = lambda at: ScoreTransform(0.0, torch.ones(2), torch.tensor([at, at + 1]), torch.tensor([at, at + 1]))   # noqa: E731
+    assert torch.equal(scored_attention(x, x, x, L, tr(lim)), scored_attention(x, x, x, L, tr(0)))
+
+
 def test_padded_positions_follow_the_tensors():
     pos = document_positions([5])
     tr = ScoreTransform(0.0, torch.ones(2), pos, pos)
@@ -396,6 +415,41 @@ def test_few_rows_graph_follows_the_metadata():
         a.copy_(b)
     graph.replay()
     assert torch.equal(held, scored_attention(q, k, v, M, transform_for("both", 8, mq, mk, "cuda")))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("Hq,rows", [(2, 5), (6, 40), (8, 40)])
+def test_positions_beyond_the_limit_are_refused_or_spoil_their_rows(Hq, rows, dtype):
+    """One key position that floats do not hold: the call by tile lists refuses it, calls of few rows, whose positions stay on
+    the device, and a captured graph give NaN to the rows that see the key, and to no other."""
+    from turbo_dllm_b200.ops import scored_attention as sa
+
+    n = 300
+    whole, pos = document_layout([n], device="cuda"), torch.arange(n, device="cuda", dtype=dtype)
+    at = torch.arange(n - rows, n, device="cuda")
+    L = MaskLayout(whole.q_lo[at], whole.q_hi[at], whole.q_grp[at], whole.k_code)
+    q, k, v = _operands(rows, n, Hq, 2, 21)
+    bad = n - rows + 3        # rows 3 and later see it
+    slopes = torch.full((Hq,), 0.25, device="cuda")
+    want = scored_attention(q, k, v, L, ScoreTransform(0.0, slopes, pos[at], pos))
+    for value in (1 << 24, -(1 << 24), torch.iinfo(dtype).min, torch.iinfo(dtype).max):
+        far = pos.clone()
+        far[bad] = value
+        tr = ScoreTransform(0.0, slopes, pos[at], far)
+        out, lse = scored_attention(q, k, v, L, tr, return_lse=True)
+        assert torch.equal(out[:3], want[:3]) and bool(out[3:].isnan().all()) and bool(lse[:, 3:].isnan().all())
+        leaf = q.detach().requires_grad_()
+        with pytest.raises(ValueError, match="positions"):
+            scored_attention(leaf, k, v, L, tr)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.MonkeyPatch.context() as mp, torch.no_grad():
+        mp.setattr(sa, "_few", lambda *a: False)
+        with torch.cuda.graph(graph):
+            held = scored_attention(q, k, v, L, tr)
+    graph.replay()
+    assert not bool(held[:3].isnan().any()) and bool(held[3:].isnan().all())
 
 
 @pytest.mark.gpu

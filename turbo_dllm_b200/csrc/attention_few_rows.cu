@@ -205,7 +205,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         grp[x] = p.q_grp[i];
         if constexpr ((MOD & score::BIAS) != 0) {
           slope2[x] = p.slopes[h] * 1.4426950408889634f;
-          qpos[x] = (float)p.q_pos[i];
+          qpos[x] = score::position(p.q_pos[i]);
         }
         const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (long long)i * p.ldq + h * HD) + t4;
 #pragma unroll
@@ -270,7 +270,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             s_code[s * BK + e * 32 + lane] = code[e];
-            if constexpr ((MOD & score::BIAS) != 0) s_kpos[s * BK + e * 32 + lane] = (float)kp[e];
+            if constexpr ((MOD & score::BIAS) != 0) s_kpos[s * BK + e * 32 + lane] = score::position(kp[e]);
           }
           mbar_arrive(bar_full + 8 * s);
           ++j;
@@ -713,7 +713,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     if (prow < rows) {
       if constexpr ((MOD & score::BIAS) != 0) {
         slope = p.slopes[kvh * G + prow % G] * 1.4426950408889634f / scl;
-        qpos = (float)p.q_pos[qi];
+        qpos = score::position(p.q_pos[qi]);
       }
     }
     Walk walk(s_vis);
@@ -729,7 +729,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int k = k0 + x * 32 + lane;
-          kpos[x] = k < p.nk ? (float)__ldg(p.k_pos + k) : 0.f;
+          kpos[x] = k < p.nk ? score::position(__ldg(p.k_pos + k)) : 0.f;
         }
       }
       bool good = __all_sync(0xffffffffu, mbar_wait_spin(bar_sfull + 8 * i, (j >> 1) & 1, KID, 30));

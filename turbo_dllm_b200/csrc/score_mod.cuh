@@ -47,6 +47,11 @@ struct Mod {
   const float* k_pos;   // [nk_pad]
 };
 
+// a position as the float that distances are taken with; one of 2^24 or more, which floats do not hold, becomes NaN, and with
+// it what the rows that meet it get
+__device__ __forceinline__ float position(int p) {
+  return (unsigned)(p + 0xffffff) <= 2u * 0xffffff ? (float)p : __int_as_float(0x7fffffff);
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -111,7 +111,9 @@ class ScoreTransform:
     """What happens to the scores before the softmax.
 
     softcap: cap of the tanh, 0 for none. slopes: [Hq] float32, one slope per query head, with q_pos [nq] and k_pos [nk]
-    (int32 or int64, absolute value below 2^24): the distance bias. Slopes are constants: they get no gradient."""
+    (int32 or int64, absolute value below 2^24): the distance bias. Slopes are constants: they get no gradient. A position
+    beyond the limit is refused; where the host does not see positions, as in calls of few rows, which read them on the
+    device, and in captured graphs, rows that meet one get NaN."""
 
     softcap: float = 0.0
     slopes: torch.Tensor | None = None
@@ -152,11 +154,12 @@ class ScoreTransform:
     def _pad(self, nq_pad: int, nk_pad: int):
         out = [(self.slopes * LOG2E).contiguous()]
         for t, n in ((self.q_pos, nq_pad), (self.k_pos, nk_pad)):
-            # (the check waits for the device, which a capture may not)
-            if t.numel() and not (t.is_cuda and torch.cuda.is_current_stream_capturing()) and int(t.abs().max()) >= MAX_POSITION:
-                raise ValueError(f"positions of the distance bias must lie within +-{MAX_POSITION}")
             f = torch.zeros(n, dtype=torch.float32, device=t.device)
             f[: t.shape[0]] = t
+            if t.is_cuda and torch.cuda.is_current_stream_capturing():      # (which may not wait for the device)
+                f.masked_fill_(f.abs() >= MAX_POSITION, math.nan)
+            elif t.numel() and float(f.abs().max()) >= MAX_POSITION:
+                raise ValueError(f"positions of the distance bias must lie between +-{MAX_POSITION}")
             out.append(f)
         return tuple(out)
 
@@ -252,7 +255,7 @@ def scored_attention_reference(q, k, v, layout: MaskLayout, transform: ScoreTran
     if transform is not None and transform.softcap:
         z = transform.softcap * torch.tanh(z / transform.softcap)
     if transform is not None and transform.biased:
-        far = (transform.q_pos.to(wide)[:, None] - transform.k_pos.to(wide)[None, :]).abs()
+        far = (transform.q_pos.long()[:, None] - transform.k_pos.long()[None, :]).abs().to(wide)
         z = z - transform.slopes.to(wide)[:, None, None] * far
     z = z.masked_fill(~(seen | ~row_live[:, None]), float("-inf"))      # (rows without a key are taken out below)
     if layout.nk == 0:
@@ -317,6 +320,11 @@ def _few(nq: int, nk: int, Hq: int, Hkv: int) -> bool:
     return TILE % G == 0 and nk > 2 * TILE and (nq * G + TILE - 1) // TILE * Hkv <= SMS
 
 
+def _int32_positions(t: torch.Tensor) -> torch.Tensor:
+    """(int64 positions that int32 does not hold stay beyond the limit)"""
+    return _int32(t.clamp(-MAX_POSITION, MAX_POSITION) if t.dtype == torch.int64 else t)
+
+
 def _int32(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
@@ -335,7 +343,7 @@ def _forward_few_rows(q, k, v, layout, transform, scale):
     meta = [_int32(t) for t in (layout.q_lo, layout.q_hi, layout.q_grp, layout.k_code)]
     bias = (None, None, None)
     if transform is not None and transform.biased:
-        bias = [transform.slopes.contiguous(), _int32(transform.q_pos), _int32(transform.k_pos)]
+        bias = [transform.slopes.contiguous(), _int32_positions(transform.q_pos), _int32_positions(transform.k_pos)]
     rc = lib.tdllm_attn_few_rows(
         ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(part), nq, nk, Hq, Hkv, _row_stride(q), _row_stride(k),
         _row_stride(v), Hq * D, nq, *[t.data_ptr() for t in meta], float(scale),
