@@ -239,6 +239,16 @@ def test_copies_keep_nothing_that_was_built(way):
     assert M.tile_lists()["f_idx"].tolist() == lists["f_idx"].tolist()
 
 
+def test_writes_that_are_told():
+    pos = torch.arange(5)
+    tr = ScoreTransform(0.0, torch.ones(2), pos, pos)
+    held = tr._padded(128, 128)
+    assert tr._padded(128, 128)[2] is held[2]
+    pos.data[4] = 9        # (not counted)
+    tr.changed()
+    assert tr._padded(128, 128)[2][:5].tolist() == [0, 1, 2, 3, 9]
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 def _operands(nq, nk, Hq, Hkv, seed, packed=False, gain=2.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -646,6 +656,31 @@ def test_changed_copies_and_assigned_tensors_are_followed(listed):
     assert torch.equal(out[100], v[100].repeat_interleave(2, 0))      # (the second document's first row sees itself alone)
     one.q_lo, one.q_hi = two.q_lo.clone(), two.q_hi.clone()
     assert not torch.equal(first, want) and torch.equal(scored_attention(q, k, v, one, other), want)
+
+
+@pytest.mark.gpu
+def test_a_replayed_graph_that_writes_the_layout_and_the_positions(listed):
+    """Eager calls by tile lists after a replay that moved the metadata on, once they are told."""
+    q, k, v = _operands(300, 300, 4, 2, 20)
+    pos = torch.arange(300, dtype=torch.int32, device="cuda")
+    L, tr = document_layout([300], device="cuda"), transform_for("bias", 4, pos.clone(), pos.clone(), "cuda")
+    M = document_layout([100, 200], device="cuda")
+    before = scored_attention(q, k, v, L, tr)
+    want = scored_attention(q, k, v, M, transform_for("bias", 4, pos * 2, pos * 2, "cuda"))
+    writes = [(L.q_lo, M.q_lo.clone()), (L.q_hi, M.q_hi.clone()), (tr.q_pos, pos * 2), (tr.k_pos, pos * 2)]
+    back = [(a, a.clone()) for a, _ in writes]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for a, b in writes:
+            a.copy_(b)
+    for a, b in back:
+        a.copy_(b)
+    assert torch.equal(scored_attention(q, k, v, L, tr), before)
+    graph.replay()
+    L.changed()
+    tr.changed()
+    assert torch.equal(scored_attention(q, k, v, L, tr), want)
 
 
 @pytest.mark.gpu

@@ -50,6 +50,11 @@ class MaskLayout:
         """Copies and pickles without what was built, which holds addresses of this object's buffers."""
         return {**self.__dict__, "_cache": {}}
 
+    def changed(self) -> None:
+        """Tells scored attention that the tensors hold something else now, where torch does not count the write: a replayed
+        graph's, or a kernel's through a pointer. Its next call builds new lists. (The lists of `tile_lists` stay as they are.)"""
+        self._cache["changes"] = self._cache.get("changes", 0) + 1
+
     @property
     def nq(self) -> int:
         return int(self.q_lo.shape[0])

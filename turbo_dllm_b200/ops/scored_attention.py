@@ -21,7 +21,8 @@ a prefix that is read in both directions). On CUDA bf16 tensors with head width 
 (`csrc/attention_fwd_sm100.cu`, `csrc/attention_bwd_fused_sm100.cu` with the transforms of `csrc/score_mod.cuh`);
 everything else takes `scored_attention_reference`. A layout's tile lists and a transform's padded positions are built on
 first use and again when one of their tensors has been written to (in every call where the tensors were made in inference
-mode, which does not count writes). A captured graph uses the lists that its layout and
+mode, which does not count writes). Writes that torch does not count, those of a replayed graph or of a kernel that was given a
+pointer, are told by `layout.changed()` and `transform.changed()`. A captured graph uses the lists that its layout and
 transform had then (or builds its own at every replay, if they had none): keep both objects as long as the graph. The form
 for few query rows has no lists and follows its tensors. Before a training step is captured, let go of eager autograd graphs
 over the same leaves: torch adds into a leaf on the stream of the oldest graph that is alive, which a capture may not use.
@@ -81,7 +82,7 @@ def _kept(cache: dict, name: str, sources: tuple, sizes: tuple, build):
     streams are done; what is made while a graph is captured belongs to that graph and is not kept, nor is what is made from
     tensors of inference mode. What a capture uses stays with its owner as long as that lives, also when a newer one takes its
     place."""
-    like, key = sources[0], (*(_version(t) for t in sources), *sizes)
+    like, key = sources[0], (*(_version(t) for t in sources), *sizes, cache.get("changes", 0))
     if None in key:
         return build()
     hit = cache.get(name)
@@ -140,6 +141,10 @@ class ScoreTransform:
     def __getstate__(self):
         """Copies and pickles without what was built."""
         return {**self.__dict__, "_cache": {}}
+
+    def changed(self) -> None:
+        """Says that the tensors hold something else now, as `MaskLayout.changed` does."""
+        self._cache["changes"] = self._cache.get("changes", 0) + 1
 
     @property
     def biased(self) -> bool:
