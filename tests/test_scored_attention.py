@@ -249,6 +249,21 @@ def test_writes_that_are_told():
     assert tr._padded(128, 128)[2][:5].tolist() == [0, 1, 2, 3, 9]
 
 
+@pytest.mark.parametrize("nq,nk", [(3, 0), (0, 3), (0, 0)])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_gradients_of_calls_without_rows_or_keys(nq, nk, device):
+    """Zeros, whatever the operands hold, on the path of the caller's loss."""
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    z = torch.zeros(nq, dtype=torch.int32, device=device)
+    L = MaskLayout(z, z + 9, z, torch.arange(nk, dtype=torch.int32, device=device))
+    leaves = [torch.full((n, h, D), float("nan"), dtype=dtype, device=device).requires_grad_() for n, h in ((nq, 4), (nk, 2), (nk, 2))]
+    out, lse = scored_attention(*leaves, L, ScoreTransform(3.0), return_lse=True)
+    assert out.shape == (nq, 4, D) and out.dtype == dtype and lse.shape == (4, nq) and not lse.requires_grad
+    assert lse.dtype == torch.float32 and bool((lse == -math.inf).all()) and bool((out == 0).all())
+    for got, leaf in zip(torch.autograd.grad(out.sum(), leaves), leaves):
+        assert got.shape == leaf.shape and got.dtype == dtype and bool((got == 0).all())
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 def _operands(nq, nk, Hq, Hkv, seed, packed=False, gain=2.0):
     g = torch.Generator(device="cuda").manual_seed(seed)

@@ -263,8 +263,9 @@ def scored_attention_reference(q, k, v, layout: MaskLayout, transform: ScoreTran
         far = (transform.q_pos.long()[:, None] - transform.k_pos.long()[None, :]).abs().to(wide)
         z = z - transform.slopes.to(wide)[:, None, None] * far
     z = z.masked_fill(~(seen | ~row_live[:, None]), float("-inf"))      # (rows without a key are taken out below)
-    if layout.nk == 0:
-        return torch.zeros_like(q), torch.full((Hq, nq), float("-inf"), dtype=wide, device=q.device)
+    if layout.nk == 0:      # (zeros that hang on the operands, whose gradients are zeros)
+        zeros = q.masked_fill(torch.ones((), dtype=torch.bool, device=q.device), 0) + (k.sum() + v.sum())
+        return zeros, torch.full((Hq, nq), float("-inf"), dtype=wide, device=q.device)
     lse = torch.logsumexp(z, dim=-1)
     p = torch.where(row_live[None, :, None], torch.exp(z - lse[..., None]), torch.zeros((), dtype=wide, device=q.device))
     out = torch.matmul(p, vf).permute(1, 0, 2)
@@ -444,6 +445,7 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
             raise native.NativeKernelError("scored attention has the one-pass backward only; unset TDLLM_ATTN_BWD=split")
         if q.shape[0] == 0 or k.shape[0] == 0:
             out, lse = scored_attention_reference(q, k, v, layout, transform, scale)
+            lse = lse.detach()
         else:
             out, lse = _ScoredAttention.apply(q, k, v, layout, transform, scale, return_lse)
     elif q.shape[0] == 0 or k.shape[0] == 0:
