@@ -198,6 +198,18 @@ def test_positions_at_the_limit(dtype):
     assert torch.equal(scored_attention(x, x, x, L, tr(lim)), scored_attention(x, x, x, L, tr(0)))
 
 
+def test_caps_and_scales_that_32_bits_do_not_hold_are_refused():
+    L, x = document_layout([3]), torch.randn(3, 2, 8)
+    for cap in (5e-324, 1e-46, 1e-19, 1e31, 1e39):
+        with pytest.raises(ValueError, match="softcap"):
+            ScoreTransform(cap)
+    for scale in (1e-21, 1e19, 1e39):
+        with pytest.raises(ValueError, match="scale"):
+            scored_attention(x, x, x, L, scale=scale)
+    for cap in (1e-18, 1e30):
+        assert torch.isfinite(scored_attention(x, x, x, L, ScoreTransform(cap))).all()
+
+
 def test_padded_positions_follow_the_tensors():
     pos = document_positions([5])
     tr = ScoreTransform(0.0, torch.ones(2), pos, pos)
@@ -753,6 +765,24 @@ def test_caps_of_every_size(cap, gain):
         # probabilities are off by half a step (2^-8) and by tol, the output by half a step
         size = scored_attention_reference(q.double(), k.double(), v.double().abs(), L, tr)[0][:rows]
         assert bool(((out.double() - want[:rows]).abs() <= 2.0 ** -8 * want[:rows].abs() + (2.0 ** -8 + 4 * tol) * size).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("few", [True, False])
+def test_caps_and_scales_at_their_limits(few, monkeypatch):
+    """Caps of 1e-18 leave scores of nothing (the mean of v over the visible rows), caps of 1e30 leave them as they are."""
+    from turbo_dllm_b200.ops import scored_attention as sa
+
+    monkeypatch.setattr(sa, "_few", lambda *a: few)
+    L = document_layout([200], causal=False, device="cuda")
+    q, k, v = _operands(200, 200, 4, 2, 24)
+    for cap, scale in ((1e-18, 1e18), (1e-18, 1e-20), (1e-18, 0.1), (1e30, 1e-20), (1e30, 0.1)):
+        out, lse = scored_attention(q, k, v, L, ScoreTransform(cap), scale=scale, return_lse=True)
+        want, want_lse = scored_attention_reference(q.double(), k.double(), v.double(), L, ScoreTransform(cap), scale)
+        size = scored_attention_reference(q.double(), k.double(), v.double().abs(), L, ScoreTransform(cap), scale)[0]
+        # scores up to 200 in 32 bits (2^-22 each), probabilities and the output off by half a step
+        assert float((lse.double() - want_lse).abs().max()) <= 2.0 ** -14 * (1 + float(want_lse.abs().max()))
+        assert bool(((out.double() - want).abs() <= HALF * want.abs() + (HALF + 2.0 ** -12) * size).all())
 
 
 @pytest.mark.gpu

@@ -56,6 +56,8 @@ native.register_signatures({
 DEAD_KEY = -(2 ** 31)      # key code that no query row matches
 MAX_POSITION = 1 << 24     # distances are taken between positions held as floats
 LOG2E = 1.4426950408889634
+# caps and scales that 32 bits hold, with their ratio times 2 log2 e and its inverse (a smaller cap would become none there)
+CAPS, SCALES = (1e-18, 1e30), (1e-20, 1e18)
 # A forward without gradients packs the query heads of a KV head into rows and splits the keys over the GPU (`_few`), instead
 # of giving a CTA the whole list of a 128-row query tile, for up to FEW_ROWS query rows, and for as many as one 128-row tile
 # of packed rows per SM holds. B200, scores capped, us (split / listed): 32 / 8 heads: 1 row x 20000 keys 23 / 485, 32 x 32768
@@ -111,7 +113,7 @@ def _kept(cache: dict, name: str, sources: tuple, sizes: tuple, build):
 class ScoreTransform:
     """What happens to the scores before the softmax.
 
-    softcap: cap of the tanh, 0 for none. slopes: [Hq] float32, one slope per query head, with q_pos [nq] and k_pos [nk]
+    softcap: cap of the tanh (1e-18 to 1e30), 0 for none. slopes: [Hq] float32, one slope per query head, with q_pos [nq] and k_pos [nk]
     (int32 or int64, absolute value below 2^24): the distance bias. Slopes are constants: they get no gradient. A position
     beyond the limit is refused; where the host does not see positions, as in calls of few rows, which read them on the
     device, and in captured graphs, rows that meet one get NaN."""
@@ -123,8 +125,8 @@ class ScoreTransform:
     _cache: dict = field(default_factory=dict, init=False, repr=False)      # (a replaced copy begins with its own)
 
     def __post_init__(self):
-        if not (math.isfinite(self.softcap) and self.softcap >= 0.0):
-            raise ValueError(f"softcap must be a finite number >= 0, got {self.softcap}")
+        if not (self.softcap == 0.0 or CAPS[0] <= self.softcap <= CAPS[1]):
+            raise ValueError(f"softcap must be 0 or a number from {CAPS[0]} to {CAPS[1]}, got {self.softcap}")
         given = [t is not None for t in (self.slopes, self.q_pos, self.k_pos)]
         if any(given) and not all(given):
             raise ValueError("a distance bias needs slopes, q_pos and k_pos together")
@@ -432,8 +434,8 @@ def scored_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
     fp32 adds whose order is not fixed, as in `block_attention`'s one-pass backward."""
     _check(q, k, v, layout, transform)
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
-    if not 1e-20 <= scale < math.inf:      # (the row maximum is taken before the scale is applied)
-        raise ValueError(f"scale must be a positive number, got {scale}")
+    if not SCALES[0] <= scale <= SCALES[1]:      # (positive: the row maximum is taken before the scale is applied)
+        raise ValueError(f"scale must be a number from {SCALES[0]} to {SCALES[1]}, got {scale}")
     if not q.is_cuda or q.dtype != torch.bfloat16:
         out, lse = scored_attention_reference(q, k, v, layout, transform, scale)
         return (out, lse.detach()) if return_lse else out
