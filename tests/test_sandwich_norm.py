@@ -246,6 +246,32 @@ def test_threads_with_rows_of_different_widths():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gate", [None, "full"])
+@pytest.mark.parametrize("rows,H", [(4000, 4096), (3000, 136), (3000, 1411)])
+def test_a_recorded_error_ends_the_kernels(rows, H, gate):
+    """While an error of another kernel stands, waits may give up: the kernels end, and once it is cleared results are right."""
+    from turbo_dllm_b200.kernels import native
+
+    t, dy, dh = operands(rows, H, gate, torch.bfloat16, "cuda", 6)
+    want = run(t, dy, dh)
+    lib = native.lib()
+    native.check(lib.tdllm_set_wait_timeout_ns(2_000_000), "set timeout")
+    try:
+        native.check(lib.tdllm_test_wait_timeout(None), "launch")      # (a wait that nobody ends records an error)
+        for _ in range(3):
+            run(t, dy, dh)
+        torch.cuda.synchronize()
+        err = native.device_error()
+        assert err["code"] == 1 and err["kernel"] == 99
+    finally:
+        lib.tdllm_clear_error()
+        lib.tdllm_set_wait_timeout_ns(2_000_000_000)
+    got = run(t, dy, dh)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    native.raise_on_device_error()
+
+
+@pytest.mark.gpu
 def test_two_captured_graphs_side_by_side():
     t, dy, dh = operands(300, 512, None, torch.bfloat16, "cuda")
     u, ey, eh = operands(300, 512, None, torch.bfloat16, "cuda", seed=5)
