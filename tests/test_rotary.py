@@ -92,6 +92,13 @@ def test_refusals():
         rotary(x, pos, f, pairs="quarter")
 
 
+@pytest.mark.parametrize("device", ["meta", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_more_rows_than_32_bits_count_are_refused(device):
+    x, pos = torch.zeros(1, 1, 2, device=device).expand(2 ** 31 + 5, 1, 2), torch.zeros(1, dtype=torch.int32, device=device)
+    with pytest.raises(ValueError, match="rows"):
+        rotary(x, pos.expand(2 ** 31 + 5), torch.ones(1, device=device))
+
+
 def test_frequencies_that_want_a_gradient_are_refused():
     f = rotary_frequencies(8, 1e4)[0].requires_grad_()
     x, pos = torch.randn(3, 2, 8), torch.arange(3)

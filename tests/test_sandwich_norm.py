@@ -108,6 +108,13 @@ def test_refusals():
         sandwich_norm(x[:, :0], res[:, :0], wq[:0], wp[:0])
 
 
+@pytest.mark.parametrize("device", ["meta", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_more_rows_than_32_bits_count_are_refused(device):
+    x, w = torch.zeros(1, 2, device=device).expand(2 ** 31 + 5, 2), torch.zeros(2, device=device)
+    with pytest.raises(ValueError, match="rows"):
+        sandwich_norm(x, x, w, w)
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])

@@ -29,6 +29,8 @@ def use_native(*tensors: torch.Tensor) -> bool:
     return True
 
 
+MAX_ROWS = 2 ** 31 - 1024      # row counts are 32-bit integers in the kernels, rounded up to whole blocks
+
 _DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 

@@ -9,8 +9,8 @@ from __future__ import annotations
 import torch
 
 from ..kernels import native
-from ._util import (dtype_code, grad_sink, mark_grad_written, on_device, ptr, refuse_tangents, refuse_twice, scratch, stream,
-                    stream_of, use_native)
+from ._util import (MAX_ROWS, dtype_code, grad_sink, mark_grad_written, on_device, ptr, refuse_tangents, refuse_twice, scratch,
+                    stream, stream_of, use_native)
 
 
 native.register_signatures({
@@ -220,6 +220,8 @@ def sandwich_norm(x: torch.Tensor, res: torch.Tensor, w_post: torch.Tensor, w_pr
         raise ValueError(f"w_post and w_pre must be vectors of {H} values")
     if gate is not None and gate.shape != (H,) and gate.shape != x.shape:
         raise ValueError(f"gate must be a vector of {H} values or have x's shape, got {tuple(gate.shape)}")
+    if x.numel() // H > MAX_ROWS:
+        raise ValueError(f"sandwich_norm takes up to {MAX_ROWS} rows, got {x.numel() // H}")
     dtype, dev, grad = x.dtype, x.device, x.requires_grad
     for t in (res, w_post, w_pre) if gate is None else (res, w_post, w_pre, gate):
         if t.dtype != dtype or t.device != dev:

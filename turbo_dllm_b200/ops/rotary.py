@@ -20,7 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from ..kernels import native
-from ._util import dtype_code, on_device, refuse_tangents, refuse_twice, stream_of
+from ._util import MAX_ROWS, dtype_code, on_device, refuse_tangents, refuse_twice, stream_of
 
 native.register_signatures({
     "tdllm_rotary": (native.c_int, [native.c_void_p] * 4 + [native.c_int] * 4 + [native.c_ll] * 2 + [native.c_int] * 2
@@ -151,6 +151,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, pai
         raise ValueError(f"pairs must be one of {PAIRS}, got {pairs!r}")
     if positions.device != x.device or freqs.device != x.device:
         raise ValueError(f"positions and freqs must lie on {x.device}")
+    if x.shape[0] > MAX_ROWS:
+        raise ValueError(f"rotary takes up to {MAX_ROWS} rows, got {x.shape[0]}")
     if dtype_code(x) is None:
         return rotary_reference(x, positions, freqs, pairs, scale)
     refuse_tangents("rotary", x, freqs)
