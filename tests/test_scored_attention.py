@@ -234,6 +234,13 @@ def test_changed_copies_have_their_own_lists_and_positions():
     assert dataclasses.replace(L, q_hi=L.q_hi + 1)._cache == {}
 
 
+def test_documents_under_another_default_device():
+    with torch.device("meta"):
+        got, at = document_layout([3, 5], prefix=[1, 0], rows=11), document_positions([3, 5], rows=11)
+    want = document_layout([3, 5], prefix=[1, 0], rows=11)
+    assert torch.equal(got.dense_mask(), want.dense_mask()) and torch.equal(at, document_positions([3, 5], rows=11))
+
+
 @pytest.mark.parametrize("way", ["copy", "deepcopy", "pickle"])
 def test_copies_keep_nothing_that_was_built(way):
     """What is kept holds addresses of one process's device memory, which a copy does not own."""
@@ -327,6 +334,18 @@ def blocks(tokens, block, device="cuda", window=None):
     p = torch.arange(tokens, device=device)
     L = block_diffusion_layout(p, p // block, p, block, window=window)
     return L, torch.cat([p, p]).to(torch.int32)
+
+
+@pytest.mark.gpu
+def test_document_lengths_that_lie_on_the_gpu():
+    lens, pre = torch.tensor([3, 0, 5], device="cuda"), torch.tensor([2, 0, 3], device="cuda", dtype=torch.int32)
+    for device in ("cpu", "cuda"):
+        for causal in (True, False):
+            got = document_layout(lens, prefix=pre, rows=11, causal=causal, device=device)
+            want = document_layout([3, 0, 5], prefix=[2, 0, 3], rows=11, causal=causal)
+            assert got.q_lo.device.type == device and torch.equal(got.dense_mask().cpu(), want.dense_mask())
+        at = document_positions(lens, rows=11, device=device)
+        assert at.device.type == device and torch.equal(at.cpu(), document_positions([3, 0, 5], rows=11))
 
 
 @pytest.mark.gpu

@@ -176,10 +176,10 @@ def document_layout(lengths, *, prefix=None, rows: int | None = None, causal: bo
     at least the document's first `prefix[d]` rows, so that a prefix is read in both directions. `lengths` are the
     documents' row counts in packing order (zero is allowed); rows behind the last document, up to `rows`, see nothing and
     are seen by nothing."""
-    lens = torch.as_tensor(lengths, dtype=torch.int64).reshape(-1)
+    lens = torch.as_tensor(lengths, dtype=torch.int64, device="cpu").reshape(-1)      # (the layout is built there)
     if lens.numel() and int(lens.min()) < 0:
         raise ValueError("document lengths must not be negative")
-    pre = torch.zeros_like(lens) if prefix is None else torch.as_tensor(prefix, dtype=torch.int64).reshape(-1)
+    pre = torch.zeros_like(lens) if prefix is None else torch.as_tensor(prefix, dtype=torch.int64, device="cpu").reshape(-1)
     if pre.shape != lens.shape or bool((pre < 0).any()) or bool((pre > lens).any()):
         raise ValueError("prefix needs one value per document, between 0 and its length")
     total = int(lens.sum())
@@ -189,20 +189,20 @@ def document_layout(lengths, *, prefix=None, rows: int | None = None, causal: bo
     start = torch.repeat_interleave(lens.cumsum(0) - lens, lens)
     stop = torch.repeat_interleave(lens.cumsum(0), lens)
     first = torch.repeat_interleave(pre, lens)
-    at = torch.arange(total)
+    at = torch.arange(total, device="cpu")
     hi = torch.maximum(at + 1, start + first) if causal else stop
     pad = rows - total
-    z = torch.zeros(pad, dtype=torch.int64)
-    out = [torch.cat([start, z]), torch.cat([hi, z]), torch.zeros(rows, dtype=torch.int64), torch.cat([at, z + DEAD_KEY])]
+    z = torch.zeros(pad, dtype=torch.int64, device="cpu")
+    out = [torch.cat([start, z]), torch.cat([hi, z]), torch.zeros(rows, dtype=torch.int64, device="cpu"), torch.cat([at, z + DEAD_KEY])]
     return MaskLayout(*(t.to(torch.int32).to(device) for t in out))
 
 
 def document_positions(lengths, *, rows: int | None = None, device="cpu") -> torch.Tensor:
     """[rows] int32 positions inside the documents of `document_layout` (0 behind the last one)."""
-    lens = torch.as_tensor(lengths, dtype=torch.int64).reshape(-1)
+    lens = torch.as_tensor(lengths, dtype=torch.int64, device="cpu").reshape(-1)
     total = int(lens.sum())
-    pos = torch.zeros(total if rows is None else int(rows), dtype=torch.int32)
-    pos[:total] = (torch.arange(total) - torch.repeat_interleave(lens.cumsum(0) - lens, lens)).to(torch.int32)
+    pos = torch.zeros(total if rows is None else int(rows), dtype=torch.int32, device="cpu")
+    pos[:total] = (torch.arange(total, device="cpu") - torch.repeat_interleave(lens.cumsum(0) - lens, lens)).to(torch.int32)
     return pos.to(device)
 
 
