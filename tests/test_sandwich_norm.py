@@ -134,6 +134,34 @@ def test_kernels(dtype, gate, rows, H):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gate", [None, "full"])
+@pytest.mark.parametrize("H", [1, 2, 3, 5, 9])
+@pytest.mark.parametrize("rows", [20001, 20004, 20008])
+def test_many_rows_of_a_few_values(dtype, gate, H, rows):
+    """Several rows to a line of 16 bytes, more rows than blocks, ends of the tensors at every place in a line."""
+    t, dy, dh = operands(rows, H, gate, dtype, "cuda", rows + H)
+    got = run(t, dy, dh)
+    part = slice(rows - 300, rows)
+    less = {n: v[part] if v.dim() == 2 else v for n, v in t.items()}
+    want, tol = exact(less["x"], less["res"], less["w_post"], less["w_pre"], less.get("gate"), 0.9, dy[part], dh[part])
+    for n in ("y", "h", "x", "res") + (("gate",) if gate else ()):
+        near(got[n][part], want[n], tol[n], n)
+
+
+@pytest.mark.gpu
+def test_rows_that_overlap_or_repeat():
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for H, ld in ((16, 0), (16, 8), (12, 4), (9, 1), (7, 0)):
+        rows = 4000
+        flat = torch.randn(rows * max(ld, 1) + H, generator=g, device="cuda").bfloat16()
+        x = flat.as_strided((rows, H), (ld, 1))
+        w = torch.ones(H, dtype=torch.bfloat16, device="cuda")
+        for a, b in zip(sandwich_norm(x, x, w, w), sandwich_norm(x.contiguous(), x.contiguous(), w, w)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("which", ["dy", "dh"])
 @pytest.mark.parametrize("gate", [None, "full"])
 def test_one_incoming_gradient(which, gate):

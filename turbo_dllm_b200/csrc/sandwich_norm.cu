@@ -25,8 +25,8 @@
 //
 // Any width goes in 16-byte lines: with V values to a line, a row that starts s values behind a 16-byte boundary is cut
 // into units [V c - s, V c - s + V). Its lines are bulk-copied as they are, the neighbours' values at both ends included,
-// and what lies outside the row is masked off when a line is read; only behind the tensors' last row, where no neighbour
-// is, the last values come one by one. Ragged lines are stored value by value. The number of blocks is a multiple of V, so
+// and what lies outside the row is masked off when a line is read; only at the tensors' last rows, behind which no neighbour
+// may be, the last values come one by one. Ragged lines are stored value by value. The number of blocks is a multiple of V, so
 // s is the same for all rows of a block. All row operands have to be shifted alike (the caller copies one that is not).
 // 2999 x 1411 fp32: 15.6 us forward, 44 us backward.
 #include "common.cuh"
@@ -110,11 +110,13 @@ struct Ring {
           for (int i = threadIdx.x; i < line_bytes / 16; i += blockDim.x)
             reinterpret_cast<uint4*>(slot(s, b))[i] = make_uint4(0u, 0u, 0u, 0u);
   }
-  // all threads: a row's lines into a stage (one thread copies; the last row's last values go in by themselves, and the
+  // rows whose last line may reach behind the tensor: a line holds up to V rows
+  __device__ __forceinline__ bool near_end(long long row) const { return SHIFT && row > last - V; }
+  // all threads: a row's lines into a stage (one thread copies; the last rows' last values go in by themselves, and the
   // caller puts a block barrier between this and their use)
   __device__ __forceinline__ void bring(int s, long long row) {
     if (!RING) return;
-    const int tail = SHIFT && row == last ? (H + shift) % V : 0;
+    const int tail = near_end(row) ? (H + shift) % V : 0;
     if (threadIdx.x == 0) {
       const int lines = SHIFT ? (tail ? (H + shift) / V : (H + shift + V - 1) / V) : H / V;
       uint32_t total = 0;
@@ -519,8 +521,8 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
         for (int j = 0; j < P; ++j) sum_post[i][j] = fma_f32x2(u[j], d[j], sum_post[i][j]);
       }
     }
-    // the tensors' last row may have had values put in by themselves: a barrier before they are read
-    if (RING && SHIFT && row + (S - 1) * step == p.rows - 1) __syncthreads();
+    // the tensors' last rows may have had values put in by themselves: a barrier before they are read
+    if (RING && SHIFT && ring.near_end(row + (S - 1) * step)) __syncthreads();
     if (++s == S) {
       s = 0;
       parity ^= 1;

@@ -113,7 +113,8 @@ def _rows2d(t: torch.Tensor) -> torch.Tensor:
     if t.is_contiguous():
         return t if t.data_ptr() % 16 == 0 else t.clone()
     H = t.shape[1]
-    if (t.stride(1) == 1 or H == 1) and t.data_ptr() % 16 == 0 and (t.stride(0) - H) * t.element_size() % 16 == 0:
+    if (t.stride(1) == 1 or H == 1) and t.data_ptr() % 16 == 0 and (t.stride(0) - H) * t.element_size() % 16 == 0 \
+            and (t.stride(0) >= H or H * t.element_size() % 16 == 0):      # (rows that overlap have no line of their own)
         return t
     return t.contiguous()
 
