@@ -478,8 +478,9 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 // exponentials of one tile overlap the products of the next; the two accumulators are joined at the end like two splits.
 //   warps 0-15 softmax, warp 16 TMA (Q once: a 3-D box of 128 / G rows x G heads lands as packed rows; K and V, three
 //   stages), warp 17 issues the MMAs.  TMEM: S0 [0,128) S1 [128,256) O0 [256,384) O1 [384,512), P over S as bf16.
-// Tiles that every row sees whole skip the mask; in the others, V rows of keys that none of the CTA's rows sees (an OR over
-// its rows, per key: the bounds' hull also holds unused cache slots between two sequences) are overwritten with zeros.
+// Tiles that every row sees whole skip the mask; in the others, V rows of keys that none of the CTA's rows sees are overwritten
+// with zeros. The bounds' hull also holds unused cache slots between two sequences, so that takes the rows' own masks: each
+// softmax warp leaves the OR over its rows, and warp 17, which has registers to spare, clears before it issues P V.
 namespace fewt {
 
 constexpr int KID = 13;
@@ -490,7 +491,7 @@ constexpr int OFF_X = OFF_STAGE + STAGES * 2 * TILE_BYTES;        // row exchang
 constexpr int OFF_BITS = OFF_X + 2048;                            // visible tiles, then fully visible tiles
 constexpr int OFF_BOUND = OFF_BITS + 2 * ROUND / 8;
 constexpr int OFF_BARS = OFF_BOUND + 32;
-constexpr int OFF_SEEN = OFF_BARS + 256;                          // keys seen: [pipeline][lane quarter][128 bits]
+constexpr int OFF_SEEN = OFF_BARS + 256;                          // keys seen: [softmax warp][its 64 keys]
 // no alignment slack: the kernel checks that its dynamic shared memory starts 1 KiB aligned
 constexpr int SMEM_BYTES = OFF_SEEN + 2 * 4 * 16;
 static_assert(SMEM_BYTES <= 232448, "shared memory budget of one CTA");
@@ -661,6 +662,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         }
         if (leader) tc_commit(bar_sfull + 8 * (j & 1));
       };
+      Walk walk(s_vis);
       bool ok = wait_all(bar_q, 0, 20);
       for (int j = 0; j < 2 && j < n && ok; ++j) {
         ok = wait_all(bar_kfull + 8 * j, 0, 21);
@@ -671,9 +673,30 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       }
       for (int j = 0; j < n && ok; ++j) {
         const int i = j & 1, s = j % STAGES;
+        const int o = walk.next();   // (before the waits, which it would lengthen)
+        const bool masked = !((s_full[o >> 5] >> (o & 31)) & 1u);
         if (!wait_all(bar_vfull + 8 * s, (j / STAGES) & 1, 22)) break;
         if (!wait_all(bar_pfull + 8 * i, (j >> 1) & 1, 23)) break;
         tc_fence_after();
+        if (masked) {   // V rows that no row of the CTA sees (behind the last key they are zeros)
+          const uint4* seen = reinterpret_cast<const uint4*>(s_seen + i * 16);
+          const uint4 a = seen[0], b = seen[1], c = seen[2], d = seen[3];   // two warps each: keys 0-63, then 64-127
+          const uint32_t some[4] = {a.x | a.z | b.x | b.z, a.y | a.w | b.y | b.w, c.x | c.z | d.x | d.z, c.y | c.w | d.y | d.w};
+          const int left = p.nk - (split + o * p.splits) * BK;
+          bool any = false;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int key = w * 32 + lane;   // (pieces of a row in an order by key: no two lanes meet in a bank)
+            if (((some[w] >> lane) & 1u) || key >= left) continue;
+            any = true;
+            uint8_t* vrow = sKV + s * 2 * TILE_BYTES + TILE_BYTES + key * 128;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              *reinterpret_cast<uint4*>(vrow + (e >> 3) * HALF_BYTES + ((e + lane) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          if (any) fence_proxy_async_smem();
+          __syncwarp();
+        }
         const uint32_t va = smem_u32(sKV + s * 2 * TILE_BYTES + TILE_BYTES);
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k) {
@@ -756,12 +779,14 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll 4
             for (int e = 0; e < 32; ++e) h |= (uint32_t)!mask.sees(__shfl_sync(0xffffffffu, code, e)) << e;
             hidden[x] = h;
-            const uint32_t some = __reduce_or_sync(0xffffffffu, ~h);   // the keys that a row of this warp sees
-            if (lane == 0) s_seen[(i * 4 + qd) * 4 + sub * 2 + x] = some;
           }
 #pragma unroll
           for (int e = 0; e < 64; ++e)
             if ((hidden[e >> 5] >> (e & 31)) & 1u) r[e] = 0xff800000u;   // -inf
+          {
+            const uint32_t s0 = ~__reduce_and_sync(0xffffffffu, hidden[0]), s1 = ~__reduce_and_sync(0xffffffffu, hidden[1]);
+            if (lane == 0) *reinterpret_cast<uint2*>(s_seen + warp * 2) = make_uint2(s0, s1);
+          }
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -770,19 +795,6 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       }
       // the barrier also orders the P stores below after the partner's loads of its score columns
       if (!named_bar_all(1 + i, 256, good)) { ok = false; break; }
-      if (masked) {
-        // this thread's key of the tile: a V row that no row of the CTA sees is cleared (half a row per thread)
-        const uint32_t* w = s_seen + i * 16 + qd;   // key `row`: word qd of the four lane quarters
-        const bool none = !(((w[0] | w[4] | w[8] | w[12]) >> lane) & 1u);
-        if (__any_sync(0xffffffffu, none)) {
-          if (none && mbar_wait_spin(bar_vfull + 8 * (j % STAGES), (j / STAGES) & 1, KID, 33)) {
-            uint4* vrow = reinterpret_cast<uint4*>(sKV + (j % STAGES) * 2 * TILE_BYTES + TILE_BYTES + sub * HALF_BYTES + row * 128);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) vrow[e] = make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-        }
-      }
       const float mx = fmaxf(*xmine, *xother);
       float alpha = 1.f;   // the reference maximum moves only when the new one is 2^8 larger
       if (mx > -INFINITY && (m == -INFINITY || (mx - m) * scl > 8.f)) {
