@@ -53,15 +53,15 @@ struct Args {
   int stages, line_bytes;         // ring: rows, bytes of one tensor's row
 };
 
-// sum of N values over the block; every thread gets the sums. CHECK: true if any thread came with `bad`
-template <int N, bool CHECK = false>
-__device__ __forceinline__ bool row_sum(float (&v)[N], float* red, bool bad = false) {
+// sum of N values over the block; every thread gets the sums
+template <int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* red) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
   const int nw = blockDim.x >> 5;
   if (nw == 1) {
     __syncwarp();
-    return CHECK && __any_sync(0xffffffffu, bad);
+    return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __syncthreads();   // the previous sums have been read
@@ -69,10 +69,9 @@ __device__ __forceinline__ bool row_sum(float (&v)[N], float* red, bool bad = fa
 #pragma unroll
     for (int i = 0; i < N; ++i) red[i * 32 + warp] = v[i];
   }
-  const bool any = CHECK ? __syncthreads_or(bad) != 0 : (__syncthreads(), false);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < nw ? red[i * 32 + lane] : 0.f);
-  return any;
 }
 
 // The ring of rows of NB tensors. RING false (rows too wide for two stages, or no more than one row per block): rows are
@@ -136,15 +135,12 @@ struct Ring {
         if (base[b] && e >= 0) slot(s, b)[shift + e] = base[b][row * ld[b] + e];
     }
   }
-  // false: the wait gave up (it ran out, or another kernel has recorded an error). No stage may be filled again then, and the
-  // block gives its copies time to land before its shared memory goes to another one; the results are undefined.
-  __device__ __forceinline__ bool wait(int s, uint32_t parity) const {
-    return !RING || mbar_wait(bars + 8 * s, parity, KID, s);
-  }
-  __device__ __forceinline__ void give_up() const {
+  // A wait gives up at once while another kernel's recorded error stands, but this block's copies are its own and land all the
+  // same: each gets up to 0.2 ms more, so that no stage is filled again, and no block ends, under a copy on its way.
+  __device__ __forceinline__ void wait(int s, uint32_t parity) const {
+    if (!RING || mbar_wait(bars + 8 * s, parity, KID, s)) return;
     const unsigned long long t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    __syncthreads();
+    while (!mbar_try_wait(bars + 8 * s, parity) && globaltimer_ns() - t0 < 200000ull) __nanosleep(100);
   }
   // line c of a tensor's row (values e ..) as pairs, zeros outside the row; keep: the bits of the line that are the row's
   __device__ __forceinline__ void read(int s, int b, long long row, int c, int e, bool whole, const uint4& keep, uint64_t* f) const {
@@ -281,7 +277,7 @@ fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h, float* __restrict
   uint32_t parity = 0;
   for (int k = 0; k < n; ++k) {
     const long long row = blockIdx.x + k * step;
-    const bool late = !ring.wait(s, parity);
+    ring.wait(s, parity);
     uint64_t hv[NV][P], sq = 0ull;
     float ss[1];
 #pragma unroll
@@ -293,10 +289,7 @@ fwd_kernel(const Args p, T* __restrict__ y, T* __restrict__ h, float* __restrict
       }
     }
     ss[0] = vio::sum_of(sq);
-    if (row_sum<1, RING>(ss, red, late)) {
-      ring.give_up();
-      break;
-    }
+    row_sum(ss, red);
     // every thread is past the previous row: its stage takes the row S - 1 ahead
     const int sn = s ? s - 1 : S - 1;
     if (RING && k + S - 1 < n) ring.bring(sn, row + (S - 1) * step);
@@ -445,7 +438,7 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
       n1 = rstd[row + step];
       n2 = rstd[p.rows + row + step];
     }
-    const bool late = !ring.wait(s, parity);
+    ring.wait(s, parity);
     uint64_t s0 = 0ull, s1 = 0ull, s2 = 0ull;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -469,10 +462,7 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
       }
     }
     float sums[3] = {vio::sum_of(s0), vio::sum_of(s1), vio::sum_of(s2)};
-    if (row_sum<3, RING>(sums, red, late)) {
-      ring.give_up();
-      break;
-    }
+    row_sum(sums, red);
     const int sn = s ? s - 1 : S - 1;
     if (RING && k + S - 1 < n) ring.bring(sn, row + (S - 1) * step);
     const float m1 = sums[0] * inv_h * r2;
@@ -521,8 +511,8 @@ bwd_kernel(const Args p, const T* __restrict__ dy, const T* __restrict__ dh, con
         for (int j = 0; j < P; ++j) sum_post[i][j] = fma_f32x2(u[j], d[j], sum_post[i][j]);
       }
     }
-    // the tensors' last rows may have had values put in by themselves: a barrier before they are read
-    if (RING && SHIFT && ring.near_end(row + (S - 1) * step)) __syncthreads();
+    // the block's last row has come in: values may have been put in by themselves, a barrier before they are read
+    if (RING && SHIFT && k + S == n) __syncthreads();
     if (++s == S) {
       s = 0;
       parity ^= 1;
