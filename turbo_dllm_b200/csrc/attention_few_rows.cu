@@ -17,10 +17,11 @@
 // bits); they meet in shared memory at the end, and the splits' partial results (fp32, with their maximum and sum) in a
 // second small kernel, in a fixed order.
 //
-// Measured with 8 KV heads of 4 query heads, joining kernel included: 1 token x 20000 keys 22.7 us (82 MB, 3.6 TB/s), 4
-// sequences x 32 tokens x 8192 keys capped 43 us (135 MB; the steady rate of one CTA per SM is 6 TB/s, so what a call pays
-// beside its bytes are about 15 us of launches, first loads, the last tile's chain and the joining kernel), 1 token x 300
-// keys 8.5 us.
+// Measured with 8 KV heads of 4 query heads, scores capped, joining kernel included, calls replayed back to back in a graph
+// (what L2 keeps of the call before helps): 1 token x 20000 keys 17.8 us (82 MB; with flushed caches 22.1 us at 3.8 TB/s and
+// the join), 4 sequences x 32 tokens x 8192 keys 42.4 us (135 MB; flushed 43.4 and the join), 1 token x 300 keys 8.7 us. From
+// 32 rows x 2048 keys (14.7 us) to 32 x 32768 (37.8) the bytes come at 5.4 TB/s, so what a call pays beside them are about
+// 13 us of launches, first loads, the last tile's chain and the joining kernel.
 //
 // Probabilities are rounded to bf16 for the product with V (as in the tile kernels), sums use them unrounded. V rows of
 // keys that none of a warp's 16 rows sees enter the product as zeros, whatever they hold.
@@ -953,8 +954,9 @@ static cudaError_t launch(const CUtensorMap& tq, const CUtensorMap& tk, const CU
 // Joins the splits of a (query row, head), W warps to each. Launched while the splits still run; the dependency wait returns
 // when that grid has ended and its results are visible. The sums run in a fixed order.
 // Four warps to a row when there are more than 8 splits, whose loads one warp would take in several rounds (one token
-// against 20000 keys, 18 splits: 22.7 us for both kernels against 23.4), else one, and few blocks (128 rows against 1024
-// keys, 4 splits: 18 us against 22 with four warps to a row). Blocks of 256 threads cost another 1 us.
+// against 20000 keys, 18 splits: 17.9 us for both kernels against 18.8; 8 rows against 4000: 14.2 against 16.2), else one, and
+// few blocks (128 rows against 1024 keys, 4 splits: 14.8 us against 19.7 with four warps to a row). Blocks of 256 threads cost
+// another 1 us.
 constexpr int JOIN_WARPS_FROM = 9;
 constexpr int JOIN_THREADS = 128;
 template <int W>
@@ -1012,9 +1014,9 @@ struct Plan {
   int wr, row_tiles, splits;
   bool tiles;   // tcgen05 on 128-row tiles
 };
-// Packed rows of a KV head from which the tcgen05 form is taken. B200, 8 KV heads of 4 query heads, us (mma form against
-// tcgen05 form): 64 rows x 2048 keys 16.2 / 16.4, 64 x 32768 63 / 37, 128 x 300 18.1 / 14.6, 128 x 2048 21 / 17.3,
-// 128 x 32768 110 / 38; up to 32 rows the tcgen05 form computes at least four times what is asked for.
+// Packed rows of a KV head from which the tcgen05 form is taken. B200, 8 KV heads of 4 query heads, capped, us (mma form against
+// tcgen05 form): 64 rows x 2048 keys 15.6 / 12.8, 64 x 32768 65 / 35, 128 x 300 19.9 / 14.5, 128 x 2048 21.9 / 14.7,
+// 128 x 32768 114 / 38; up to 32 rows the tcgen05 form computes at least four times what is asked for.
 constexpr int TILE_ROWS_FROM = 33;
 static Plan plan_of(int nq, int nk, int Hq, int Hkv) {
   Plan pl;

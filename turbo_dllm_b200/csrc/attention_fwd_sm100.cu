@@ -132,7 +132,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const uint32_t bar_epi = b0 + 120;         // [2] output staged in shared memory
   uint32_t* tmem_slot = (uint32_t*)(bars + 17);
   float* sX = (float*)((uint8_t*)bars + 512);   // [head][column half][128 rows]: row maxima, then row sums
-  // MOD: codes and positions of a tile's keys come into shared memory with its K tile. Slot j & 3 of tile j is free for
+  // MOD: codes (of tiles with a mask) and positions of a tile's keys come into shared memory with its K tile. Slot j & 3 of tile j is free for
   // tile j + 4: K of that tile waits for the scores of tile j + 2, whose products follow both heads' softmax of tile j.
   uint8_t* sMeta = (uint8_t*)bars + 512 + 2048;
   const uint32_t bar_meta = b0 + 144;           // [4]

@@ -17,7 +17,8 @@
 // gridDim.x apart and keeps a ring of them in shared memory, filled by bulk copies two or more rows ahead, so the copies
 // run while a row's sums are joined and its results are stored; the passes over a row read shared memory. (Rows loaded
 // into registers, one ahead, reached 3.4 TB/s forward and 2.9 TB/s backward at 16384 x 4096 bf16; the ring reaches 5.8 TB/s
-// (92 us) and 5.3 TB/s (152 us, both kernels).) The backward pass needs two row sums, the second of which depends on the first; it is split into
+// (92 us without a gate, 98 with one per channel) and 5.5 TB/s (147 us, both kernels).) The backward pass needs two row sums, the
+// second of which depends on the first; it is split into
 //   sum du u = sum g w_post u (dh + dt / rms(h)) - mean(dt t) / rms(h) * sum g w_post u t
 // so that all three sums are taken together in one reduction. The sums over rows stay in registers, one partial row per
 // block goes to memory, and a second kernel adds the partial rows in a fixed order, so results repeat bit for bit. For a
@@ -28,7 +29,9 @@
 // and what lies outside the row is masked off when a line is read; only at the tensors' last rows, behind which no neighbour
 // may be, the last values come one by one. Ragged lines are stored value by value. The number of blocks is a multiple of V, so
 // s is the same for all rows of a block. All row operands have to be shifted alike (the caller copies one that is not).
-// 2999 x 1411 fp32: 15.6 us forward, 44 us backward.
+// 2999 x 1411 with a full gate, forward / backward: fp16 16 / 44 us, fp32 31 / 33 us. Backward, 16-bit rows have 376 blocks
+// of three warps (the cap on partial rows), 11 % of an SM's warps, too few to cover one another's latency: they spend 23 % of
+// their time on fixed latencies, 21 % on loads and copies, 13 % each on the block barriers of the row sums and on shared memory.
 #include "common.cuh"
 #include "vec_io.cuh"
 #include "api.h"

@@ -190,8 +190,8 @@ class _SandwichNorm(torch.autograd.Function):
             part = torch.empty((lib.tdllm_sandwich_norm_parts(rows, H) * 2 * H,), dtype=torch.float32, device=dev)
             native.check(lib.tdllm_sandwich_norm_bwd(
                 x.data_ptr(), res.data_ptr(), w_post.data_ptr(), w_pre.data_ptr(), ptr(gate), ptr(dy), ptr(dh),
-                stats.data_ptr(), dx.data_ptr(), dres.data_ptr(), ptr(dgate), *(ptr(t) for t in targets), *flags, ptr(part), _row_stride(x), _row_stride(res),
-                _row_stride(gate) if kind == GATE_FULL else H, rows, H, kind, _DTYPES[dtype], res_scale, stream_of(x)),
+                stats.data_ptr(), dx.data_ptr(), dres.data_ptr(), ptr(dgate), *(ptr(t) for t in targets), *flags, ptr(part),
+                _row_stride(x), _row_stride(res), _row_stride(gate) if kind == GATE_FULL else H, rows, H, kind, _DTYPES[dtype], res_scale, stream_of(x)),
                 "sandwich_norm_bwd")
         for sink, more in again:
             sink.add_(more)

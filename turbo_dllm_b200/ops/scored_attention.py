@@ -16,6 +16,8 @@ summed over the query heads that share a KV head. Rows that see no key give out 
 rows without a visible key and keys that no row sees may hold anything, infinities and NaN included; a value that is not
 finite and that some row does see may reach the other rows of its 128-row tile.
 
+A layout's values are those of int32 tensors, noisy groups up to 2^31 - 3 (the codes behind that mark dead keys and padding).
+
 The block-diffusion masks come from `block_diffusion_layout`; `document_layout` gives packed documents (causal, or with
 a prefix that is read in both directions). On CUDA bf16 tensors with head width 128 the tcgen05 kernels run
 (`csrc/attention_fwd_sm100.cu`, `csrc/attention_bwd_fused_sm100.cu` with the transforms of `csrc/score_mod.cuh`);
@@ -60,9 +62,9 @@ LOG2E = 1.4426950408889634
 CAPS, SCALES = (1e-18, 1e30), (1e-20, 1e18)
 # A forward without gradients packs the query heads of a KV head into rows and splits the keys over the GPU (`_few`), instead
 # of giving a CTA the whole list of a 128-row query tile, for up to FEW_ROWS query rows, and for as many as one 128-row tile
-# of packed rows per SM holds. B200, scores capped, us (split / listed): 32 / 8 heads: 1 row x 20000 keys 23 / 485, 32 x 32768
-# 41 / 797, 128 x 1024 19 / 36, 512 x 512 21 / 22, 512 x 8192 114 / 188, 1024 x 8192 (two packed tiles per SM) 241 / 208; 16 / 8
-# heads: 1024 x 1024 26 / 32, 1024 x 32768 387 / 689; two key tiles: 200 x 200 20 / 16
+# of packed rows per SM holds. B200, scores capped, all keys seen, device time in us (split / listed): 32 / 8 heads: 1 row x 20000
+# keys 18 / 408, 32 x 32768 38 / 654, 128 x 1024 15 / 27, 512 x 512 15 / 17, 512 x 8192 98 / 170, 1024 x 8192 (two packed tiles
+# per SM) 195 / 171; 16 / 8 heads: 1024 x 1024 20 / 28, 1024 x 32768 369 / 659; two key tiles: 200 x 200 17 / 14
 FEW_ROWS = 128
 SMS = 148
 # The backward pass has an item of work per (key tile, chunk of query tiles, KV head). Where the key tiles and heads alone are
@@ -113,10 +115,11 @@ def _kept(cache: dict, name: str, sources: tuple, sizes: tuple, build):
 class ScoreTransform:
     """What happens to the scores before the softmax.
 
-    softcap: cap of the tanh (1e-18 to 1e30), 0 for none. slopes: [Hq] float32, one slope per query head, with q_pos [nq] and k_pos [nk]
-    (int32 or int64, absolute value below 2^24): the distance bias. Slopes are constants: they get no gradient. A position
-    beyond the limit is refused; where the host does not see positions, as in calls of few rows, which read them on the
-    device, and in captured graphs, rows that meet one get NaN."""
+    softcap: cap of the tanh (1e-18 to 1e30), 0 for none. slopes: [Hq] float32, one slope per query head, with q_pos [nq] and
+    k_pos [nk] (int32 or int64, absolute value below 2^24): the distance bias. Slopes are constants: they get no gradient. A
+    position beyond the limit is refused; where the host does not see positions, as in calls of few rows, which read them on
+    the device, and in captured graphs, rows that meet one get NaN. Scores are 32-bit numbers: a row all of whose keys are far
+    away knows them to 2^-24 of slope * distance."""
 
     softcap: float = 0.0
     slopes: torch.Tensor | None = None
@@ -193,7 +196,8 @@ def document_layout(lengths, *, prefix=None, rows: int | None = None, causal: bo
     hi = torch.maximum(at + 1, start + first) if causal else stop
     pad = rows - total
     z = torch.zeros(pad, dtype=torch.int64, device="cpu")
-    out = [torch.cat([start, z]), torch.cat([hi, z]), torch.zeros(rows, dtype=torch.int64, device="cpu"), torch.cat([at, z + DEAD_KEY])]
+    grp = torch.zeros(rows, dtype=torch.int64, device="cpu")
+    out = [torch.cat([start, z]), torch.cat([hi, z]), grp, torch.cat([at, z + DEAD_KEY])]
     return MaskLayout(*(t.to(torch.int32).to(device) for t in out))
 
 
