@@ -137,8 +137,8 @@ class _Rotary(torch.autograd.Function):
 def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, pairs: str = "half",
            scale: float = 1.0) -> torch.Tensor:
     """x [rows, H, D] (any row and head stride, e.g. the query and key heads of a packed projection) -> [rows, H, D].
-    positions [rows] int32 or int64 (within int32), freqs [n / 2] float32 with n <= D, from `rotary_frequencies`
-    (constants: they get no gradient)."""
+    positions [rows] int32 or int64 (within int32), freqs [n / 2] float32 with n <= D (2048 at most in
+    the kernel), from `rotary_frequencies` (constants: they get no gradient)."""
     if x.dim() != 3 or positions.shape != x.shape[:1]:
         raise ValueError(f"need x [rows, H, D] and one position per row, got {tuple(x.shape)} and {tuple(positions.shape)}")
     if positions.dtype not in (torch.int32, torch.int64):
